@@ -12,6 +12,9 @@ and the attention helpers of train/wan/rcm/utils/jvp_helper.py):
 * ``FlexOrSdpaLocalAttentionWithT`` -- dense / block-sparse dispatcher of the masked JVP students
 * ``MinimalA2AAttnOpWithT``, ``RopeCache`` -- RoPE-with-tangent then local attention (one-GPU branch)
 * ``apply_rope_with_tangent``       -- interleaved RoPE of a BSHD pair, differentiable
+* ``qk_norm_rope_with_tangent``     -- RMSNorm of queries and keys per head and RoPE, with tangents, differentiable
+* ``PagedKVCache``                  -- a paged key-value cache: ``qk_norm_rope_append`` (norm, rotate, write),
+  ``append_kv``, ``paged_attention`` (one or a few new tokens), ``evict_low_weight``
 """
 from .jvp_attention import (  # noqa: F401
     _attention, attention, backward_mode, backward_score_budget, current_backward_mode, plain_attention,
@@ -24,6 +27,11 @@ from .jvp_helper import (  # noqa: F401
     torch_attention_op,
     torch_attention_op_withT,
 )
-from .prologue import apply_rope_with_tangent, rmsnorm_rope_with_tangent  # noqa: F401
+from .kv_cache import (  # noqa: F401
+    PagedKVCache, append_kv, evict_low_weight, paged_attention, qk_norm_rope_append,
+)
+from .prologue import (  # noqa: F401
+    apply_rope_with_tangent, qk_norm_rope_with_tangent, rmsnorm_rope_with_tangent,
+)
 from . import magimask  # noqa: F401
 from .magimask import MagiMask, prepare_magi_csr_and_tasks  # noqa: F401

@@ -58,6 +58,29 @@ class Plan(ctypes.Structure):
         return out
 
 
+class KvCache(ctypes.Structure):
+    """``dmad_kv_cache``: the pages of a key-value cache and what its sequences hold."""
+
+    _fields_ = [
+        ("num_pages", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("batch", ctypes.c_int64),
+        ("pages_per_seq", ctypes.c_int64),
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("seen", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("position", ctypes.c_void_p),
+    ]
+
+
 # Every function the header declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -67,6 +90,7 @@ _SZ = ctypes.c_size_t
 _SZP = ctypes.POINTER(ctypes.c_size_t)
 _INT = ctypes.c_int
 _F = ctypes.c_float
+_KV = ctypes.POINTER(KvCache)
 
 SIGNATURES = {
     "dmad_abi_version": (_INT, []),
@@ -93,6 +117,18 @@ SIGNATURES = {
     "dmad_set_kernel_events": (_INT, [ctypes.POINTER(ctypes.c_void_p), _INT]),
     "dmad_probe_mfma": (_INT, [_INT, _I64, _I64, _P, _P]),
     "dmad_rmsnorm_rope_jvp": (_INT, [_INT, _I64, _I64, _I64, _I64, _P, _P, _I64, _P, _FP, _F, _P, _P, _I64, _P]),
+    "dmad_qk_norm_rope": (_INT, [_INT, _INT, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64P, _I64P, _I64P, _I64P,
+                                 _P, _P, _P, _I64, _F, _P, _P, _P, _P, _P]),
+    "dmad_qk_norm_rope_bwd_workspace_bytes": (_INT, [_I64, _I64, _I64, _I64, _I64, _SZP]),
+    "dmad_qk_norm_rope_bwd": (_INT, [_INT, _INT, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P,
+                                     _I64P, _I64P, _I64P, _I64P, _P, _P, _P, _I64, _F,
+                                     _P, _P, _P, _P, _P, _SZ, _P]),
+    "dmad_qk_norm_rope_append": (_INT, [_INT, _INT, _I64, _I64, _P, _P, _P, _I64P, _I64P, _I64P, _P, _P, _P, _I64, _F,
+                                        _P, _KV, _P]),
+    "dmad_paged_attn_workspace_bytes": (_INT, [_KV, _I64, _I64, _INT, _SZP]),
+    "dmad_paged_attn": (_INT, [_INT, _KV, _I64, _I64, _P, _I64P, _INT, _INT, _F, _P, _P, _P, _SZ, _P]),
+    "dmad_kv_evict_workspace_bytes": (_INT, [_KV, _I64, _SZP]),
+    "dmad_kv_evict": (_INT, [_INT, _KV, _I64, _I64, _I64, _P, _SZ, _P]),
     "dmad_attn_bwd_workspace_bytes": (_INT, [_INT, _I64, _I64, _I64, _I64, _I64, _SZP]),
     "dmad_attn_fwd_plan": (_INT, [_INT, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _I64, ctypes.POINTER(Plan)]),
     "dmad_attn_bwd_plan": (_INT, [_INT, _INT, _INT, _I64, _I64, _I64, _I64, _I64, ctypes.POINTER(Plan)]),
@@ -176,6 +212,16 @@ def strides4(t: torch.Tensor):
     return arr
 
 
+def int64_array(values: tuple):
+    """A ctypes array of int64, made once per tuple of values."""
+    arr = _strides_cache.get(values)
+    if arr is None:
+        if len(_strides_cache) > 4096:
+            _strides_cache.clear()
+        arr = _strides_cache[values] = (ctypes.c_int64 * len(values))(*values)
+    return arr
+
+
 def ptr(t):
     """Device address of ``t`` (None -> NULL) as an int, which ctypes passes as c_void_p."""
     return None if t is None else t.data_ptr()
@@ -189,6 +235,24 @@ def stream_ptr(device: torch.device) -> int:
     if _raw_stream is not None:
         return _raw_stream(device.index if device.index is not None else torch.cuda.current_device())
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class _HereAlready:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _HereAlready()
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one (launches need its streams' device current)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _here
+    return torch.cuda.device(device)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -268,6 +332,25 @@ def bwd_workspace_bytes_of(dtype: int, mode: int, B: int, H: int, Lq: int, Lk: i
     """Workspace of a backward whose operands have dtype code ``dtype`` (``mode`` as in
     ``bwd_workspace_bytes``): fp32 operands need only the per-row statistics."""
     return int(bwd_plan(dtype, B, H, Lq, Lk, D, full=mode > 0, tangent_grads=mode == 2)["workspace_bytes"])
+
+
+@functools.lru_cache(maxsize=1024)
+def qk_norm_rope_bwd_workspace_bytes(B: int, S: int, Hq: int, Hk: int, D: int) -> int:
+    n = ctypes.c_size_t(0)
+    check(lib().dmad_qk_norm_rope_bwd_workspace_bytes(B, S, Hq, Hk, D, ctypes.byref(n)))
+    return int(n.value)
+
+
+def paged_attn_workspace_bytes(cache: KvCache, S: int, Hq: int, accumulate: bool) -> int:
+    n = ctypes.c_size_t(0)
+    check(lib().dmad_paged_attn_workspace_bytes(ctypes.byref(cache), S, Hq, int(accumulate), ctypes.byref(n)))
+    return int(n.value)
+
+
+def kv_evict_workspace_bytes(cache: KvCache, keep: int) -> int:
+    n = ctypes.c_size_t(0)
+    check(lib().dmad_kv_evict_workspace_bytes(ctypes.byref(cache), keep, ctypes.byref(n)))
+    return int(n.value)
 
 
 def workspace(nbytes: int, device: torch.device):

@@ -57,6 +57,9 @@ def units():
     """(source, object name, extra flags) for every compilation unit."""
     out = [("capi.hip", "capi", []), ("aux.hip", "aux", []), ("prologue.hip", "prologue", []),
            ("probe.hip", "probe", [])]
+    # the per-head norm and the paged cache test for NaN (weights, positions without angles)
+    out += [("qk_norm_rope.hip", "qk_norm_rope", ["-fhonor-nans"]), ("kv_evict.hip", "kv_evict", ["-fhonor-nans"]),
+            ("paged_attn.hip", "paged_attn", ["-fhonor-nans", "-mllvm", "-amdgpu-mfma-vgpr-form"])]
     for t, tname in ((0, "bf16"), (1, "f16")):
         out.append(("fwd32_inst.hip", f"fwd32_{tname}", [f"-DDMAD_T={t}", "-mllvm", "-amdgpu-mfma-vgpr-form"]))
         out.append(("bwd_dq_inst.hip", f"bwd_dq_{tname}", [f"-DDMAD_T={t}", "-mllvm", "-amdgpu-mfma-vgpr-form"]))

@@ -7,6 +7,7 @@
 #include <string>
 
 #include "dmad_attn.h"
+#include "kv_cache.h"
 #include "launch.h"
 
 namespace dmad {
@@ -1188,6 +1189,209 @@ int bwd_impl(int dtype, int64_t B, int64_t H, int64_t Lq, int64_t Lk, int64_t D,
 }
 
 
+// ---------------------------------------------------------------- per-head norm and rotation, paged cache
+
+// Passes whose loads a wave of the norm and rotation has in flight together (it
+// rounds a wave's share up to them), and the waves that fill the chip twice over.
+constexpr int64_t kQkShare = 2, kQkFill = 16384;
+
+// One [B, S, H, D] operand by strides {b, s, h, d}: rows start 16-byte aligned.
+int check_rows(const char* name, const void* ptr, const int64_t* st, int esz) {
+  if (ptr == nullptr) return fail(DMAD_ERR_INVALID, "%s: null pointer", name);
+  if (st == nullptr) return fail(DMAD_ERR_INVALID, "%s: null strides", name);
+  if (st[3] != 1) return fail(DMAD_ERR_INVALID, "%s: stride of the head dim must be 1, got %lld", name, (long long)st[3]);
+  const int align = 16 / esz;
+  for (int i = 0; i < 3; ++i)
+    if (st[i] < 0 || st[i] % align != 0)
+      return fail(DMAD_ERR_INVALID, "%s: strides must be non-negative multiples of %d elements, got %lld", name, align,
+                  (long long)st[i]);
+  if (((uintptr_t)ptr & 15) != 0) return fail(DMAD_ERR_INVALID, "%s: base pointer must be 16-byte aligned", name);
+  return DMAD_OK;
+}
+
+// Sizes shared by the forward, the backward and the append; fills the
+// parameters' work split.
+int qk_sizes(int dtype, int wdtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t Hv, int64_t D, float eps,
+             dmad::QkNormRopeParams& p) {
+  if (dtype != DMAD_BF16 && dtype != DMAD_F16 && dtype != DMAD_F32)
+    return fail(DMAD_ERR_UNSUPPORTED, "unsupported dtype code %d", dtype);
+  if (wdtype != dtype && wdtype != DMAD_F32)
+    return fail(DMAD_ERR_UNSUPPORTED, "weights must have the operands' type or float32");
+  if (!head_dim_ok(D)) return fail(DMAD_ERR_UNSUPPORTED, "head dim must be 16, 32, 64, 128 or 256, got %lld", (long long)D);
+  if (B < 0 || S < 0 || Hq < 0 || Hk < 0 || Hq + Hk == 0)
+    return fail(DMAD_ERR_INVALID, "bad sizes B=%lld S=%lld Hq=%lld Hk=%lld", (long long)B, (long long)S, (long long)Hq,
+                (long long)Hk);
+  if (!(eps >= 0.f)) return fail(DMAD_ERR_INVALID, "eps must be non-negative");
+  const int64_t lim = (int64_t)1 << 31;
+  if (Hq >= (1 << 20) || Hk >= (1 << 20) || B >= lim || S >= lim || (B > 0 && S > (lim - 1) / B))
+    return fail(DMAD_ERR_UNSUPPORTED, "too many heads or tokens");
+  const int64_t heads[3] = {Hq, Hk, Hv}, per_pass = 512 / D;
+  int64_t passes = 0;
+  for (int i = 0; i < 3; ++i) {
+    p.op[i].H = (int)heads[i];
+    p.op[i].passes = (int)((heads[i] + per_pass - 1) / per_pass);
+    passes += p.op[i].passes;
+  }
+  // small calls spread a token's passes over waves, large ones share its angles
+  int64_t share = B * S * passes / kQkFill;
+  share = share < 1 ? 1 : (share + kQkShare - 1) / kQkShare * kQkShare;
+  if (share > passes) share = passes;
+  p.B = (int)B;
+  p.S = (int)S;
+  p.D = (int)D;
+  p.passes = (int)passes;
+  p.per_wave = (int)share;
+  p.units = B * S * ((passes + share - 1) / share);
+  // 64 threads per unit, of which a launch takes fewer than 2^32
+  if (p.units >= ((int64_t)1 << 26)) return fail(DMAD_ERR_UNSUPPORTED, "too many heads and tokens");
+  p.eps = eps;
+  return DMAD_OK;
+}
+
+// Fills operand i; t (a tangent or an output's gradient) by its own strides, or null.
+int qk_operand(dmad::QkNormRopeParams& p, int i, const char* name, int esz, const void* x, const int64_t* xs,
+               const void* t, const int64_t* ts, const void* w, void* out, void* tout) {
+  dmad::QkOperand& o = p.op[i];
+  if (o.H == 0) {
+    if (x != nullptr) return fail(DMAD_ERR_INVALID, "%s: given, but with no heads", name);
+    return DMAD_OK;
+  }
+  int rc = check_rows(name, x, xs, esz);
+  if (rc != DMAD_OK) return rc;
+  if (t != nullptr && (rc = check_rows(name, t, ts, esz)) != DMAD_OK) return rc;
+  for (const void* ptr : {w, (const void*)out, (const void*)tout})
+    if (ptr != nullptr && ((uintptr_t)ptr & 15) != 0)
+      return fail(DMAD_ERR_INVALID, "%s: weight and outputs must be 16-byte aligned", name);
+  o.x = x;
+  o.t = t;
+  o.w = w;
+  o.out = out;
+  o.tout = tout;
+  o.xb = xs[0]; o.xs = xs[1]; o.xh = xs[2];
+  if (t != nullptr) { o.tb = ts[0]; o.ts = ts[1]; o.th = ts[2]; }
+  return DMAD_OK;
+}
+
+// Checks a cache and fills the kernels' view of it.
+int check_cache(int dtype, const dmad_kv_cache* c, dmad::KvPages& kv) {
+  if (dtype != DMAD_BF16 && dtype != DMAD_F16) return fail(DMAD_ERR_UNSUPPORTED, "the cache takes bf16 or fp16");
+  if (c == nullptr) return fail(DMAD_ERR_INVALID, "cache: null pointer");
+  if (!head_dim_ok(c->head_dim))
+    return fail(DMAD_ERR_UNSUPPORTED, "head dim must be 16, 32, 64, 128 or 256, got %lld", (long long)c->head_dim);
+  if (c->page_size < 16 || c->page_size % 16 != 0)
+    return fail(DMAD_ERR_UNSUPPORTED, "page_size must be a multiple of 16, got %lld", (long long)c->page_size);
+  const int64_t lim = (int64_t)1 << 30, slots = (int64_t)1 << 26;
+  if (c->num_pages < 1 || c->kv_heads < 1 || c->batch < 0 || c->pages_per_seq < 0)
+    return fail(DMAD_ERR_INVALID, "bad cache sizes");
+  if (c->num_pages >= lim || c->kv_heads >= 65536 || c->batch >= 65536 || c->page_size > slots ||
+      (c->pages_per_seq > 0 && c->page_size > slots / c->pages_per_seq) || c->batch * c->kv_heads >= ((int64_t)1 << 22))
+    return fail(DMAD_ERR_UNSUPPORTED, "cache too large: at most 65535 sequences and heads (2^22 together) of 2^26 slots");
+  for (const void* ptr : {(const void*)c->k_pages, (const void*)c->v_pages}) {
+    if (ptr == nullptr) return fail(DMAD_ERR_INVALID, "cache pages: null pointer");
+    if (((uintptr_t)ptr & 15) != 0) return fail(DMAD_ERR_INVALID, "cache pages must be 16-byte aligned");
+  }
+  for (const int64_t* st : {c->k_strides, c->v_strides}) {
+    for (int i = 0; i < 3; ++i)
+      if (st[i] < c->head_dim || st[i] % 8 != 0)
+        return fail(DMAD_ERR_INVALID, "cache strides must be multiples of 8 elements and at least the head dim, got %lld",
+                    (long long)st[i]);
+    // a lane's offset from its 16 slots' base is a 32-bit byte offset
+    if (st[2] > ((int64_t)1 << 31) / 64) return fail(DMAD_ERR_UNSUPPORTED, "cache: stride of a slot too large");
+  }
+  if (c->batch > 0 && (c->lengths == nullptr || c->seen == nullptr))
+    return fail(DMAD_ERR_INVALID, "cache lengths and seen: null pointer");
+  if (c->batch > 0 && c->pages_per_seq > 0 && c->page_table == nullptr)
+    return fail(DMAD_ERR_INVALID, "cache page_table: null pointer");
+  if (c->batch > 1 && c->table_stride < c->pages_per_seq)
+    return fail(DMAD_ERR_INVALID, "cache page_table: rows overlap");
+  if ((c->weight == nullptr) != (c->position == nullptr))
+    return fail(DMAD_ERR_INVALID, "cache weight and position must be both set or both null");
+  kv.k = c->k_pages;
+  kv.v = c->v_pages;
+  kv.k_sp = c->k_strides[0]; kv.k_sh = c->k_strides[1]; kv.k_sl = c->k_strides[2];
+  kv.v_sp = c->v_strides[0]; kv.v_sh = c->v_strides[1]; kv.v_sl = c->v_strides[2];
+  kv.table = c->page_table;
+  kv.table_stride = c->table_stride;
+  kv.lengths = c->lengths;
+  kv.seen = c->seen;
+  kv.weight = c->weight;
+  kv.position = c->position;
+  kv.num_pages = (int)c->num_pages;
+  kv.heads = (int)c->kv_heads;
+  kv.P = (int)c->page_size;
+  kv.M = (int)c->pages_per_seq;
+  kv.B = (int)c->batch;
+  return DMAD_OK;
+}
+
+// Pieces that all sequences together aim at, per key head and row group: three
+// workgroups of the attention share a CU.
+constexpr int64_t kPagedFill = 3 * 256;
+
+struct PagedLayout {
+  int64_t R, row_groups, splits, max_splits;
+  size_t part_o, part_ml, scores, lse2, total;  // offsets; equal to the next where a part is absent
+};
+int paged_layout(const dmad_kv_cache* c, int64_t S, int64_t Hq, bool accumulate, PagedLayout& w) {
+  if (S < 0 || Hq < 1 || Hq % c->kv_heads != 0)
+    return fail(DMAD_ERR_INVALID, "query heads (%lld) must be a multiple of the cache's key heads (%lld)", (long long)Hq,
+                (long long)c->kv_heads);
+  const int64_t lim = (int64_t)1 << 31;
+  if (S >= lim / Hq) return fail(DMAD_ERR_UNSUPPORTED, "too many query rows");
+  w.R = S * (Hq / c->kv_heads);
+  const int64_t rows = dmad::paged_attn_rows((int)c->head_dim, (int)w.R);
+  w.row_groups = (w.R + rows - 1) / rows;
+  const int64_t cap = c->pages_per_seq * c->page_size;
+  const int64_t tiles = cap > 0 ? (cap + dmad::kPagedTile - 1) / dmad::kPagedTile : 1;
+  const int64_t per = c->kv_heads * (w.row_groups > 0 ? w.row_groups : 1);
+  w.splits = per < kPagedFill ? kPagedFill / per : 1;
+  w.max_splits = w.splits + c->batch;
+  if (w.max_splits > c->batch * tiles) w.max_splits = c->batch * tiles;
+  const bool join = tiles > 1;
+  const size_t BR = (size_t)c->batch * c->kv_heads * w.R;
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  size_t at = 0;
+  w.part_o = at;
+  if (join) at += up((size_t)w.max_splits * c->kv_heads * w.R * c->head_dim * 4);
+  w.part_ml = at;
+  if (join) at += up((size_t)w.max_splits * c->kv_heads * w.R * 8);
+  w.scores = at;
+  if (accumulate) at += up(BR * (size_t)cap * 4);
+  w.lse2 = at;
+  if (accumulate) at += up(BR * 4);
+  w.total = at;
+  // 256 threads per workgroup, of which a launch takes fewer than 2^32 threads
+  const int64_t groups = (int64_t)1 << 24;
+  if (w.max_splits * per >= groups || c->batch * c->kv_heads * w.R >= groups || c->batch * tiles >= lim)
+    return fail(DMAD_ERR_UNSUPPORTED, "too many pieces for one launch");
+  if (accumulate && c->batch * c->kv_heads >= 65536)
+    return fail(DMAD_ERR_UNSUPPORTED, "weights are accumulated for fewer than 65536 sequences times heads");
+  return DMAD_OK;
+}
+
+int64_t evict_moves(const dmad_kv_cache* c, int64_t keep) {
+  const int64_t cap = c->pages_per_seq * c->page_size, over = cap - keep;
+  return over <= 0 ? 0 : over < keep ? over : keep;
+}
+struct EvictLayout {
+  size_t keys, moves, counts, total;
+};
+EvictLayout evict_layout(const dmad_kv_cache* c, int64_t keep) {
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  const size_t BH = (size_t)c->batch * c->kv_heads;
+  EvictLayout w{};
+  if (c->pages_per_seq * c->page_size <= keep) return w;  // nothing can be longer
+  w.moves = up(BH * c->pages_per_seq * c->page_size * 4);
+  w.counts = w.moves + up(BH * 2 * evict_moves(c, keep) * 4);
+  w.total = w.counts + up(BH * 4);
+  return w;
+}
+int evict_sizes(const dmad_kv_cache* c, int64_t keep) {
+  if (keep < 1) return fail(DMAD_ERR_INVALID, "keep must be at least 1, got %lld", (long long)keep);
+  if (c->weight == nullptr) return fail(DMAD_ERR_INVALID, "the cache has no weights and positions");
+  return DMAD_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1475,6 +1679,201 @@ int dmad_rmsnorm_rope_jvp(int dtype, int64_t rows, int64_t L, int64_t H, int64_t
   const hipError_t e = dmad::launch_rmsnorm_rope(p, dtype, s);
   mark(0, true, s);
   if (e != hipSuccess) return fail(DMAD_ERR_HIP, "prologue launch: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int dmad_qk_norm_rope(int dtype, int wdtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, const void* q,
+                      const void* tq, const void* k, const void* tk, const int64_t q_strides[4],
+                      const int64_t tq_strides[4], const int64_t k_strides[4], const int64_t tk_strides[4],
+                      const void* wq, const void* wk, const float* freqs, int64_t freqs_stride_b, float eps, void* oq,
+                      void* otq, void* ok_, void* otk, void* stream) {
+  dmad::QkNormRopeParams p{};
+  int rc = qk_sizes(dtype, wdtype, B, S, Hq, Hk, 0, D, eps, p);
+  if (rc != DMAD_OK) return rc;
+  if (B == 0 || S == 0) return ok();
+  const bool jvp = tq != nullptr || tk != nullptr;
+  if (jvp && ((Hq > 0 && tq == nullptr) || (Hk > 0 && tk == nullptr)))
+    return fail(DMAD_ERR_INVALID, "tangents must be given for q and k, or for neither");
+  const int esz = elem_size(dtype);
+  if ((rc = qk_operand(p, 0, "q", esz, q, q_strides, tq, tq_strides, wq, oq, otq)) != DMAD_OK) return rc;
+  if ((rc = qk_operand(p, 1, "k", esz, k, k_strides, tk, tk_strides, wk, ok_, otk)) != DMAD_OK) return rc;
+  for (int i = 0; i < 2; ++i)
+    if (p.op[i].H > 0 && (p.op[i].out == nullptr || (jvp && p.op[i].tout == nullptr)))
+      return fail(DMAD_ERR_INVALID, "output: null pointer");
+  if (freqs_stride_b < 0) return fail(DMAD_ERR_INVALID, "freqs: negative stride");
+  p.freqs = freqs;
+  p.freqs_b = freqs_stride_b;
+  hipStream_t s = (hipStream_t)stream;
+  mark(0, false, s);
+  const hipError_t e = dmad::launch_qk_norm_rope(p, dtype, wdtype, jvp ? dmad::QkMode::kTangent : dmad::QkMode::kPrimal, s);
+  mark(0, true, s);
+  if (e != hipSuccess) return fail(DMAD_ERR_HIP, "norm and rotation launch: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int dmad_qk_norm_rope_bwd_workspace_bytes(int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, size_t* bytes) {
+  if (bytes == nullptr) return fail(DMAD_ERR_INVALID, "bytes: null pointer");
+  dmad::QkNormRopeParams p{};
+  const int rc = qk_sizes(DMAD_F32, DMAD_F32, B, S, Hq, Hk, 0, D, 0.f, p);
+  if (rc != DMAD_OK) return rc;
+  *bytes = (size_t)dmad::qk_norm_rope_bwd_blocks(p.units) * 2 * D * sizeof(float);
+  return ok();
+}
+
+int dmad_qk_norm_rope_bwd(int dtype, int wdtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D,
+                          const void* q, const void* gq, const void* k, const void* gk, const int64_t q_strides[4],
+                          const int64_t gq_strides[4], const int64_t k_strides[4], const int64_t gk_strides[4],
+                          const void* wq, const void* wk, const float* freqs, int64_t freqs_stride_b, float eps,
+                          void* dq, void* dk, void* dwq, void* dwk, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  dmad::QkNormRopeParams p{};
+  int rc = qk_sizes(dtype, wdtype, B, S, Hq, Hk, 0, D, eps, p);
+  if (rc != DMAD_OK) return rc;
+  const int esz = elem_size(dtype);
+  if ((dwq != nullptr && (wq == nullptr || Hq == 0)) || (dwk != nullptr && (wk == nullptr || Hk == 0)))
+    return fail(DMAD_ERR_INVALID, "the gradient of a weight that is not there");
+  if (B == 0 || S == 0) {
+    if (dwq != nullptr || dwk != nullptr) return fail(DMAD_ERR_INVALID, "no rows to sum the weights' gradients over");
+    return ok();
+  }
+  if ((Hq > 0 && gq == nullptr) || (Hk > 0 && gk == nullptr)) return fail(DMAD_ERR_INVALID, "gradient: null pointer");
+  if ((rc = qk_operand(p, 0, "q", esz, q, q_strides, gq, gq_strides, wq, dq, nullptr)) != DMAD_OK) return rc;
+  if ((rc = qk_operand(p, 1, "k", esz, k, k_strides, gk, gk_strides, wk, dk, nullptr)) != DMAD_OK) return rc;
+  for (int i = 0; i < 2; ++i)
+    if (p.op[i].H > 0 && p.op[i].out == nullptr) return fail(DMAD_ERR_INVALID, "output: null pointer");
+  if (freqs_stride_b < 0) return fail(DMAD_ERR_INVALID, "freqs: negative stride");
+  p.freqs = freqs;
+  p.freqs_b = freqs_stride_b;
+  if (dwq != nullptr || dwk != nullptr) {
+    const size_t need = (size_t)dmad::qk_norm_rope_bwd_blocks(p.units) * 2 * D * sizeof(float);
+    if (workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)
+      return fail(DMAD_ERR_WORKSPACE, "workspace: %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
+    p.partial = (float*)workspace;
+  }
+  hipStream_t s = (hipStream_t)stream;
+  mark(0, false, s);
+  const hipError_t e = dmad::launch_qk_norm_rope_bwd(p, dtype, wdtype, dwq, dwk, s);
+  mark(0, true, s);
+  if (e != hipSuccess) return fail(DMAD_ERR_HIP, "norm and rotation backward launch: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int dmad_qk_norm_rope_append(int dtype, int wdtype, int64_t S, int64_t Hq, const void* q, const void* k, const void* v,
+                             const int64_t q_strides[4], const int64_t k_strides[4], const int64_t v_strides[4],
+                             const void* wq, const void* wk, const float* freqs, int64_t freqs_rows, float eps,
+                             void* oq, const dmad_kv_cache* cache, void* stream) {
+  dmad::QkNormRopeParams p{};
+  int rc = check_cache(dtype, cache, p.kv);
+  if (rc != DMAD_OK) return rc;
+  const int64_t B = cache->batch, Hk = cache->kv_heads, D = cache->head_dim;
+  if ((rc = qk_sizes(dtype, wdtype, B, S, Hq, Hk, Hk, D, eps, p)) != DMAD_OK) return rc;
+  if (B == 0 || S == 0) return ok();
+  if ((rc = qk_operand(p, 0, "q", 2, q, q_strides, nullptr, nullptr, wq, oq, nullptr)) != DMAD_OK) return rc;
+  if ((rc = qk_operand(p, 1, "k", 2, k, k_strides, nullptr, nullptr, wk, nullptr, nullptr)) != DMAD_OK) return rc;
+  if ((rc = qk_operand(p, 2, "v", 2, v, v_strides, nullptr, nullptr, nullptr, nullptr, nullptr)) != DMAD_OK) return rc;
+  if (Hq > 0 && oq == nullptr) return fail(DMAD_ERR_INVALID, "output: null pointer");
+  if (freqs != nullptr && (freqs_rows < 1 || freqs_rows >= ((int64_t)1 << 31)))
+    return fail(DMAD_ERR_INVALID, "freqs: bad number of rows %lld", (long long)freqs_rows);
+  p.freqs = freqs;
+  p.freqs_rows = (int)(freqs != nullptr ? freqs_rows : 0);
+  hipStream_t s = (hipStream_t)stream;
+  mark(0, false, s);
+  const hipError_t e = dmad::launch_qk_norm_rope(p, dtype, wdtype, dmad::QkMode::kAppend, s);
+  mark(0, true, s);
+  if (e != hipSuccess) return fail(DMAD_ERR_HIP, "append launch: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int dmad_paged_attn_workspace_bytes(const dmad_kv_cache* cache, int64_t S, int64_t Hq, int accumulate, size_t* bytes) {
+  if (bytes == nullptr) return fail(DMAD_ERR_INVALID, "bytes: null pointer");
+  dmad::KvPages kv;
+  int rc = check_cache(DMAD_BF16, cache, kv);
+  if (rc != DMAD_OK) return rc;
+  PagedLayout w;
+  if ((rc = paged_layout(cache, S, Hq, accumulate != 0, w)) != DMAD_OK) return rc;
+  *bytes = w.total;
+  return ok();
+}
+
+int dmad_paged_attn(int dtype, const dmad_kv_cache* cache, int64_t S, int64_t Hq, const void* q,
+                    const int64_t q_strides[4], int causal, int accumulate, float sm_scale, void* o, float* lse,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  dmad::PagedAttnParams p{};
+  int rc = check_cache(dtype, cache, p.kv);
+  if (rc != DMAD_OK) return rc;
+  if (!(sm_scale > 0.f)) return fail(DMAD_ERR_UNSUPPORTED, "sm_scale must be positive");
+  PagedLayout w;
+  if ((rc = paged_layout(cache, S, Hq, accumulate != 0, w)) != DMAD_OK) return rc;
+  if (accumulate && cache->weight == nullptr) return fail(DMAD_ERR_INVALID, "the cache has no weights to accumulate");
+  if (cache->batch == 0 || S == 0) return ok();
+  if ((rc = check_rows("q", q, q_strides, 2)) != DMAD_OK) return rc;
+  if (o == nullptr || lse == nullptr) return fail(DMAD_ERR_INVALID, "output: null pointer");
+  if (((uintptr_t)o & 15) != 0) return fail(DMAD_ERR_INVALID, "o must be 16-byte aligned");
+  if (w.total > 0 && (workspace == nullptr || workspace_bytes < w.total || ((uintptr_t)workspace & 255) != 0))
+    return fail(DMAD_ERR_WORKSPACE, "workspace: %zu bytes (256-byte aligned) needed, %zu given", w.total, workspace_bytes);
+  char* ws = (char*)workspace;
+  p.q = q;
+  p.qb = q_strides[0]; p.qs = q_strides[1]; p.qh = q_strides[2];
+  p.o = o;
+  p.lse = lse;
+  p.S = (int)S;
+  p.G = (int)(Hq / cache->kv_heads);
+  p.R = (int)w.R;
+  p.row_groups = (int)w.row_groups;
+  p.causal = causal != 0;
+  p.splits = (int)w.splits;
+  p.max_splits = (int)w.max_splits;
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  if (w.part_ml > w.part_o) {
+    p.part_o = (float*)(ws + w.part_o);
+    p.part_ml = (float*)(ws + w.part_ml);
+  }
+  if (accumulate) {
+    p.scores = (float*)(ws + w.scores);
+    p.lse2 = (float*)(ws + w.lse2);
+  }
+  hipStream_t s = (hipStream_t)stream;
+  mark(0, false, s);
+  const hipError_t e = dmad::launch_paged_attn(p, dtype, (int)cache->head_dim, s);
+  mark(0, true, s);
+  if (e != hipSuccess) return fail(DMAD_ERR_HIP, "paged attention launch: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int dmad_kv_evict_workspace_bytes(const dmad_kv_cache* cache, int64_t keep, size_t* bytes) {
+  if (bytes == nullptr) return fail(DMAD_ERR_INVALID, "bytes: null pointer");
+  dmad::KvPages kv;
+  int rc = check_cache(DMAD_BF16, cache, kv);
+  if (rc != DMAD_OK || (rc = evict_sizes(cache, keep)) != DMAD_OK) return rc;
+  *bytes = evict_layout(cache, keep).total;
+  return ok();
+}
+
+int dmad_kv_evict(int dtype, const dmad_kv_cache* cache, int64_t keep, int64_t recent, int64_t sink, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  dmad::KvEvictParams p{};
+  int rc = check_cache(dtype, cache, p.kv);
+  if (rc != DMAD_OK || (rc = evict_sizes(cache, keep)) != DMAD_OK) return rc;
+  if (recent < 0 || sink < 0 || recent > keep || sink > keep - recent)
+    return fail(DMAD_ERR_INVALID, "recent and sink must be non-negative and together at most keep");
+  const EvictLayout w = evict_layout(cache, keep);
+  if (cache->batch == 0 || w.total == 0) return ok();
+  if (workspace == nullptr || workspace_bytes < w.total || ((uintptr_t)workspace & 255) != 0)
+    return fail(DMAD_ERR_WORKSPACE, "workspace: %zu bytes (256-byte aligned) needed, %zu given", w.total, workspace_bytes);
+  char* ws = (char*)workspace;
+  p.D = (int)cache->head_dim;
+  p.keep = (int)keep;
+  p.recent = (int)recent;
+  p.sink = (int)sink;
+  p.max_moves = (int)evict_moves(cache, keep);
+  p.keys = (uint32_t*)(ws + w.keys);
+  p.moves = (int32_t*)(ws + w.moves);
+  p.counts = (int32_t*)(ws + w.counts);
+  hipStream_t s = (hipStream_t)stream;
+  mark(0, false, s);
+  const hipError_t e = dmad::launch_kv_evict(p, s);
+  mark(0, true, s);
+  if (e != hipSuccess) return fail(DMAD_ERR_HIP, "eviction launch: %s", hipGetErrorString(e));
   return ok();
 }
 

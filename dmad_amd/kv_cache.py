@@ -1,0 +1,257 @@
+"""A paged key-value cache for token-by-token and block-by-block inference on the gfx950 kernels.
+
+``PagedKVCache`` holds the pages and what its sequences hold. Three calls work on it:
+
+  * ``qk_norm_rope_append``: the new tokens' queries and keys are normalised per head and rotated
+    (as ``qk_norm_rope_with_tangent`` does), keys and values go into the pages; ``append_kv`` is
+    the same without queries, norm and rotation;
+  * ``paged_attention``: attention of those queries over the cache, optionally adding up the
+    attention weight every slot receives;
+  * ``evict_low_weight``: cuts long sequences to their heaviest slots.
+
+They run without gradients, put only kernel launches on the current stream and read lengths and
+page table on the device, so a captured step follows them. Nothing is copied to the host: what
+the device holds is checked by the kernels (see ``PagedKVCache``). Device work only: tensors off
+the GPU raise.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _native as nat
+from .prologue import HEAD_DIMS, _check_same_device, _norm_weights, readable_rows
+
+
+class PagedKVCache:
+    """Pages of keys and values, one page list per sequence.
+
+    k_pages, v_pages  [N, Hk, P, D] bf16 or fp16; P a multiple of 16; D one of 16, 32, 64, 128, 256.
+                      Any strides with contiguous rows and multiples of 8 elements: an
+                      [N, P, Hk, D] pool is passed as its transpose(1, 2)
+    page_table        [B, M] int32: slot s of sequence b is slot s % P of page page_table[b, s // P].
+                      An id outside [0, N) (-1) marks a page that holds nothing: its slots are not
+                      read or written and no query sees them, so a window may drop pages in front
+    lengths           [B] int32, slots in use; values outside [0, M * P] count as the nearer end
+    seen              [B] int32, tokens appended so far: the position of the next one. Equal to
+                      lengths until something is evicted
+    weight, position  [N, Hk, P] float32 and int32: each slot's accumulated attention weight and
+                      its token's position; both or neither (None: no accumulation, no eviction)
+
+    The tensors are used in place and stay the caller's: pages are handed out, shared or dropped
+    by writing to ``page_table`` and ``lengths``. A page may appear in several sequences as long
+    as it is only read; pages that are appended to, evicted from or whose weights are accumulated
+    belong to one sequence.
+    """
+
+    def __init__(self, k_pages, v_pages, page_table, lengths, seen, weight=None, position=None):
+        op = "PagedKVCache"
+        self.device = _check_same_device(op, k_pages, v_pages, page_table, lengths, seen, weight, position)
+        if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+            raise ValueError(f"{op}: k_pages and v_pages must be [N, Hk, P, D], got {tuple(k_pages.shape)} and "
+                             f"{tuple(v_pages.shape)}")
+        if k_pages.dtype not in (torch.bfloat16, torch.float16) or v_pages.dtype != k_pages.dtype:
+            raise NotImplementedError(f"{op}: pages must be bfloat16 or float16, got {k_pages.dtype} and {v_pages.dtype}")
+        N, Hk, P, D = k_pages.shape
+        if D not in HEAD_DIMS:
+            raise NotImplementedError(f"{op}: head dim {D} is not one of {HEAD_DIMS}")
+        if P < 16 or P % 16:
+            raise NotImplementedError(f"{op}: the page size must be a multiple of 16, got {P}")
+        if N < 1 or Hk < 1:
+            raise ValueError(f"{op}: an empty pool {tuple(k_pages.shape)}")
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise ValueError(f"{op}: page_table must be [B, M] int32 with contiguous rows")
+        B, M = page_table.shape
+        for name, t in (("lengths", lengths), ("seen", seen)):
+            if t.shape != (B,) or t.dtype != torch.int32 or not t.is_contiguous():
+                raise ValueError(f"{op}: {name} must be [{B}] int32, contiguous")
+        if (weight is None) != (position is None):
+            raise ValueError(f"{op}: weight and position together, or neither")
+        for name, t, dtype in (("weight", weight, torch.float32), ("position", position, torch.int32)):
+            if t is not None and (t.shape != (N, Hk, P) or t.dtype != dtype or not t.is_contiguous()):
+                raise ValueError(f"{op}: {name} must be [{N}, {Hk}, {P}] {dtype}, contiguous")
+
+        def strides(name, t):
+            if t.stride(3) != 1 or t.data_ptr() % 16:
+                raise ValueError(f"{op}: rows of {name} must be contiguous and 16-byte aligned")
+            st = [D if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
+            if any(s % 8 or s < D for s in st):
+                raise ValueError(f"{op}: strides of {name} must be multiples of 8 elements and at least {D}, got {t.stride()}")
+            return (ctypes.c_int64 * 3)(*st)
+
+        self.k_pages, self.v_pages, self.page_table = k_pages, v_pages, page_table
+        self.lengths, self.seen, self.weight, self.position = lengths, seen, weight, position
+        self.dtype, self.batch, self.kv_heads, self.page_size, self.head_dim = k_pages.dtype, B, Hk, P, D
+        self.capacity = M * P
+        self._sizes = {}
+        self._c = nat.KvCache(N, Hk, P, D, B, M, nat.ptr(k_pages), nat.ptr(v_pages), strides("k_pages", k_pages),
+                              strides("v_pages", v_pages), nat.ptr(page_table), page_table.stride(0) if B > 1 else M,
+                              nat.ptr(lengths), nat.ptr(seen), nat.ptr(weight), nat.ptr(position))
+        self._ref = ctypes.byref(self._c)
+
+    def __setattr__(self, name, value):
+        if hasattr(self, "_ref"):
+            raise AttributeError(f"PagedKVCache.{name} cannot be replaced: write into the tensors in place")
+        object.__setattr__(self, name, value)
+
+    @classmethod
+    def allocate(cls, batch, capacity, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda", page_size=64,
+                 track_weights=True):
+        """An empty cache of ``batch`` sequences of up to ``capacity`` slots (rounded up to whole
+        pages), each with its own pages in order. ``track_weights``: room for weights and positions."""
+        if batch < 1 or capacity < 1 or kv_heads < 1:
+            raise ValueError(f"PagedKVCache.allocate: batch {batch}, capacity {capacity}, kv_heads {kv_heads}")
+        if page_size < 16 or page_size % 16:
+            raise NotImplementedError(f"PagedKVCache: the page size must be a multiple of 16, got {page_size}")
+        M = -(-capacity // page_size)
+        N = batch * M
+        pages = (N, kv_heads, page_size)
+        return cls(
+            torch.empty((*pages, head_dim), device=device, dtype=dtype),
+            torch.empty((*pages, head_dim), device=device, dtype=dtype),
+            torch.arange(N, device=device, dtype=torch.int32).view(batch, M),
+            torch.zeros(batch, device=device, dtype=torch.int32),
+            torch.zeros(batch, device=device, dtype=torch.int32),
+            torch.zeros(pages, device=device, dtype=torch.float32) if track_weights else None,
+            torch.zeros(pages, device=device, dtype=torch.int32) if track_weights else None,
+        )
+
+    def _workspace(self, key, query):
+        """A fresh workspace whose size ``query`` gives, asked once per ``key``."""
+        size = self._sizes.get(key)
+        if size is None:
+            size = self._sizes[key] = query()
+        return nat.workspace(size, self.device)
+
+
+def _check_new(op, cache, *named):
+    """Shapes of new tokens' q, k, v against the cache: (S, Hq)."""
+    if not isinstance(cache, PagedKVCache):
+        raise TypeError(f"{op}: cache must be a PagedKVCache, got {type(cache).__name__}")
+    given = [(n, t) for n, t in named if t is not None]
+    dev = _check_same_device(op, *(t for _, t in given))
+    if dev != cache.device:
+        raise ValueError(f"{op}: tensors on {dev}, the cache on {cache.device}")
+    for n, t in given:
+        if t.dim() != 4 or t.shape[0] != cache.batch or t.shape[3] != cache.head_dim or t.shape[1] != given[0][1].shape[1]:
+            raise ValueError(f"{op}: {n} must be [{cache.batch}, S, H, {cache.head_dim}], got {tuple(t.shape)}")
+        if t.dtype != cache.dtype:
+            raise ValueError(f"{op}: {n} is {t.dtype}, the cache {cache.dtype}")
+        if n != "q" and t.shape[2] != cache.kv_heads:
+            raise ValueError(f"{op}: {n} has {t.shape[2]} heads, the cache {cache.kv_heads}")
+
+
+def _no_grad_only(op, *ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"{op} has no backward: call it under torch.no_grad()")
+
+
+def qk_norm_rope_append(q, k, v, q_weight, k_weight, eps, freqs, cache):
+    """Appends S new tokens to every sequence of the cache and returns their queries.
+
+    q [B, S, Hq, D] comes back normalised per head and rotated, k [B, S, Hk, D] goes into the cache
+    so, v [B, S, Hk, D] as it is. The tokens take the slots after ``cache.lengths`` and the positions
+    from ``cache.seen`` on; then both advance by S. ``freqs`` [T, D/2] are angles by position, shared
+    by the sequences: a token whose position has no row gets NaN in q and k. A weight of None skips
+    that norm, freqs None the rotation. New slots start with weight 0. Tokens beyond the capacity
+    are dropped (``lengths`` stays at it, ``seen`` advances), and those whose page holds nothing.
+    """
+    op = "qk_norm_rope_append"
+    if k is None or v is None:
+        raise ValueError(f"{op}: k and v must be given")
+    _check_new(op, cache, ("k", k), ("v", v), ("q", q))
+    _check_same_device(op, k, q_weight, k_weight, freqs)
+    _no_grad_only(op, q, k, v, q_weight, k_weight)
+    if not eps >= 0:
+        raise ValueError(f"{op}: eps must be non-negative, got {eps}")
+    B, S, D = cache.batch, k.shape[1], cache.head_dim
+    if q is None and q_weight is not None:
+        raise ValueError(f"{op}: q_weight without q")
+    cq, ck, wcode = _norm_weights(op, k, D, q_weight, k_weight)
+    if freqs is not None:
+        if freqs.dim() != 2 or freqs.shape[1] != D // 2 or freqs.shape[0] < 1:
+            raise ValueError(f"{op}: freqs must be [positions, {D // 2}], got {tuple(freqs.shape)}")
+        freqs = freqs.to(torch.float32).contiguous()
+    Hq = 0 if q is None else q.shape[2]
+    out = None if q is None else torch.empty((B, S, Hq, D), device=q.device, dtype=q.dtype)
+    if Hq == 0:
+        q = None
+    ops = [(None, None) if t is None else readable_rows(t) for t in (q, k, v)]
+    with nat.on_device(cache.device):
+        nat.check(nat.lib().dmad_qk_norm_rope_append(
+            nat.dtype_code(cache.dtype), wcode, S, Hq, *(nat.ptr(t) for t, _ in ops), *(s for _, s in ops),
+            nat.ptr(cq if q is not None else None), nat.ptr(ck), nat.ptr(freqs), 0 if freqs is None else freqs.shape[0],
+            float(eps), nat.ptr(out), cache._ref, nat.stream_ptr(cache.device)))
+    return out
+
+
+def append_kv(k, v, cache):
+    """Appends k and v [B, S, Hk, D] to the cache as they are (see ``qk_norm_rope_append``)."""
+    qk_norm_rope_append(None, k, v, None, None, 0.0, None, cache)
+
+
+def paged_attention(q, cache, sm_scale=None, causal=False, accumulate=False, return_lse=False):
+    """Attention of q [B, S, Hq, D] over each sequence's cache: o [B, S, Hq, D] (and lse [B, Hq, S]).
+
+    Made for few new tokens (S = 1, a draft of a few, a small block): the work is split over the
+    cache's length. Hq is a multiple of the cache's heads; query head h reads key head
+    h // (Hq // Hk). ``sm_scale`` defaults to D^-1/2. Every token sees all slots in use;
+    with ``causal`` the S tokens are the last S slots (just appended, nothing evicted since) and
+    each sees the slots up to its own. A token that sees no slot gets o = 0 and lse = -inf, and so
+    does one whose scores are all -inf. With ``causal``, an infinity or NaN in a new token's value
+    reaches the other new tokens of its sequence and key head.
+
+    ``accumulate`` adds to ``cache.weight`` what each slot receives: its softmax weight summed over
+    the S tokens and the query heads of its key head.
+    """
+    op = "paged_attention"
+    _check_new(op, cache, ("q", q))
+    _no_grad_only(op, q)
+    S, Hq = q.shape[1], q.shape[2]
+    if Hq < 1 or Hq % cache.kv_heads:
+        raise ValueError(f"{op}: {Hq} query heads are not a multiple of the cache's {cache.kv_heads}")
+    scale = cache.head_dim ** -0.5 if sm_scale is None else float(sm_scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise NotImplementedError(f"{op}: sm_scale must be positive and finite, got {sm_scale}")
+    if accumulate and cache.weight is None:
+        raise ValueError(f"{op}: the cache keeps no weights to accumulate")
+    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    lse = torch.empty((cache.batch, Hq, S), device=q.device, dtype=torch.float32)
+    q, strides = readable_rows(q)
+    accumulate = bool(accumulate)
+    ws_ptr, ws_size, ws = cache._workspace(
+        (S, Hq, accumulate), lambda: nat.paged_attn_workspace_bytes(cache._c, S, Hq, accumulate))
+    with nat.on_device(cache.device):
+        nat.check(nat.lib().dmad_paged_attn(
+            nat.dtype_code(cache.dtype), cache._ref, S, Hq, nat.ptr(q), strides, int(bool(causal)), int(accumulate), scale,
+            nat.ptr(o), nat.ptr(lse), ws_ptr, ws_size, nat.stream_ptr(cache.device)))
+    return (o, lse) if return_lse else o
+
+
+def evict_low_weight(cache, keep, recent=0, sink=0):
+    """Cuts every sequence of more than ``keep`` slots to ``keep``, in place, each key head by itself.
+
+    Slots of the first ``sink`` positions and of the last ``recent`` ones (of ``cache.seen``) stay,
+    then those with the largest accumulated weight; of equal ones the lower slots. Slots below
+    ``keep`` that go are filled, in order, with those beyond that stay, with their weights and
+    positions: slots are in no order of position afterwards, and a key head's slot holds another
+    token than another head's. Pages beyond ``keep`` slots are free then. A NaN weight counts as
+    the largest. Slots of missing pages stay below ``keep`` and go beyond it.
+    """
+    op = "evict_low_weight"
+    if not isinstance(cache, PagedKVCache):
+        raise TypeError(f"{op}: cache must be a PagedKVCache, got {type(cache).__name__}")
+    if cache.weight is None:
+        raise ValueError(f"{op}: the cache keeps no weights and positions")
+    keep, recent, sink = int(keep), int(recent), int(sink)
+    if keep < 1 or recent < 0 or sink < 0 or recent + sink > keep:
+        raise ValueError(f"{op}: keep must be at least 1, recent and sink non-negative and together at most keep; got "
+                         f"keep={keep}, recent={recent}, sink={sink}")
+    if keep >= cache.capacity or cache.batch == 0:
+        return  # no sequence can be longer
+    ws_ptr, ws_size, ws = cache._workspace(("evict", keep), lambda: nat.kv_evict_workspace_bytes(cache._c, keep))
+    with nat.on_device(cache.device):
+        nat.check(nat.lib().dmad_kv_evict(nat.dtype_code(cache.dtype), cache._ref, keep, recent, sink, ws_ptr, ws_size,
+                                          nat.stream_ptr(cache.device)))

@@ -324,6 +324,112 @@ int dmad_attn_bwd_plan_ws(int dtype, int full, int tangent_grads, int64_t B, int
 int dmad_attn_bwd_score_bytes(int dtype, int full, int64_t Lq, int64_t Lk, int64_t D, size_t* bytes);
 
 /*
+ * RMSNorm of queries and keys for each head with the rotation of their pairs
+ * in the same pass (no counterpart in the reference, whose norm runs over the
+ * whole model width; the rotation is train/wan/rcm/utils/rope.py:56-70).
+ *   q, k  : [B, S, Hq, D], [B, S, Hk, D] by element strides {b, s, h, d},
+ *           d = 1; k null with Hk = 0, or q null with Hq = 0
+ *   tq, tk: tangents by their own strides, or both null; an operand that is
+ *           absent has none
+ *   wq, wk: [D] weights of type wdtype (the operands' or DMAD_F32); null skips
+ *           that operand's norm
+ *   freqs : [S][D/2] float32 angles, freqs_stride_b elements from one batch
+ *           entry's to the next (0: shared); null skips the rotation
+ *   oq, ok, otq, otk: contiguous [B, S, H, D] outputs
+ * D in {16, 32, 64, 128, 256}; bf16, fp16 and fp32. Rows start 16-byte
+ * aligned. Computed in float32 and rounded once.
+ */
+int dmad_qk_norm_rope(int dtype, int wdtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, const void* q,
+                      const void* tq, const void* k, const void* tk, const int64_t q_strides[4],
+                      const int64_t tq_strides[4], const int64_t k_strides[4], const int64_t tk_strides[4],
+                      const void* wq, const void* wk, const float* freqs, int64_t freqs_stride_b, float eps, void* oq,
+                      void* otq, void* ok, void* otk, void* stream);
+
+/* Bytes of workspace of dmad_qk_norm_rope_bwd (0 where no weight gradient is asked for is also accepted there). */
+int dmad_qk_norm_rope_bwd_workspace_bytes(int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, size_t* bytes);
+
+/*
+ * Its backward over the primal outputs: gq, gk the outputs' gradients (strides
+ * as the operands'; null with the operand null), dq, dk contiguous
+ * [B, S, H, D], dwq, dwk [D] of type wdtype or null. The weights' gradients
+ * are summed in a fixed order.
+ */
+int dmad_qk_norm_rope_bwd(int dtype, int wdtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D,
+                          const void* q, const void* gq, const void* k, const void* gk, const int64_t q_strides[4],
+                          const int64_t gq_strides[4], const int64_t k_strides[4], const int64_t gk_strides[4],
+                          const void* wq, const void* wk, const float* freqs, int64_t freqs_stride_b, float eps,
+                          void* dq, void* dk, void* dwq, void* dwk, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/*
+ * A paged key-value cache in device memory. Sequence b's slot s is slot
+ * s % page_size of page page_table[b * table_stride + s / page_size]; an id
+ * outside [0, num_pages) marks a page that holds nothing: its slots are
+ * neither read nor written, and no row attends to them. Lengths outside
+ * [0, pages_per_seq * page_size] are clipped. Pages that are written belong to
+ * one sequence.
+ *   k_strides, v_strides: elements between pages, heads and slots; the head
+ *           dim's is 1
+ *   weight, position: [num_pages][kv_heads][page_size], or both null where
+ *           nothing is accumulated or evicted
+ * page_size: a multiple of 16. bf16 and fp16.
+ */
+typedef struct dmad_kv_cache {
+  int64_t num_pages, kv_heads, page_size, head_dim, batch, pages_per_seq;
+  void* k_pages;
+  void* v_pages;
+  int64_t k_strides[3], v_strides[3];
+  const int32_t* page_table;
+  int64_t table_stride;
+  int32_t* lengths;  /* [batch] slots in use */
+  int32_t* seen;     /* [batch] tokens appended so far: the next one's position */
+  float* weight;     /* attention weight each slot has received */
+  int32_t* position; /* position of each slot's token */
+} dmad_kv_cache;
+
+/*
+ * Appends S new tokens to every sequence: q [B, S, Hq, D] (null with Hq = 0)
+ * is normalised and rotated into oq, k [B, S, kv_heads, D] likewise into its
+ * slots, v copied; weight 0 and the position are set, then lengths and seen
+ * advance by S. wq, wk, freqs null skip norm and rotation. freqs: [freqs_rows][D/2]
+ * angles by position; a position without a row gives NaN. Tokens beyond the
+ * capacity are dropped and lengths stay at it.
+ */
+int dmad_qk_norm_rope_append(int dtype, int wdtype, int64_t S, int64_t Hq, const void* q, const void* k, const void* v,
+                             const int64_t q_strides[4], const int64_t k_strides[4], const int64_t v_strides[4],
+                             const void* wq, const void* wk, const float* freqs, int64_t freqs_rows, float eps,
+                             void* oq, const dmad_kv_cache* cache, void* stream);
+
+/* Bytes of workspace of dmad_paged_attn. */
+int dmad_paged_attn_workspace_bytes(const dmad_kv_cache* cache, int64_t S, int64_t Hq, int accumulate, size_t* bytes);
+
+/*
+ * Attention of q [B, S, Hq, D] over the cache, query head h on key head
+ * h / (Hq / kv_heads). causal = 0: every row sees the sequence's slots;
+ * causal = 1: the S tokens are the last S slots and token i sees the slots up
+ * to its own. A row that sees none gets o = 0, lse = -inf. accumulate: adds
+ * each slot's softmax weight over all rows to cache->weight.
+ *   o: contiguous [B, S, Hq, D]; lse: [B, Hq, S] float32, natural log
+ */
+int dmad_paged_attn(int dtype, const dmad_kv_cache* cache, int64_t S, int64_t Hq, const void* q,
+                    const int64_t q_strides[4], int causal, int accumulate, float sm_scale, void* o, float* lse,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of dmad_kv_evict. */
+int dmad_kv_evict_workspace_bytes(const dmad_kv_cache* cache, int64_t keep, size_t* bytes);
+
+/*
+ * Cuts every sequence of more than `keep` slots to `keep`, each key head by
+ * itself: slots of positions below `sink` and of the last `recent` positions
+ * stay, then those of the largest weight (NaN above all, equal ones by the
+ * lower slot). The i-th slot below `keep` that goes takes over the i-th slot
+ * at or beyond `keep` that stays, with its weight and position.
+ * sink + recent <= keep.
+ */
+int dmad_kv_evict(int dtype, const dmad_kv_cache* cache, int64_t keep, int64_t recent, int64_t sink, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
+/*
  * Timing hook (no counterpart in the reference; for benchmarks and profilers
  * that time kernels live). `events` points to `count` hipEvent_t handles; while
  * set, every dmad_attn_jvp_fwd / dmad_attn_fwd / dmad_attn_jvp_bwd call on

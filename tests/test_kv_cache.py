@@ -1,0 +1,759 @@
+"""The paged key-value cache: append with norm and rotation, attention of new tokens, eviction.
+
+CPU: the address and bounds arithmetic the kernels use (csrc/kv_pages.h, compiled for the host), the
+oracle's eviction on a hand-made case, and what the C entries refuse. GPU: every call against
+oracle/streaming.py in float64 on copies of the same cache, in pools whose unused slots hold NaN.
+
+Bounds for attention, from u = finfo.eps / 2 of the 16-bit type: P is rounded to that type for its
+product (u of sum p|v|; in fp16 also half a subnormal step, 2^-25, of sum |v|), O once more (u of |o|).
+A score is a float32 sum of D products and a scaling, off by at most es = (D + 8) 2^-24 of the largest
+scaled sum |q k| of its row, which moves each p by the factor 1 +- 2 es; exponentials, sums and joins add less than
+64 half steps of float32.
+"""
+import ctypes
+import math
+import os
+import subprocess
+
+import pytest
+import torch
+
+from oracle import streaming as st
+
+F32 = 2.0 ** -24
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+# ---------------------------------------------------------------- on the CPU
+
+
+def test_addresses_stay_inside_the_pool(tmp_path):
+    """Whatever table, lengths and slots hold: a located slot lies on a page of the pool, lengths are
+    clipped to the capacity, and appended slots stay below it."""
+    src = tmp_path / "pages.cpp"
+    src.write_text(r"""
+#include <climits>
+#include <cstdio>
+#include <vector>
+#include "kv_pages.h"
+using namespace dmad;
+int main() {
+  const int ids[] = {-1, 0, 1, 5, 6, 7, INT_MAX, INT_MIN, -7};
+  const int nums[] = {0, 1, 15, 16, 17, 47, 48, 95, 96, 97, 143, 144, 145, INT_MAX, INT_MAX - 1, INT_MIN, -1, -16};
+  long checked = 0;
+  for (int P : {16, 48}) for (int M : {0, 1, 3}) {
+    const int N = 6, H = 2, B = 2;
+    std::vector<int32_t> table(B * (M + 1)), lengths(B), seen(B);
+    KvPages kv{};
+    kv.table = table.data(); kv.table_stride = M + 1; kv.lengths = lengths.data(); kv.seen = seen.data();
+    kv.num_pages = N; kv.heads = H; kv.P = P; kv.M = M; kv.B = B;
+    kv.k_sp = kv.v_sp = H * P * 16; kv.k_sh = kv.v_sh = P * 16; kv.k_sl = kv.v_sl = 16;
+    for (int id : ids) {
+      for (auto& t : table) t = id;
+      for (int n : nums) {
+        lengths[0] = lengths[1] = n;
+        const int len = kv.length(1);
+        if (len < 0 || len > M * P || (n >= 0 && n <= M * P && len != n)) return 1;
+        for (int s : nums) {
+          const KvSlot at = kv.locate(1, s);
+          const bool should = s >= 0 && s < M * P && id >= 0 && id < N;
+          if (should != (at.page >= 0)) return 2;
+          if (should && (at.page != id || at.slot != s % P)) return 3;
+          if (should && (kv.index(at, H - 1) < 0 || kv.index(at, H - 1) >= (int64_t)N * H * P)) return 4;
+          if (should && (kv.k_offset(at, H - 1) + 16 > (int64_t)N * H * P * 16 || kv.v_offset(at, 0) < 0)) return 5;
+          if (!should && (at.page != -1 || at.slot != 0)) return 6;
+          if (s >= 0) {
+            const int slot = kv_append_slot(len, s, M * P);
+            if (slot != -1 && (slot < len || slot >= M * P || slot - len != s)) return 7;
+            if (slot == -1 && (int64_t)len + s < (int64_t)M * P) return 8;
+            const int after = kv_append_length(len, s, M * P);
+            if (after < len || after > M * P || (after < M * P && after - len != s)) return 9;
+          }
+          ++checked;
+        }
+      }
+    }
+  }
+  // offsets beyond 32 bits
+  KvPages big{};
+  int32_t page = 70000;
+  big.table = &page; big.table_stride = 1; big.num_pages = 100000; big.heads = 8; big.P = 64; big.M = 1; big.B = 1;
+  big.k_sp = big.v_sp = 8 * 64 * 128; big.k_sh = big.v_sh = 64 * 128; big.k_sl = big.v_sl = 128;
+  if (big.k_offset(big.locate(0, 63), 7) != 70000LL * 65536 + 7 * 8192 + 63 * 128) return 10;
+  printf("%ld\n", checked);
+  return 0;
+}
+""")
+    exe = tmp_path / "pages"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover",
+                    "-I", os.path.join(ROOT, "dmad_amd", "csrc"), str(src), "-o", str(exe)], check=True)
+    done = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert done.returncode == 0 and int(done.stdout) > 1000, (done.returncode, done.stderr)
+
+
+def test_oracle_eviction_by_hand():
+    """Six slots, four stay: the sink 0, the two last positions (4 and 5) and the heavier of 1, 2, 3."""
+    c = dict(k_pages=torch.arange(16.0).view(1, 1, 16, 1).expand(1, 1, 16, 16).clone(), v_pages=torch.zeros(1, 1, 16, 16),
+             page_table=torch.zeros(1, 1, dtype=torch.int32), lengths=torch.tensor([6]), seen=torch.tensor([6]),
+             weight=torch.tensor([0.0, 1.0, 3.0, 1.0, 0.0, 0.0] + [9.0] * 10).view(1, 1, 16),
+             position=torch.arange(16).view(1, 1, 16))
+    st.evict(c, 4, recent=2, sink=1)
+    assert c["lengths"].tolist() == [4]
+    assert c["position"][0, 0, :6].tolist() == [0, 4, 2, 5, 4, 5]
+    assert c["k_pages"][0, 0, :4, 0].tolist() == [0, 4, 2, 5] and c["weight"][0, 0, :4].tolist() == [0, 0, 3, 0]
+
+
+def test_oracle_attention_matches_loops():
+    g = torch.Generator().manual_seed(0)
+    c = dict(k_pages=torch.randn(3, 1, 16, 16, generator=g), v_pages=torch.randn(3, 1, 16, 16, generator=g),
+             page_table=torch.tensor([[2, 0]], dtype=torch.int32), lengths=torch.tensor([20]), seen=torch.tensor([20]),
+             weight=torch.zeros(3, 1, 16), position=torch.zeros(3, 1, 16, dtype=torch.int32))
+    q = torch.randn(1, 2, 2, 16, generator=g)
+    o, lse, _ = st.attend(c, q, causal=True, accumulate=True)
+    for i in range(2):
+        for h in range(2):
+            rows = [(2, s) for s in range(16)] + [(0, s) for s in range(3 + i)]
+            s = [sum(float(q[0, i, h, d]) * float(c["k_pages"][p, 0, j, d]) for d in range(16)) / 4 for p, j in rows]
+            z = sum(math.exp(v) for v in s)
+            assert abs(math.log(z) - float(lse[0, h, i])) < 1e-5
+            for d in (0, 7):
+                want = sum(math.exp(v) / z * float(c["v_pages"][p, 0, j, d]) for v, (p, j) in zip(s, rows))
+                assert abs(want - float(o[0, i, h, d])) < 1e-5
+    assert abs(float(c["weight"].sum()) - 4) < 1e-9  # four rows' weights
+
+
+def _c_cache(nat, **over):
+    a = dict(num_pages=8, kv_heads=2, page_size=16, head_dim=64, batch=2, pages_per_seq=4, k_pages=4096, v_pages=4096,
+             ks=(2048, 1024, 64), vs=(2048, 1024, 64), page_table=4096, table_stride=4, lengths=4096, seen=4096, weight=4096,
+             position=4096)
+    a.update(over)
+    return nat.KvCache(a["num_pages"], a["kv_heads"], a["page_size"], a["head_dim"], a["batch"], a["pages_per_seq"], a["k_pages"],
+                       a["v_pages"], (ctypes.c_int64 * 3)(*a["ks"]), (ctypes.c_int64 * 3)(*a["vs"]), a["page_table"],
+                       a["table_stride"], a["lengths"], a["seen"], a["weight"], a["position"])
+
+
+BAD_CACHES = [
+    (dict(head_dim=96), 2, "head dim"),
+    (dict(page_size=24), 2, "multiple of 16"),
+    (dict(page_size=0), 2, "multiple of 16"),
+    (dict(num_pages=0), 1, "sizes"),
+    (dict(batch=-1), 1, "sizes"),
+    (dict(batch=70000), 2, "too large"),
+    (dict(pages_per_seq=1 << 26), 2, "too large"),
+    (dict(k_pages=0), 1, "null"),
+    (dict(v_pages=4100), 1, "aligned"),
+    (dict(ks=(2048, 1024, 60)), 1, "multiples of 8"),
+    (dict(vs=(2048, 0, 64)), 1, "multiples of 8"),
+    (dict(ks=(2048, 1024, 1 << 26)), 2, "slot"),
+    (dict(lengths=0), 1, "lengths"),
+    (dict(page_table=0), 1, "page_table"),
+    (dict(table_stride=3), 1, "overlap"),
+    (dict(weight=0), 1, "both"),
+]
+
+
+@pytest.mark.parametrize("over,code,needle", BAD_CACHES)
+def test_c_entries_reject_bad_caches(over, code, needle):
+    from dmad_amd import _native as nat
+
+    lib, p = nat.lib(), ctypes.c_void_p
+    c = ctypes.byref(_c_cache(nat, **over))
+    n = ctypes.c_size_t(0)
+    s = (ctypes.c_int64 * 4)(256, 128, 64, 1)
+    calls = [
+        lambda: lib.dmad_paged_attn_workspace_bytes(c, 1, 4, 1, ctypes.byref(n)),
+        lambda: lib.dmad_paged_attn(0, c, 1, 4, p(256), s, 0, 0, 0.125, p(256), p(256), p(256), 1 << 40, p(0)),
+        lambda: lib.dmad_kv_evict_workspace_bytes(c, 8, ctypes.byref(n)),
+        lambda: lib.dmad_kv_evict(0, c, 8, 0, 0, p(256), 1 << 40, p(0)),
+        lambda: lib.dmad_qk_norm_rope_append(0, 0, 1, 4, p(256), p(256), p(256), s, s, s, p(0), p(0), p(0), 0, 0.0, p(256), c, p(0)),
+    ]
+    for call in calls:
+        assert call() == code
+        assert needle in lib.dmad_last_error().decode()
+
+
+def test_c_entries_reject_bad_arguments():
+    from dmad_amd import _native as nat
+
+    lib, p = nat.lib(), ctypes.c_void_p
+    c, bare = ctypes.byref(_c_cache(nat)), ctypes.byref(_c_cache(nat, weight=0, position=0))
+    s = (ctypes.c_int64 * 4)(256, 128, 64, 1)
+
+    def attn(cache=c, dtype=0, S=1, Hq=4, q=256, acc=0, scale=0.125, o=256, ws=256, size=1 << 40, strides=s):
+        return lib.dmad_paged_attn(dtype, cache, S, Hq, p(q), strides, 0, acc, scale, p(o), p(256), p(ws), size, p(0))
+
+    assert attn(cache=None) == 1
+    assert attn(dtype=2) == 2 and attn(dtype=5) == 2
+    assert attn(Hq=3) == 1 and attn(Hq=0) == 1 and attn(S=-1) == 1
+    assert attn(q=0) == 1 and attn(q=264) == 1 and attn(o=0) == 1 and attn(o=8) == 1
+    assert attn(scale=0.0) == 2 and attn(scale=-1.0) == 2 and attn(scale=math.nan) == 2
+    assert attn(cache=bare, acc=1) == 1
+    assert attn(acc=1, ws=0) == 3 and attn(acc=1, size=64) == 3 and attn(acc=1, ws=272) == 3
+    assert attn(S=1 << 28, Hq=64) == 2
+    assert attn(S=0) == 0
+
+    def evict(cache=c, keep=8, recent=0, sink=0, ws=256, size=1 << 40):
+        return lib.dmad_kv_evict(0, cache, keep, recent, sink, p(ws), size, p(0))
+
+    assert evict(cache=bare) == 1 and evict(keep=0) == 1 and evict(recent=-1) == 1 and evict(sink=-1) == 1
+    assert evict(recent=9) == 1 and evict(recent=5, sink=4) == 1 and evict(recent=1 << 62, sink=1 << 62) == 1
+    assert evict(ws=0) == 3 and evict(size=8) == 3
+    assert evict(keep=64) == 0  # nothing can be longer
+
+    def app(cache=c, S=1, Hq=4, q=256, k=256, oq=256, f=0, rows=0, eps=0.0, wd=0):
+        return lib.dmad_qk_norm_rope_append(0, wd, S, Hq, p(q), p(k), p(256), s, s, s, p(0), p(0), p(f), rows, eps, p(oq), cache, p(0))
+
+    assert app(q=0) == 1 and app(k=0) == 1 and app(oq=0) == 1 and app(Hq=0) == 1 and app(f=256, rows=0) == 1
+    assert app(eps=-1.0) == 1 and app(wd=1) == 2 and app(S=0) == 0
+
+
+def test_calls_off_the_gpu_raise():
+    from dmad_amd import PagedKVCache
+
+    with pytest.raises(RuntimeError, match="GPU only"):
+        PagedKVCache.allocate(1, 16, 1, 16, device="cpu")
+
+
+# ---------------------------------------------------------------- on the GPU
+
+
+def _make(dev, B, Hk, D, dtype, page, lengths, room=0, extra=2, nhd=False, seed=0, weights=True, seen_ahead=0):
+    """A cache of mixed pages holding `lengths` slots; everything else in the pool is NaN."""
+    from dmad_amd import PagedKVCache
+
+    g = torch.Generator().manual_seed(seed)
+    M = max(1, -(-(max(lengths) + room) // page))
+    N = B * M + extra
+    table = torch.randperm(N, generator=g)[:B * M].view(B, M).to(torch.int32)
+    shape = (N, page, Hk, D) if nhd else (N, Hk, page, D)
+    c = dict(k_pages=torch.full(shape, math.nan, dtype=dtype), v_pages=torch.full(shape, math.nan, dtype=dtype),
+             weight=torch.full((N, Hk, page), math.nan), position=torch.full((N, Hk, page), -1, dtype=torch.int32))
+    if nhd:
+        c["k_pages"], c["v_pages"] = c["k_pages"].transpose(1, 2), c["v_pages"].transpose(1, 2)
+    for b, n in enumerate(lengths):
+        k, v = (torch.randn(n, Hk, D, generator=g) * sd for sd in (1.5, 1.0))
+        w = torch.rand(n, Hk, generator=g) ** 4
+        w[torch.rand(n, Hk, generator=g) < 0.2] = 0.0
+        for j in range(-(-n // page)):
+            m = min(page, n - j * page)
+            rows = slice(j * page, j * page + m)
+            at = int(table[b, j])
+            c["k_pages"][at, :, :m] = k[rows].transpose(0, 1).to(dtype)
+            c["v_pages"][at, :, :m] = v[rows].transpose(0, 1).to(dtype)
+            c["weight"][at, :, :m] = w[rows].t()
+            c["position"][at, :, :m] = torch.arange(rows.start, rows.stop, dtype=torch.int32)
+    lens = torch.tensor(lengths, dtype=torch.int32)
+
+    def up(t):
+        return torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=dev).copy_(t)
+
+    return PagedKVCache(up(c["k_pages"]), up(c["v_pages"]), table.to(dev), lens.to(dev), (lens + seen_ahead).to(dev),
+                        up(c["weight"]) if weights else None, up(c["position"]) if weights else None)
+
+
+def _same(name, a, b):
+    """Equal, NaN to NaN."""
+    a, b = a.cpu().float(), b.cpu().float()
+    assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(0.0), b.nan_to_num(0.0)), name
+
+
+def _check_attention(got, ref, dtype, D, accumulated=None, before=None):
+    o, lse = got
+    ro, rlse, (pv, sv, size) = ref
+    u = torch.finfo(dtype).eps / 2
+    es = (D + 8) * F32 * size + 64 * F32 * (1 + rlse.transpose(1, 2)[..., None].abs().nan_to_num(0, posinf=0))
+    tol = (u * (1 + 1e-3) + 2 * es) * pv + u * (1 + 1e-3) * ro.abs() + 1e-30
+    if dtype == torch.float16:
+        tol = tol + 2.0 ** -25 * (sv + 1)
+    err = (o.cpu().double() - ro).abs()
+    assert torch.isfinite(o).all()
+    print(f"  o: {float((err / tol).max()):.2f} of its bound", flush=True)
+    assert (err <= tol).all()
+    none = torch.isinf(rlse)
+    assert torch.equal(lse.cpu() == -math.inf, none)
+    err = (lse.cpu().double() - rlse).abs()[~none]
+    assert (err <= es.amax(-1).transpose(1, 2)[~none]).all()
+
+
+ATTEND = [
+    # B, S, Hq, Hk, D, dtype, page, lengths, causal, accumulate
+    (1, 1, 1, 1, 128, "bf16", 16, [1], False, True),
+    (2, 1, 2, 2, 64, "fp16", 16, [0, 16], False, True),
+    (3, 1, 4, 1, 128, "bf16", 16, [17, 31, 33], False, True),
+    (1, 1, 12, 12, 64, "fp16", 16, [257], False, False),
+    (2, 1, 8, 2, 16, "bf16", 32, [127, 129], False, True),
+    (2, 2, 6, 3, 32, "fp16", 48, [500, 95], True, True),
+    (1, 4, 64, 8, 128, "bf16", 64, [1000], True, True),
+    (2, 7, 24, 8, 128, "fp16", 16, [300, 3], True, True),
+    (1, 1, 5, 5, 256, "bf16", 16, [700], False, True),
+    (2, 5, 10, 2, 256, "fp16", 64, [130, 4], True, False),
+    (1, 40, 2, 1, 64, "bf16", 128, [390], True, True),
+    (1, 33, 3, 3, 128, "bf16", 16, [33], True, False),
+    (70, 1, 2, 1, 64, "bf16", 16, [(7 * i) % 61 for i in range(70)], False, True),
+    (1, 1, 2, 2, 128, "bf16", 16, [9001], False, True),
+    (3, 3, 16, 1, 32, "bf16", 16, [2, 1500, 640], True, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,Hq,Hk,D,dtype,page,lengths,causal,accumulate", ATTEND)
+def test_attention(gpu, B, S, Hq, Hk, D, dtype, page, lengths, causal, accumulate):
+    from dmad_amd import paged_attention
+
+    print(f"case attend B={B} S={S} Hq={Hq} Hk={Hk} D={D} {dtype} page={page} lengths={lengths[:4]} causal={causal}", flush=True)
+    t = DTYPES[dtype]
+    cache = _make(gpu, B, Hk, D, t, page, lengths, room=5, seed=D + S, nhd=page == 48)
+    q = (torch.randn(B, S, Hq, D, generator=torch.Generator().manual_seed(1)) * 1.5).to(t)
+    c = st.cache_of(cache)
+    ref = st.attend(c, q, causal=causal, accumulate=accumulate)
+    before = cache.weight.clone()
+    got = paged_attention(q.to(gpu), cache, causal=causal, accumulate=accumulate, return_lse=True)
+    torch.cuda.synchronize()
+    _check_attention(got, ref, t, D)
+    if accumulate:
+        w, r = cache.weight.cpu().double(), c["weight"].double()
+        _same("weights of unused slots", torch.isnan(w).float(), torch.isnan(r).float())
+        share = (r - before.cpu().double()).nan_to_num(0)
+        # each p is off by the factor of its score and lse, the sum by float32's steps
+        worst = float(ref[2][2].max()) * (D + 8) * F32 * 2 + 128 * F32 * (1 + float(ref[1][~torch.isinf(ref[1])].abs().max()) if (~torch.isinf(ref[1])).any() else 1)
+        assert ((w - r).abs().nan_to_num(0) <= worst * share + 2 * F32 * r.abs().nan_to_num(0) + 1e-30).all()
+    else:
+        _same("weights", cache.weight, before)
+    # the same again bit for bit, and without lse
+    again = paged_attention(q.to(gpu), cache, causal=causal)
+    assert torch.equal(again, got[0])
+
+
+@pytest.mark.gpu
+def test_attention_of_missing_pages_and_odd_lengths(gpu):
+    """Ids outside the pool hide their slots; lengths beyond the table or negative are clipped; a sequence
+    without a readable slot gives zeros and -inf."""
+    from dmad_amd import paged_attention
+
+    cache = _make(gpu, 6, 2, 64, torch.bfloat16, 16, [100, 100, 100, 100, 100, 100], seed=3)
+    N = cache.k_pages.shape[0]
+    cache.page_table[0, 0] = -1
+    cache.page_table[1, 3] = N
+    cache.page_table[1, 6] = 2 ** 31 - 1
+    cache.page_table[2, :] = -(2 ** 31)
+    cache.lengths[3] = -5
+    cache.lengths[4] = 0
+    cache.page_table[5, 1:5] = -1
+    q = torch.randn(6, 2, 4, 64, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    for causal in (False, True):
+        c = st.cache_of(cache)
+        ref = st.attend(c, q, causal=causal, accumulate=True)
+        w = cache.weight.clone()
+        got = paged_attention(q.to(gpu), cache, causal=causal, accumulate=True, return_lse=True)
+        torch.cuda.synchronize()
+        _check_attention(got, ref, torch.bfloat16, 64)
+        assert torch.equal(got[0][2:5], torch.zeros_like(got[0][2:5])) and torch.isneginf(got[1][2:5]).all()
+        assert torch.allclose(cache.weight.cpu().double(), c["weight"].double(), rtol=1e-4, atol=1e-6, equal_nan=True)
+        cache.weight.copy_(w)
+    # a length beyond the table: all its slots, the NaN ones beyond the data among them, reach that sequence alone
+    cache.lengths[4] = 10 ** 9
+    o = paged_attention(q.to(gpu), cache)
+    assert torch.isnan(o[4]).all() and torch.isfinite(o[:4]).all() and torch.isfinite(o[5]).all()
+
+
+@pytest.mark.gpu
+def test_attention_scores_of_any_size(gpu):
+    """Scores far apart and all very low keep their softmax; an infinite or NaN key or value reaches its own
+    sequence and key head and no other."""
+    from dmad_amd import paged_attention
+
+    for dtype in (torch.bfloat16, torch.float16):
+        cache = _make(gpu, 2, 2, 64, dtype, 16, [300, 260], seed=4)
+        c = st.cache_of(cache)
+        q = torch.randn(2, 1, 4, 64, generator=torch.Generator().manual_seed(5)).to(dtype)
+        for scale in (1e-3, 1.0, 30.0):
+            ref = st.attend(c, q, scale=scale)
+            got = paged_attention(q.to(gpu), cache, sm_scale=scale, return_lse=True)
+            _check_attention(got, ref, dtype, 64)
+        low = torch.full((2, 1, 4, 64), -200.0).to(dtype)
+        page, slot = st.locate(c, 0, 290)
+        cache.k_pages[cache.page_table[0].long()] = 200.0
+        c = st.cache_of(cache)
+        _check_attention(paged_attention(low.to(gpu), cache, return_lse=True), st.attend(c, low), dtype, 64)
+        clean = paged_attention(q.to(gpu), cache)
+        for where, value in (("k_pages", math.nan), ("v_pages", math.inf), ("v_pages", math.nan)):
+            keep = getattr(cache, where)[page, 1, slot].clone()
+            getattr(cache, where)[page, 1, slot] = value
+            o = paged_attention(q.to(gpu), cache)
+            assert not torch.isfinite(o[0, 0, 2:]).any(), where
+            assert torch.equal(o[0, 0, :2], clean[0, 0, :2]) and torch.equal(o[1], clean[1])
+            getattr(cache, where)[page, 1, slot] = keep
+
+
+@pytest.mark.gpu
+def test_attention_equals_the_dense_one(gpu):
+    """Against the package's own dense attention over the same keys."""
+    from dmad_amd import paged_attention, plain_attention
+
+    cache = _make(gpu, 1, 8, 128, torch.bfloat16, 16, [4000], seed=6)
+    q = torch.randn(1, 16, 8, 128, generator=torch.Generator().manual_seed(7)).to(torch.bfloat16).to(gpu)
+    used = cache.page_table[0].long()
+    k, v = (p[used].transpose(0, 1).reshape(1, 8, -1, 128)[:, :, :4000].contiguous() for p in (cache.k_pages, cache.v_pages))
+    dense = plain_attention(q.transpose(1, 2), k, v).transpose(1, 2).float()
+    o = paged_attention(q, cache).float()
+    assert float((o - dense).norm() / dense.norm()) < 5e-3
+
+
+APPEND = [
+    # B, S, Hq, Hk, D, dtype, page, lengths, weights' type
+    (1, 1, 1, 1, 16, "bf16", 16, [0], "bf16"),
+    (3, 1, 8, 2, 128, "bf16", 16, [15, 16, 0], "fp32"),
+    (2, 5, 6, 3, 64, "fp16", 48, [46, 100], "fp16"),
+    (1, 130, 40, 40, 128, "bf16", 64, [61], "bf16"),
+    (2, 3, 9, 1, 32, "fp16", 16, [0, 31], "fp32"),
+    (2, 2, 4, 4, 256, "bf16", 32, [31, 64], "bf16"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,Hq,Hk,D,dtype,page,lengths,wtype", APPEND)
+def test_append(gpu, B, S, Hq, Hk, D, dtype, page, lengths, wtype):
+    from dmad_amd import qk_norm_rope_append
+    from test_qk_norm_rope import _check, _pair_size
+
+    print(f"case append B={B} S={S} Hq={Hq} Hk={Hk} D={D} {dtype} page={page} lengths={lengths}", flush=True)
+    t = DTYPES[dtype]
+    cache = _make(gpu, B, Hk, D, t, page, lengths, room=S, seed=D, nhd=page == 48, seen_ahead=3)
+    g = torch.Generator().manual_seed(8)
+    qkv = torch.randn(B, S, Hq + 2 * Hk, D, generator=g).to(t)
+    wq, wk = ((1 + 0.2 * torch.randn(D, generator=g)).to({"fp32": torch.float32, **DTYPES}[wtype]) for _ in range(2))
+    freqs = torch.rand(max(lengths) + 3 + S, D // 2, generator=g) * 300
+    c, before = st.cache_of(cache), st.cache_of(cache)
+    q, k, v = qkv.split((Hq, Hk, Hk), dim=2)
+    rq, rk = st.append(c, q, k, v, wq, wk, 1e-6, freqs)
+    dq, dk, dv = qkv.to(gpu).split((Hq, Hk, Hk), dim=2)
+    got = qk_norm_rope_append(dq, dk, dv, wq.to(gpu), wk.to(gpu), 1e-6, freqs.to(gpu), cache)
+    torch.cuda.synchronize()
+    _check("q", got, rq, _pair_size(rq))
+    after = st.cache_of(cache)
+    for b in range(B):
+        for i in range(S):
+            at = st.locate(c, b, lengths[b] + i)
+            _check(f"k {b} {i}", after["k_pages"][at[0], :, at[1]], rk[b, i], _pair_size(rk[b, i]))
+            before["k_pages"][at[0], :, at[1]] = after["k_pages"][at[0], :, at[1]]
+    _same("other slots", after["k_pages"], before["k_pages"])
+    for n in ("v_pages", "weight", "position", "lengths", "seen"):
+        _same(n, after[n], c[n])
+
+
+@pytest.mark.gpu
+def test_append_where_there_is_no_room(gpu):
+    """Tokens beyond the capacity or on missing pages are dropped, positions beyond the angles give NaN, and
+    keys appended as they are keep their bits."""
+    from dmad_amd import append_kv, qk_norm_rope_append
+
+    cache = _make(gpu, 4, 2, 32, torch.bfloat16, 16, [30, 10, 32, 5], seed=9)
+    cache.page_table[1, 0] = -1
+    cache.lengths[3] = -7
+    g = torch.Generator().manual_seed(10)
+    k, v = (torch.randn(4, 5, 2, 32, generator=g).to(torch.bfloat16) for _ in range(2))
+    k[0, 0, 0, 0] = math.inf
+    c = st.cache_of(cache)
+    st.append(c, None, k, v, None, None, 0.0, None)
+    append_kv(k.to(gpu), v.to(gpu), cache)
+    torch.cuda.synchronize()
+    for n in st.FIELDS:
+        _same(n, getattr(cache, n), c[n])
+    assert cache.lengths.tolist() == [32, 15, 32, 5] and cache.seen.tolist() == [35, 15, 37, 10]
+    # angles for positions 0..35 only
+    cache.lengths.zero_()
+    q = torch.randn(4, 2, 6, 32, generator=g).to(torch.bfloat16).to(gpu)
+    w, f = torch.ones(32, device=gpu), torch.rand(36, 16, generator=g).to(gpu)
+    got = qk_norm_rope_append(q, q[:, :, :2], q[:, :, 2:4], w, w, 1e-6, f, cache)
+    bad = torch.tensor([[s + i >= 36 for i in range(2)] for s in (35, 15, 37, 10)])
+    assert torch.equal(torch.isnan(got.float()).all(-1).all(-1).cpu(), bad)
+    assert torch.equal(torch.isnan(got.float()).any(-1).any(-1).cpu(), bad)
+    # negative counts have no angles either
+    cache.seen.fill_(-2 ** 31)
+    assert torch.isnan(qk_norm_rope_append(q, q[:, :, :2], q[:, :, 2:4], w, w, 1e-6, f, cache).float()).all()
+
+
+EVICT = [
+    # B, Hk, D, dtype, page, lengths, keep, recent, sink
+    (1, 1, 16, "bf16", 16, [2], 1, 0, 0),
+    (2, 2, 64, "fp16", 16, [33, 32], 32, 4, 1),
+    (3, 1, 128, "bf16", 16, [0, 100, 64], 64, 16, 4),
+    (2, 3, 32, "bf16", 48, [500, 333], 100, 0, 0),
+    (1, 2, 256, "fp16", 64, [1100], 1000, 100, 0),
+    (2, 2, 64, "bf16", 16, [2500, 90], 77, 30, 47),
+    (1, 1, 64, "bf16", 16, [5000], 4999, 0, 3),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Hk,D,dtype,page,lengths,keep,recent,sink", EVICT)
+def test_evict(gpu, B, Hk, D, dtype, page, lengths, keep, recent, sink):
+    from dmad_amd import evict_low_weight
+
+    print(f"case evict B={B} Hk={Hk} D={D} page={page} lengths={lengths} keep={keep} recent={recent} sink={sink}", flush=True)
+    cache = _make(gpu, B, Hk, D, DTYPES[dtype], page, lengths, room=7, seed=keep, nhd=page == 48)
+    for again in range(2):  # a second cut finds slots out of order
+        c = st.cache_of(cache)
+        k = keep if again == 0 else max(1, keep // 2)
+        r, s = (recent, sink) if again == 0 else (recent // 2, sink // 2)
+        st.evict(c, k, r, s)
+        evict_low_weight(cache, k, recent=r, sink=s)
+        torch.cuda.synchronize()
+        for n in st.FIELDS:
+            _same(n, getattr(cache, n), c[n])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["equal", "zeros of both signs", "infinities and NaN", "all recent", "negative", "missing pages"])
+def test_evict_order(gpu, kind):
+    from dmad_amd import evict_low_weight
+
+    print(f"case evict order {kind}", flush=True)
+    cache = _make(gpu, 2, 2, 64, torch.bfloat16, 16, [300, 211], seed=11)
+    g = torch.Generator().manual_seed(12)
+    w = torch.rand(cache.weight.shape, generator=g)
+    if kind == "equal":
+        w = torch.ones_like(w)
+    elif kind == "zeros of both signs":
+        w = torch.where(w < 0.5, torch.tensor(-0.0), torch.tensor(0.0))
+    elif kind == "infinities and NaN":
+        w = torch.where(w < 0.1, torch.tensor(math.nan), torch.where(w < 0.4, torch.tensor(math.inf), torch.where(w < 0.7, torch.tensor(-math.inf), w)))
+    elif kind == "negative":
+        w = w - 0.7
+    elif kind == "all recent":
+        cache.position.fill_(10 ** 6)
+    cache.weight.copy_(w)
+    if kind == "missing pages":
+        cache.page_table[0, 2] = -1
+        cache.page_table[0, 15] = cache.k_pages.shape[0]
+        cache.page_table[1, 12] = -9
+    c = st.cache_of(cache)
+    st.evict(c, 128, 16, 4)
+    evict_low_weight(cache, 128, recent=16, sink=4)
+    torch.cuda.synchronize()
+    for n in st.FIELDS:
+        _same(n, getattr(cache, n), c[n])
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(gpu):
+    """A pool of 5 GiB per side, a few pages at its end."""
+    from dmad_amd import PagedKVCache, evict_low_weight, paged_attention, qk_norm_rope_append
+
+    N, Hk, P, D = 5 * 2 ** 30 // (8 * 64 * 128 * 2), 8, 64, 128
+    k_pages = torch.empty((N, Hk, P, D), device=gpu, dtype=torch.bfloat16)
+    v_pages = torch.empty_like(k_pages)
+    table = torch.tensor([[N - 1, N - 3], [N - 2, 0]], device=gpu, dtype=torch.int32)
+    small = table.long().view(-1)
+    g = torch.Generator(device=gpu).manual_seed(0)
+    for pages in (k_pages, v_pages):
+        pages[small] = torch.randn((4, Hk, P, D), generator=g, device=gpu).to(torch.bfloat16)
+    lens = torch.tensor([100, 64], device=gpu, dtype=torch.int32)
+    weight = torch.rand((N, Hk, P), generator=g, device=gpu)
+    position = torch.arange(P, device=gpu, dtype=torch.int32).expand(N, Hk, P).contiguous()
+    big = PagedKVCache(k_pages, v_pages, table, lens, lens.clone(), weight, position)
+    ids = torch.arange(4, device=gpu, dtype=torch.int32).view(2, 2)
+    little = PagedKVCache(k_pages[small].clone(), v_pages[small].clone(), ids, lens.clone(), lens.clone(), weight[small].clone(),
+                          position[small].clone())
+    q = torch.randn((2, 1, 16, D), generator=g, device=gpu).to(torch.bfloat16)
+    kv = torch.randn((2, 1, Hk, D), generator=g, device=gpu).to(torch.bfloat16)
+    w, f = torch.ones(D, device=gpu), torch.rand((200, D // 2), generator=g, device=gpu)
+    outs = []
+    for cache in (big, little):
+        a = qk_norm_rope_append(q, kv, kv, w, w, 1e-6, f, cache)
+        o = paged_attention(a, cache, accumulate=True)
+        evict_low_weight(cache, 60, recent=3)
+        outs.append((a, o, paged_attention(a, cache)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    for n in ("k_pages", "v_pages", "weight", "position"):
+        assert torch.equal(getattr(big, n)[small], getattr(little, n)), n
+
+
+def _decode(cache, steps, wq, wk, freqs, keep):
+    from dmad_amd import evict_low_weight, paged_attention, qk_norm_rope_append
+
+    outs = []
+    for q, k, v in steps:
+        q = qk_norm_rope_append(q, k, v, wq, wk, 1e-6, freqs, cache)
+        outs.append(paged_attention(q, cache, causal=True, accumulate=True))
+        evict_low_weight(cache, keep, recent=8, sink=2)
+    return outs
+
+
+def _steps(dev, B, Hq, Hk, D, dtype, sizes, seed):
+    g = torch.Generator().manual_seed(seed)
+    return [[torch.randn(B, S, h, D, generator=g).to(dtype).to(dev) for h in (Hq, Hk, Hk)] for S in sizes]
+
+
+@pytest.mark.gpu
+def test_decoding_with_eviction(gpu):
+    """A prompt, then tokens one, three and one at a time against a cache that is cut to 40 slots after every
+    step, each call against the oracle on a copy of the cache it found. Slots and positions agree in every step."""
+    from dmad_amd import PagedKVCache
+
+    B, Hq, Hk, D, dtype = 2, 8, 2, 64, torch.bfloat16
+    cache = PagedKVCache.allocate(B, 80, Hk, D, dtype, gpu, page_size=16)
+    assert cache.capacity == 80
+    g = torch.Generator().manual_seed(20)
+    wq, wk = ((1 + 0.2 * torch.randn(D, generator=g)).to(dtype) for _ in range(2))
+    freqs = torch.rand(200, D // 2, generator=g) * 50
+    total = 0
+    for n, (q, k, v) in enumerate(_steps(gpu, B, Hq, Hk, D, dtype, [37, 1, 3, 1, 1, 8, 1], 21)):
+        from dmad_amd import evict_low_weight, paged_attention, qk_norm_rope_append
+
+        c = st.cache_of(cache)
+        st.append(c, q.cpu(), k.cpu(), v.cpu(), wq, wk, 1e-6, freqs)
+        qn = qk_norm_rope_append(q, k, v, wq.to(gpu), wk.to(gpu), 1e-6, freqs.to(gpu), cache)
+        total += q.shape[1]
+        assert cache.lengths.tolist() == c["lengths"].tolist() and cache.seen.tolist() == [total] * B
+        c = st.cache_of(cache)
+        ref = st.attend(c, qn.cpu(), causal=True, accumulate=True)
+        got = paged_attention(qn, cache, causal=True, accumulate=True, return_lse=True)
+        _check_attention(got, ref, dtype, D)
+        c = st.cache_of(cache)
+        st.evict(c, 40, 8, 2)
+        evict_low_weight(cache, 40, recent=8, sink=2)
+        for name in st.FIELDS:
+            _same(f"{name} after step {n}", getattr(cache, name)[:] if name != "lengths" else cache.lengths, c[name])
+        for h in range(Hk):  # positions of the slots in use are distinct, the last ones and the sinks among them
+            at = [int(cache.position[p, h, s]) for p, s in (st.locate(c, 0, j) for j in range(int(cache.lengths[0])))]
+            assert len(set(at)) == len(at) and {0, 1, *range(max(0, total - 8), total)} <= set(at)
+
+
+@pytest.mark.gpu
+def test_captured_steps_follow_the_cache(gpu):
+    """One captured step replayed token by token: lengths, pages and evictions are the device's, so every
+    replay is the eager step that stands there. Two graphs of the same calls do not disturb each other."""
+    from dmad_amd import PagedKVCache
+
+    B, Hq, Hk, D, dtype = 3, 8, 2, 128, torch.bfloat16
+    g = torch.Generator().manual_seed(30)
+    wq, wk = ((1 + 0.2 * torch.randn(D, generator=g)).to(gpu) for _ in range(2))
+    freqs = (torch.rand(600, D // 2, generator=g) * 50).to(gpu)
+    steps = _steps(gpu, B, Hq, Hk, D, dtype, [1] * 6, 31)
+
+    def fresh():
+        cache = PagedKVCache.allocate(B, 400, Hk, D, dtype, gpu, page_size=16)
+        _decode(cache, _steps(gpu, B, Hq, Hk, D, dtype, [300], 32), wq, wk, freqs, 301)
+        cache.lengths[1] = 7
+        return cache
+
+    eager = fresh()
+    want = [o.clone() for o in _decode(eager, steps, wq, wk, freqs, 300)]
+    torch.cuda.synchronize()
+    caches, graphs, ins, outs = [fresh() for _ in range(2)], [], [], []
+    for cache in caches:
+        saved = {n: getattr(cache, n).clone() for n in st.FIELDS}
+        x = [t.clone() for t in steps[0]]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _decode(cache, [x], wq, wk, freqs, 300)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_decode(cache, [x], wq, wk, freqs, 300)[0])
+        for n, t in saved.items():
+            getattr(cache, n).copy_(t)
+        graphs.append(graph)
+        ins.append(x)
+    for n, step in enumerate(steps):
+        for i in range(2):
+            for a, b in zip(ins[i], step):
+                a.copy_(b)
+            graphs[i].replay()
+        junk = torch.randn(1024, 1024, device=gpu)
+        (junk @ junk).sum().item()
+        for i in range(2):
+            assert torch.equal(outs[i], want[n]), (n, i)
+    for cache in caches:
+        for name in ("lengths", "seen"):
+            assert torch.equal(getattr(cache, name), getattr(eager, name))
+
+
+@pytest.mark.gpu
+def test_refusals(gpu):
+    from dmad_amd import PagedKVCache, append_kv, evict_low_weight, paged_attention, qk_norm_rope_append
+
+    ok = PagedKVCache.allocate(2, 40, 2, 64, torch.bfloat16, gpu, page_size=16)
+    assert ok.capacity == 48
+    f = [getattr(ok, n) for n in ("k_pages", "v_pages", "page_table", "lengths", "seen", "weight", "position")]
+
+    def built(**over):
+        names = ("k_pages", "v_pages", "page_table", "lengths", "seen", "weight", "position")
+        return PagedKVCache(**{**dict(zip(names, f)), **over})
+
+    built()
+    for error, over in [
+        (ValueError, dict(v_pages=f[1][:1])),
+        (ValueError, dict(k_pages=f[0][0])),
+        (NotImplementedError, dict(v_pages=f[1].half())),
+        (NotImplementedError, dict(k_pages=f[0].float(), v_pages=f[1].float())),
+        (NotImplementedError, dict(k_pages=f[0][:, :, :8], v_pages=f[1][:, :, :8])),
+        (NotImplementedError, dict(k_pages=f[0][..., :48], v_pages=f[1][..., :48])),
+        (ValueError, dict(k_pages=f[0].transpose(2, 3).contiguous().transpose(2, 3))),
+        (ValueError, dict(k_pages=f[0][:1].expand_as(f[0]))),
+        (ValueError, dict(page_table=f[2].long())),
+        (ValueError, dict(page_table=f[2].t())),
+        (ValueError, dict(lengths=f[3][:1])),
+        (ValueError, dict(seen=f[4].long())),
+        (ValueError, dict(weight=None)),
+        (ValueError, dict(weight=f[5].double())),
+        (ValueError, dict(position=f[6][:, :1])),
+        (RuntimeError, dict(lengths=f[3].cpu())),
+    ]:
+        with pytest.raises(error):
+            built(**over)
+    with pytest.raises(AttributeError, match="in place"):
+        ok.lengths = f[3]
+    with pytest.raises(NotImplementedError, match="multiple of 16"):
+        PagedKVCache.allocate(1, 10, 1, 64, device=gpu, page_size=20)
+    with pytest.raises(ValueError):
+        PagedKVCache.allocate(0, 10, 1, 64, device=gpu)
+
+    q, k = torch.zeros(2, 1, 4, 64, device=gpu, dtype=torch.bfloat16), torch.zeros(2, 1, 2, 64, device=gpu, dtype=torch.bfloat16)
+    w = torch.ones(64, device=gpu)
+    bare = built(weight=None, position=None)
+    for error, call in [
+        (TypeError, lambda: paged_attention(q, f[0])),
+        (ValueError, lambda: paged_attention(q[:1], ok)),
+        (ValueError, lambda: paged_attention(q[0], ok)),
+        (ValueError, lambda: paged_attention(q[..., :32], ok)),
+        (ValueError, lambda: paged_attention(q[:, :, :3], ok)),
+        (ValueError, lambda: paged_attention(q.half(), ok)),
+        (RuntimeError, lambda: paged_attention(q.cpu(), ok)),
+        (NotImplementedError, lambda: paged_attention(q, ok, sm_scale=0.0)),
+        (NotImplementedError, lambda: paged_attention(q, ok, sm_scale=math.nan)),
+        (ValueError, lambda: paged_attention(q, bare, accumulate=True)),
+        (RuntimeError, lambda: paged_attention(q.clone().requires_grad_(True), ok)),
+        (ValueError, lambda: append_kv(k, None, ok)),
+        (ValueError, lambda: append_kv(k, q, ok)),
+        (ValueError, lambda: append_kv(k, k.half(), ok)),
+        (ValueError, lambda: append_kv(k, torch.cat((k, k), 1), ok)),
+        (TypeError, lambda: append_kv(k, k, None)),
+        (ValueError, lambda: qk_norm_rope_append(q, k, k, w, w, -1.0, None, ok)),
+        (ValueError, lambda: qk_norm_rope_append(q, k, k, w[:32], w, 1e-6, None, ok)),
+        (ValueError, lambda: qk_norm_rope_append(None, k, k, w, w, 1e-6, None, ok)),
+        (ValueError, lambda: qk_norm_rope_append(q, k, k, w, w, 1e-6, torch.zeros(5, 64, device=gpu), ok)),
+        (RuntimeError, lambda: qk_norm_rope_append(q, k, k, w.clone().requires_grad_(True), w, 1e-6, None, ok)),
+        (ValueError, lambda: evict_low_weight(bare, 8)),
+        (TypeError, lambda: evict_low_weight(None, 8)),
+        (ValueError, lambda: evict_low_weight(ok, 0)),
+        (ValueError, lambda: evict_low_weight(ok, 8, recent=-1)),
+        (ValueError, lambda: evict_low_weight(ok, 8, recent=5, sink=4)),
+    ]:
+        with pytest.raises(error):
+            call()
+    assert ok.lengths.tolist() == [0, 0]
+    # without weights everything else works
+    append_kv(k, k, bare)
+    assert torch.equal(paged_attention(q, bare), torch.zeros_like(q)) and bare.lengths.tolist() == [1, 1]
+    # no new tokens, no sequences
+    assert paged_attention(q[:, :0], bare).shape == (2, 0, 4, 64)
+    append_kv(k[:, :0], k[:, :0], bare)
+    assert bare.lengths.tolist() == [1, 1]
+    none = PagedKVCache(f[0], f[1], f[2][:0], f[3][:0], f[4][:0])
+    assert paged_attention(q[:0], none).shape == (0, 1, 4, 64)
+    append_kv(k[:0], k[:0], none)

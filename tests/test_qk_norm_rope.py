@@ -1,0 +1,463 @@
+"""RMSNorm of queries and keys per head with the rotation in the same pass (qk_norm_rope_with_tangent).
+
+CPU: the oracle (oracle/streaming.py) against differences and element-wise loops. GPU: the kernels
+against the oracle on the same inputs. The kernels compute in float32 and round once, so an element is
+off by half a step of its type, u = finfo.eps / 2, plus float32 errors of the terms it is made of: the
+mean of D squares (8 sequential and at most 5 pairwise additions), one reciprocal root, sine and cosine
+and four products come to less than 64 half steps of float32 of the larger element of its pair.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import streaming as st
+
+F32 = 2.0 ** -24
+FP32_STEPS = 64
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _pair_size(x):
+    """The larger magnitude of each pair, for both of its elements."""
+    a = x.abs().reshape(*x.shape[:-1], -1, 2).amax(-1, keepdim=True)
+    return a.expand(*a.shape[:-1], 2).reshape(x.shape)
+
+
+def _check(name, got, ref, scale):
+    """|got - ref| <= u |ref| + steps of float32 of `scale` (+ half the smallest subnormal)."""
+    tiny = torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
+    tol = _half_step(got.dtype) * ref.abs() * (1 + 1e-3) + FP32_STEPS * F32 * scale + tiny
+    err = (got.detach().cpu().double() - ref).abs()
+    assert torch.isfinite(got.detach().cpu().double()).all(), name
+    worst = float((err / tol).max()) if err.numel() else 0.0
+    print(f"  {name}: worst error {worst:.2f} of its bound", flush=True)
+    assert worst <= 1.0, name
+
+
+# ---------------------------------------------------------------- the oracle
+
+
+def test_oracle_matches_loops():
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(2, 3, 2, 8, generator=g, dtype=torch.float64)
+    w = torch.rand(8, generator=g, dtype=torch.float64)
+    f = torch.rand(3, 4, generator=g, dtype=torch.float64) * 6
+    y = st.norm_rope(x, w, 1e-3, f)
+    for b in range(2):
+        for s in range(3):
+            for h in range(2):
+                row = x[b, s, h].tolist()
+                r = 1 / math.sqrt(sum(v * v for v in row) / 8 + 1e-3)
+                z = [v * r * float(w[i]) for i, v in enumerate(row)]
+                for i in range(4):
+                    c, n = math.cos(float(f[s, i])), math.sin(float(f[s, i]))
+                    assert abs(z[2 * i] * c - z[2 * i + 1] * n - float(y[b, s, h, 2 * i])) < 1e-12
+                    assert abs(z[2 * i + 1] * c + z[2 * i] * n - float(y[b, s, h, 2 * i + 1])) < 1e-12
+
+
+def test_oracle_tangent_is_the_difference_quotient():
+    g = torch.Generator().manual_seed(1)
+    x, t = (torch.randn(1, 2, 3, 16, generator=g, dtype=torch.float64) for _ in range(2))
+    w, f = torch.rand(16, generator=g, dtype=torch.float64), torch.rand(2, 8, generator=g, dtype=torch.float64)
+    d = (st.norm_rope(x + 1e-6 * t, w, 1e-6, f) - st.norm_rope(x - 1e-6 * t, w, 1e-6, f)) / 2e-6
+    assert torch.allclose(st.norm_rope_tangent(x, t, w, 1e-6, f), d, rtol=1e-6, atol=1e-8)
+
+
+# ---------------------------------------------------------------- inputs
+
+
+def _inputs(B, S, Hq, Hk, D, dtype, wdtype, seed, layout):
+    g = torch.Generator().manual_seed(seed)
+
+    def r(*shape, sd=1.0):
+        return (torch.randn(shape, generator=g) * sd).to(dtype)
+
+    if layout == "fused":  # slices of one projection's output
+        qkv = r(B, S, Hq + 2 * Hk, D)
+        q, k = qkv[:, :, :Hq], qkv[:, :, Hq:Hq + Hk]
+    elif layout == "bhsd":
+        q, k = r(B, Hq, S, D).transpose(1, 2), r(B, Hk, S, D).transpose(1, 2)
+    else:
+        q, k = r(B, S, Hq, D), r(B, S, Hk, D)
+    x = dict(q=q, k=k, tq=r(B, S, Hq, D, sd=0.1), tk=r(B, Hk, S, D, sd=0.1).transpose(1, 2), gq=r(B, S, Hq, D),
+             gk=r(B, S, Hk, D))
+    for n in ("wq", "wk"):
+        x[n] = (1 + 0.3 * torch.randn(D, generator=g)).to(wdtype)
+    x["freqs"] = torch.rand(S, D // 2, generator=g) * 200 - 100
+    x["freqs3"] = torch.rand(B, S, D // 2, generator=g) * 200 - 100
+    return x
+
+
+def _to(x, dev):
+    """The same tensor on the device, with its strides."""
+    base = torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=dev) if x.is_contiguous() or 0 not in x.stride() else x.to(dev)
+    base.copy_(x)
+    return base
+
+
+def _reference(x, wq, wk, eps, freqs, jvp):
+    out = {}
+    for n, w in (("q", wq), ("k", wk)):
+        z = x[n].double().requires_grad_(True)
+        wz = None if w is None else w.double().requires_grad_(True)
+        y = st.norm_rope(z, wz, eps, freqs)
+        y.backward(x["g" + n].double())
+        out[n], out["d" + n] = y.detach(), z.grad
+        if w is not None:
+            out["dw" + n] = wz.grad
+            u = st.rotate(x["g" + n].double(), None if freqs is None else -freqs.double())
+            m = z.detach() / (z.detach().pow(2).mean(-1, keepdim=True) + eps).sqrt()
+            out["sum" + n] = (u * m).abs().sum((0, 1, 2))  # what the weight's gradient is the sum of
+            a, r = u * w.double(), (z.detach().pow(2).mean(-1, keepdim=True) + eps).rsqrt()
+            out["size" + n] = r * (_pair_size(a) + m.abs() * (a * m).abs().mean(-1, keepdim=True))
+        else:
+            out["size" + n] = _pair_size(out["d" + n])
+        if jvp:
+            out["t" + n] = st.norm_rope_tangent(x[n], x["t" + n], w, eps, freqs)
+            z, t = x[n].double(), x["t" + n].double()
+            if w is not None:
+                r = (z.pow(2).mean(-1, keepdim=True) + eps).rsqrt()
+                parts = (t.abs() + (z * r).abs() * (z * r * t).abs().mean(-1, keepdim=True)) * r * w.double().abs()
+            else:
+                parts = t
+            out["tsize" + n] = _pair_size(parts)
+    return out
+
+
+CASES = [
+    # B, S, Hq, Hk, D, dtype, weights' dtype, layout, weights, rotation
+    (1, 1, 1, 1, 16, "bf16", "bf16", "plain", True, "shared"),
+    (2, 37, 3, 1, 16, "fp16", "fp32", "fused", True, "batch"),
+    (1, 65, 40, 8, 32, "bf16", "fp32", "bhsd", True, "shared"),
+    (3, 21, 5, 5, 64, "fp16", "fp16", "fused", True, "shared"),
+    (1, 256, 2, 2, 64, "fp32", "fp32", "plain", True, "shared"),
+    (2, 130, 12, 12, 128, "bf16", "bf16", "plain", True, "shared"),
+    (1, 77, 9, 3, 128, "fp32", "fp32", "fused", True, "batch"),
+    (1, 999, 40, 40, 128, "bf16", "bf16", "fused", True, "shared"),
+    (2, 33, 7, 1, 256, "bf16", "fp32", "bhsd", True, "batch"),
+    (1, 50, 4, 2, 256, "fp32", "fp32", "plain", True, "shared"),
+    (2, 40, 6, 2, 128, "bf16", "bf16", "plain", False, "shared"),
+    (2, 40, 6, 2, 64, "fp16", "fp16", "plain", True, None),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,S,Hq,Hk,D,dtype,wdtype,layout,norm,rope", CASES)
+def test_forward_tangent_backward(gpu, B, S, Hq, Hk, D, dtype, wdtype, layout, norm, rope):
+    from dmad_amd import qk_norm_rope_with_tangent
+
+    print(f"case norm B={B} S={S} Hq={Hq} Hk={Hk} D={D} {dtype} weights {wdtype if norm else None} {layout} rope={rope}", flush=True)
+    x = _inputs(B, S, Hq, Hk, D, DTYPES[dtype], DTYPES[wdtype], seed=D + S, layout=layout)
+    wq, wk = (x["wq"], x["wk"]) if norm else (None, None)
+    freqs = {"shared": x["freqs"], "batch": x["freqs3"], None: None}[rope]
+    ref = _reference(x, wq, wk, 1e-6, freqs, True)
+    d = {n: _to(v, gpu) for n, v in x.items()}
+    leaves = [d["q"].requires_grad_(True), d["k"].requires_grad_(True)]
+    if norm:
+        leaves += [d["wq"].requires_grad_(True), d["wk"].requires_grad_(True)]
+    f = None if freqs is None else freqs.to(gpu)
+    args = ((d["wq"], d["wk"]) if norm else (None, None)) + (1e-6, f)
+    (q, tq), (k, tk) = qk_norm_rope_with_tangent((d["q"], d["tq"]), (d["k"], d["tk"]), *args)
+    assert q.requires_grad and k.requires_grad and not tq.requires_grad and not tk.requires_grad
+    assert q.is_contiguous() and q.shape == (B, S, Hq, D) and k.shape == (B, S, Hk, D)
+    grads = torch.autograd.grad((q, k), leaves, (d["gq"], d["gk"]))
+    torch.cuda.synchronize()
+    for n, y, ty in (("q", q, tq), ("k", k, tk)):
+        _check(n, y, ref[n], _pair_size(ref[n]))
+        _check("t" + n, ty, ref["t" + n], ref["tsize" + n])
+    for n, got in zip(("q", "k"), grads):
+        _check("d" + n, got, ref["d" + n], ref["size" + n])
+    if norm:
+        for n, got in zip(("q", "k"), grads[2:]):
+            assert got.dtype == DTYPES[wdtype]
+            _check("dw" + n, got, ref["dw" + n], ref["sum" + n])
+    # the primal alone is the same
+    with torch.no_grad():
+        (q2, t2), (k2, _) = qk_norm_rope_with_tangent((d["q"], None), (d["k"], None), *args)
+    assert t2 is None and torch.equal(q2, q) and torch.equal(k2, k)
+
+
+@pytest.mark.gpu
+def test_gradient_is_the_difference_quotient(gpu):
+    """fp32 gradients against central differences of the kernel's own outputs. With step h = 2^-6 the
+    quotient of sum(y g) is off by h^2 / 6 times a third derivative of order 10 and by the outputs' float32
+    errors, 64 half steps of sum |y g| over h: together under 1e-3 of the gradient's size here."""
+    from dmad_amd import qk_norm_rope_with_tangent
+
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(1, 3, 2, 16, generator=g).to(gpu).requires_grad_(True)
+    w = (1 + 0.2 * torch.randn(16, generator=g)).to(gpu).requires_grad_(True)
+    f, go, dx, dw = torch.rand(3, 8, generator=g).to(gpu), *(torch.randn(s, generator=g).to(gpu) for s in ((1, 3, 2, 16), (1, 3, 2, 16), (16,)))
+
+    def loss(a, b):
+        return (qk_norm_rope_with_tangent((a, None), (None, None), b, None, 1e-6, f)[0][0].double() * go.double()).sum()
+
+    gx, gw = torch.autograd.grad(loss(x, w), (x, w))
+    h = 2.0 ** -6
+    with torch.no_grad():
+        num_x = (loss(x + h * dx, w) - loss(x - h * dx, w)) / (2 * h)
+        num_w = (loss(x, w + h * dw) - loss(x, w - h * dw)) / (2 * h)
+    size_x, size_w = float((gx * dx).abs().sum()), float((gw * dw).abs().sum())
+    assert abs(float((gx.double() * dx).sum() - num_x)) <= 1e-3 * size_x
+    assert abs(float((gw.double() * dw).sum() - num_w)) <= 1e-3 * size_w
+
+
+@pytest.mark.gpu
+def test_one_operand_and_partial_gradients(gpu):
+    from dmad_amd import qk_norm_rope_with_tangent
+
+    x = _inputs(2, 19, 4, 2, 64, torch.bfloat16, torch.bfloat16, 7, "plain")
+    d = {n: v.to(gpu) for n, v in x.items()}
+    both = qk_norm_rope_with_tangent((d["q"], d["tq"]), (d["k"], d["tk"]), d["wq"], d["wk"], 1e-6, d["freqs"])
+    (q, tq), none = qk_norm_rope_with_tangent((d["q"], d["tq"]), (None, None), d["wq"], None, 1e-6, d["freqs"])
+    assert none == (None, None) and torch.equal(q, both[0][0]) and torch.equal(tq, both[0][1])
+    none, (k, _) = qk_norm_rope_with_tangent((None, None), (d["k"], None), None, d["wk"], 1e-6, d["freqs"])
+    assert none == (None, None) and torch.equal(k, both[1][0])
+    # a loss of k alone leaves q and its weight without a gradient
+    for n in ("q", "k", "wq", "wk"):
+        d[n].requires_grad_(True)
+    (_, _), (k, _) = qk_norm_rope_with_tangent((d["q"], None), (d["k"], None), d["wq"], d["wk"], 1e-6, d["freqs"])
+    k.float().square().sum().backward()
+    assert d["q"].grad is None and d["wq"].grad is None and d["k"].grad is not None and d["wk"].grad is not None
+    # a summed output's gradient is an expanded scalar; a frozen weight gets none
+    d["wk"].requires_grad_(False)
+    (q, _), (k, _) = qk_norm_rope_with_tangent((d["q"], None), (d["k"], None), d["wq"], d["wk"], 1e-6, d["freqs"])
+    gq, gw = torch.autograd.grad(q.sum() + k.sum(), (d["q"], d["wq"]))
+    ones = torch.ones_like(q)
+    (q, _), (k, _) = qk_norm_rope_with_tangent((d["q"], None), (d["k"], None), d["wq"], d["wk"], 1e-6, d["freqs"])
+    hq, hw = torch.autograd.grad((q,), (d["q"], d["wq"]), (ones,))
+    assert torch.equal(gq, hq) and torch.equal(gw, hw)
+
+
+@pytest.mark.gpu
+def test_broadcast_and_unaligned_inputs(gpu):
+    """An expanded operand is read in place and its gradient summed; rows that start unaligned are copied."""
+    from dmad_amd import qk_norm_rope_with_tangent
+
+    g = torch.Generator().manual_seed(9)
+    one = torch.randn(1, 11, 1, 128, generator=g).to(torch.bfloat16).to(gpu).requires_grad_(True)
+    w, f = torch.ones(128, device=gpu, dtype=torch.bfloat16), torch.rand(11, 64, generator=g).to(gpu)
+    (q, _), _ = qk_norm_rope_with_tangent((one.expand(2, 11, 3, 128), None), (None, None), w, None, 1e-6, f)
+    (r, _), _ = qk_norm_rope_with_tangent((one, None), (None, None), w, None, 1e-6, f)
+    assert torch.equal(q, r.expand_as(q))
+    q.float().sum().backward()
+    assert one.grad.shape == one.shape
+    flat = torch.randn(1 * 5 * 2 * 64 + 1, generator=g).to(torch.bfloat16).to(gpu)
+    odd = flat[1:].view(1, 5, 2, 64)
+    w, f = torch.ones(64, device=gpu, dtype=torch.bfloat16), torch.rand(5, 32, generator=g).to(gpu)
+    a = qk_norm_rope_with_tangent((odd, None), (None, None), w, None, 1e-6, f)[0][0]
+    b = qk_norm_rope_with_tangent((odd.clone(), None), (None, None), w, None, 1e-6, f)[0][0]
+    assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_extremes(gpu):
+    """Zero rows, with eps = 0 too (0/0 is NaN in that row alone), large and small values, an empty batch."""
+    from dmad_amd import qk_norm_rope_with_tangent
+
+    w, f = torch.ones(32, device=gpu), torch.rand(4, 16, device=gpu)
+    x = torch.zeros(1, 4, 3, 32, device=gpu)
+    x[0, 1] = 1e18
+    x[0, 2] = 1e-18
+    x.requires_grad_(True)
+    (y, _), _ = qk_norm_rope_with_tangent((x, None), (None, None), w, None, 1e-30, f)
+    ref = st.norm_rope(x.detach().cpu(), w.cpu(), 1e-30, f.cpu())
+    _check("y", y, ref, _pair_size(ref))
+    (y, _), _ = qk_norm_rope_with_tangent((x, None), (None, None), w, None, 0.0, f)
+    assert torch.isnan(y[0, 0]).all() and torch.isfinite(y[0, 1]).all()
+    # three heads of 32 leave most of a wave without a row: those add nothing to the weight's gradient
+    z = torch.randn(1, 4, 3, 32, device=gpu)
+    wz = w.clone().requires_grad_(True)
+    (y, _), _ = qk_norm_rope_with_tangent((z, None), (None, None), wz, None, 0.0, f)
+    assert torch.isfinite(torch.autograd.grad(y.sum(), wz)[0]).all()
+    e = torch.zeros(0, 4, 3, 32, device=gpu, requires_grad=True)
+    we = w.clone().requires_grad_(True)
+    (y, _), _ = qk_norm_rope_with_tangent((e, None), (None, None), we, None, 1e-6, f)
+    ge, gw = torch.autograd.grad(y.sum(), (e, we))
+    assert y.shape == e.shape and ge.shape == e.shape and torch.equal(gw, torch.zeros_like(gw))
+
+
+@pytest.mark.gpu
+def test_long_sums_of_the_weight_gradient_repeat(gpu):
+    from dmad_amd import qk_norm_rope_with_tangent
+
+    x = _inputs(1, 7000, 12, 4, 128, torch.bfloat16, torch.float32, 11, "plain")
+    ref = _reference(x, x["wq"], x["wk"], 1e-6, x["freqs"], False)
+    d = {n: v.to(gpu) for n, v in x.items()}
+    for n in ("q", "k", "wq", "wk"):
+        d[n].requires_grad_(True)
+    runs = []
+    for _ in range(3):
+        (q, _), (k, _) = qk_norm_rope_with_tangent((d["q"], None), (d["k"], None), d["wq"], d["wk"], 1e-6, d["freqs"])
+        runs.append(torch.autograd.grad((q, k), (d["wq"], d["wk"]), (d["gq"], d["gk"])))
+    _check("dwq", runs[0][0], ref["dwq"], ref["sumq"])
+    _check("dwk", runs[0][1], ref["dwk"], ref["sumk"])
+    for r in runs[1:]:
+        assert torch.equal(r[0], runs[0][0]) and torch.equal(r[1], runs[0][1])
+
+
+@pytest.mark.gpu
+def test_feeds_the_jvp_attention(gpu):
+    """The operator in its place: projections' outputs and tangents, normed and rotated, into the JVP attention."""
+    from dmad_amd import qk_norm_rope_with_tangent, torch_attention_op_withT
+    from oracle import attention as orc
+
+    x = _inputs(1, 200, 4, 4, 64, torch.bfloat16, torch.bfloat16, 13, "fused")
+    g = torch.Generator().manual_seed(14)
+    v = torch.randn(1, 200, 4, 64, generator=g).to(torch.bfloat16)
+    tv = (torch.randn(1, 200, 4, 64, generator=g) * 0.1).to(torch.bfloat16)
+    d = {n: t.to(gpu) for n, t in x.items()}
+    d["q"].requires_grad_(True)
+    qT, kT = qk_norm_rope_with_tangent((d["q"], d["tq"]), (d["k"], d["tk"]), d["wq"], d["wk"], 1e-6, d["freqs"])
+    o, to = torch_attention_op_withT(qT, kT, (v.to(gpu), tv.to(gpu)))
+    o.float().sum().backward()
+    hd = lambda t: t.transpose(1, 2).double()  # noqa: E731
+    q, k = (st.norm_rope(x[n], x["w" + n], 1e-6, x["freqs"]).to(torch.bfloat16) for n in ("q", "k"))
+    tq, tk = (st.norm_rope_tangent(x[n], x["t" + n], x["w" + n], 1e-6, x["freqs"]).to(torch.bfloat16) for n in ("q", "k"))
+    ro, rto, _, _ = orc.jvp_closed_form(hd(q), hd(k), hd(v), hd(tq), hd(tk), hd(tv))
+    assert orc.rel_l2(o.detach().transpose(1, 2).cpu(), ro) < 1e-2
+    assert orc.rel_l2(to.transpose(1, 2).cpu(), rto) < 1e-2
+    assert torch.isfinite(d["q"].grad.float()).all() and float(d["q"].grad.float().norm()) > 0
+
+
+@pytest.mark.gpu
+def test_captured_and_on_another_stream(gpu):
+    from dmad_amd import qk_norm_rope_with_tangent
+
+    x = _inputs(2, 300, 6, 2, 128, torch.bfloat16, torch.bfloat16, 15, "plain")
+    d = {n: v.to(gpu) for n, v in x.items()}
+
+    def step():
+        leaves = [d[n].detach().requires_grad_(True) for n in ("q", "k", "wq", "wk")]
+        (q, _), (k, _) = qk_norm_rope_with_tangent((leaves[0], None), (leaves[1], None), leaves[2], leaves[3], 1e-6, d["freqs"])
+        return [q.detach(), k.detach(), *torch.autograd.grad((q, k), leaves, (d["gq"], d["gk"]))]
+
+    ref = [t.clone() for t in step()]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(other, ref))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        junk = torch.randn(1024, 1024, device=gpu)
+        (junk @ junk).sum().item()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, ref))
+
+
+# ---------------------------------------------------------------- refusals
+
+
+def test_refusals_on_the_cpu():
+    from dmad_amd import qk_norm_rope_with_tangent
+
+    q = torch.randn(1, 2, 3, 32)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        qk_norm_rope_with_tangent((q, None), (None, None), None, None, 1e-6, torch.zeros(2, 16))
+
+
+@pytest.mark.gpu
+def test_refusals(gpu):
+    from dmad_amd import qk_norm_rope_with_tangent as op
+
+    q = torch.randn(2, 5, 4, 64, device=gpu, dtype=torch.bfloat16)
+    k, w, f = q[:, :, :2].contiguous(), torch.ones(64, device=gpu, dtype=torch.bfloat16), torch.zeros(5, 32, device=gpu)
+    bad = [
+        (ValueError, "neither", (None, None), (None, None), w, w, 1e-6, f),
+        (ValueError, "heads", (q, None), (k[:, :4], None), w, w, 1e-6, f),
+        (ValueError, "and k", (q, None), (k.half(), None), w, w, 1e-6, f),
+        (NotImplementedError, "head dim", (q[..., :48], None), (None, None), None, None, 1e-6, None),
+        (NotImplementedError, "dtype", (q.double(), None), (None, None), None, None, 1e-6, f),
+        (ValueError, "weights", (q, None), (k, None), w[:32], w, 1e-6, f),
+        (ValueError, "weights", (q, None), (k, None), w.double(), w, 1e-6, f),
+        (ValueError, "freqs", (q, None), (k, None), w, w, 1e-6, f[:4]),
+        (ValueError, "freqs", (q, None), (k, None), w, w, 1e-6, f[None].expand(3, 5, 32)),
+        (ValueError, "eps", (q, None), (k, None), w, w, -1.0, f),
+        (ValueError, "eps", (q, None), (k, None), w, w, math.nan, f),
+        (ValueError, "tangent", (q, q[:1]), (k, k), w, w, 1e-6, f),
+        (ValueError, "tangents of both", (q, q), (k, None), w, w, 1e-6, f),
+        (ValueError, r"\[B, S, H, D\]", (q[0], None), (None, None), w, w, 1e-6, f),
+        (RuntimeError, "GPU only", (q, None), (k.cpu(), None), w, w, 1e-6, f),
+    ]
+    for error, match, *args in bad:
+        with pytest.raises(error, match=match):
+            op(*args)
+    # a weight of another 16-bit type is widened with its partner
+    a = op((q, None), (k, None), w, w.float(), 1e-6, f)
+    b = op((q, None), (k, None), w.float(), w.float(), 1e-6, f)
+    assert torch.equal(a[0][0], b[0][0]) and torch.equal(a[1][0], b[1][0])
+
+
+def _strides(*v):
+    import ctypes
+
+    return (ctypes.c_int64 * 4)(*v)
+
+
+@pytest.mark.parametrize("over,code,needle", [
+    (dict(D=48), 2, "head dim"),
+    (dict(dtype=9), 2, "dtype"),
+    (dict(wdtype=1), 2, "weights"),
+    (dict(Hq=0, Hk=0), 1, "sizes"),
+    (dict(S=-1), 1, "sizes"),
+    (dict(eps=-1.0), 1, "eps"),
+    (dict(q=0), 1, "q: null"),
+    (dict(Hk=0), 1, "no heads"),
+    (dict(tq=256), 1, "neither"),
+    (dict(q=264), 1, "aligned"),
+    (dict(wq=2), 1, "aligned"),
+    (dict(qs=_strides(512, 256, 60, 1)), 1, "multiples of 8"),
+    (dict(qs=_strides(512, 256, 64, 2)), 1, "head dim must be 1"),
+    (dict(ks=_strides(512, -256, 64, 1)), 1, "non-negative"),
+    (dict(ok=0), 1, "output"),
+    (dict(fb=-1), 1, "freqs"),
+    (dict(B=1 << 20, S=1 << 20), 2, "too many"),
+    (dict(B=1 << 15, S=1 << 15, Hq=64), 2, "too many"),
+])
+def test_c_entry_rejects_bad_arguments(over, code, needle):
+    import ctypes
+
+    from dmad_amd import _native as nat
+
+    a = dict(dtype=0, wdtype=0, B=1, S=2, Hq=4, Hk=2, D=64, q=256, tq=0, k=256, tk=0, qs=_strides(512, 256, 64, 1), wq=256,
+             ks=_strides(256, 128, 64, 1), wk=256, f=256, fb=0, eps=1e-6, oq=256, ok=256)
+    a.update(over)
+    p = ctypes.c_void_p
+    rc = nat.lib().dmad_qk_norm_rope(a["dtype"], a["wdtype"], a["B"], a["S"], a["Hq"], a["Hk"], a["D"], p(a["q"]), p(a["tq"]),
+                                     p(a["k"]), p(a["tk"]), a["qs"], a["qs"], a["ks"], a["ks"], p(a["wq"]), p(a["wk"]),
+                                     p(a["f"]), a["fb"], a["eps"], p(a["oq"]), p(0), p(a["ok"]), p(0), p(0))
+    assert rc == code, nat.lib().dmad_last_error()
+    assert needle in nat.lib().dmad_last_error().decode()
+
+
+def test_c_backward_rejects_bad_arguments():
+    import ctypes
+
+    from dmad_amd import _native as nat
+
+    p, n = ctypes.c_void_p, ctypes.c_size_t(0)
+    lib = nat.lib()
+    assert lib.dmad_qk_norm_rope_bwd_workspace_bytes(1, 5, 4, 2, 64, ctypes.byref(n)) == 0 and n.value > 0
+    s = _strides(512, 256, 64, 1)
+
+    def call(wq=256, dwq=256, gq=256, ws=256, size=1 << 30, B=1):
+        return lib.dmad_qk_norm_rope_bwd(0, 0, B, 2, 4, 4, 64, p(256), p(gq), p(256), p(256), s, s, s, s, p(wq), p(256), p(256),
+                                         0, 1e-6, p(256), p(256), p(dwq), p(256), p(ws), size, p(0))
+
+    assert call(wq=0) == 1 and b"weight" in lib.dmad_last_error()
+    assert call(gq=0) == 1 and b"gradient" in lib.dmad_last_error()
+    assert call(ws=0) == 3 and call(size=16) == 3
+    assert call(B=0) == 1
