@@ -1318,18 +1318,34 @@ int check_cache(int dtype, const dmad_kv_cache* c, dmad::KvPages& kv) {
   kv.position = c->position;
   kv.num_pages = (int)c->num_pages;
   kv.heads = (int)c->kv_heads;
-  kv.P = (int)c->page_size;
-  kv.M = (int)c->pages_per_seq;
+  kv.set_pages((int)c->page_size, (int)c->pages_per_seq);
   kv.B = (int)c->batch;
   return DMAD_OK;
 }
 
-// Pieces that all sequences together aim at, per key head and row group: three
-// workgroups of the attention share a CU.
-constexpr int64_t kPagedFill = 3 * 256;
+// Pieces per key head and row group, of which there are `per`: as many as make
+// rounds of the workgroups that 256 CUs hold at least nine tenths full, the
+// fewest first (every further round costs each workgroup its start and end).
+constexpr int64_t kPagedCus = 256;
+int64_t paged_splits(int64_t per, int64_t resident) {
+  const int64_t slots = kPagedCus * resident;
+  if (per <= slots / 10) return slots / per;  // one round, at least nine tenths of it
+  int64_t best = 1;
+  double fullest = 0;
+  for (int64_t n = 1; n <= 16; ++n) {
+    const int64_t rounds = (n * per + slots - 1) / slots;
+    const double full = (double)(n * per) / (double)(rounds * slots);
+    if (full >= 0.9) return n;
+    if (full > fullest) {
+      fullest = full;
+      best = n;
+    }
+  }
+  return best;
+}
 
 struct PagedLayout {
-  int64_t R, row_groups, splits, max_splits;
+  int64_t R, row_groups, splits;
   size_t part_o, part_ml, scores, lse2, total;  // offsets; equal to the next where a part is absent
 };
 int paged_layout(const dmad_kv_cache* c, int64_t S, int64_t Hq, bool accumulate, PagedLayout& w) {
@@ -1339,22 +1355,21 @@ int paged_layout(const dmad_kv_cache* c, int64_t S, int64_t Hq, bool accumulate,
   const int64_t lim = (int64_t)1 << 31;
   if (S >= lim / Hq) return fail(DMAD_ERR_UNSUPPORTED, "too many query rows");
   w.R = S * (Hq / c->kv_heads);
-  const int64_t rows = dmad::paged_attn_rows((int)c->head_dim, (int)w.R);
+  const int64_t rows = dmad::paged_attn_rows((int)w.R);
   w.row_groups = (w.R + rows - 1) / rows;
   const int64_t cap = c->pages_per_seq * c->page_size;
   const int64_t tiles = cap > 0 ? (cap + dmad::kPagedTile - 1) / dmad::kPagedTile : 1;
   const int64_t per = c->kv_heads * (w.row_groups > 0 ? w.row_groups : 1);
-  w.splits = per < kPagedFill ? kPagedFill / per : 1;
-  w.max_splits = w.splits + c->batch;
-  if (w.max_splits > c->batch * tiles) w.max_splits = c->batch * tiles;
+  w.splits = paged_splits(per, dmad::paged_attn_resident((int)c->head_dim));
+  if (w.splits > c->batch * tiles) w.splits = c->batch * tiles;
   const bool join = tiles > 1;
   const size_t BR = (size_t)c->batch * c->kv_heads * w.R;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   size_t at = 0;
   w.part_o = at;
-  if (join) at += up((size_t)w.max_splits * c->kv_heads * w.R * c->head_dim * 4);
+  if (join) at += up((size_t)(w.splits + c->batch) * c->kv_heads * w.R * c->head_dim * 4);
   w.part_ml = at;
-  if (join) at += up((size_t)w.max_splits * c->kv_heads * w.R * 8);
+  if (join) at += up((size_t)(w.splits + c->batch) * c->kv_heads * w.R * 8);
   w.scores = at;
   if (accumulate) at += up(BR * (size_t)cap * 4);
   w.lse2 = at;
@@ -1362,10 +1377,8 @@ int paged_layout(const dmad_kv_cache* c, int64_t S, int64_t Hq, bool accumulate,
   w.total = at;
   // 256 threads per workgroup, of which a launch takes fewer than 2^32 threads
   const int64_t groups = (int64_t)1 << 24;
-  if (w.max_splits * per >= groups || c->batch * c->kv_heads * w.R >= groups || c->batch * tiles >= lim)
+  if (w.splits * per + 8 * w.row_groups >= groups || c->batch * c->kv_heads * w.R >= groups || c->batch * tiles >= lim / 2)
     return fail(DMAD_ERR_UNSUPPORTED, "too many pieces for one launch");
-  if (accumulate && c->batch * c->kv_heads >= 65536)
-    return fail(DMAD_ERR_UNSUPPORTED, "weights are accumulated for fewer than 65536 sequences times heads");
   return DMAD_OK;
 }
 
@@ -1381,7 +1394,7 @@ EvictLayout evict_layout(const dmad_kv_cache* c, int64_t keep) {
   const size_t BH = (size_t)c->batch * c->kv_heads;
   EvictLayout w{};
   if (c->pages_per_seq * c->page_size <= keep) return w;  // nothing can be longer
-  w.moves = up(BH * c->pages_per_seq * c->page_size * 4);
+  if (c->pages_per_seq * c->page_size > dmad::kSelectInLds) w.moves = up(BH * c->pages_per_seq * c->page_size * 4);
   w.counts = w.moves + up(BH * 2 * evict_moves(c, keep) * 4);
   w.total = w.counts + up(BH * 4);
   return w;
@@ -1822,7 +1835,6 @@ int dmad_paged_attn(int dtype, const dmad_kv_cache* cache, int64_t S, int64_t Hq
   p.row_groups = (int)w.row_groups;
   p.causal = causal != 0;
   p.splits = (int)w.splits;
-  p.max_splits = (int)w.max_splits;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   if (w.part_ml > w.part_o) {
     p.part_o = (float*)(ws + w.part_o);

@@ -50,24 +50,28 @@ struct PagedAttnParams {
   int S, G, R;             // new tokens, query heads per key head, rows per key head (S * G)
   int row_groups;          // workgroups that share a key head's rows
   int causal;
-  int splits;              // target number of pieces of all sequences together, per head and row group
-  int max_splits;          // bound on the pieces there are
+  int splits;              // pieces of all sequences together, per head and row group
   float scale_log2;
-  float* part_o;           // [max_splits][heads][R][D]
-  float* part_ml;          // [max_splits][heads][R][2]: maximum (log2 domain) and sum
+  float* part_o;           // [splits + B][heads][R][D], or null: no sequence has more than a tile
+  float* part_ml;          // [splits + B][heads][R][2]: maximum (log2 domain) and sum
   float* scores;           // [B][heads][R][M P], log2 domain; null: weights are not accumulated
   float* lse2;             // [B][heads][R], log2 domain (with scores)
 };
-// Rows of a workgroup of paged attention at head dim D and R rows per key head.
-int paged_attn_rows(int D, int R);
+// Rows of a workgroup of paged attention, of R rows per key head.
+int paged_attn_rows(int R);
+// Its workgroups per CU that a launch aims at.
+int paged_attn_resident(int D);
 hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, int D, hipStream_t s);
 
 // ---------------------------------------------------------------- eviction
+// Up to this many slots per sequence the selection keeps its keys in LDS (128 KiB).
+constexpr int kSelectInLds = 32 * 1024;
+
 struct KvEvictParams {
   KvPages kv;
   int D, keep, recent, sink;
   int max_moves;       // bound on the slots that move, per sequence and head
-  uint32_t* keys;      // [B][heads][M P]
+  uint32_t* keys;      // [B][heads][M P], for more than kSelectInLds slots
   int32_t* moves;      // [B][heads][2][max_moves]: destination slots, source slots
   int32_t* counts;     // [B][heads] slots that move; -1 where nothing is evicted
 };

@@ -9,14 +9,20 @@
 // or beyond `keep` and one to which it moves below: the copies need no order.
 //
 // Selection is one workgroup per sequence and head: a radix search for the
-// keep-th largest key, 8 bits at a time with a histogram per wave, then counts
-// and ranks in slot order. Copies are a second launch over all moved rows.
+// keep-th largest key, 8 bits at a time with a histogram in LDS, then counts and
+// ranks in slot order. Copies are a second launch over all moved rows.
 #include "kv_cache.h"
 #include "lanes.h"
 
 namespace dmad {
 
 constexpr int kSelectWaves = 16;
+constexpr int kSelectThreads = 64 * kSelectWaves;
+constexpr int kSelectBatch = 4;  // keys a lane reads together
+
+// Copies of the histogram, by lane: lanes that count one digit meet in a copy
+// four at a time, not 64.
+constexpr int kHistCopies = 16;
 
 // Order of weights as unsigned keys: 1 .. 0xfffffffe, NaN above all of them;
 // 0xffffffff stays unconditionally and 0 goes first.
@@ -26,8 +32,11 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__global__ __launch_bounds__(64 * kSelectWaves) void kv_select_kernel(KvEvictParams p) {
-  __shared__ uint32_t hist[kSelectWaves][256];
+// SLOTS > 0: keys stay in LDS (sequences of up to SLOTS slots); 0: in memory.
+template <int SLOTS>
+__global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams p) {
+  __shared__ uint32_t lds_keys[SLOTS > 0 ? SLOTS : 1];
+  __shared__ uint32_t hist[256 * kHistCopies];
   __shared__ uint32_t total[256];
   __shared__ uint32_t found[2];
   __shared__ int before_eq[kSelectWaves], before_hole[kSelectWaves], before_move[kSelectWaves];
@@ -40,37 +49,68 @@ __global__ __launch_bounds__(64 * kSelectWaves) void kv_select_kernel(KvEvictPar
     return;
   }
   // each wave has a range of slots, so that ranks in slot order need only its running counts
-  const int span = ((n + 64 * kSelectWaves - 1) / (64 * kSelectWaves)) * 64;
+  const int span = ((n + kSelectThreads - 1) / kSelectThreads) * 64;
   const int begin = min(n, wave * span), end = min(n, begin + span);
-  uint32_t* keys = p.keys + (int64_t)blockIdx.x * kv.capacity();
+  uint32_t* keys = SLOTS > 0 ? lds_keys : p.keys + (int64_t)blockIdx.x * kv.capacity();
   const int oldest = kv.seen[b] - p.recent;
 
-  for (int s = begin + lane; s < end; s += 64) {
-    const KvSlot where = kv.locate(b, s);
-    uint32_t key = s < p.keep ? 0xffffffffu : 0u;  // slots of a missing page: none moves, none is moved to
-    if (where.page >= 0) {
-      const int64_t at = kv.index(where, h);
-      const int position = kv.position[at];
-      key = position < p.sink || position >= oldest ? 0xffffffffu : weight_key(kv.weight[at]);
+  // Keys from weights and positions, LOADS slots of a lane under way together
+  // (the page ids, then what is there); a lane reads back only its own.
+  constexpr int LOADS = SLOTS == kSelectInLds / 8 ? 4 : 16;
+  for (int s0 = begin; s0 < end; s0 += 64 * LOADS) {
+    KvSlot at[LOADS];
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const int s = s0 + 64 * j + lane;
+      at[j] = KvSlot{-1, 0};
+      if (s < end) at[j] = kv.locate(b, s);
     }
-    keys[s] = key;
+    float w[LOADS];
+    int position[LOADS];
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      if (at[j].page < 0) continue;
+      w[j] = kv.weight[kv.index(at[j], h)];
+      position[j] = kv.position[kv.index(at[j], h)];
+    }
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const int s = s0 + 64 * j + lane;
+      // slots of a missing page: none moves, none is moved to
+      uint32_t key = s < p.keep ? 0xffffffffu : 0u;
+      if (at[j].page >= 0) key = position[j] < p.sink || position[j] >= oldest ? 0xffffffffu : weight_key(w[j]);
+      if (s < end) keys[s] = key;
+    }
   }
+  // f(slot, its key, whether there is one) for this wave's slots, 64 at a time in order
+  auto each = [&](auto f) {
+    for (int s0 = begin; s0 < end; s0 += 64 * kSelectBatch) {
+      uint32_t key[kSelectBatch];
+#pragma unroll
+      for (int j = 0; j < kSelectBatch; ++j) {
+        const int s = s0 + 64 * j + lane;
+        key[j] = s < end ? keys[s] : 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < kSelectBatch; ++j)
+        if (s0 + 64 * j < end) f(s0 + 64 * j + lane, key[j], s0 + 64 * j + lane < end);  // the test is the wave's
+    }
+  };
 
   // the keep-th largest key, and how many of its equals stay
   uint32_t prefix = 0, mask = 0;
   uint32_t left = (uint32_t)p.keep;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256 * kSelectWaves; i += 64 * kSelectWaves) (&hist[0][0])[i] = 0;
+    for (int i = threadIdx.x; i < 256 * kHistCopies; i += kSelectThreads) hist[i] = 0;
     __syncthreads();
-    for (int s = begin + lane; s < end; s += 64) {
-      const uint32_t key = keys[s];
-      if ((key & mask) == prefix) atomicAdd(&hist[wave][(key >> shift) & 255], 1u);
-    }
+    each([&](int, uint32_t k, bool there) {
+      if (there && (k & mask) == prefix) atomicAdd(&hist[((k >> shift) & 255) * kHistCopies + (lane & (kHistCopies - 1))], 1u);
+    });
     __syncthreads();
     if (threadIdx.x < 256) {
       uint32_t t = 0;
 #pragma unroll
-      for (int w = 0; w < kSelectWaves; ++w) t += hist[w][threadIdx.x];
+      for (int c = 0; c < kHistCopies; ++c) t += hist[threadIdx.x * kHistCopies + ((c + threadIdx.x) & (kHistCopies - 1))];
       total[threadIdx.x] = t;
     }
     __syncthreads();
@@ -103,34 +143,28 @@ __global__ __launch_bounds__(64 * kSelectWaves) void kv_select_kernel(KvEvictPar
   }
 
   // equals before each wave
-  auto ballot_count = [](bool x) { return (int)__popcll(__ballot(x)); };
   const uint64_t below = ((uint64_t)1 << lane) - 1;
   int count = 0;
-  for (int s0 = begin; s0 < end; s0 += 64) {
-    const int s = s0 + lane;
-    count += ballot_count(s < end && keys[s] == prefix);
-  }
+  each([&](int, uint32_t k, bool there) { count += (int)__popcll(__ballot(there && k == prefix)); });
   if (lane == 0) before_eq[wave] = count;
   __syncthreads();
   int eq0 = 0;
   for (int w = 0; w < wave; ++w) eq0 += before_eq[w];
 
   // whether a slot stays; eq runs over the equals
-  auto stays = [&](int s, int& eq) {
-    const uint32_t key = s < end ? keys[s] : 0u;
-    const bool equal = s < end && key == prefix;
+  auto stays = [&](uint32_t k, bool there, int& eq) {
+    const bool equal = there && k == prefix;
     const uint64_t votes = __ballot(equal);
     const int rank = eq + (int)__popcll(votes & below);
     eq += (int)__popcll(votes);
-    return s < end && (key > prefix || (equal && (uint32_t)rank < left));
+    return there && (k > prefix || (equal && (uint32_t)rank < left));
   };
   int holes = 0, moves = 0, eq = eq0;
-  for (int s0 = begin; s0 < end; s0 += 64) {
-    const int s = s0 + lane;
-    const bool st = stays(s, eq);
-    holes += ballot_count(s < p.keep && s < end && !st);
-    moves += ballot_count(s >= p.keep && st);
-  }
+  each([&](int s, uint32_t k, bool there) {
+    const bool st = stays(k, there, eq);
+    holes += (int)__popcll(__ballot(s < p.keep && there && !st));
+    moves += (int)__popcll(__ballot(s >= p.keep && st));
+  });
   if (lane == 0) {
     before_hole[wave] = holes;
     before_move[wave] = moves;
@@ -144,10 +178,9 @@ __global__ __launch_bounds__(64 * kSelectWaves) void kv_select_kernel(KvEvictPar
   int32_t* to = p.moves + (int64_t)blockIdx.x * 2 * p.max_moves;
   int32_t* from = to + p.max_moves;
   eq = eq0;
-  for (int s0 = begin; s0 < end; s0 += 64) {
-    const int s = s0 + lane;
-    const bool st = stays(s, eq);
-    const bool hole = s < p.keep && s < end && !st, move = s >= p.keep && st;
+  each([&](int s, uint32_t k, bool there) {
+    const bool st = stays(k, there, eq);
+    const bool hole = s < p.keep && there && !st, move = s >= p.keep && st;
     const uint64_t hv = __ballot(hole), mv = __ballot(move);
     // as many slots move as go below keep: min(keep, n - keep) at most
     const int hi = hole0 + (int)__popcll(hv & below), mi = move0 + (int)__popcll(mv & below);
@@ -155,8 +188,8 @@ __global__ __launch_bounds__(64 * kSelectWaves) void kv_select_kernel(KvEvictPar
     if (move && mi < p.max_moves) from[mi] = s;
     hole0 += (int)__popcll(hv);
     move0 += (int)__popcll(mv);
-  }
-  if (threadIdx.x == 64 * kSelectWaves - 1) p.counts[blockIdx.x] = min(move0, p.max_moves);
+  });
+  if (threadIdx.x == kSelectThreads - 1) p.counts[blockIdx.x] = min(move0, p.max_moves);
 }
 
 // A row per D/8 lanes, K and V together.
@@ -192,7 +225,11 @@ static hipError_t move_launch(const KvEvictParams& p, hipStream_t s) {
 }
 
 hipError_t launch_kv_evict(const KvEvictParams& p, hipStream_t s) {
-  hipLaunchKernelGGL(kv_select_kernel, dim3((unsigned)(p.kv.B * p.kv.heads)), dim3(64 * kSelectWaves), 0, s, p);
+  const dim3 grid((unsigned)(p.kv.B * p.kv.heads)), block(kSelectThreads);
+  const int slots = p.kv.M * p.kv.P;
+  if (slots <= kSelectInLds / 8) hipLaunchKernelGGL((kv_select_kernel<kSelectInLds / 8>), grid, block, 0, s, p);
+  else if (slots <= kSelectInLds) hipLaunchKernelGGL((kv_select_kernel<kSelectInLds>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((kv_select_kernel<0>), grid, block, 0, s, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   switch (p.D) {

@@ -30,7 +30,21 @@ struct KvPages {
   float* weight;      // [num_pages][heads][P], or null
   int32_t* position;  // [num_pages][heads][P], or null (both or none)
   int num_pages, heads, P, M, B;
+  uint32_t p_mul;  // s / P = (s p_mul) >> (32 + p_shift) for s < 2^26 (set_pages)
+  int p_shift;
 
+  // Page size and pages per sequence, P M <= 2^26. With 2^l >= P the multiplier
+  // ceil(2^sh / P) at sh = max(32, 26 + l) is off by less than P / 2^sh, which
+  // times s < 2^26 stays below 1 / P: the quotient is exact.
+  inline void set_pages(int page_size, int pages) {
+    P = page_size;
+    M = pages;
+    int l = 0;
+    while (((int64_t)1 << l) < page_size) ++l;
+    const int sh = l < 6 ? 32 : 26 + l;
+    p_mul = (uint32_t)((((uint64_t)1 << sh) + page_size - 1) / page_size);
+    p_shift = sh - 32;
+  }
   DMAD_HD int capacity() const { return M * P; }
   // Slots of sequence b, whatever its length says.
   DMAD_HD int length(int b) const {
@@ -40,9 +54,10 @@ struct KvPages {
   // Slot s of sequence b; s may be any number.
   DMAD_HD KvSlot locate(int b, int s) const {
     if ((unsigned)s >= (unsigned)(M * P)) return KvSlot{-1, 0};
-    const int page = table[b * table_stride + (int)((unsigned)s / (unsigned)P)];
+    const int entry = (int)((uint32_t)(((uint64_t)(uint32_t)s * p_mul) >> 32) >> p_shift);
+    const int page = table[b * table_stride + entry];
     if ((unsigned)page >= (unsigned)num_pages) return KvSlot{-1, 0};
-    return KvSlot{page, (int)((unsigned)s % (unsigned)P)};
+    return KvSlot{page, s - entry * P};
   }
   // Index into weight and position, and offsets (elements) into k and v.
   DMAD_HD int64_t index(KvSlot at, int head) const { return ((int64_t)at.page * heads + head) * P + at.slot; }

@@ -21,12 +21,12 @@
 // The next step's K is requested when this step's scores are done, and V
 // when its products are.
 //
-// Split: the launch aims at `splits` pieces for all sequences together; the
-// device turns that into a number of 128-slot tiles per piece from the lengths
-// it finds, so ragged batches load the chip evenly and a captured graph
-// follows the lengths. Each piece leaves (maximum, sum, O) in float32 and a
-// second kernel joins them in order. A sequence of one piece is finished by
-// the first kernel.
+// Split: the launch has `splits` pieces of equal work for all sequences
+// together; the device finds from the lengths which tiles are whose, so ragged
+// batches load the chip evenly and a captured graph follows the lengths. A
+// sequence that lies in several pieces leaves (maximum, sum, O) of each in
+// float32 and a second kernel joins them in order; one that lies in a single
+// piece is finished by the first kernel.
 #include "kv_cache.h"
 #include "lanes.h"
 
@@ -35,71 +35,96 @@ namespace dmad {
 constexpr int kPagedWaves = 4;
 constexpr int kStep = 32;  // slots per wave step
 
-__device__ __forceinline__ int wave_sum_int(int x) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
+// Running sum over the lanes, the lane's own included: within rows of 16
+// lanes, then the row before's last lane, then lane 31's.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_step(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+  x = scan_step<0x111, 0xf>(x);  // from 1, 2, 4 and 8 lanes below
+  x = scan_step<0x112, 0xf>(x);
+  x = scan_step<0x114, 0xf>(x);
+  x = scan_step<0x118, 0xf>(x);
+  x = scan_step<0x142, 0xa>(x);  // lane 15 to rows 1, 3
+  x = scan_step<0x143, 0xc>(x);  // lane 31 to rows 2, 3
   return x;
 }
-__device__ __forceinline__ int wave_scan_int(int x, int lane) {  // inclusive
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int y = __shfl_up(x, m);
-    if (lane >= m) x += y;
-  }
-  return x;
-}
+__device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
-// How the sequences are cut: tiles per piece, from all lengths.
+// How the work is cut. Each sequence is a run of 128-slot tiles (one at least),
+// the runs follow one another, and piece x takes tiles [x chunk, (x + 1) chunk)
+// of that line, whatever sequences they belong to: equal work for every
+// workgroup of a ragged batch. A piece's part of a sequence is a segment; with
+// the pieces and the sequences both in order, x + b numbers the segments
+// without a clash.
 __device__ __forceinline__ int paged_tiles(int n) { return max(1, (n + kPagedTile - 1) / kPagedTile); }
-__device__ __forceinline__ int paged_chunk(const KvPages& kv, int splits, int lane) {
-  int tiles = 0;
-  for (int b = lane; b < kv.B; b += 64) tiles += paged_tiles(kv.length(b));
-  tiles = wave_sum_int(tiles);
-  return max(1, (tiles + splits - 1) / splits);
-}
 
-struct PagedPiece {
-  int b, n;          // sequence and its length; b < 0: no such piece
-  int index, count;  // this piece among the sequence's, and how many it has
-  int first;         // number of its first piece among all
-  int chunk;         // tiles per piece
+// Lengths of all sequences, a lane each; the first 64 are read once.
+struct PagedLengths {
+  const KvPages& kv;
+  int lane, first;
+  __device__ __forceinline__ PagedLengths(const KvPages& k, int l) : kv(k), lane(l), first(l < k.B ? k.length(l) : 0) {}
+  // length of sequence b0 + lane (b0 a multiple of 64), and its tiles (0 beyond the last)
+  __device__ __forceinline__ int at(int b0) const { return b0 == 0 ? first : b0 + lane < kv.B ? kv.length(b0 + lane) : 0; }
+  __device__ __forceinline__ int tiles(int b0) const { return b0 + lane < kv.B ? paged_tiles(at(b0)) : 0; }
+  __device__ __forceinline__ int total() const {
+    int t = 0;
+    for (int b0 = 0; b0 < kv.B; b0 += 64) t += tiles(b0);
+    return wave_total(t);
+  }
 };
 
-// Piece `x` of all sequences in order (every wave finds it for itself).
-__device__ __forceinline__ PagedPiece find_piece(const KvPages& kv, int splits, int x, int lane) {
-  PagedPiece r{-1, 0, 0, 0, 0, 0};
-  r.chunk = paged_chunk(kv, splits, lane);
+// A sequence and where its run of tiles begins.
+struct PagedRun {
+  int b, n, base;
+};
+__device__ __forceinline__ PagedRun run_of_tile(const PagedLengths& len, int tile) {
   int before = 0;
-  for (int b0 = 0; b0 < kv.B; b0 += 64) {
-    const int b = b0 + lane;
-    const int n = b < kv.B ? kv.length(b) : 0;
-    const int mine = b < kv.B ? (paged_tiles(n) + r.chunk - 1) / r.chunk : 0;
-    const int end = before + wave_scan_int(mine, lane);
-    const uint64_t past = __ballot(end > x);
+  for (int b0 = 0; b0 < len.kv.B; b0 += 64) {
+    const int n = len.at(b0), end = before + wave_scan(len.tiles(b0));
+    const uint64_t past = __ballot(end > tile);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
-      r.b = b0 + at;
-      r.n = __builtin_amdgcn_readlane(n, at);
-      r.count = __builtin_amdgcn_readlane(mine, at);
-      r.first = __builtin_amdgcn_readlane(end, at) - r.count;
-      r.index = x - r.first;
-      return r;
+      const int m = __builtin_amdgcn_readlane(n, at);
+      return PagedRun{b0 + at, m, __builtin_amdgcn_readlane(end, at) - paged_tiles(m)};
     }
     before = __builtin_amdgcn_readlane(end, 63);
   }
-  return r;
+  return PagedRun{len.kv.B, 0, before};  // beyond the last tile: not asked for
+}
+__device__ __forceinline__ PagedRun run_of_sequence(const PagedLengths& len, int b) {
+  int before = 0;
+  for (int b0 = 0; b0 < b; b0 += 64) before += b0 + len.lane < b ? len.tiles(b0) : 0;
+  return PagedRun{b, len.kv.length(b), wave_total(before)};
 }
 
-// The pieces of sequence b.
-__device__ __forceinline__ PagedPiece pieces_of(const KvPages& kv, int splits, int b, int lane) {
-  PagedPiece r{b, kv.length(b), 0, 0, 0, 0};
-  r.chunk = paged_chunk(kv, splits, lane);
-  int first = 0;
-  for (int i = lane; i < b; i += 64) first += (paged_tiles(kv.length(i)) + r.chunk - 1) / r.chunk;
-  r.first = wave_sum_int(first);
-  r.count = (paged_tiles(r.n) + r.chunk - 1) / r.chunk;
-  return r;
-}
+// Piece x, segment by segment.
+struct PagedPiece {
+  const KvPages& kv;
+  PagedRun run;
+  int tile, stop, end;  // this segment's first tile, the piece's end, the segment's end
+  __device__ __forceinline__ PagedPiece(const KvPages& k, int splits, int x, int lane) : kv(k), run{0, 0, 0}, tile(0), stop(0), end(0) {
+    const PagedLengths len(kv, lane);
+    const int total = len.total(), chunk = max(1, (total + splits - 1) / splits);
+    tile = x * chunk;
+    stop = min(total, tile + chunk);
+    if (tile < stop) run = run_of_tile(len, tile);
+    end = min(stop, run.base + paged_tiles(run.n));
+  }
+  __device__ __forceinline__ bool done() const { return tile >= stop; }
+  __device__ __forceinline__ bool last() const { return end >= stop; }
+  __device__ __forceinline__ void next() {
+    tile = end;
+    if (done()) return;
+    run = PagedRun{run.b + 1, kv.length(run.b + 1), run.base + paged_tiles(run.n)};
+    end = min(stop, run.base + paged_tiles(run.n));
+  }
+  // the segment's slots, and whether it is the whole sequence
+  __device__ __forceinline__ int first_slot() const { return (tile - run.base) * kPagedTile; }
+  __device__ __forceinline__ int end_slot() const { return min(run.n, (end - run.base) * kPagedTile); }
+  __device__ __forceinline__ bool whole() const { return tile == run.base && end == run.base + paged_tiles(run.n); }
+};
 
 // Elements of O, or of a partial: 4 floats to 4 elements.
 template <typename T>
@@ -138,21 +163,22 @@ __device__ __forceinline__ void load_v(const char* base, uint32_t off, uint32_t 
 }
 
 template <typename T, int D, int NT, bool ACC>
-__global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_attn_kernel(PagedAttnParams p) {
+__global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged_attn_kernel(PagedAttnParams p) {
   using C = PagedCfg<D>;
   __shared__ float sm_o[kPagedWaves][16][C::OP];
   __shared__ float sm_m[kPagedWaves][NT * 16], sm_l[kPagedWaves][NT * 16];
   const KvPages& kv = p.kv;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = lane & 15, g = lane >> 4;
-  const int rg = (int)blockIdx.x % p.row_groups, hk = ((int)blockIdx.x / p.row_groups) % kv.heads;
-  const int x = (int)blockIdx.x / (p.row_groups * kv.heads);
-  const PagedPiece piece = find_piece(kv, p.splits, x, lane);
-  if (piece.b < 0) return;  // the whole workgroup
-  const int b = piece.b, n = piece.n;
-  const int first = piece.index * piece.chunk * kPagedTile;
-  // a sequence of several pieces has fewer tiles than int holds
-  const int last = piece.index + 1 == piece.count ? n : first + piece.chunk * kPagedTile;
+  // Blocks are dealt to the 8 XCDs in turn: the row groups of one piece and head
+  // are 8 blocks apart, on one XCD, whose L2 then reads K and V once for them.
+  const int work = (int)blockIdx.x / (8 * p.row_groups) * 8 + ((int)blockIdx.x & 7), rg = (int)blockIdx.x / 8 % p.row_groups;
+  const int hk = work % kv.heads, x = work / kv.heads;
+  if (x >= p.splits) return;
+  PagedPiece piece(kv, p.splits, x, lane);
+  for (; !piece.done(); piece.next()) {  // the same segments in every wave
+  const int b = piece.run.b, n = piece.run.n;
+  const int first = piece.first_slot(), last = piece.end_slot();
   const int steps = (last - first + kStep - 1) / kStep;
   const int mine = steps > wave ? (steps - wave + kPagedWaves - 1) / kPagedWaves : 0;  // this wave's: wave, wave + 4, ...
 
@@ -224,6 +250,11 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_attn_kernel(PagedAt
     }
   };
 
+  float* score_row[NT];  // this lane's row, from its 4 slots of a half on
+#pragma unroll
+  for (int t = 0; t < NT && ACC; ++t)
+    score_row[t] = p.scores + (((int64_t)b * kv.heads + hk) * p.R + (rg * NT + t) * 16 + row) * kv.capacity() + g * 4;
+
   f32x4_t acc[NT][C::VE];
   float m[NT], l[NT];
 #pragma unroll
@@ -234,12 +265,18 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_attn_kernel(PagedAt
     for (int j = 0; j < C::VE; ++j) acc[t][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
 
+  // Q and the page ids have to be here before the loop, on every path to it:
+  // with them still on their way the compiler waits, in every step, for all
+  // loads in flight
+  look_up(0);
+  wait_vmem();
   if (mine > 0) {
-    look_up(0);
     request_k(0);
     request_v(0);
   }
-  for (int step = 0; step < mine; ++step) {
+  // One step; all but the last request the next one's K and V without a branch
+  // around them, so that each product waits for its own operand alone.
+  auto run_step = [&](int step, auto more) {
     const int key0 = first + (wave + kPagedWaves * step) * kStep;
     const int page[2] = {half(step, 0).page, half(step, 1).page};
     const bool whole = key0 + kStep <= min(all_see, last) && page[0] >= 0 && page[1] >= 0;  // uniform
@@ -253,8 +290,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_attn_kernel(PagedAt
 #pragma unroll
         for (int c = 0; c < C::KC; ++c) s[t][hh] = mfma16(kf[hh][c], qf[t][c], s[t][hh], T{});
       }
-    const bool more = step + 1 < mine;
-    if (more) {
+    if constexpr (more.value) {
       if ((step & 31) == 31) look_up(step + 1);
       request_k(step + 1);
     }
@@ -290,12 +326,10 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_attn_kernel(PagedAt
           top = fmaxf(top, s[t][hh][v]);
         }
       if constexpr (ACC) {
-        const int r = (rg * NT + t) * 16 + row;
-        if (r < p.R) {
-          float* out = p.scores + (((int64_t)b * kv.heads + hk) * p.R + r) * kv.capacity();
+        if ((rg * NT + t) * 16 + row < p.R) {
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh)
-            if (key0 + hh * 16 < last) *(f32x4_t*)(out + key0 + hh * 16 + g * 4) = s[t][hh];
+            if (key0 + hh * 16 < last) *(f32x4_t*)(score_row[t] + key0 + hh * 16) = s[t][hh];
         }
       }
       top = across32<LaneMax>(across16<LaneMax>(top));
@@ -330,8 +364,10 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_attn_kernel(PagedAt
 #pragma unroll
       for (int t = 0; t < NT; ++t) acc[t][j] = mfma16(a, pf[t], acc[t][j], T{});
     }
-    if (more) request_v(step + 1);
-  }
+    if constexpr (more.value) request_v(step + 1);
+  };
+  for (int step = 0; step + 1 < mine; ++step) run_step(step, IC<1>{});
+  if (mine > 0) run_step(mine - 1, IC<0>{});
 
   // The waves' results joined through LDS, 16 rows at a time.
 #pragma unroll
@@ -368,7 +404,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_attn_kernel(PagedAt
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = fmaf(f, y[k], o[k]);
       }
-      if (piece.count == 1) {
+      if (piece.whole()) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const int hq = hk * p.G + r % p.G, tok = r / p.G, Hq = kv.heads * p.G;
         store4<T>((T*)p.o + (((int64_t)b * p.S + tok) * Hq + hq) * D + d, o * inv);
@@ -378,7 +414,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_attn_kernel(PagedAt
           if constexpr (ACC) p.lse2[((int64_t)b * kv.heads + hk) * p.R + r] = sum == 0.f ? __builtin_inff() : l2;
         }
       } else {
-        const int64_t at = ((int64_t)x * kv.heads + hk) * p.R + r;
+        const int64_t at = ((int64_t)(x + b) * kv.heads + hk) * p.R + r;
         *(f32x4_t*)(p.part_o + at * D + d) = o;
         if (d == 0) {
           p.part_ml[2 * at] = top;
@@ -386,6 +422,8 @@ __global__ __launch_bounds__(64 * kPagedWaves, 2) void paged_attn_kernel(PagedAt
         }
       }
     }
+  }
+  if (!piece.last()) __syncthreads();  // the next segment writes the same LDS
   }
 }
 
@@ -396,13 +434,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
   __shared__ float sm_o[STRANDS][D], sm_m[STRANDS], sm_l[STRANDS];
   const KvPages& kv = p.kv;
   const int r = (int)blockIdx.x % p.R, hk = ((int)blockIdx.x / p.R) % kv.heads, b = (int)blockIdx.x / (p.R * kv.heads);
-  const PagedPiece piece = pieces_of(kv, p.splits, b, lane_id());
-  if (piece.count == 1) return;  // finished
+  const PagedLengths len(kv, lane_id());
+  const int chunk = max(1, (len.total() + p.splits - 1) / p.splits);
+  const PagedRun run = run_of_sequence(len, b);
+  const int first = run.base / chunk, last = (run.base + paged_tiles(run.n) - 1) / chunk;  // pieces
+  if (first == last) return;  // finished
   const int strand = threadIdx.x / LANES, d = (threadIdx.x % LANES) * 4;
   float m = -__builtin_inff(), l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int i = strand; i < piece.count; i += STRANDS) {
-    const int64_t at = ((int64_t)(piece.first + i) * kv.heads + hk) * p.R + r;
+  for (int i = first + strand; i <= last; i += STRANDS) {
+    const int64_t at = ((int64_t)(i + b) * kv.heads + hk) * p.R + r;
     const float mi = p.part_ml[2 * at], li = p.part_ml[2 * at + 1];
     const f32x4_t oi = *(const f32x4_t*)(p.part_o + at * D + d);
     const float up = fmaxf(m, mi), base = up == -__builtin_inff() ? 0.f : up;
@@ -438,40 +479,55 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
   }
 }
 
-// weight_j += sum over the rows of exp2(score - lse2), 4 slots per thread.
-__global__ __launch_bounds__(256) void paged_weight_kernel(PagedAttnParams p) {
+// weight_j += sum over the rows of exp2(score - lse2), a tile of slots at a time
+// and a slot per thread. The line of tiles is cut finer than for the attention:
+// short sequences follow one another through the same wait for every one.
+__global__ __launch_bounds__(kPagedTile) void paged_weight_kernel(PagedAttnParams p, int splits) {
   const KvPages& kv = p.kv;
-  const int hk = (int)blockIdx.y % kv.heads, b = (int)blockIdx.y / kv.heads;
-  const int key = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
-  if (key >= kv.length(b)) return;  // a group of 4 slots never leaves its page
-  const KvSlot at = kv.locate(b, key);
-  if (at.page < 0) return;
-  const int64_t bh = (int64_t)b * kv.heads + hk;
-  const float* s = p.scores + bh * p.R * kv.capacity() + key;
-  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-  for (int r = 0; r < p.R; ++r) {
-    const float lse = p.lse2[bh * p.R + r];
-    const f32x4_t x = *(const f32x4_t*)(s + (int64_t)r * kv.capacity());
+  const int hk = (int)blockIdx.x % kv.heads;
+  for (PagedPiece piece(kv, splits, (int)blockIdx.x / kv.heads, lane_id()); !piece.done(); piece.next()) {
+    const int b = piece.run.b, last = piece.end_slot();
+    const int64_t bh = (int64_t)b * kv.heads + hk;
+    for (int key = piece.first_slot() + (int)threadIdx.x; key < last; key += kPagedTile) {
+      const KvSlot at = kv.locate(b, key);
+      const float* s = p.scores + bh * p.R * kv.capacity() + key;
+      float sum = 0.f;
+      for (int r0 = 0; r0 < p.R; r0 += 8) {
+        float x[8], lse[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) sum[k] += fast_exp2(x[k] - lse);
+        for (int j = 0; j < 8; ++j) {
+          const int r = min(r0 + j, p.R - 1);
+          lse[j] = r0 + j < p.R ? p.lse2[bh * p.R + r] : __builtin_inff();
+          x[j] = s[(int64_t)r * kv.capacity()];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += fast_exp2(x[j] - lse[j]);
+      }
+      if (at.page >= 0) kv.weight[kv.index(at, hk)] += sum;
+    }
   }
-  float* w = kv.weight + kv.index(at, hk);
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (key + k < kv.length(b)) w[k] += sum[k];
 }
+// Its workgroups: up to 32 per CU.
+constexpr int kPagedWeightGroups = 8192;
 
-// Two row tiles share one reading of K and V where their registers leave two
-// waves per SIMD (not for 256-wide heads).
-static int paged_row_tiles(int D, int R) { return R > 16 && D <= 128 ? 2 : 1; }
-int paged_attn_rows(int D, int R) { return 16 * paged_row_tiles(D, R); }
+// Two row tiles share one reading of K and V. Four (as many as the registers of
+// one wave per SIMD hold) were no faster up to 64 rows, whose two groups meet
+// in one L2: 67 us either way for 4 x 8 tokens of 8 query heads per key head.
+static int paged_row_tiles(int R) { return R <= 16 ? 1 : 2; }
+int paged_attn_rows(int R) { return 16 * paged_row_tiles(R); }
+// Workgroups per CU that the cut aims at. Four waves with 16 KiB of K and V on
+// their way each (128-wide heads) keep a CU's share of the memory busy: two or
+// three workgroups were 0-17% slower, for their starts and ends, and one of
+// 64-wide heads 6% slower than two.
+int paged_attn_resident(int D) { return D >= 128 ? 1 : 2; }
 
 template <typename T, int D, bool ACC>
 static hipError_t paged_launch(const PagedAttnParams& p, hipStream_t s) {
-  const dim3 grid((unsigned)(p.max_splits * p.kv.heads * p.row_groups)), block(64 * kPagedWaves);
-  if (paged_row_tiles(D, p.R) == 1) {
+  const int work = (p.splits * p.kv.heads + 7) / 8 * 8;
+  const dim3 grid((unsigned)(work * p.row_groups)), block(64 * kPagedWaves);
+  if (paged_row_tiles(p.R) == 1) {
     hipLaunchKernelGGL((paged_attn_kernel<T, D, 1, ACC>), grid, block, 0, s, p);
-  } else if constexpr (D <= 128) {
+  } else {
     hipLaunchKernelGGL((paged_attn_kernel<T, D, 2, ACC>), grid, block, 0, s, p);
   }
   hipError_t e = hipGetLastError();
@@ -481,8 +537,8 @@ static hipError_t paged_launch(const PagedAttnParams& p, hipStream_t s) {
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if constexpr (ACC) {
-    const dim3 wgrid((unsigned)((p.kv.M * p.kv.P + 1023) / 1024), (unsigned)(p.kv.B * p.kv.heads));
-    hipLaunchKernelGGL(paged_weight_kernel, wgrid, dim3(256), 0, s, p);
+    const int splits = max(p.splits, kPagedWeightGroups / p.kv.heads);
+    hipLaunchKernelGGL(paged_weight_kernel, dim3((unsigned)(splits * p.kv.heads)), dim3(kPagedTile), 0, s, p, splits);
     e = hipGetLastError();
   }
   return e;

@@ -283,22 +283,31 @@ __global__ __launch_bounds__(64 * kQkWaves) void qk_norm_rope_bwd_kernel(QkNormR
   }
 }
 
-// dw[c] = sum of column c of partial [blocks][2 D]: 16 columns and 16 strands
-// of rows per workgroup.
+// dw[c] = sum of column c of partial [blocks][2 D]: 16 columns and 64 strands
+// of rows per workgroup, at most kQkBwdBlocks / 64 rows each.
 template <typename W>
-__global__ __launch_bounds__(256) void qk_weight_grad_kernel(const float* partial, int blocks, int D, W* dwq, W* dwk) {
-  __shared__ float sums[16][17];
+__global__ __launch_bounds__(1024) void qk_weight_grad_kernel(const float* partial, int blocks, int D, W* dwq, W* dwk) {
+  __shared__ float sums[64][17];
   const int col = threadIdx.x & 15, strand = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
+  float x[kQkBwdBlocks / 64];
+#pragma unroll
+  for (int j = 0; j < kQkBwdBlocks / 64; ++j) {
+    const int i = strand + 64 * j;
+    x[j] = i < blocks ? partial[(int64_t)i * 2 * D + c] : 0.f;
+  }
   float s = 0.f;
-  for (int i = strand; i < blocks; i += 16) s += partial[(int64_t)i * 2 * D + c];
+#pragma unroll
+  for (int j = 0; j < kQkBwdBlocks / 64; ++j) s += x[j];
   sums[strand][col] = s;
   __syncthreads();
-  if (strand != 0) return;
+  if (threadIdx.x >= 64) return;
+  // strands 16 apart in each of four lane groups, then the groups
   s = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s += sums[i][col];
+  for (int i = 0; i < 16; ++i) s += sums[4 * i + strand][col];
+  s = across32<LaneAdd>(across16<LaneAdd>(s));
   W* out = c < D ? dwq : dwk;
-  if (out != nullptr) out[c < D ? c : c - D] = (W)s;
+  if (strand == 0 && out != nullptr) out[c < D ? c : c - D] = (W)s;
 }
 
 int64_t qk_norm_rope_bwd_blocks(int64_t units) {
@@ -326,7 +335,7 @@ static hipError_t qk_launch_bwd_d(const QkNormRopeParams& p, void* dwq, void* dw
   hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, D>), dim3(blocks), dim3(64 * kQkWaves), 0, s, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.partial == nullptr) return e;
-  hipLaunchKernelGGL((qk_weight_grad_kernel<W>), dim3(2 * D / 16), dim3(256), 0, s, p.partial, blocks, D, (W*)dwq, (W*)dwk);
+  hipLaunchKernelGGL((qk_weight_grad_kernel<W>), dim3(2 * D / 16), dim3(1024), 0, s, p.partial, blocks, D, (W*)dwq, (W*)dwk);
   return hipGetLastError();
 }
 

@@ -141,45 +141,62 @@ def _check_same_device(op, *ts):
     for t in ts:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise RuntimeError(f"{op} runs on the GPU only (HIP kernel); got a tensor on {t.device}")
-        if dev is not None and t.device != dev:
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
             raise ValueError(f"{op}: tensors on {dev} and on {t.device}")
-        dev = t.device
     return dev
 
 
-def row_strides(t):
-    """Strides the kernels take for a [.., D] operand (an axis of one element counts as 0), or None
-    where rows are not contiguous and 16-byte aligned."""
-    if t.shape[-1] != 1 and t.stride(-1) != 1 or t.data_ptr() % 16:
-        return None
-    st = [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
-    step = 16 // t.element_size()
-    return None if any(s % step for s in st) else (*st, 1)
+# ctypes strides by (shape, strides, element size); None where the kernels cannot read the rows in place
+_row_strides: dict = {}
+
+
+def _strides_of_rows(t):
+    key = (t.shape, t.stride(), t.element_size())
+    arr = _row_strides.get(key, 0)
+    if arr == 0:
+        *shape, D = t.shape
+        # an axis of one element is never stepped along
+        st = [0 if n == 1 else s for n, s in zip(shape, t.stride()[:-1])]
+        step = 16 // t.element_size()
+        bad = (D != 1 and t.stride(-1) != 1) or any(s % step for s in st)
+        if len(_row_strides) > 4096:
+            _row_strides.clear()
+        arr = _row_strides[key] = None if bad else nat.int64_array((*st, 1))
+    return arr
 
 
 def readable_rows(t):
-    """(tensor, ctypes strides): ``t`` itself or a contiguous copy the kernels can read."""
-    st = row_strides(t)
-    if st is None:
-        # a contiguous tensor may still start unaligned
-        t = t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
-        st = row_strides(t)
-    return t, nat.int64_array(st)
+    """(tensor, ctypes strides): ``t`` itself where its rows are contiguous and 16-byte aligned, else a
+    contiguous copy."""
+    st = _strides_of_rows(t)
+    if st is None or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = _strides_of_rows(t)
+    return t, st
 
 
 def _norm_weights(op, x, D, wq, wk):
-    """(wq, wk, their type code): one type for both, the operands' own or float32."""
+    """(wq, wk, their type code) as the kernels take them: one type for both, the operands' own or float32."""
+    dtype = x.dtype
     for w in (wq, wk):
-        if w is not None and (w.shape != (D,) or not w.is_floating_point() or w.dtype == torch.float64):
+        if w is None:
+            continue
+        if w.dim() != 1 or w.shape[0] != D or w.dtype not in (torch.float32, torch.bfloat16, torch.float16):
             raise ValueError(f"{op}: weights must be [{D}] in the operands' type or float32, "
                              f"got {tuple(w.shape)} {w.dtype}")
-    given = [w for w in (wq, wk) if w is not None]
-    dtype = x.dtype if all(w.dtype == x.dtype for w in given) else torch.float32
-    aligned = [None if w is None else w.to(dtype).contiguous() for w in (wq, wk)]
-    aligned = [w.clone() if w is not None and w.data_ptr() % 16 else w for w in aligned]
-    return aligned[0], aligned[1], nat.dtype_code(dtype)
+        if w.dtype != dtype:
+            dtype = torch.float32
+
+    def as_read(w):
+        if w is None or w.dtype == dtype and w.is_contiguous() and not w.data_ptr() % 16:
+            return w
+        return torch.empty(D, device=w.device, dtype=dtype).copy_(w.detach())
+
+    return as_read(wq), as_read(wk), nat.dtype_code(dtype)
 
 
 def _angle_table(op, freqs, B, S, D):
@@ -189,84 +206,127 @@ def _angle_table(op, freqs, B, S, D):
     if freqs.shape[-1] != D // 2 or freqs.dim() not in (2, 3) or freqs.shape[-2] != S or \
             (freqs.dim() == 3 and freqs.shape[0] not in (1, B)):
         raise ValueError(f"{op}: freqs must be [{S}, {D // 2}] or [{B}, {S}, {D // 2}], got {tuple(freqs.shape)}")
-    f = freqs.to(torch.float32).contiguous()
-    return f, (S * (D // 2) if f.dim() == 3 and f.shape[0] == B and B > 1 else 0)
+    if freqs.dtype != torch.float32 or not freqs.is_contiguous():
+        freqs = freqs.to(torch.float32).contiguous()
+    return freqs, (S * (D // 2) if freqs.dim() == 3 and B > 1 and freqs.shape[0] == B else 0)
 
 
 def _qk_shapes(op, q, k):
-    given = [x for x in (q, k) if x is not None]
-    if not given:
+    x = q if q is not None else k
+    if x is None:
         raise ValueError(f"{op}: neither q nor k")
-    for x in given:
-        if x.dim() != 4:
-            raise ValueError(f"{op}: q and k must be [B, S, H, D], got {tuple(x.shape)}")
-    B, S, _, D = given[0].shape
-    if len(given) == 2 and (k.shape[0], k.shape[1], k.shape[3]) != (B, S, D):
-        raise ValueError(f"{op}: q {tuple(q.shape)} and k {tuple(k.shape)} differ in more than their heads")
-    if len(given) == 2 and q.dtype != k.dtype:
-        raise ValueError(f"{op}: q is {q.dtype} and k {k.dtype}")
+    if x.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError(f"{op}: q and k must be [B, S, H, D], got {tuple(x.shape if x.dim() != 4 else k.shape)}")
+    B, S, H, D = x.shape
+    if q is None:
+        Hq, Hk = 0, H
+    elif k is None:
+        Hq, Hk = H, 0
+    else:
+        Bk, Sk, Hk, Dk = k.shape
+        Hq = H
+        if Bk != B or Sk != S or Dk != D:
+            raise ValueError(f"{op}: q {tuple(q.shape)} and k {tuple(k.shape)} differ in more than their heads")
+        if q.dtype != k.dtype:
+            raise ValueError(f"{op}: q is {q.dtype} and k {k.dtype}")
     if D not in HEAD_DIMS:
         raise NotImplementedError(f"{op}: head dim {D} is not one of {HEAD_DIMS}")
-    return B, S, 0 if q is None else q.shape[2], 0 if k is None else k.shape[2], D
+    return x, B, S, Hq, Hk, D
+
+
+_NOTHING = (None, None)
+
+
+class _QkCall:
+    """What forward and backward of one call share, besides its operands: sizes, the weights and the
+    angles as the kernels take them."""
+
+    __slots__ = ("device", "code", "B", "S", "Hq", "Hk", "D", "wq", "wk", "wcode", "freqs", "freqs_b", "eps")
+
+
+def _qk_forward(call, q, tq, k, tk):
+    """The launch: (q', tq', k', tk') and q and k as they were read."""
+    q, sq = _NOTHING if q is None else readable_rows(q)
+    k, sk = _NOTHING if k is None else readable_rows(k)
+    tq, stq = _NOTHING if tq is None else readable_rows(tq)
+    tk, stk = _NOTHING if tk is None else readable_rows(tk)
+    dev = call.device
+    oq, otq, ok, otk = (None if t is None else torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, tq, k, tk))
+    with nat.on_device(dev):
+        nat.check(nat.lib().dmad_qk_norm_rope(
+            call.code, call.wcode, call.B, call.S, call.Hq, call.Hk, call.D, nat.ptr(q), nat.ptr(tq), nat.ptr(k),
+            nat.ptr(tk), sq, stq, sk, stk, nat.ptr(call.wq), nat.ptr(call.wk), nat.ptr(call.freqs), call.freqs_b,
+            call.eps, nat.ptr(oq), nat.ptr(otq), nat.ptr(ok), nat.ptr(otk), nat.stream_ptr(dev)))
+    return oq, otq, ok, otk, q, k
 
 
 class _QkNormRope(torch.autograd.Function):
-    """(q, tq, k, tk, wq, wk, freqs, eps) -> (q', tq', k', tk'); gradients of the primal outputs."""
+    """(call, q, tq, k, tk, wq, wk) -> (q', tq', k', tk'); gradients of the primal outputs."""
 
     @staticmethod
-    def forward(ctx, q, tq, k, tk, wq, wk, freqs, eps):
-        op = "qk_norm_rope_with_tangent"
-        B, S, Hq, Hk, D = _qk_shapes(op, q, k)
-        x = q if q is not None else k
-        cq, ck, wcode = _norm_weights(op, x, D, wq, wk)
-        f, fb = _angle_table(op, freqs, B, S, D)
-        ops, outs = [], []
-        for t in (q, tq, k, tk):
-            ops.append((None, None) if t is None else readable_rows(t))
-            outs.append(None if t is None else torch.empty(t.shape, device=t.device, dtype=t.dtype))
-        with nat.on_device(x.device):
-            nat.check(nat.lib().dmad_qk_norm_rope(
-                nat.dtype_code(x.dtype), wcode, B, S, Hq, Hk, D, *(nat.ptr(t) for t, _ in ops), *(s for _, s in ops),
-                nat.ptr(cq), nat.ptr(ck), nat.ptr(f), fb, float(eps), *(nat.ptr(t) for t in outs),
-                nat.stream_ptr(x.device)))
-        ctx.save_for_backward(q, k, wq, wk, freqs)
-        ctx.eps = float(eps)
+    def forward(ctx, call, q, tq, k, tk, wq, wk):
+        oq, otq, ok, otk, q, k = _qk_forward(call, q, tq, k, tk)
+        ctx.save_for_backward(q, k, wq, wk, call.freqs)
+        ctx.call = call
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*(t for t in (outs[1], outs[3]) if t is not None))
-        return tuple(outs)
+        if tq is not None or tk is not None:
+            ctx.mark_non_differentiable(*(t for t in (otq, otk) if t is not None))
+        return oq, otq, ok, otk
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gq, _gtq, gk, _gtk):
-        q, k, wq, wk, freqs = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        # an output whose gradient did not arrive adds nothing
-        q, k = (q if gq is not None else None), (k if gk is not None else None)
-        if q is None and k is None:
-            return (None,) * 8
-        op = "qk_norm_rope_with_tangent"
-        B, S, Hq, Hk, D = _qk_shapes(op, q, k)
-        x = q if q is not None else k
-        cq, ck, wcode = _norm_weights(op, x, D, wq, wk)
-        f, fb = _angle_table(op, freqs, B, S, D)
-        grads = [None if g is None else g.to(x.dtype) for g in (gq, gk)]
-        ops = [(None, None) if t is None else readable_rows(t) for t in (q, grads[0], k, grads[1])]
-        dx = [None if t is None else torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k)]
-        dw = [torch.empty_like(w) if w is not None and t is not None and need[i] else None
-              for w, t, i in ((cq, q, 4), (ck, k, 5))]
-        if x.numel() == 0:
-            dw = [None if w is None else w.zero_() for w in dw]
-        else:
-            size = nat.qk_norm_rope_bwd_workspace_bytes(B, S, Hq, Hk, D) if any(w is not None for w in dw) else 0
-            ws_ptr, ws_size, ws = nat.workspace(size, x.device)
-            with nat.on_device(x.device):
-                nat.check(nat.lib().dmad_qk_norm_rope_bwd(
-                    nat.dtype_code(x.dtype), wcode, B, S, Hq, Hk, D, *(nat.ptr(t) for t, _ in ops),
-                    *(s for _, s in ops), nat.ptr(cq if q is not None else None),
-                    nat.ptr(ck if k is not None else None), nat.ptr(f), fb, ctx.eps,
-                    *(nat.ptr(t) for t in dx), *(nat.ptr(t) for t in dw), ws_ptr, ws_size, nat.stream_ptr(x.device)))
-        dw = [None if g is None else g.to(w.dtype) for g, w in zip(dw, (wq, wk))]
-        return dx[0], None, dx[1], None, dw[0], dw[1], None, None
+        # a backward that is itself recorded (create_graph) must refuse to be differentiated
+        if torch.is_grad_enabled():
+            return _qk_backward_once(ctx, gq, gk)
+        return _qk_backward(ctx, gq, gk)
+
+
+def _qk_backward(ctx, gq, gk):
+    q, k, wq, wk, _ = ctx.saved_tensors  # unpacked, so that a change in place is noticed
+    call, need = ctx.call, ctx.needs_input_grad
+    cq, ck, Hq, Hk, dev = call.wq, call.wk, call.Hq, call.Hk, call.device
+    sq = sgq = sk = sgk = dq = dk = dwq = dwk = ws = ws_ptr = None
+    ws_size = 0
+    # an output whose gradient did not arrive adds nothing
+    if gq is not None:
+        q, sq = readable_rows(q)
+        gq, sgq = readable_rows(gq)
+        dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        if cq is not None and need[5]:
+            dwq = torch.empty_like(cq)
+    else:
+        q, cq, Hq = None, None, 0
+    if gk is not None:
+        k, sk = readable_rows(k)
+        gk, sgk = readable_rows(gk)
+        dk = torch.empty(k.shape, device=dev, dtype=k.dtype)
+        if ck is not None and need[6]:
+            dwk = torch.empty_like(ck)
+    else:
+        k, ck, Hk = None, None, 0
+    if gq is None and gk is None:
+        return (None,) * 7
+    if call.B * call.S == 0:
+        for dw in (dwq, dwk):
+            if dw is not None:
+                dw.zero_()
+    else:
+        if dwq is not None or dwk is not None:
+            ws_ptr, ws_size, ws = nat.workspace(
+                nat.qk_norm_rope_bwd_workspace_bytes(call.B, call.S, Hq, Hk, call.D), dev)
+        with nat.on_device(dev):
+            nat.check(nat.lib().dmad_qk_norm_rope_bwd(
+                call.code, call.wcode, call.B, call.S, Hq, Hk, call.D, nat.ptr(q), nat.ptr(gq), nat.ptr(k), nat.ptr(gk),
+                sq, sgq, sk, sgk, nat.ptr(cq), nat.ptr(ck), nat.ptr(call.freqs), call.freqs_b, call.eps, nat.ptr(dq),
+                nat.ptr(dk), nat.ptr(dwq), nat.ptr(dwk), ws_ptr, ws_size, nat.stream_ptr(dev)))
+    if dwq is not None and dwq.dtype != wq.dtype:
+        dwq = dwq.to(wq.dtype)
+    if dwk is not None and dwk.dtype != wk.dtype:
+        dwk = dwk.to(wk.dtype)
+    return None, dq, None, dk, None, dwq, dwk
+
+
+_qk_backward_once = torch.autograd.function.once_differentiable(_qk_backward)
 
 
 def qk_norm_rope_with_tangent(q_withT, k_withT, q_weight, k_weight, eps, freqs):
@@ -282,19 +342,30 @@ def qk_norm_rope_with_tangent(q_withT, k_withT, q_weight, k_weight, eps, freqs):
     ``tq``/``tk``: tangents, given for both or for neither; their outputs are detached. ``k_withT``
     (or ``q_withT``) may be ``(None, None)``: the other alone. A weight of None skips that norm,
     ``freqs`` None the rotation; freqs are [S, D/2], or [B, S, D/2] for angles per sequence.
-    Weights have the operands' type or float32. Differentiable in q, k and the weights.
+    Weights have the operands' type or float32. Differentiable (once) in q, k and the weights.
     """
     op = "qk_norm_rope_with_tangent"
     (q, tq), (k, tk) = q_withT, k_withT
     _check_same_device(op, q, tq, k, tk, q_weight, k_weight, freqs)
-    _qk_shapes(op, q, k)
-    nat.dtype_code((q if q is not None else k).dtype)
-    if not eps >= 0:
+    call = _QkCall()
+    x, call.B, call.S, call.Hq, call.Hk, call.D = _qk_shapes(op, q, k)
+    call.code, call.device = nat.dtype_code(x.dtype), x.device
+    call.eps = float(eps)
+    if not call.eps >= 0:
         raise ValueError(f"{op}: eps must be non-negative, got {eps}")
-    for x, t in ((q, tq), (k, tk)):
-        if t is not None and (x is None or t.shape != x.shape or t.dtype != x.dtype):
-            raise ValueError(f"{op}: a tangent has its operand's shape and type")
-    if (tq is not None or tk is not None) and any(x is not None and t is None for x, t in ((q, tq), (k, tk))):
-        raise ValueError(f"{op}: tangents of both q and k, or of neither")
-    q, tq, k, tk = _QkNormRope.apply(q, tq, k, tk, q_weight, k_weight, freqs, eps)
+    if tq is not None or tk is not None:
+        for y, t in ((q, tq), (k, tk)):
+            if (y is None) != (t is None):
+                raise ValueError(f"{op}: tangents of both q and k, or of neither")
+            if t is not None and (t.shape != y.shape or t.dtype != y.dtype):
+                raise ValueError(f"{op}: a tangent has its operand's shape and type")
+    if (q is None and q_weight is not None) or (k is None and k_weight is not None):
+        raise ValueError(f"{op}: a weight without its operand")
+    # the weights' gradients are the operator's own
+    call.wq, call.wk, call.wcode = _norm_weights(op, x, call.D, q_weight, k_weight)
+    call.freqs, call.freqs_b = _angle_table(op, freqs, call.B, call.S, call.D)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        q, tq, k, tk = _QkNormRope.apply(call, q, tq, k, tk, q_weight, k_weight)
+    else:
+        q, tq, k, tk = _qk_forward(call, q, tq, k, tk)[:4]
     return (q, tq), (k, tk)

@@ -47,7 +47,7 @@ int main() {
     std::vector<int32_t> table(B * (M + 1)), lengths(B), seen(B);
     KvPages kv{};
     kv.table = table.data(); kv.table_stride = M + 1; kv.lengths = lengths.data(); kv.seen = seen.data();
-    kv.num_pages = N; kv.heads = H; kv.P = P; kv.M = M; kv.B = B;
+    kv.num_pages = N; kv.heads = H; kv.B = B; kv.set_pages(P, M);
     kv.k_sp = kv.v_sp = H * P * 16; kv.k_sh = kv.v_sh = P * 16; kv.k_sl = kv.v_sl = 16;
     for (int id : ids) {
       for (auto& t : table) t = id;
@@ -78,9 +78,23 @@ int main() {
   // offsets beyond 32 bits
   KvPages big{};
   int32_t page = 70000;
-  big.table = &page; big.table_stride = 1; big.num_pages = 100000; big.heads = 8; big.P = 64; big.M = 1; big.B = 1;
+  big.table = &page; big.table_stride = 1; big.num_pages = 100000; big.heads = 8; big.B = 1; big.set_pages(64, 1);
   big.k_sp = big.v_sp = 8 * 64 * 128; big.k_sh = big.v_sh = 64 * 128; big.k_sl = big.v_sl = 128;
   if (big.k_offset(big.locate(0, 63), 7) != 70000LL * 65536 + 7 * 8192 + 63 * 128) return 10;
+  // the quotient by the page size, at its steps and at the largest slot
+  for (int P = 16; P <= 1 << 26; P += P < 4096 ? 16 : P % 32 ? 16 : P / 3 / 16 * 16) {
+    const int M = (1 << 26) / P;
+    std::vector<int32_t> pages(M);
+    for (int i = 0; i < M; ++i) pages[i] = i;
+    KvPages kv{};
+    kv.table = pages.data(); kv.num_pages = M; kv.B = 1; kv.set_pages(P, M);
+    for (int i = 0; i < M; i = i < 100 ? i + 1 : i + 1 + i / 7) {
+      const KvSlot a = kv.locate(0, i * P), z = kv.locate(0, i * P + P - 1);
+      if (a.page != i || a.slot != 0 || z.page != i || z.slot != P - 1) return 11;
+      ++checked;
+    }
+    if (kv.locate(0, M * P - 1).page != M - 1) return 12;
+  }
   printf("%ld\n", checked);
   return 0;
 }

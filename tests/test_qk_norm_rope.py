@@ -235,6 +235,24 @@ def test_one_operand_and_partial_gradients(gpu):
 
 
 @pytest.mark.gpu
+def test_no_second_derivative(gpu):
+    """A gradient taken with create_graph is right, and differentiating it raises instead of giving zero."""
+    from dmad_amd import qk_norm_rope_with_tangent
+
+    x = torch.randn(1, 4, 2, 32, device=gpu, requires_grad=True)
+    w, f = torch.ones(32, device=gpu), torch.rand(4, 16, device=gpu)
+
+    def grad(create_graph):
+        (y, _), _ = qk_norm_rope_with_tangent((x, None), (None, None), w, None, 1e-6, f)
+        return torch.autograd.grad(y.square().sum() + y.sum(), x, create_graph=create_graph)[0]
+
+    g = grad(True)
+    assert torch.equal(g.detach(), grad(False))
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        g.sum().backward()
+
+
+@pytest.mark.gpu
 def test_broadcast_and_unaligned_inputs(gpu):
     """An expanded operand is read in place and its gradient summed; rows that start unaligned are copied."""
     from dmad_amd import qk_norm_rope_with_tangent
