@@ -1306,6 +1306,8 @@ int check_cache(int dtype, const dmad_kv_cache* c, dmad::KvPages& kv) {
     return fail(DMAD_ERR_INVALID, "cache page_table: rows overlap");
   if ((c->weight == nullptr) != (c->position == nullptr))
     return fail(DMAD_ERR_INVALID, "cache weight and position must be both set or both null");
+  if ((((uintptr_t)c->weight | (uintptr_t)c->position) & 15) != 0)
+    return fail(DMAD_ERR_INVALID, "cache weight and position must be 16-byte aligned");
   kv.k = c->k_pages;
   kv.v = c->v_pages;
   kv.k_sp = c->k_strides[0]; kv.k_sh = c->k_strides[1]; kv.k_sl = c->k_strides[2];
@@ -1789,6 +1791,7 @@ int dmad_qk_norm_rope_append(int dtype, int wdtype, int64_t S, int64_t Hq, const
     return fail(DMAD_ERR_INVALID, "freqs: bad number of rows %lld", (long long)freqs_rows);
   p.freqs = freqs;
   p.freqs_rows = (int)(freqs != nullptr ? freqs_rows : 0);
+  dmad::qk_append_split(p);
   hipStream_t s = (hipStream_t)stream;
   mark(0, false, s);
   const hipError_t e = dmad::launch_qk_norm_rope(p, dtype, wdtype, dmad::QkMode::kAppend, s);

@@ -18,11 +18,12 @@ namespace dmad {
 
 constexpr int kSelectWaves = 16;
 constexpr int kSelectThreads = 64 * kSelectWaves;
-constexpr int kSelectBatch = 4;  // keys a lane reads together
-
+constexpr int kSelectRow = 4 * 64;  // slots a wave takes at a time, 4 neighbours per lane
 // Copies of the histogram, by lane: lanes that count one digit meet in a copy
 // four at a time, not 64.
 constexpr int kHistCopies = 16;
+
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 
 // Order of weights as unsigned keys: 1 .. 0xfffffffe, NaN above all of them;
 // 0xffffffff stays unconditionally and 0 goes first.
@@ -33,12 +34,14 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 // SLOTS > 0: keys stay in LDS (sequences of up to SLOTS slots); 0: in memory.
-template <int SLOTS>
+// LOADS: rows whose weights and positions a wave has on their way together.
+template <int SLOTS, int LOADS>
 __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams p) {
-  __shared__ uint32_t lds_keys[SLOTS > 0 ? SLOTS : 1];
+  static_assert(SLOTS % (kSelectRow * kSelectWaves) == 0, "whole rows for every wave");
+  __shared__ __attribute__((aligned(16))) uint32_t lds_keys[SLOTS > 0 ? SLOTS : 4];
   __shared__ uint32_t hist[256 * kHistCopies];
   __shared__ uint32_t total[256];
-  __shared__ uint32_t found[2];
+  __shared__ uint32_t found[3];
   __shared__ int before_eq[kSelectWaves], before_hole[kSelectWaves], before_move[kSelectWaves];
   const KvPages& kv = p.kv;
   const int h = (int)blockIdx.x % kv.heads, b = (int)blockIdx.x / kv.heads;
@@ -48,52 +51,60 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams
     if (threadIdx.x == 0) p.counts[blockIdx.x] = 0;
     return;
   }
-  // each wave has a range of slots, so that ranks in slot order need only its running counts
-  const int span = ((n + kSelectThreads - 1) / kSelectThreads) * 64;
+  // Each wave has a range of whole rows, so that ranks in slot order need only
+  // its running counts; a lane reads back only the keys it wrote. Slots from n
+  // on to the end of a row have key 0: with at least keep slots below them they
+  // are never among the ones that stay.
+  const int span = (n + kSelectRow * kSelectWaves - 1) / (kSelectRow * kSelectWaves) * kSelectRow;
   const int begin = min(n, wave * span), end = min(n, begin + span);
   uint32_t* keys = SLOTS > 0 ? lds_keys : p.keys + (int64_t)blockIdx.x * kv.capacity();
   const int oldest = kv.seen[b] - p.recent;
 
-  // Keys from weights and positions, LOADS slots of a lane under way together
-  // (the page ids, then what is there); a lane reads back only its own.
-  constexpr int LOADS = SLOTS == kSelectInLds / 8 ? 4 : 16;
-  for (int s0 = begin; s0 < end; s0 += 64 * LOADS) {
+  for (int row = begin; row < end; row += kSelectRow * LOADS) {
     KvSlot at[LOADS];
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
-      const int s = s0 + 64 * j + lane;
+      const int s = row + kSelectRow * j + 4 * lane;
       at[j] = KvSlot{-1, 0};
-      if (s < end) at[j] = kv.locate(b, s);
+      if (s < end) at[j] = kv.locate(b, s);  // 4 slots from a multiple of 4 lie on one page
     }
-    float w[LOADS];
-    int position[LOADS];
+    f32x4_t w[LOADS];
+    i32x4_t position[LOADS];
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
       if (at[j].page < 0) continue;
-      w[j] = kv.weight[kv.index(at[j], h)];
-      position[j] = kv.position[kv.index(at[j], h)];
+      const int64_t i = kv.index(at[j], h);
+      w[j] = *(const f32x4_t*)(kv.weight + i);
+      position[j] = *(const i32x4_t*)(kv.position + i);
     }
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
-      const int s = s0 + 64 * j + lane;
-      // slots of a missing page: none moves, none is moved to
-      uint32_t key = s < p.keep ? 0xffffffffu : 0u;
-      if (at[j].page >= 0) key = position[j] < p.sink || position[j] >= oldest ? 0xffffffffu : weight_key(w[j]);
-      if (s < end) keys[s] = key;
+      if (row + kSelectRow * j >= end) continue;
+      const int s = row + kSelectRow * j + 4 * lane;
+      u32x4_t key;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // slots of a missing page: none moves, none is moved to
+        key[e] = s + e < p.keep ? 0xffffffffu : 0u;
+        if (at[j].page >= 0 && s + e < n)
+          key[e] = position[j][e] < p.sink || position[j][e] >= oldest ? 0xffffffffu : weight_key(w[j][e]);
+      }
+      if (SLOTS > 0 || s < n) *(u32x4_t*)(keys + s) = key;
     }
   }
-  // f(slot, its key, whether there is one) for this wave's slots, 64 at a time in order
+  // f(row, the lane's first slot of it, its 4 keys) for this wave's rows in order
   auto each = [&](auto f) {
-    for (int s0 = begin; s0 < end; s0 += 64 * kSelectBatch) {
-      uint32_t key[kSelectBatch];
+    for (int row = begin; row < end; row += 4 * kSelectRow) {
+      u32x4_t key[4];
 #pragma unroll
-      for (int j = 0; j < kSelectBatch; ++j) {
-        const int s = s0 + 64 * j + lane;
-        key[j] = s < end ? keys[s] : 0u;
+      for (int j = 0; j < 4; ++j) {
+        const int s = row + kSelectRow * j + 4 * lane;
+        key[j] = u32x4_t{0, 0, 0, 0};
+        if (row + kSelectRow * j < end && (SLOTS > 0 || s < n)) key[j] = *(const u32x4_t*)(keys + s);
       }
 #pragma unroll
-      for (int j = 0; j < kSelectBatch; ++j)
-        if (s0 + 64 * j < end) f(s0 + 64 * j + lane, key[j], s0 + 64 * j + lane < end);  // the test is the wave's
+      for (int j = 0; j < 4; ++j)
+        if (row + kSelectRow * j < end) f(row + kSelectRow * j, row + kSelectRow * j + 4 * lane, key[j]);
     }
   };
 
@@ -103,8 +114,10 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams
   for (int shift = 24; shift >= 0; shift -= 8) {
     for (int i = threadIdx.x; i < 256 * kHistCopies; i += kSelectThreads) hist[i] = 0;
     __syncthreads();
-    each([&](int, uint32_t k, bool there) {
-      if (there && (k & mask) == prefix) atomicAdd(&hist[((k >> shift) & 255) * kHistCopies + (lane & (kHistCopies - 1))], 1u);
+    each([&](int, int, u32x4_t k) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if ((k[e] & mask) == prefix) atomicAdd(&hist[((k[e] >> shift) & 255) * kHistCopies + (lane & (kHistCopies - 1))], 1u);
     });
     __syncthreads();
     if (threadIdx.x < 256) {
@@ -131,6 +144,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams
           if (above < left && left <= above + d[k]) {
             found[0] = 255 - 4 * lane - k;
             found[1] = left - above;
+            found[2] = d[k];
           }
           above += d[k];
         }
@@ -141,29 +155,68 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams
     mask |= 255u << shift;
     left = found[1];
   }
+  const bool ties = left != found[2];  // only some of the equals stay: the first ones
 
-  // equals before each wave
+  // what a row's 4 votes per lane come to below this lane, and in all
   const uint64_t below = ((uint64_t)1 << lane) - 1;
-  int count = 0;
-  each([&](int, uint32_t k, bool there) { count += (int)__popcll(__ballot(there && k == prefix)); });
-  if (lane == 0) before_eq[wave] = count;
-  __syncthreads();
-  int eq0 = 0;
-  for (int w = 0; w < wave; ++w) eq0 += before_eq[w];
-
-  // whether a slot stays; eq runs over the equals
-  auto stays = [&](uint32_t k, bool there, int& eq) {
-    const bool equal = there && k == prefix;
-    const uint64_t votes = __ballot(equal);
-    const int rank = eq + (int)__popcll(votes & below);
-    eq += (int)__popcll(votes);
-    return there && (k > prefix || (equal && (uint32_t)rank < left));
+  struct Votes {
+    int before, all;
+  };
+  auto vote = [&](const bool (&x)[4]) {
+    Votes v{0, 0};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint64_t m = __ballot(x[e]);
+      v.before += (int)__popcll(m & below);
+      v.all += (int)__popcll(m);
+    }
+    return v;
+  };
+  int eq0 = 0;  // equals before this wave
+  if (ties) {
+    int count = 0;
+    each([&](int, int, u32x4_t k) {
+      const bool equal[4] = {k[0] == prefix, k[1] == prefix, k[2] == prefix, k[3] == prefix};
+      count += vote(equal).all;
+    });
+    if (lane == 0) before_eq[wave] = count;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) eq0 += before_eq[w];
+  }
+  // which of a lane's 4 slots stay; eq runs over the equals
+  auto stays = [&](u32x4_t k, int& eq, bool (&st)[4]) {
+    if (!ties) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st[e] = k[e] >= prefix;
+      return;
+    }
+    const bool equal[4] = {k[0] == prefix, k[1] == prefix, k[2] == prefix, k[3] == prefix};
+    const Votes v = vote(equal);
+    int rank = eq + v.before;
+    eq += v.all;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      st[e] = k[e] > prefix || (equal[e] && (uint32_t)rank < left);
+      rank += equal[e];
+    }
+  };
+  // which of them change: slots below keep that go, or beyond that stay
+  auto changes = [&](int s, const bool (&st)[4], bool hole, bool (&x)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = hole ? s + e < p.keep && !st[e] : s + e >= p.keep && st[e];
   };
   int holes = 0, moves = 0, eq = eq0;
-  each([&](int s, uint32_t k, bool there) {
-    const bool st = stays(k, there, eq);
-    holes += (int)__popcll(__ballot(s < p.keep && there && !st));
-    moves += (int)__popcll(__ballot(s >= p.keep && st));
+  each([&](int row, int s, u32x4_t k) {
+    bool st[4], x[4];
+    stays(k, eq, st);
+    if (row < p.keep) {
+      changes(s, st, true, x);
+      holes += vote(x).all;
+    }
+    if (row + kSelectRow > p.keep) {
+      changes(s, st, false, x);
+      moves += vote(x).all;
+    }
   });
   if (lane == 0) {
     before_hole[wave] = holes;
@@ -177,17 +230,29 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams
   }
   int32_t* to = p.moves + (int64_t)blockIdx.x * 2 * p.max_moves;
   int32_t* from = to + p.max_moves;
+  auto list = [&](int32_t* out, int& base, int s, const bool (&x)[4]) {
+    const Votes v = vote(x);
+    int at = base + v.before;
+    base += v.all;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // as many slots move as go below keep: min(keep, n - keep) at most
+      if (x[e] && at < p.max_moves) out[at] = s + e;
+      at += x[e];
+    }
+  };
   eq = eq0;
-  each([&](int s, uint32_t k, bool there) {
-    const bool st = stays(k, there, eq);
-    const bool hole = s < p.keep && there && !st, move = s >= p.keep && st;
-    const uint64_t hv = __ballot(hole), mv = __ballot(move);
-    // as many slots move as go below keep: min(keep, n - keep) at most
-    const int hi = hole0 + (int)__popcll(hv & below), mi = move0 + (int)__popcll(mv & below);
-    if (hole && hi < p.max_moves) to[hi] = s;
-    if (move && mi < p.max_moves) from[mi] = s;
-    hole0 += (int)__popcll(hv);
-    move0 += (int)__popcll(mv);
+  each([&](int row, int s, u32x4_t k) {
+    bool st[4], x[4];
+    stays(k, eq, st);
+    if (row < p.keep) {
+      changes(s, st, true, x);
+      list(to, hole0, s, x);
+    }
+    if (row + kSelectRow > p.keep) {
+      changes(s, st, false, x);
+      list(from, move0, s, x);
+    }
   });
   if (threadIdx.x == kSelectThreads - 1) p.counts[blockIdx.x] = min(move0, p.max_moves);
 }
@@ -227,9 +292,9 @@ static hipError_t move_launch(const KvEvictParams& p, hipStream_t s) {
 hipError_t launch_kv_evict(const KvEvictParams& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.kv.B * p.kv.heads)), block(kSelectThreads);
   const int slots = p.kv.M * p.kv.P;
-  if (slots <= kSelectInLds / 8) hipLaunchKernelGGL((kv_select_kernel<kSelectInLds / 8>), grid, block, 0, s, p);
-  else if (slots <= kSelectInLds) hipLaunchKernelGGL((kv_select_kernel<kSelectInLds>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((kv_select_kernel<0>), grid, block, 0, s, p);
+  if (slots <= kSelectInLds / 8) hipLaunchKernelGGL((kv_select_kernel<kSelectInLds / 8, 1>), grid, block, 0, s, p);
+  else if (slots <= kSelectInLds) hipLaunchKernelGGL((kv_select_kernel<kSelectInLds, 4>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((kv_select_kernel<0, 4>), grid, block, 0, s, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   switch (p.D) {

@@ -70,8 +70,8 @@ class PagedKVCache:
         if (weight is None) != (position is None):
             raise ValueError(f"{op}: weight and position together, or neither")
         for name, t, dtype in (("weight", weight, torch.float32), ("position", position, torch.int32)):
-            if t is not None and (t.shape != (N, Hk, P) or t.dtype != dtype or not t.is_contiguous()):
-                raise ValueError(f"{op}: {name} must be [{N}, {Hk}, {P}] {dtype}, contiguous")
+            if t is not None and (t.shape != (N, Hk, P) or t.dtype != dtype or not t.is_contiguous() or t.data_ptr() % 16):
+                raise ValueError(f"{op}: {name} must be [{N}, {Hk}, {P}] {dtype}, contiguous and 16-byte aligned")
 
         def strides(name, t):
             if t.stride(3) != 1 or t.data_ptr() % 16:

@@ -370,8 +370,8 @@ int dmad_qk_norm_rope_bwd(int dtype, int wdtype, int64_t B, int64_t S, int64_t H
  * one sequence.
  *   k_strides, v_strides: elements between pages, heads and slots; the head
  *           dim's is 1
- *   weight, position: [num_pages][kv_heads][page_size], or both null where
- *           nothing is accumulated or evicted
+ *   weight, position: [num_pages][kv_heads][page_size], 16-byte aligned, or
+ *           both null where nothing is accumulated or evicted
  * page_size: a multiple of 16. bf16 and fp16.
  */
 typedef struct dmad_kv_cache {

@@ -164,6 +164,8 @@ BAD_CACHES = [
     (dict(page_table=0), 1, "page_table"),
     (dict(table_stride=3), 1, "overlap"),
     (dict(weight=0), 1, "both"),
+    (dict(weight=4104), 1, "aligned"),
+    (dict(position=4100), 1, "aligned"),
 ]
 
 
@@ -307,6 +309,8 @@ ATTEND = [
     (70, 1, 2, 1, 64, "bf16", 16, [(7 * i) % 61 for i in range(70)], False, True),
     (1, 1, 2, 2, 128, "bf16", 16, [9001], False, True),
     (3, 3, 16, 1, 32, "bf16", 16, [2, 1500, 640], True, True),
+    (2, 1, 1, 1, 16, "bf16", 16, [9000, 700], False, True),
+    (130, 1, 1, 1, 16, "fp16", 16, [(37 * i) % 400 for i in range(130)], False, True),
 ]
 
 
@@ -497,6 +501,8 @@ EVICT = [
     (1, 2, 256, "fp16", 64, [1100], 1000, 100, 0),
     (2, 2, 64, "bf16", 16, [2500, 90], 77, 30, 47),
     (1, 1, 64, "bf16", 16, [5000], 4999, 0, 3),
+    (1, 2, 16, "bf16", 128, [36000], 20001, 77, 0),
+    (2, 1, 16, "bf16", 16, [4096, 4097], 4095, 0, 0),
 ]
 
 
@@ -519,12 +525,14 @@ def test_evict(gpu, B, Hk, D, dtype, page, lengths, keep, recent, sink):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("size", [300, 5000, 33100])
 @pytest.mark.parametrize("kind", ["equal", "zeros of both signs", "infinities and NaN", "all recent", "negative", "missing pages"])
-def test_evict_order(gpu, kind):
+def test_evict_order(gpu, kind, size):
+    """Ties, signs and what is not a number, for keys in a little and in much LDS and in memory."""
     from dmad_amd import evict_low_weight
 
-    print(f"case evict order {kind}", flush=True)
-    cache = _make(gpu, 2, 2, 64, torch.bfloat16, 16, [300, 211], seed=11)
+    print(f"case evict order {kind} {size}", flush=True)
+    cache = _make(gpu, 2, 1, 16, torch.bfloat16, 16, [size, 211], seed=11)
     g = torch.Generator().manual_seed(12)
     w = torch.rand(cache.weight.shape, generator=g)
     if kind == "equal":
@@ -543,8 +551,9 @@ def test_evict_order(gpu, kind):
         cache.page_table[0, 15] = cache.k_pages.shape[0]
         cache.page_table[1, 12] = -9
     c = st.cache_of(cache)
-    st.evict(c, 128, 16, 4)
-    evict_low_weight(cache, 128, recent=16, sink=4)
+    keep = 128 if size < 1000 else size // 2 + 9
+    st.evict(c, keep, 16, 4)
+    evict_low_weight(cache, keep, recent=16, sink=4)
     torch.cuda.synchronize()
     for n in st.FIELDS:
         _same(n, getattr(cache, n), c[n])
@@ -716,6 +725,7 @@ def test_refusals(gpu):
         (ValueError, dict(weight=None)),
         (ValueError, dict(weight=f[5].double())),
         (ValueError, dict(position=f[6][:, :1])),
+        (ValueError, dict(weight=torch.zeros(f[5].numel() + 1, device=gpu)[1:].view(f[5].shape))),
         (RuntimeError, dict(lengths=f[3].cpu())),
     ]:
         with pytest.raises(error):
