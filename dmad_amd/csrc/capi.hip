@@ -1720,6 +1720,7 @@ int dmad_qk_norm_rope(int dtype, int wdtype, int64_t B, int64_t S, int64_t Hq, i
   p.freqs_b = freqs_stride_b;
   hipStream_t s = (hipStream_t)stream;
   mark(0, false, s);
+  p.past_caches = dmad::qk_past_caches(4 * B * S * (Hq + Hk) * D * esz);
   const hipError_t e = dmad::launch_qk_norm_rope(p, dtype, wdtype, jvp ? dmad::QkMode::kTangent : dmad::QkMode::kPrimal, s);
   mark(0, true, s);
   if (e != hipSuccess) return fail(DMAD_ERR_HIP, "norm and rotation launch: %s", hipGetErrorString(e));
@@ -1767,6 +1768,7 @@ int dmad_qk_norm_rope_bwd(int dtype, int wdtype, int64_t B, int64_t S, int64_t H
   }
   hipStream_t s = (hipStream_t)stream;
   mark(0, false, s);
+  p.past_caches = dmad::qk_past_caches(3 * B * S * (Hq + Hk) * D * esz);
   const hipError_t e = dmad::launch_qk_norm_rope_bwd(p, dtype, wdtype, dwq, dwk, s);
   mark(0, true, s);
   if (e != hipSuccess) return fail(DMAD_ERR_HIP, "norm and rotation backward launch: %s", hipGetErrorString(e));

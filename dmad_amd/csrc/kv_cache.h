@@ -27,12 +27,15 @@ struct QkNormRopeParams {
   int passes, per_wave;    // passes per token, and per wave
   int64_t units;           // waves' worth of work: tokens * ceil(passes / per_wave)
   float eps;
+  bool past_caches;        // tangents, backward: more than the caches hold (qk_past_caches)
   bool by_sequence;        // append: a workgroup per sequence (qk_append_split)
   float* partial;          // backward: [blocks][2][D] sums of the weights' gradients
   KvPages kv;              // append
 };
 
 enum class QkMode { kPrimal, kTangent, kAppend };
+// Whether a call that reads and writes that many bytes does so past the caches.
+bool qk_past_caches(int64_t bytes);
 // Decides whether an append runs a workgroup per sequence, and cuts it so.
 void qk_append_split(QkNormRopeParams& p);
 hipError_t launch_qk_norm_rope(const QkNormRopeParams& p, int dtype, int wdtype, QkMode mode, hipStream_t s);

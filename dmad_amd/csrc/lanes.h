@@ -50,34 +50,50 @@ __device__ __forceinline__ float group_sum(float x) {
   return group_reduce<W, LaneAdd>(x);
 }
 
+// A vector load or store; NT: not to be kept in the caches.
+template <bool NT, typename V>
+__device__ __forceinline__ V load_vec(const void* p) {
+  if constexpr (NT) return __builtin_nontemporal_load((const V*)p);
+  else return *(const V*)p;
+}
+template <bool NT, typename V>
+__device__ __forceinline__ void store_vec(void* p, V v) {
+  if constexpr (NT) __builtin_nontemporal_store(v, (V*)p);
+  else *(V*)p = v;
+}
+
 // 8 consecutive elements of a row, as loaded (16 bytes, or 32 in fp32).
 template <typename T>
 struct Row8 {
   i32x4_t v;
-  __device__ __forceinline__ void load(const T* p) { v = *(const i32x4_t*)p; }
+  template <bool NT = false>
+  __device__ __forceinline__ void load(const T* p) { v = load_vec<NT, i32x4_t>(p); }
   __device__ __forceinline__ void zero() { v = i32x4_t{0, 0, 0, 0}; }
   __device__ __forceinline__ float get(int e) const {
     return Elem<T>::to_f32((uint16_t)(((uint32_t)v[e >> 1] >> ((e & 1) * 16)) & 0xffff));
   }
+  template <bool NT = false>
   __device__ __forceinline__ static void store(T* p, const float (&x)[8]) {
     i32x4_t o;
 #pragma unroll
     for (int k = 0; k < 4; ++k) o[k] = (int)Elem<T>::pack2(x[2 * k], x[2 * k + 1]);
-    *(i32x4_t*)p = o;
+    store_vec<NT>(p, o);
   }
 };
 template <>
 struct Row8<float> {
   f32x4_t lo, hi;
+  template <bool NT = false>
   __device__ __forceinline__ void load(const float* p) {
-    lo = *(const f32x4_t*)p;
-    hi = *(const f32x4_t*)(p + 4);
+    lo = load_vec<NT, f32x4_t>(p);
+    hi = load_vec<NT, f32x4_t>(p + 4);
   }
   __device__ __forceinline__ void zero() { lo = hi = f32x4_t{0.f, 0.f, 0.f, 0.f}; }
   __device__ __forceinline__ float get(int e) const { return e < 4 ? lo[e & 3] : hi[e & 3]; }
+  template <bool NT = false>
   __device__ __forceinline__ static void store(float* p, const float (&x)[8]) {
-    *(f32x4_t*)p = f32x4_t{x[0], x[1], x[2], x[3]};
-    *(f32x4_t*)(p + 4) = f32x4_t{x[4], x[5], x[6], x[7]};
+    store_vec<NT>(p, f32x4_t{x[0], x[1], x[2], x[3]});
+    store_vec<NT>(p + 4, f32x4_t{x[4], x[5], x[6], x[7]});
   }
 };
 

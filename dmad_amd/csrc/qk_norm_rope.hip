@@ -77,8 +77,8 @@ __device__ __forceinline__ int qk_operand(const QkNormRopeParams& p, int& pass) 
   return 2;
 }
 
-// One wave's rows.
-template <typename T, typename W, int D, QkMode MODE>
+// One wave's rows. NT: operands and results past the caches.
+template <typename T, typename W, int D, QkMode MODE, bool NT = false>
 __device__ __forceinline__ void qk_norm_rope_rows(const QkNormRopeParams& p, const QkUnit u) {
   constexpr int LPH = D / 8, HPP = 64 / LPH;
   constexpr bool JVP = MODE == QkMode::kTangent, APPEND = MODE == QkMode::kAppend;
@@ -121,8 +121,8 @@ __device__ __forceinline__ void qk_norm_rope_rows(const QkNormRopeParams& p, con
       x[j].zero();
       if constexpr (JVP) t[j].zero();
       if (h < o.H) {
-        x[j].load((const T*)o.x + u.b * o.xb + u.i * o.xs + h * o.xh + el);
-        if constexpr (JVP) t[j].load((const T*)o.t + u.b * o.tb + u.i * o.ts + h * o.th + el);
+        x[j].template load<NT>((const T*)o.x + u.b * o.xb + u.i * o.xs + h * o.xh + el);
+        if constexpr (JVP) t[j].template load<NT>((const T*)o.t + u.b * o.tb + u.i * o.ts + h * o.th + el);
       }
       if (o.w != nullptr) w[j].load((const W*)o.w + el);
     }
@@ -163,8 +163,8 @@ __device__ __forceinline__ void qk_norm_rope_rows(const QkNormRopeParams& p, con
       if (h >= o.H) continue;
       if (!APPEND || which == 0) {
         const int64_t out = (((int64_t)u.b * p.S + u.i) * o.H + h) * D + el;
-        Row8<T>::store((T*)o.out + out, y);
-        if constexpr (JVP) Row8<T>::store((T*)o.tout + out, ty);
+        Row8<T>::template store<NT>((T*)o.out + out, y);
+        if constexpr (JVP) Row8<T>::template store<NT>((T*)o.tout + out, ty);
       } else if constexpr (APPEND) {
         if (at.page < 0) continue;
         if (which == 1) {
@@ -181,10 +181,10 @@ __device__ __forceinline__ void qk_norm_rope_rows(const QkNormRopeParams& p, con
   }
 }
 
-template <typename T, typename W, int D, QkMode MODE>
+template <typename T, typename W, int D, QkMode MODE, bool NT>
 __global__ __launch_bounds__(64 * kQkWaves) void qk_norm_rope_kernel(QkNormRopeParams p) {
   const int64_t unit = (int64_t)blockIdx.x * kQkWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (unit < p.units) qk_norm_rope_rows<T, W, D, MODE>(p, qk_unit(p, unit));  // the whole wave
+  if (unit < p.units) qk_norm_rope_rows<T, W, D, MODE, NT>(p, qk_unit(p, unit));  // the whole wave
 }
 
 __device__ __forceinline__ void kv_advance(const KvPages& kv, int b, int S) {
@@ -216,7 +216,7 @@ __global__ void kv_advance_kernel(KvPages kv, int S) {
 // not change from call to call.
 constexpr int kQkBwdBlocks = 1024;
 
-template <typename T, typename W, int D>
+template <typename T, typename W, int D, bool NT>
 __global__ __launch_bounds__(64 * kQkWaves) void qk_norm_rope_bwd_kernel(QkNormRopeParams p) {
   constexpr int LPH = D / 8, HPP = 64 / LPH;
   __shared__ float sums[kQkWaves][2][D];
@@ -240,8 +240,8 @@ __global__ __launch_bounds__(64 * kQkWaves) void qk_norm_rope_bwd_kernel(QkNormR
         x[j].zero();
         g[j].zero();
         if (h < o.H) {
-          x[j].load((const T*)o.x + u.b * o.xb + u.i * o.xs + h * o.xh + el);
-          g[j].load((const T*)o.t + u.b * o.tb + u.i * o.ts + h * o.th + el);
+          x[j].template load<NT>((const T*)o.x + u.b * o.xb + u.i * o.xs + h * o.xh + el);
+          g[j].template load<NT>((const T*)o.t + u.b * o.tb + u.i * o.ts + h * o.th + el);
         }
         if (o.w != nullptr) w[j].load((const W*)o.w + el);
       }
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(64 * kQkWaves) void qk_norm_rope_bwd_kernel(QkNormR
 #pragma unroll
           for (int e = 0; e < 8; ++e) a[e] = r * fmaf(-(x[j].get(e) * r), m, a[e]);
         }
-        if (h < o.H) Row8<T>::store((T*)o.out + (((int64_t)u.b * p.S + u.i) * o.H + h) * D + el, a);
+        if (h < o.H) Row8<T>::template store<NT>((T*)o.out + (((int64_t)u.b * p.S + u.i) * o.H + h) * D + el, a);
       }
     }
   }
@@ -329,6 +329,15 @@ __global__ __launch_bounds__(1024) void qk_weight_grad_kernel(const float* parti
   if (strand == 0 && out != nullptr) out[c < D ? c : c - D] = (W)s;
 }
 
+// A backward pass or a forward with tangents that moves more than the 256 MB
+// memory-side cache holds goes past it (non-temporal loads and stores). A plain
+// forward does not: its results are read next by the attention, and its
+// operands again by the backward pass. Forward and backward together, none past
+// the cache -> backward only -> both: 201 MB of 1.3B queries and keys 194 ->
+// 187 -> 184 us, 671 MB of 14B 652 -> 627 -> 614 us, 168 MB of 256-wide heads
+// 170 -> 143 -> 155 us; with tangents 518 -> 499 us for 14B.
+bool qk_past_caches(int64_t bytes) { return bytes > (int64_t)256 << 20; }
+
 // A workgroup per sequence saves the launch that advances the lengths and is
 // slower where a wave takes more than two passes (48 passes: 8.1 us against
 // 6.7 us; 12: 5.8 against 6.8 us for 32 sequences).
@@ -350,16 +359,19 @@ int64_t qk_norm_rope_bwd_blocks(int64_t units) {
 template <typename T, typename W, int D>
 static hipError_t qk_launch_d(const QkNormRopeParams& p, QkMode mode, hipStream_t s) {
   const dim3 grid((unsigned)((p.units + kQkWaves - 1) / kQkWaves)), block(64 * kQkWaves);
-  if (mode == QkMode::kPrimal) hipLaunchKernelGGL((qk_norm_rope_kernel<T, W, D, QkMode::kPrimal>), grid, block, 0, s, p);
-  else if (mode == QkMode::kTangent) hipLaunchKernelGGL((qk_norm_rope_kernel<T, W, D, QkMode::kTangent>), grid, block, 0, s, p);
-  else if constexpr (sizeof(T) == 2) {
+  if (mode == QkMode::kPrimal) {
+    hipLaunchKernelGGL((qk_norm_rope_kernel<T, W, D, QkMode::kPrimal, false>), grid, block, 0, s, p);
+  } else if (mode == QkMode::kTangent) {
+    if (p.past_caches) hipLaunchKernelGGL((qk_norm_rope_kernel<T, W, D, QkMode::kTangent, true>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((qk_norm_rope_kernel<T, W, D, QkMode::kTangent, false>), grid, block, 0, s, p);
+  } else if constexpr (sizeof(T) == 2) {
     if (p.by_sequence) {
       const int64_t units = p.units / p.B;
       const unsigned waves = (unsigned)(units < kQkAppendWaves ? units : kQkAppendWaves);
       hipLaunchKernelGGL((kv_append_kernel<T, W, D>), dim3((unsigned)p.B), dim3(64 * waves), 0, s, p);
       return hipGetLastError();
     }
-    hipLaunchKernelGGL((qk_norm_rope_kernel<T, W, D, QkMode::kAppend>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((qk_norm_rope_kernel<T, W, D, QkMode::kAppend, false>), grid, block, 0, s, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kv_advance_kernel, dim3((unsigned)((p.B + 255) / 256)), dim3(256), 0, s, p.kv, p.S);
@@ -370,7 +382,8 @@ static hipError_t qk_launch_d(const QkNormRopeParams& p, QkMode mode, hipStream_
 template <typename T, typename W, int D>
 static hipError_t qk_launch_bwd_d(const QkNormRopeParams& p, void* dwq, void* dwk, hipStream_t s) {
   const int blocks = (int)qk_norm_rope_bwd_blocks(p.units);
-  hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, D>), dim3(blocks), dim3(64 * kQkWaves), 0, s, p);
+  if (p.past_caches) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, D, true>), dim3(blocks), dim3(64 * kQkWaves), 0, s, p);
+  else hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<T, W, D, false>), dim3(blocks), dim3(64 * kQkWaves), 0, s, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.partial == nullptr) return e;
   hipLaunchKernelGGL((qk_weight_grad_kernel<W>), dim3(2 * D / 16), dim3(1024), 0, s, p.partial, blocks, D, (W*)dwq, (W*)dwk);
