@@ -1357,7 +1357,7 @@ int paged_layout(const dmad_kv_cache* c, int64_t S, int64_t Hq, bool accumulate,
   const int64_t lim = (int64_t)1 << 31;
   if (S >= lim / Hq) return fail(DMAD_ERR_UNSUPPORTED, "too many query rows");
   w.R = S * (Hq / c->kv_heads);
-  const int64_t rows = dmad::paged_attn_rows((int)w.R);
+  const int64_t rows = dmad::paged_attn_rows((int)c->head_dim, (int)w.R);
   w.row_groups = (w.R + rows - 1) / rows;
   const int64_t cap = c->pages_per_seq * c->page_size;
   const int64_t tiles = cap > 0 ? (cap + dmad::kPagedTile - 1) / dmad::kPagedTile : 1;

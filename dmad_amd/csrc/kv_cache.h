@@ -63,8 +63,8 @@ struct PagedAttnParams {
   float* scores;           // [B][heads][R][M P], log2 domain; null: weights are not accumulated
   float* lse2;             // [B][heads][R], log2 domain (with scores)
 };
-// Rows of a workgroup of paged attention, of R rows per key head.
-int paged_attn_rows(int R);
+// Rows of a workgroup of paged attention at head dim D, of R rows per key head.
+int paged_attn_rows(int D, int R);
 // Its workgroups per CU that a launch aims at.
 int paged_attn_resident(int D);
 hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, int D, hipStream_t s);

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams
   const int span = (n + kSelectRow * kSelectWaves - 1) / (kSelectRow * kSelectWaves) * kSelectRow;
   const int begin = min(n, wave * span), end = min(n, begin + span);
   uint32_t* keys = SLOTS > 0 ? lds_keys : p.keys + (int64_t)blockIdx.x * kv.capacity();
-  const int oldest = kv.seen[b] - p.recent;
+  const int seen = kv.seen[b], oldest = seen < INT32_MIN + p.recent ? INT32_MIN : seen - p.recent;
 
   for (int row = begin; row < end; row += kSelectRow * LOADS) {
     KvSlot at[LOADS];

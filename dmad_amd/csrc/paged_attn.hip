@@ -132,6 +132,13 @@ __device__ __forceinline__ void store4(T* p, f32x4_t x) {
   *(u32x2_t*)p = u32x2_t{Elem<T>::pack2(x[0], x[1]), Elem<T>::pack2(x[2], x[3])};
 }
 
+// Whether one of two packed elements is infinite or not a number.
+template <typename T>
+__device__ __forceinline__ bool any_nonfinite(uint32_t w) {
+  constexpr uint32_t EXP = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+  return (w & EXP) == EXP || ((w >> 16) & EXP) == EXP;
+}
+
 template <int D>
 struct PagedCfg {
   static constexpr int KC = D >= 32 ? D / 32 : 1;   // 32-wide slices of a K row
@@ -162,7 +169,8 @@ __device__ __forceinline__ void load_v(const char* base, uint32_t off, uint32_t 
   }
 }
 
-template <typename T, int D, int NT, bool ACC>
+// CAUSAL: rows of different tokens see different slots.
+template <typename T, int D, int NT, bool ACC, bool CAUSAL>
 __global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged_attn_kernel(PagedAttnParams p) {
   using C = PagedCfg<D>;
   __shared__ float sm_o[kPagedWaves][16][C::OP];
@@ -189,7 +197,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged
   for (int t = 0; t < NT; ++t) {
     const int r = (rg * NT + t) * 16 + row;
     const int i = r / p.G, h = hk * p.G + r % p.G;
-    sees[t] = r < p.R ? (p.causal ? n - (p.S - 1 - i) : n) : 0;
+    sees[t] = r < p.R ? (CAUSAL ? n - (p.S - 1 - i) : n) : 0;
 #pragma unroll
     for (int c = 0; c < C::KC; ++c) {
       qf[t][c] = i32x4_t{0, 0, 0, 0};
@@ -198,7 +206,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged
     }
   }
   // slots below this are seen by every row
-  const int all_see = p.causal ? n - (p.S - 1) : n;
+  const int all_see = CAUSAL ? n - (p.S - 1) : n;
 
   const uint32_t koff = (uint32_t)(row * kv.k_sl + g * 8) * 2;
   uint32_t voff[4];
@@ -274,12 +282,19 @@ __global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged
     request_k(0);
     request_v(0);
   }
-  // One step; all but the last request the next one's K and V without a branch
-  // around them, so that each product waits for its own operand alone.
-  auto run_step = [&](int step, auto more) {
+  // Whether every row sees every slot of a step, and another step follows.
+  auto plain_step = [&](int step) {
+    return step + 1 < mine && first + (wave + kPagedWaves * step + 1) * kStep <= min(all_see, last) &&
+           half(step, 0).page >= 0 && half(step, 1).page >= 0;  // uniform
+  };
+  // One step. Those that need no mask, nearly all, request the next one's K and V
+  // without a branch around them, so that each product waits for its own
+  // operand alone; the others (EDGE) mask what is not there or not seen.
+  auto run_step = [&](int step, auto edge) {
+    constexpr bool EDGE = edge.value != 0;
     const int key0 = first + (wave + kPagedWaves * step) * kStep;
     const int page[2] = {half(step, 0).page, half(step, 1).page};
-    const bool whole = key0 + kStep <= min(all_see, last) && page[0] >= 0 && page[1] >= 0;  // uniform
+    const bool more = !EDGE || step + 1 < mine;
 
     f32x4_t s[NT][2];
 #pragma unroll
@@ -290,12 +305,13 @@ __global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged
 #pragma unroll
         for (int c = 0; c < C::KC; ++c) s[t][hh] = mfma16(kf[hh][c], qf[t][c], s[t][hh], T{});
       }
-    if constexpr (more.value) {
+    if (more) {
       if ((step & 31) == 31) look_up(step + 1);
       request_k(step + 1);
     }
 
-    if (!whole) {
+    bool hidden = false;  // an infinity or NaN in V that some row must not see
+    if constexpr (EDGE) {
       // slots beyond the sequence, this piece or the row's view, and of missing pages
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
@@ -310,8 +326,12 @@ __global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged
           if (!there) {
 #pragma unroll
             for (int k = 0; k < C::VD; ++k) vf[hh * 4 + v][k] = 0;
+          } else if (CAUSAL && key >= all_see) {
+#pragma unroll
+            for (int k = 0; k < C::VD; ++k) hidden |= any_nonfinite<T>(vf[hh * 4 + v][k]);
           }
         }
+      if constexpr (CAUSAL) hidden = __ballot(hidden) != 0;
     }
 
     i32x4_t pf[NT];
@@ -329,7 +349,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged
         if ((rg * NT + t) * 16 + row < p.R) {
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh)
-            if (key0 + hh * 16 < last) *(f32x4_t*)(score_row[t] + key0 + hh * 16) = s[t][hh];
+            if (!EDGE || key0 + hh * 16 < last) *(f32x4_t*)(score_row[t] + key0 + hh * 16) = s[t][hh];
         }
       }
       top = across32<LaneMax>(across16<LaneMax>(top));
@@ -355,19 +375,47 @@ __global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged
       for (int k = 0; k < 4; ++k) pf[t][k] = (int)Elem<T>::pack2(e[2 * k], e[2 * k + 1]);
     }
 
+    if (EDGE && CAUSAL && hidden) {
+      // Zero times such a value is NaN: token by token, with the slots it does
+      // not see zeroed in V, and only its own rows taking the result.
+      for (int i = 0; i < p.S; ++i) {
+        const int see = all_see + i;
+        bool any = false;
 #pragma unroll
-    for (int j = 0; j < C::VE; ++j) {
-      i32x4_t a;
+        for (int t = 0; t < NT; ++t) any |= sees[t] == see;
+        if (__ballot(any) == 0) continue;
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        a[k] = (int)__builtin_amdgcn_perm(vf[2 * k + 1][j >> 1], vf[2 * k][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
+        for (int j = 0; j < C::VE; ++j) {
+          auto seen = [&](int e) { return key0 + (e >> 2) * 16 + g * 4 + (e & 3) < see ? vf[e][j >> 1] : 0u; };
+          i32x4_t a;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) acc[t][j] = mfma16(a, pf[t], acc[t][j], T{});
+          for (int k = 0; k < 4; ++k)
+            a[k] = (int)__builtin_amdgcn_perm(seen(2 * k + 1), seen(2 * k), (j & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const f32x4_t o = mfma16(a, pf[t], acc[t][j], T{});
+            if (sees[t] == see) acc[t][j] = o;
+          }
+          __builtin_amdgcn_sched_barrier(0);  // one column of V at a time: few registers
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < C::VE; ++j) {
+        i32x4_t a;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          a[k] = (int)__builtin_amdgcn_perm(vf[2 * k + 1][j >> 1], vf[2 * k][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t][j] = mfma16(a, pf[t], acc[t][j], T{});
+      }
     }
-    if constexpr (more.value) request_v(step + 1);
+    if (more) request_v(step + 1);
   };
-  for (int step = 0; step + 1 < mine; ++step) run_step(step, IC<1>{});
-  if (mine > 0) run_step(mine - 1, IC<0>{});
+  for (int step = 0; step < mine; ++step) {
+    for (; plain_step(step); ++step) run_step(step, IC<0>{});
+    run_step(step, IC<1>{});
+  }
 
   // The waves' results joined through LDS, 16 rows at a time.
 #pragma unroll
@@ -510,26 +558,35 @@ __global__ __launch_bounds__(kPagedTile) void paged_weight_kernel(PagedAttnParam
 // Its workgroups: up to 32 per CU.
 constexpr int kPagedWeightGroups = 8192;
 
-// Two row tiles share one reading of K and V. Four (as many as the registers of
-// one wave per SIMD hold) were no faster up to 64 rows, whose two groups meet
-// in one L2: 67 us either way for 4 x 8 tokens of 8 query heads per key head.
-static int paged_row_tiles(int R) { return R <= 16 ? 1 : 2; }
-int paged_attn_rows(int R) { return 16 * paged_row_tiles(R); }
+// Two row tiles share one reading of K and V, where their registers allow (not
+// for 256-wide heads). Four were no faster up to 64 rows, whose two groups meet
+// in one L2: 67 us either way for 4 sequences of 8 tokens with 8 query heads
+// per key head.
+static int paged_row_tiles(int D, int R) { return R <= 16 || D == 256 ? 1 : 2; }
+int paged_attn_rows(int D, int R) { return 16 * paged_row_tiles(D, R); }
 // Workgroups per CU that the cut aims at. Four waves with 16 KiB of K and V on
 // their way each (128-wide heads) keep a CU's share of the memory busy: two or
 // three workgroups were 0-17% slower, for their starts and ends, and one of
 // 64-wide heads 6% slower than two.
 int paged_attn_resident(int D) { return D >= 128 ? 1 : 2; }
 
-template <typename T, int D, bool ACC>
-static hipError_t paged_launch(const PagedAttnParams& p, hipStream_t s) {
+template <typename T, int D, bool ACC, bool CAUSAL>
+static void paged_launch_rows(const PagedAttnParams& p, hipStream_t s) {
   const int work = (p.splits * p.kv.heads + 7) / 8 * 8;
   const dim3 grid((unsigned)(work * p.row_groups)), block(64 * kPagedWaves);
-  if (paged_row_tiles(p.R) == 1) {
-    hipLaunchKernelGGL((paged_attn_kernel<T, D, 1, ACC>), grid, block, 0, s, p);
-  } else {
-    hipLaunchKernelGGL((paged_attn_kernel<T, D, 2, ACC>), grid, block, 0, s, p);
+  if constexpr (D < 256) {
+    if (paged_row_tiles(D, p.R) == 2) {
+      hipLaunchKernelGGL((paged_attn_kernel<T, D, 2, ACC, CAUSAL>), grid, block, 0, s, p);
+      return;
+    }
   }
+  hipLaunchKernelGGL((paged_attn_kernel<T, D, 1, ACC, CAUSAL>), grid, block, 0, s, p);
+}
+
+template <typename T, int D, bool ACC>
+static hipError_t paged_launch(const PagedAttnParams& p, hipStream_t s) {
+  if (p.causal && p.S > 1) paged_launch_rows<T, D, ACC, true>(p, s);
+  else paged_launch_rows<T, D, ACC, false>(p, s);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (p.part_o != nullptr) {

@@ -200,8 +200,8 @@ def paged_attention(q, cache, sm_scale=None, causal=False, accumulate=False, ret
     h // (Hq // Hk). ``sm_scale`` defaults to D^-1/2. Every token sees all slots in use;
     with ``causal`` the S tokens are the last S slots (just appended, nothing evicted since) and
     each sees the slots up to its own. A token that sees no slot gets o = 0 and lse = -inf, and so
-    does one whose scores are all -inf. With ``causal``, an infinity or NaN in a new token's value
-    reaches the other new tokens of its sequence and key head.
+    does one whose scores are all -inf. What a slot that a token does not see holds, infinities and
+    NaN among it, does not reach the token.
 
     ``accumulate`` adds to ``cache.weight`` what each slot receives: its softmax weight summed over
     the S tokens and the query heads of its key head.

@@ -405,6 +405,51 @@ def test_attention_scores_of_any_size(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,S,Hq,dtype", [(64, 4, 8, "bf16"), (16, 3, 2, "fp16"), (128, 9, 8, "bf16"), (256, 2, 2, "fp16"), (32, 40, 2, "bf16")])
+def test_hidden_tokens_do_not_reach_earlier_ones(gpu, D, S, Hq, dtype):
+    """With causal, whatever the values (and keys) of later new tokens hold: a token that does not see them is as
+    if they were not there, one that sees an infinity or NaN is not finite."""
+    from dmad_amd import paged_attention
+
+    t = DTYPES[dtype]
+    for length in (S, 37 + S, 300 + S):
+        cache = _make(gpu, 1, 2, D, t, 16, [length], seed=D + length)
+        q = torch.randn(1, S, Hq, D, generator=torch.Generator().manual_seed(3)).to(t)
+        clean = paged_attention(q.to(gpu), cache, causal=True, return_lse=True)
+        _check_attention(clean, st.attend(st.cache_of(cache), q, causal=True), t, D)
+        for token in {1, S - 1}:
+            page, slot = st.locate(st.cache_of(cache), 0, length - S + token)
+            for name, value in (("v_pages", math.inf), ("v_pages", math.nan), ("k_pages", math.nan)):
+                pages = getattr(cache, name)
+                keep = pages[page, 0, slot].clone()
+                pages[page, 0, slot] = value
+                o = paged_attention(q.to(gpu), cache, causal=True)
+                half = Hq // 2  # the query heads of key head 0
+                assert torch.equal(o[:, :token], clean[0][:, :token]), (length, token, name)
+                assert torch.equal(o[:, :, half:], clean[0][:, :, half:]), (length, token, name)
+                assert not torch.isfinite(o[:, token:, :half]).any(), (length, token, name)
+                pages[page, 0, slot] = keep
+
+
+@pytest.mark.gpu
+def test_attention_reads_strided_queries(gpu):
+    """Queries as a slice of a projection's output, as a transpose and unaligned; keys in [N, P, H, D] storage."""
+    from dmad_amd import paged_attention
+
+    cache = _make(gpu, 2, 2, 64, torch.bfloat16, 32, [70, 200], seed=21, nhd=True)
+    g = torch.Generator().manual_seed(22)
+    qkv = torch.randn(2, 3, 8, 64, generator=g).to(torch.bfloat16).to(gpu)
+    want = paged_attention(qkv[:, :, :4].contiguous(), cache, causal=True)
+    assert torch.equal(paged_attention(qkv[:, :, :4], cache, causal=True), want)
+    assert torch.equal(paged_attention(qkv[:, :, :4].transpose(1, 2).contiguous().transpose(1, 2), cache, causal=True), want)
+    flat = torch.zeros(2 * 3 * 4 * 64 + 1, device=gpu, dtype=torch.bfloat16)
+    flat[1:] = qkv[:, :, :4].reshape(-1)
+    assert torch.equal(paged_attention(flat[1:].view(2, 3, 4, 64), cache, causal=True), want)
+    one = qkv[:, :1, :4].expand(2, 3, 4, 64)
+    assert torch.equal(paged_attention(one, cache), paged_attention(one.contiguous(), cache))
+
+
+@pytest.mark.gpu
 def test_attention_equals_the_dense_one(gpu):
     """Against the package's own dense attention over the same keys."""
     from dmad_amd import paged_attention, plain_attention
