@@ -6,8 +6,11 @@
 // over the slots j the row sees, in one pass with the running maximum and sum.
 // Optionally weight_j += sum_r p_j for every slot.
 //
-// Bound by reading K and V once. A wave takes 32 slots at a time and needs no
-// LDS and no barrier for them:
+// Bound by reading K and V once: 5.9-6.2 TB/s (a 4 GiB copy reaches 4.7, reads
+// and writes together): 112 us for one token over 40 heads of 32760 slots,
+// 1.33 ms for 4 tokens of 64 query heads over 16 sequences of about 125000
+// slots (8.2 GB). A wave takes 32 slots at a time and needs no LDS and no
+// barrier for them:
 //   * S^T = K Q^T on 16x16x32 MFMAs. K's rows go from memory straight into the
 //     A operand (lane = slot, 16 bytes of its row), Q^T stays in registers.
 //   * In the C layout a lane holds slots 4 g + v (g = lane / 16) of both 16-slot
@@ -18,14 +21,17 @@
 //     8 x D/16 block, and pairing its 16-bit halves (one v_perm per two
 //     elements) gives V^T's A operands. Column m of MFMA j is element
 //     m D/16 + j of the row, so a lane's results are D/16 neighbours.
-// The next step's K is requested when this step's scores are done, and V
-// when its products are.
+// The next step's K is requested when this step's scores are done, and V when
+// its products are. The arithmetic hides behind the bytes: 16 rows per key head
+// take 82 us where 4 take 72 (352 MB).
 //
 // Split: the launch has `splits` pieces of equal work for all sequences
 // together; the device finds from the lengths which tiles are whose, so ragged
-// batches load the chip evenly and a captured graph follows the lengths. A
-// sequence that lies in several pieces leaves (maximum, sum, O) of each in
-// float32 and a second kernel joins them in order; one that lies in a single
+// batches load the chip evenly and a captured graph follows the lengths (48
+// sequences of 1 to 16000 slots: 68 us against 74 with pieces that end where a
+// sequence does, 60 for equal lengths; the 16 sequences above 1.33 ms against
+// 1.59). A sequence that lies in several pieces leaves (maximum, sum, O) of each
+// in float32 and a second kernel joins them in order; one that lies in a single
 // piece is finished by the first kernel.
 #include "kv_cache.h"
 #include "lanes.h"
@@ -529,7 +535,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
 
 // weight_j += sum over the rows of exp2(score - lse2), a tile of slots at a time
 // and a slot per thread. The line of tiles is cut finer than for the attention:
-// short sequences follow one another through the same wait for every one.
+// short sequences follow one another through the same wait for every one (17
+// -> 10 us for 48 of them). In one launch with the joins, each row's lse found
+// again from the pieces, both took what they take one after the other.
 __global__ __launch_bounds__(kPagedTile) void paged_weight_kernel(PagedAttnParams p, int splits) {
   const KvPages& kv = p.kv;
   const int hk = (int)blockIdx.x % kv.heads;

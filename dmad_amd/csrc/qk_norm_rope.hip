@@ -15,7 +15,8 @@
 // A token's rows share their angles: a wave takes up to `per_wave` passes of
 // one token (q's heads, then k's, then v's), and its lanes share the sines and
 // cosines (D <= 128: one each). HBM-bound: 2 D bytes in and out per row and
-// tensor for about 60 vector instructions per 8 elements.
+// tensor for about 60 vector instructions per 8 elements. 14B with tangents,
+// 2.7 GB: 498 us, 5.4 TB/s; gradients of 1.3B, 604 MB: 103 us, 5.8 TB/s.
 #include "kv_cache.h"
 #include "lanes.h"
 

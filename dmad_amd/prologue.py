@@ -12,6 +12,8 @@ Linear output and its tangent, one write of the rotated pair), with the
 reference's rounding points. ``apply_rope_with_tangent`` is the rotation alone
 (the reference function of that name), with a backward: the rotation's
 transpose is the rotation by the negated angles, run on the same kernel.
+``qk_norm_rope_with_tangent`` is the norm per head of queries and keys with the
+rotation in the same pass, tangents and a backward (no counterpart there).
 Device work only: tensors off the GPU raise.
 """
 from __future__ import annotations
