@@ -3,6 +3,7 @@
 // allocation-free backward uses this file's static device array `scratch`.
 #include <cstdarg>
 #include <cstdio>
+#include <limits>
 #include <mutex>
 #include <string>
 
@@ -1819,7 +1820,9 @@ int dmad_paged_attn(int dtype, const dmad_kv_cache* cache, int64_t S, int64_t Hq
   dmad::PagedAttnParams p{};
   int rc = check_cache(dtype, cache, p.kv);
   if (rc != DMAD_OK) return rc;
-  if (!(sm_scale > 0.f)) return fail(DMAD_ERR_UNSUPPORTED, "sm_scale must be positive");
+  const float scale_log2 = sm_scale * 1.4426950408889634f;
+  if (!(sm_scale > 0.f && scale_log2 <= std::numeric_limits<float>::max()))
+    return fail(DMAD_ERR_UNSUPPORTED, "sm_scale must be positive, and finite times log2(e)");
   PagedLayout w;
   if ((rc = paged_layout(cache, S, Hq, accumulate != 0, w)) != DMAD_OK) return rc;
   if (accumulate && cache->weight == nullptr) return fail(DMAD_ERR_INVALID, "the cache has no weights to accumulate");
@@ -1840,7 +1843,7 @@ int dmad_paged_attn(int dtype, const dmad_kv_cache* cache, int64_t S, int64_t Hq
   p.row_groups = (int)w.row_groups;
   p.causal = causal != 0;
   p.splits = (int)w.splits;
-  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   if (w.part_ml > w.part_o) {
     p.part_o = (float*)(ws + w.part_o);
     p.part_ml = (float*)(ws + w.part_ml);

@@ -204,6 +204,8 @@ def test_c_entries_reject_bad_arguments():
     assert attn(Hq=3) == 1 and attn(Hq=0) == 1 and attn(S=-1) == 1
     assert attn(q=0) == 1 and attn(q=264) == 1 and attn(o=0) == 1 and attn(o=8) == 1
     assert attn(scale=0.0) == 2 and attn(scale=-1.0) == 2 and attn(scale=math.nan) == 2
+    # finite in 64 bits, not in 32; and so near the largest that log2(e) times it is not
+    assert attn(scale=1e39) == 2 and attn(scale=3e38) == 2 and attn(scale=1e-50) == 2
     assert attn(cache=bare, acc=1) == 1
     assert attn(acc=1, ws=0) == 3 and attn(acc=1, size=64) == 3 and attn(acc=1, ws=272) == 3
     assert attn(S=1 << 28, Hq=64) == 2
@@ -795,6 +797,7 @@ def test_refusals(gpu):
         (RuntimeError, lambda: paged_attention(q.cpu(), ok)),
         (NotImplementedError, lambda: paged_attention(q, ok, sm_scale=0.0)),
         (NotImplementedError, lambda: paged_attention(q, ok, sm_scale=math.nan)),
+        (NotImplementedError, lambda: paged_attention(q, ok, sm_scale=1e39)),
         (ValueError, lambda: paged_attention(q, bare, accumulate=True)),
         (RuntimeError, lambda: paged_attention(q.clone().requires_grad_(True), ok)),
         (ValueError, lambda: append_kv(k, None, ok)),
