@@ -63,7 +63,9 @@ __device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readl
 // of that line, whatever sequences they belong to: equal work for every
 // workgroup of a ragged batch. A piece's part of a sequence is a segment; with
 // the pieces and the sequences both in order, x + b numbers the segments
-// without a clash.
+// without a clash. Every read of a length may find another value where a caller
+// writes them meanwhile: pieces and sequences are kept in range whatever the
+// lengths were, so that such a call gives wrong results and nothing worse.
 __device__ __forceinline__ int paged_tiles(int n) { return max(1, (n + kPagedTile - 1) / kPagedTile); }
 
 // Lengths of all sequences, a lane each; the first 64 are read once.
@@ -88,7 +90,8 @@ struct PagedRun {
 __device__ __forceinline__ PagedRun run_of_tile(const PagedLengths& len, int tile) {
   int before = 0;
   for (int b0 = 0; b0 < len.kv.B; b0 += 64) {
-    const int n = len.at(b0), end = before + wave_scan(len.tiles(b0));
+    // one reading: a tile is never before its sequence's first
+    const int n = len.at(b0), end = before + wave_scan(b0 + len.lane < len.kv.B ? paged_tiles(n) : 0);
     const uint64_t past = __ballot(end > tile);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
@@ -116,12 +119,14 @@ struct PagedPiece {
     tile = x * chunk;
     stop = min(total, tile + chunk);
     if (tile < stop) run = run_of_tile(len, tile);
+    if (run.b >= kv.B) stop = tile;
     end = min(stop, run.base + paged_tiles(run.n));
   }
   __device__ __forceinline__ bool done() const { return tile >= stop; }
   __device__ __forceinline__ bool last() const { return end >= stop; }
   __device__ __forceinline__ void next() {
     tile = end;
+    if (run.b + 1 >= kv.B) stop = tile;
     if (done()) return;
     run = PagedRun{run.b + 1, kv.length(run.b + 1), run.base + paged_tiles(run.n)};
     end = min(stop, run.base + paged_tiles(run.n));
@@ -491,7 +496,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
   const PagedLengths len(kv, lane_id());
   const int chunk = max(1, (len.total() + p.splits - 1) / p.splits);
   const PagedRun run = run_of_sequence(len, b);
-  const int first = run.base / chunk, last = (run.base + paged_tiles(run.n) - 1) / chunk;  // pieces
+  const int first = run.base / chunk, last = min((run.base + paged_tiles(run.n) - 1) / chunk, p.splits - 1);  // pieces
   if (first == last) return;  // finished
   const int strand = threadIdx.x / LANES, d = (threadIdx.x % LANES) * 4;
   float m = -__builtin_inff(), l = 0.f;

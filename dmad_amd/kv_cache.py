@@ -43,7 +43,9 @@ class PagedKVCache:
     The tensors are used in place and stay the caller's: pages are handed out, shared or dropped
     by writing to ``page_table`` and ``lengths``. A page may appear in several sequences as long
     as it is only read; pages that are appended to, evicted from or whose weights are accumulated
-    belong to one sequence.
+    belong to one sequence. Calls that only read a cache may run on several streams at once; one
+    that appends, accumulates or evicts is ordered by the caller against all others, as with any
+    tensor changed in place.
     """
 
     def __init__(self, k_pages, v_pages, page_table, lengths, seen, weight=None, position=None):
@@ -204,7 +206,8 @@ def paged_attention(q, cache, sm_scale=None, causal=False, accumulate=False, ret
     NaN among it, does not reach the token.
 
     ``accumulate`` adds to ``cache.weight`` what each slot receives: its softmax weight summed over
-    the S tokens and the query heads of its key head.
+    the S tokens and the query heads of its key head. It takes scratch of 4 bytes per query row and
+    slot of the cache's whole capacity.
     """
     op = "paged_attention"
     _check_new(op, cache, ("q", q))

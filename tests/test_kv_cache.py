@@ -452,6 +452,41 @@ def test_attention_reads_strided_queries(gpu):
 
 
 @pytest.mark.gpu
+def test_shared_pages_on_two_streams(gpu):
+    """Sequences that begin with the same pages, read by two calls at once on two streams and by one after
+    another: the same results, those of sequences with pages of their own."""
+    from dmad_amd import PagedKVCache, paged_attention
+
+    Hq, Hk, D, dtype = 8, 2, 128, torch.bfloat16
+    lengths = [700, 640, 1300, 16]
+    own = _make(gpu, 4, Hk, D, dtype, 16, lengths, seed=50)
+    table = own.page_table.clone()
+    table[1:3, :40] = table[0, :40]  # 640 slots in common
+    shared = PagedKVCache(own.k_pages, own.v_pages, table, own.lengths, own.seen)
+    g = torch.Generator().manual_seed(51)
+    qs = [torch.randn(4, S, Hq, D, generator=g).to(dtype) for S in (1, 3)]
+    calls = [dict(causal=False), dict(causal=True)]
+    dev = [q.to(gpu) for q in qs]
+    want = []
+    for q, x, kw in zip(qs, dev, calls):
+        want.append(paged_attention(x, shared, return_lse=True, **kw))
+        torch.cuda.synchronize()
+        _check_attention(want[-1], st.attend(st.cache_of(shared), q, causal=kw["causal"]), dtype, D)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(paged_attention(dev[i], shared, return_lse=True, **calls[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o, lse in got[i]:
+            assert torch.equal(o, want[i][0]) and torch.equal(lse, want[i][1])
+
+
+@pytest.mark.gpu
 def test_attention_equals_the_dense_one(gpu):
     """Against the package's own dense attention over the same keys."""
     from dmad_amd import paged_attention, plain_attention
