@@ -1390,7 +1390,7 @@ int64_t evict_moves(const dmad_kv_cache* c, int64_t keep) {
   return over <= 0 ? 0 : over < keep ? over : keep;
 }
 struct EvictLayout {
-  size_t keys, moves, counts, total;
+  size_t keys, moves, counts, ends, total;
 };
 EvictLayout evict_layout(const dmad_kv_cache* c, int64_t keep) {
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
@@ -1399,7 +1399,8 @@ EvictLayout evict_layout(const dmad_kv_cache* c, int64_t keep) {
   if (c->pages_per_seq * c->page_size <= keep) return w;  // nothing can be longer
   if (c->pages_per_seq * c->page_size > dmad::kSelectInLds) w.moves = up(BH * c->pages_per_seq * c->page_size * 4);
   w.counts = w.moves + up(BH * 2 * evict_moves(c, keep) * 4);
-  w.total = w.counts + up(BH * 4);
+  w.ends = w.counts + up(BH * 4);
+  w.total = w.ends + up((size_t)c->batch * 4);
   return w;
 }
 int evict_sizes(const dmad_kv_cache* c, int64_t keep) {
@@ -1889,6 +1890,7 @@ int dmad_kv_evict(int dtype, const dmad_kv_cache* cache, int64_t keep, int64_t r
   p.keys = (uint32_t*)(ws + w.keys);
   p.moves = (int32_t*)(ws + w.moves);
   p.counts = (int32_t*)(ws + w.counts);
+  p.ends = (int32_t*)(ws + w.ends);
   hipStream_t s = (hipStream_t)stream;
   mark(0, false, s);
   const hipError_t e = dmad::launch_kv_evict(p, s);

@@ -80,6 +80,7 @@ struct KvEvictParams {
   uint32_t* keys;      // [B][heads][M P], for more than kSelectInLds slots
   int32_t* moves;      // [B][heads][2][max_moves]: destination slots, source slots
   int32_t* counts;     // [B][heads] slots that move; 0 where nothing is evicted
+  int32_t* ends;       // [B] lengths afterwards
 };
 hipError_t launch_kv_evict(const KvEvictParams& p, hipStream_t s);
 

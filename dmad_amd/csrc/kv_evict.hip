@@ -2,11 +2,13 @@
 //
 // Per sequence of more than `keep` slots and per key head: the slots of the
 // first `sink` positions and of the last `recent` ones stay, then those of the
-// largest weight, equal ones by the lower slot, `keep` in all. The i-th slot
-// below `keep` that goes takes over the i-th slot at or beyond `keep` that
-// stays, in slot order; slots below `keep` that stay are not touched, so only
-// the rows that move are read and written. A slot from which a row moves is at
-// or beyond `keep` and one to which it moves below: the copies need no order.
+// largest weight, equal ones by the lower slot, `keep` in all. The sequence then
+// ends at slot E behind its keep-th slot: the i-th slot below E that goes takes
+// over the i-th slot at or beyond E that stays, in slot order; slots below E
+// that stay are not touched, so only the rows that move are read and written. A
+// slot from which a row moves is at or beyond E and one to which it moves
+// below: the copies need no order. Slots of missing pages are no slots here:
+// they neither count nor move, and E is `keep` where there are none.
 //
 // Selection is one workgroup per sequence and head: a radix search for the
 // keep-th largest key, 8 bits at a time with a histogram in LDS, then counts and
@@ -29,7 +31,7 @@ constexpr int kHistCopies = 16;
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 
 // Order of weights as unsigned keys: 1 .. 0xfffffffe, NaN above all of them;
-// 0xffffffff stays unconditionally and 0 goes first.
+// 0xffffffff stays unconditionally and 0 is a slot that is not there.
 __device__ __forceinline__ uint32_t weight_key(float w) {
   if (w != w) return 0xfffffffeu;
   const uint32_t u = __float_as_uint(w + 0.f);  // -0 as +0
@@ -45,24 +47,28 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams
   __shared__ uint32_t hist[256 * kHistCopies];
   __shared__ uint32_t total[256];
   __shared__ uint32_t found[3];
-  __shared__ int before_eq[kSelectWaves], before_hole[kSelectWaves], before_move[kSelectWaves];
+  __shared__ int before_held[kSelectWaves], before_eq[kSelectWaves], before_hole[kSelectWaves], before_move[kSelectWaves];
+  __shared__ int behind;
   const KvPages& kv = p.kv;
   const int h = (int)blockIdx.x % kv.heads, b = (int)blockIdx.x / kv.heads;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = kv.length(b);
-  if (n <= p.keep) {
+  // nothing goes: a uniform decision of the workgroup
+  auto leave_as_it_is = [&] {
     if (threadIdx.x == 0) p.counts[blockIdx.x] = 0;
-    return;
-  }
+    if (threadIdx.x == 0 && h == 0) p.ends[b] = n;
+  };
+  if (n <= p.keep) return leave_as_it_is();
   // Each wave has a range of whole rows, so that ranks in slot order need only
-  // its running counts; a lane reads back only the keys it wrote. Slots from n
-  // on to the end of a row have key 0: with at least keep slots below them they
-  // are never among the ones that stay.
+  // its running counts; a lane reads back only the keys it wrote. Slots of
+  // missing pages and those from n on to the end of a row have key 0: with more
+  // than keep other slots they are never among the ones that stay.
   const int span = (n + kSelectRow * kSelectWaves - 1) / (kSelectRow * kSelectWaves) * kSelectRow;
   const int begin = min(n, wave * span), end = min(n, begin + span);
   uint32_t* keys = SLOTS > 0 ? lds_keys : p.keys + (int64_t)blockIdx.x * kv.capacity();
   const int seen = kv.seen[b], oldest = seen < INT32_MIN + p.recent ? INT32_MIN : seen - p.recent;
 
+  int held = 0;  // slots of this lane that a page holds
   for (int row = begin; row < end; row += kSelectRow * LOADS) {
     KvSlot at[LOADS];
 #pragma unroll
@@ -87,10 +93,11 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams
       u32x4_t key;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        // slots of a missing page: none moves, none is moved to
-        key[e] = s + e < p.keep ? 0xffffffffu : 0u;
-        if (at[j].page >= 0 && s + e < n)
+        key[e] = 0u;
+        if (at[j].page >= 0 && s + e < n) {
           key[e] = position[j][e] < p.sink || position[j][e] >= oldest ? 0xffffffffu : weight_key(w[j][e]);
+          ++held;
+        }
       }
       if (SLOTS > 0 || s < n) *(u32x4_t*)(keys + s) = key;
     }
@@ -110,6 +117,18 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams
         if (row + kSelectRow * j < end) f(row + kSelectRow * j, row + kSelectRow * j + 4 * lane, key[j]);
     }
   };
+
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) held += __shfl_xor(held, m);
+  if (lane == 0) before_held[wave] = held;
+  __syncthreads();
+  int held0 = 0, held_all = 0;
+#pragma unroll
+  for (int w = 0; w < kSelectWaves; ++w) {
+    if (w < wave) held0 += before_held[w];
+    held_all += before_held[w];
+  }
+  if (held_all <= p.keep) return leave_as_it_is();
 
   // the keep-th largest key, and how many of its equals stay
   uint32_t prefix = 0, mask = 0;
@@ -175,6 +194,28 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams
     }
     return v;
   };
+  // where the sequence ends afterwards: behind its keep-th slot
+  int cut = p.keep;
+  if (held_all != n) {
+    if (held0 < p.keep && p.keep <= held0 + held) {  // in one wave's range
+      int rank = held0;
+      each([&](int, int s, u32x4_t k) {
+        const bool here[4] = {k[0] != 0, k[1] != 0, k[2] != 0, k[3] != 0};
+        const Votes v = vote(here);
+        int r = rank + v.before;
+        rank += v.all;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          r += here[e];
+          if (here[e] && r == p.keep) behind = s + e + 1;
+        }
+      });
+    }
+    __syncthreads();
+    cut = behind;
+  }
+  if (threadIdx.x == 0 && h == 0) p.ends[b] = cut;
+
   int eq0 = 0;  // equals before this wave
   if (ties) {
     int count = 0;
@@ -203,21 +244,21 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams
       rank += equal[e];
     }
   };
-  // which of them change: slots below keep that go, or beyond that stay
-  auto changes = [&](int s, const bool (&st)[4], bool hole, bool (&x)[4]) {
+  // which of them change: slots below the cut that go, or beyond that stay
+  auto changes = [&](int s, u32x4_t k, const bool (&st)[4], bool hole, bool (&x)[4]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = hole ? s + e < p.keep && !st[e] : s + e >= p.keep && st[e];
+    for (int e = 0; e < 4; ++e) x[e] = hole ? s + e < cut && k[e] != 0 && !st[e] : s + e >= cut && st[e];
   };
   int holes = 0, moves = 0, eq = eq0;
   each([&](int row, int s, u32x4_t k) {
     bool st[4], x[4];
     stays(k, eq, st);
-    if (row < p.keep) {
-      changes(s, st, true, x);
+    if (row < cut) {
+      changes(s, k, st, true, x);
       holes += vote(x).all;
     }
-    if (row + kSelectRow > p.keep) {
-      changes(s, st, false, x);
+    if (row + kSelectRow > cut) {
+      changes(s, k, st, false, x);
       moves += vote(x).all;
     }
   });
@@ -239,7 +280,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams
     base += v.all;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      // as many slots move as go below keep: min(keep, n - keep) at most
+      // as many slots move as go below the cut: at most keep, and at most those beyond it
       if (x[e] && at < p.max_moves) out[at] = s + e;
       at += x[e];
     }
@@ -248,12 +289,12 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(KvEvictParams
   each([&](int row, int s, u32x4_t k) {
     bool st[4], x[4];
     stays(k, eq, st);
-    if (row < p.keep) {
-      changes(s, st, true, x);
+    if (row < cut) {
+      changes(s, k, st, true, x);
       list(to, hole0, s, x);
     }
-    if (row + kSelectRow > p.keep) {
-      changes(s, st, false, x);
+    if (row + kSelectRow > cut) {
+      changes(s, k, st, false, x);
       list(from, move0, s, x);
     }
   });
@@ -267,7 +308,7 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvEvictParams p) {
   const KvPages& kv = p.kv;
   const int h = (int)blockIdx.y, b = (int)blockIdx.z;
   const int64_t bh = (int64_t)b * kv.heads + h;
-  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) kv.lengths[b] = min(kv.length(b), p.keep);
+  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) kv.lengths[b] = p.ends[b];
   const int i = (int)blockIdx.x * ROWS + (int)threadIdx.x / LANES, el = ((int)threadIdx.x % LANES) * 8;
   if (i >= p.counts[bh]) return;
   const KvSlot to = kv.locate(b, p.moves[bh * 2 * p.max_moves + i]);

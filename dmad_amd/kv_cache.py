@@ -237,11 +237,14 @@ def evict_low_weight(cache, keep, recent=0, sink=0):
     """Cuts every sequence of more than ``keep`` slots to ``keep``, in place, each key head by itself.
 
     Slots of the first ``sink`` positions and of the last ``recent`` ones (of ``cache.seen``) stay,
-    then those with the largest accumulated weight; of equal ones the lower slots. Slots below
-    ``keep`` that go are filled, in order, with those beyond that stay, with their weights and
+    then those with the largest accumulated weight; of equal ones the lower slots. A NaN weight
+    counts as the largest. The sequence then ends behind its ``keep``-th slot; slots before that
+    end that go are filled, in order, with those beyond that stay, with their weights and
     positions: slots are in no order of position afterwards, and a key head's slot holds another
-    token than another head's. Pages beyond ``keep`` slots are free then. A NaN weight counts as
-    the largest. Slots of missing pages stay below ``keep`` and go beyond it.
+    token than another head's. Pages beyond ``cache.lengths`` are free then. Slots of missing pages
+    hold nothing: they do not count towards ``keep`` and none is filled, so a window whose front
+    pages were dropped keeps ``keep`` of the slots it still has (``cache.lengths`` is then larger
+    than ``keep`` by the missing ones; without any it is ``keep``).
     """
     op = "evict_low_weight"
     if not isinstance(cache, PagedKVCache):

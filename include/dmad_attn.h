@@ -422,9 +422,10 @@ int dmad_kv_evict_workspace_bytes(const dmad_kv_cache* cache, int64_t keep, size
  * Cuts every sequence of more than `keep` slots to `keep`, each key head by
  * itself: slots of positions below `sink` and of the last `recent` positions
  * stay, then those of the largest weight (NaN above all, equal ones by the
- * lower slot). The i-th slot below `keep` that goes takes over the i-th slot
- * at or beyond `keep` that stays, with its weight and position.
- * sink + recent <= keep.
+ * lower slot). lengths becomes the slot behind the sequence's keep-th; the i-th
+ * slot below it that goes takes over the i-th slot at or beyond it that stays,
+ * with its weight and position. Slots of missing pages do not count and stay
+ * as they are: without any, lengths becomes `keep`. sink + recent <= keep.
  */
 int dmad_kv_evict(int dtype, const dmad_kv_cache* cache, int64_t keep, int64_t recent, int64_t sink, void* workspace,
                   size_t workspace_bytes, void* stream);

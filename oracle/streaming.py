@@ -121,28 +121,28 @@ def attend(c, q, scale=None, causal=False, accumulate=False):
 
 
 def evict(c, keep, recent=0, sink=0):
-    """Cuts the cache in place."""
+    """Cuts the cache in place. Only slots that a page holds count: the sequence then ends behind the
+    keep-th of them."""
     Hk = c["k_pages"].shape[1]
     for b in range(c["page_table"].shape[0]):
         n = length(c, b)
-        if n > keep:
+        held = [s for s in range(n) if locate(c, b, s) is not None]
+        end = n
+        if len(held) > keep:
+            end = held[keep - 1] + 1
             for h in range(Hk):
                 rank = []
-                for s in range(n):
+                for s in held:
                     at = locate(c, b, s)
-                    if at is None:
-                        first = 0 if s < keep else 3
-                        rank.append((first, 0.0, s))
-                        continue
                     w, p = float(c["weight"][at[0], h, at[1]]), int(c["position"][at[0], h, at[1]])
                     stays = p < sink or p >= int(c["seen"][b]) - recent
                     rank.append((0, 0.0, s) if stays else (1, 0.0, s) if math.isnan(w) else (2, -w, s))
                 kept = {s for _, _, s in sorted(rank)[:keep]}
-                holes = [s for s in range(keep) if s not in kept]
-                tail = [s for s in range(keep, n) if s in kept]
+                holes = [s for s in held if s < end and s not in kept]
+                tail = [s for s in held if s >= end and s in kept]
                 assert len(holes) == len(tail)
                 for to, source in zip(holes, tail):
                     (tp, ts), (fp, fs) = locate(c, b, to), locate(c, b, source)
                     for name in ("k_pages", "v_pages", "weight", "position"):
                         c[name][tp, h, ts] = c[name][fp, h, fs]
-        c["lengths"][b] = min(n, keep)
+        c["lengths"][b] = end

@@ -864,3 +864,72 @@ def test_refusals(gpu):
     none = PagedKVCache(f[0], f[1], f[2][:0], f[3][:0], f[4][:0])
     assert paged_attention(q[:0], none).shape == (0, 1, 4, 64)
     append_kv(k[:0], k[:0], none)
+
+
+# ---------------------------------------------------------------- windows: pages missing in front and between
+
+
+def test_oracle_eviction_of_a_window_by_hand():
+    """128 slots whose first 64 lie on dropped pages. 64 are there: cut to 64 nothing goes. Cut to 20 (a sink that
+    is no longer there, the last 16 positions, the heaviest of the rest) the sequence ends behind its 20th slot."""
+    def window():
+        c = dict(k_pages=torch.arange(128.0).view(8, 1, 16, 1).repeat(1, 1, 1, 16), v_pages=torch.zeros(8, 1, 16, 16),
+                 page_table=torch.arange(8, dtype=torch.int32).view(1, 8).clone(), lengths=torch.tensor([128]),
+                 seen=torch.tensor([128]), weight=torch.zeros(8, 1, 16), position=torch.arange(128).view(8, 1, 16).clone())
+        c["page_table"][0, :4] = -1
+        c["weight"].view(-1)[[70, 81, 90, 111]] = 2.0
+        return c
+
+    c, same = window(), window()
+    st.evict(c, 64, recent=16)
+    assert all(torch.equal(c[n], same[n]) for n in st.FIELDS)
+    st.evict(c, 20, recent=16, sink=4)
+    assert c["lengths"].tolist() == [84]
+    live = [at for s in range(84) if (at := st.locate(c, 0, s)) is not None]
+    held = [int(c["position"][p, 0, s]) for p, s in live]
+    assert sorted(held) == [70, 81, 90, 111, *range(112, 128)]
+    assert held[6] == 70 and held[17] == 81  # those that stay below the end have not moved
+    assert [float(c["k_pages"][p, 0, s, 0]) for p, s in live] == held
+
+
+WINDOW = [
+    # capacity in pages, length, missing entries, keep, recent, sink
+    (8, 128, [0, 1, 2, 3], 64, 16, 0),       # as many slots left as stay
+    (8, 128, [0, 1, 2, 3], 65, 16, 4),       # fewer left than stay
+    (8, 128, [0, 1, 2, 3], 48, 16, 0),
+    (8, 128, [0, 1, 2, 3, 4, 5, 6, 7], 5, 2, 1),
+    (8, 120, [0, 2, 5], 33, 8, 2),
+    (8, 117, [6, 7], 20, 20, 0),             # the newest pages are the ones missing
+    (40, 629, [*range(0, 20), 30], 100, 50, 3),
+    (400, 6301, [*range(0, 250), 251, 260, 399], 1000, 128, 4),  # keys in much LDS
+    (400, 6400, [*range(1, 398)], 20, 7, 9),
+    (2200, 35000, [*range(0, 1500), 1700], 3000, 64, 0),  # keys in memory
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pages,length,missing,keep,recent,sink", WINDOW)
+def test_evict_in_a_window(gpu, pages, length, missing, keep, recent, sink):
+    """Missing pages hold nothing, so they do not use up `keep`: the newest and heaviest of the slots that are
+    there stay, for a sequence beside one without missing pages."""
+    from dmad_amd import evict_low_weight, paged_attention
+
+    print(f"case evict window length={length} missing={len(missing)} keep={keep}", flush=True)
+    cache = _make(gpu, 2, 2, 16, torch.bfloat16, 16, [length, max(1, length - 9)], room=16 * pages - length, seed=keep)
+    assert cache.page_table.shape[1] == pages
+    cache.page_table[0, missing] = -1
+    for k, r, s in ((keep, recent, sink), (max(1, keep // 2), recent // 2, sink // 2)):
+        c = st.cache_of(cache)
+        there = [int(c["position"][p, 0, j]) for i in range(st.length(c, 0)) if (at := st.locate(c, 0, i)) for p, j in [at]]
+        st.evict(c, k, r, s)
+        evict_low_weight(cache, k, recent=r, sink=s)
+        torch.cuda.synchronize()
+        for n in st.FIELDS:
+            _same(n, getattr(cache, n), c[n])
+        live = [at for i in range(int(cache.lengths[0])) if (at := st.locate(c, 0, i)) is not None]
+        assert len(live) == min(k, len(there))
+        for h in range(2):
+            held = {int(c["position"][p, h, j]) for p, j in live}
+            assert held >= {t for t in there if t >= length - r or t < s}
+    if there:
+        assert torch.isfinite(paged_attention(torch.randn(2, 1, 2, 16, device=gpu).bfloat16(), cache, return_lse=True)[1]).all()
