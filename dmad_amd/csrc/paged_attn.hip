@@ -150,6 +150,18 @@ __device__ __forceinline__ bool any_nonfinite(uint32_t w) {
   return (w & EXP) == EXP || ((w >> 16) & EXP) == EXP;
 }
 
+// P = exp2(score - running maximum) <= 1 is rounded to the operand type for its
+// product with V alone (off by at most 2^-8 of each in bf16, 2^-11 in fp16; the sums of P stay
+// float32). In fp16 it goes in as 2^15 P and O is scaled back with its last
+// store: P itself would be subnormal from 14 binary orders below the maximum on
+// and zero from 25, and a long tail of equally light slots, whose P all round the
+// same way, can be what the output is made of when the heavy slot's V is small.
+// The float32 accumulators have room for 2^15 times anything fp16 holds.
+template <typename T>
+struct PagedP {
+  static constexpr float UP = __is_same(T, _Float16) ? 32768.f : 1.f;
+};
+
 template <int D>
 struct PagedCfg {
   static constexpr int KC = D >= 32 ? D / 32 : 1;   // 32-wide slices of a K row
@@ -381,9 +393,8 @@ __global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged
           e[hh * 4 + v] = fast_exp2(s[t][hh][v] - base);
           l[t] += e[hh * 4 + v];
         }
-      // rounded to the operand type for the product alone: the sum keeps float32
 #pragma unroll
-      for (int k = 0; k < 4; ++k) pf[t][k] = (int)Elem<T>::pack2(e[2 * k], e[2 * k + 1]);
+      for (int k = 0; k < 4; ++k) pf[t][k] = (int)Elem<T>::pack2(e[2 * k] * PagedP<T>::UP, e[2 * k + 1] * PagedP<T>::UP);
     }
 
     if (EDGE && CAUSAL && hidden) {
@@ -443,7 +454,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged
 #pragma unroll
     for (int v = 0; v < 4; ++v)
 #pragma unroll
-      for (int j = 0; j < C::VE; ++j) sm_o[wave][row][(g * 4 + v) * C::VE + j] = acc[t][j][v];
+      for (int j = 0; j < C::VE; ++j) sm_o[wave][row][(g * 4 + v) * C::VE + j] = acc[t][j][v] * (1.f / PagedP<T>::UP);
     __syncthreads();
     for (int i = threadIdx.x; i < 16 * (D / 4); i += 64 * kPagedWaves) {
       const int rr = i / (D / 4), d = (i % (D / 4)) * 4;

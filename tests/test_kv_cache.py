@@ -933,3 +933,54 @@ def test_evict_in_a_window(gpu, pages, length, missing, keep, recent, sink):
             assert held >= {t for t in there if t >= length - r or t < s}
     if there:
         assert torch.isfinite(paged_attention(torch.randn(2, 1, 2, 16, device=gpu).bfloat16(), cache, return_lse=True)[1]).all()
+
+
+# ---------------------------------------------------------------- light slots beside a heavy one
+
+
+LIGHT = [
+    # D, S, Hq, dtype, length, binary orders that the light slots lie below the heavy one
+    (64, 1, 1, "fp16", 3001, 16.7),
+    (64, 1, 1, "fp16", 3001, 20.3),
+    (128, 3, 2, "fp16", 2000, 18.5),
+    (16, 1, 20, "fp16", 1500, 22.6),
+    (256, 2, 1, "fp16", 900, 24.4),
+    (32, 1, 1, "fp16", 40, 26.2),
+    (64, 1, 1, "bf16", 3001, 20.3),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,S,Hq,dtype,length,orders", LIGHT)
+def test_light_slots_keep_their_share(gpu, D, S, Hq, dtype, length, orders):
+    """One heavy slot with zero values over a tail of equally light ones, which the output is made of. P enters its
+    product rounded to the type, u of it each, whatever its size next to the heaviest: an absolute step that
+    many equal slots share would add up. What is left of such a step is 2^-40 (2^-25 of half a subnormal step,
+    2^-15 of the scaling) of sum |v| in fp16, and half a subnormal step of the output."""
+    from dmad_amd import paged_attention
+
+    print(f"case light D={D} S={S} Hq={Hq} {dtype} {length} {orders}", flush=True)
+    t = DTYPES[dtype]
+    cache = _make(gpu, 1, 1, D, t, 16, [length], seed=60)
+    q = torch.zeros(1, S, Hq, D)
+    q[..., 0] = 4.0
+    c = st.cache_of(cache)
+    for s in range(length):
+        p, j = st.locate(c, 0, s)
+        cache.k_pages[p, 0, j] = 0
+        cache.v_pages[p, 0, j] = c["v_pages"][p, 0, j].abs()
+    p, j = st.locate(c, 0, 5)
+    cache.k_pages[p, 0, j, 0] = 8.0
+    cache.v_pages[p, 0, j] = 0
+    q, scale = q.to(t), orders * math.log(2) / 32
+    o, lse = paged_attention(q.to(gpu), cache, sm_scale=scale, causal=True, return_lse=True)
+    ro, rlse, (pv, sv, size) = st.attend(st.cache_of(cache), q, scale=scale, causal=True)
+    u = torch.finfo(t).eps / 2
+    es = (D + 8) * F32 * size + 64 * F32 * (1 + rlse.transpose(1, 2)[..., None].abs())
+    tol = (u * (1 + 1e-3) + 2 * es) * pv + u * (1 + 1e-3) * ro.abs()
+    if t == torch.float16:
+        tol = tol + 2.0 ** -40 * sv + 2.0 ** -25
+    worst = float(((o.cpu().double() - ro).abs() / tol).max())
+    print(f"  o: {worst:.2f} of its bound", flush=True)
+    assert worst <= 1
+    assert ((lse.cpu().double() - rlse).abs() <= es.amax(-1).transpose(1, 2)).all()
