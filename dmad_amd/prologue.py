@@ -18,9 +18,12 @@ Device work only: tensors off the GPU raise.
 """
 from __future__ import annotations
 
+from typing import Optional, Tuple
+
 import torch
 
 from . import _native as nat
+from .jvp_attention import _eager_call
 
 
 def rmsnorm_rope_with_tangent(x_with_t, weight, eps, freqs, num_heads):
@@ -138,12 +141,21 @@ def apply_rope_with_tangent(x, t_x, freqs, fused: bool = False):
 HEAD_DIMS = (16, 32, 64, 128, 256)
 
 
+def refuse_forward_mode(op, *ts):
+    """Raises where one of ``ts`` carries a forward-mode tangent, which the kernels do not see and the result
+    would lack."""
+    if torch.compiler.is_compiling() or torch.autograd.forward_ad._current_level < 0:
+        return
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError(f"{op} has no forward-mode derivative of torch's; tangents are operands of their own")
+
+
 def _check_same_device(op, *ts):
     dev = None
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        if not t.is_cuda and not t.is_meta:
             raise RuntimeError(f"{op} runs on the GPU only (HIP kernel); got a tensor on {t.device}")
         if dev is None:
             dev = t.device
@@ -181,8 +193,8 @@ def readable_rows(t):
     return t, st
 
 
-def _norm_weights(op, x, D, wq, wk):
-    """(wq, wk, their type code) as the kernels take them: one type for both, the operands' own or float32."""
+def _weights_dtype(op, x, D, wq, wk):
+    """The one type in which the kernels take both weights: the operands' own or float32."""
     dtype = x.dtype
     for w in (wq, wk):
         if w is None:
@@ -192,22 +204,31 @@ def _norm_weights(op, x, D, wq, wk):
                              f"got {tuple(w.shape)} {w.dtype}")
         if w.dtype != dtype:
             dtype = torch.float32
-
-    def as_read(w):
-        if w is None or w.dtype == dtype and w.is_contiguous() and not w.data_ptr() % 16:
-            return w
-        return torch.empty(D, device=w.device, dtype=dtype).copy_(w.detach())
-
-    return as_read(wq), as_read(wk), nat.dtype_code(dtype)
+    return dtype
 
 
-def _angle_table(op, freqs, B, S, D):
+def _weight_as_read(w, dtype):
+    if w is None or w.dtype == dtype and w.is_contiguous() and not w.data_ptr() % 16:
+        return w
+    return torch.empty(w.shape, device=w.device, dtype=dtype).copy_(w.detach())
+
+
+def _norm_weights(op, x, D, wq, wk):
+    """(wq, wk, their type code) as the kernels take them."""
+    dtype = _weights_dtype(op, x, D, wq, wk)
+    return _weight_as_read(wq, dtype), _weight_as_read(wk, dtype), nat.dtype_code(dtype)
+
+
+def _check_angles(op, freqs, B, S, D):
+    if freqs is not None and (freqs.dim() not in (2, 3) or freqs.shape[-1] != D // 2 or freqs.shape[-2] != S or
+                              (freqs.dim() == 3 and freqs.shape[0] not in (1, B))):
+        raise ValueError(f"{op}: freqs must be [{S}, {D // 2}] or [{B}, {S}, {D // 2}], got {tuple(freqs.shape)}")
+
+
+def _angle_table(freqs, B, S, D):
     """(float32 table, batch stride) of [S, D/2] or [B, S, D/2] angles."""
     if freqs is None:
         return None, 0
-    if freqs.shape[-1] != D // 2 or freqs.dim() not in (2, 3) or freqs.shape[-2] != S or \
-            (freqs.dim() == 3 and freqs.shape[0] not in (1, B)):
-        raise ValueError(f"{op}: freqs must be [{S}, {D // 2}] or [{B}, {S}, {D // 2}], got {tuple(freqs.shape)}")
     if freqs.dtype != torch.float32 or not freqs.is_contiguous():
         freqs = freqs.to(torch.float32).contiguous()
     return freqs, (S * (D // 2) if freqs.dim() == 3 and B > 1 and freqs.shape[0] == B else 0)
@@ -244,6 +265,39 @@ class _QkCall:
     angles as the kernels take them."""
 
     __slots__ = ("device", "code", "B", "S", "Hq", "Hk", "D", "wq", "wk", "wcode", "freqs", "freqs_b", "eps")
+
+    def __init__(self, sizes, wq, wk, freqs, eps):
+        x, self.B, self.S, self.Hq, self.Hk, self.D, wdtype = sizes
+        self.code, self.device, self.eps = nat.dtype_code(x.dtype), x.device, eps
+        # the weights' gradients are the operator's own
+        self.wq, self.wk, self.wcode = _weight_as_read(wq, wdtype), _weight_as_read(wk, wdtype), nat.dtype_code(wdtype)
+        self.freqs, self.freqs_b = _angle_table(freqs, self.B, self.S, self.D)
+
+
+_QK = "qk_norm_rope_with_tangent"
+
+
+def _qk_check(q, tq, k, tk, wq, wk, freqs, eps):
+    """Refuses what the operator does not take; (an operand, B, S, Hq, Hk, D, the weights' type)."""
+    op = _QK
+    _check_same_device(op, q, tq, k, tk, wq, wk, freqs)
+    x, B, S, Hq, Hk, D = _qk_shapes(op, q, k)
+    nat.dtype_code(x.dtype)
+    if not eps >= 0:
+        raise ValueError(f"{op}: eps must be non-negative, got {eps}")
+    if tq is not None or tk is not None:
+        for y, t in ((q, tq), (k, tk)):
+            if (y is None) != (t is None):
+                raise ValueError(f"{op}: tangents of both q and k, or of neither")
+            if t is not None and (t.shape != y.shape or t.dtype != y.dtype):
+                raise ValueError(f"{op}: a tangent has its operand's shape and type")
+    if (q is None and wq is not None) or (k is None and wk is not None):
+        raise ValueError(f"{op}: a weight without its operand")
+    wdtype = _weights_dtype(op, x, D, wq, wk)
+    _check_angles(op, freqs, B, S, D)
+    if freqs is not None and freqs.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{op} has no gradient of the angles: detach freqs")
+    return x, B, S, Hq, Hk, D, wdtype
 
 
 def _qk_forward(call, q, tq, k, tk):
@@ -284,17 +338,31 @@ class _QkNormRope(torch.autograd.Function):
 
 
 def _qk_backward(ctx, gq, gk):
-    q, k, wq, wk, _ = ctx.saved_tensors  # unpacked, so that a change in place is noticed
+    q, k, wq, wk, freqs = ctx.saved_tensors  # unpacked, so that a change in place is noticed
     call, need = ctx.call, ctx.needs_input_grad
+    # an output whose gradient did not arrive adds nothing
+    if gq is None and gk is None:
+        return (None,) * 7
+    if _eager_call(q, k, gq, gk, wq, wk, freqs):
+        dq, dk, dwq, dwk = _qk_gradients(call, q, k, gq, gk, wq, wk, need[5], need[6])
+    else:
+        dq, dk, dwq, dwk = _qk_gradients_op(q, k, gq, gk, wq, wk, freqs, call.eps, need[5], need[6])
+    return None, dq, None, dk, None, dwq, dwk
+
+
+_qk_backward_once = torch.autograd.function.once_differentiable(_qk_backward)
+
+
+def _qk_gradients(call, q, k, gq, gk, wq, wk, need_wq, need_wk):
+    """The launch: (dq, dk, dwq, dwk), None where there is no gradient of that output or none is asked for."""
     cq, ck, Hq, Hk, dev = call.wq, call.wk, call.Hq, call.Hk, call.device
     sq = sgq = sk = sgk = dq = dk = dwq = dwk = ws = ws_ptr = None
     ws_size = 0
-    # an output whose gradient did not arrive adds nothing
     if gq is not None:
         q, sq = readable_rows(q)
         gq, sgq = readable_rows(gq)
         dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        if cq is not None and need[5]:
+        if cq is not None and need_wq:
             dwq = torch.empty_like(cq)
     else:
         q, cq, Hq = None, None, 0
@@ -302,12 +370,10 @@ def _qk_backward(ctx, gq, gk):
         k, sk = readable_rows(k)
         gk, sgk = readable_rows(gk)
         dk = torch.empty(k.shape, device=dev, dtype=k.dtype)
-        if ck is not None and need[6]:
+        if ck is not None and need_wk:
             dwk = torch.empty_like(ck)
     else:
         k, ck, Hk = None, None, 0
-    if gq is None and gk is None:
-        return (None,) * 7
     if call.B * call.S == 0:
         for dw in (dwq, dwk):
             if dw is not None:
@@ -325,10 +391,71 @@ def _qk_backward(ctx, gq, gk):
         dwq = dwq.to(wq.dtype)
     if dwk is not None and dwk.dtype != wk.dtype:
         dwk = dwk.to(wk.dtype)
-    return None, dq, None, dk, None, dwq, dwk
+    return dq, dk, dwq, dwk
 
 
-_qk_backward_once = torch.autograd.function.once_differentiable(_qk_backward)
+# The same as registered ops, for whatever watches or replaces operators (compilers, dispatch modes, the profiler)
+# and for operands whose memory does not hold their values. What is absent comes back with 0 elements.
+def _or_empty(x, ts):
+    return tuple(x.new_empty((0,)) if t is None else t for t in ts)
+
+
+@torch.library.custom_op("dmad::qk_norm_rope_fwd", mutates_args=())
+def qk_norm_rope_fwd(q: Optional[torch.Tensor], tq: Optional[torch.Tensor], k: Optional[torch.Tensor],
+                     tk: Optional[torch.Tensor], wq: Optional[torch.Tensor], wk: Optional[torch.Tensor],
+                     freqs: Optional[torch.Tensor],
+                     eps: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(q', tq', k', tk') of ``qk_norm_rope_with_tangent``."""
+    call = _QkCall(_qk_check(q, tq, k, tk, wq, wk, freqs, eps), wq, wk, freqs, eps)
+    return _or_empty(k if q is None else q, _qk_forward(call, q, tq, k, tk)[:4])
+
+
+@qk_norm_rope_fwd.register_fake
+def _(q, tq, k, tk, wq, wk, freqs, eps):
+    return _or_empty(k if q is None else q, (None if t is None else t.new_empty(t.shape) for t in (q, tq, k, tk)))
+
+
+@torch.library.custom_op("dmad::qk_norm_rope_bwd", mutates_args=())
+def qk_norm_rope_bwd(q: Optional[torch.Tensor], k: Optional[torch.Tensor], gq: Optional[torch.Tensor],
+                     gk: Optional[torch.Tensor], wq: Optional[torch.Tensor], wk: Optional[torch.Tensor],
+                     freqs: Optional[torch.Tensor], eps: float, need_wq: bool,
+                     need_wk: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dq, dk, dwq, dwk) of qk_norm_rope_fwd over its primal outputs' gradients, of which one may be absent."""
+    call = _QkCall(_qk_check(q, None, k, None, wq, wk, freqs, eps), wq, wk, freqs, eps)
+    return _or_empty(k if q is None else q, _qk_gradients(call, q, k, gq, gk, wq, wk, need_wq, need_wk))
+
+
+@qk_norm_rope_bwd.register_fake
+def _(q, k, gq, gk, wq, wk, freqs, eps, need_wq, need_wk):
+    outs = [(q, gq is not None), (k, gk is not None), (wq, need_wq and gq is not None), (wk, need_wk and gk is not None)]
+    return _or_empty(k if q is None else q, (t.new_empty(t.shape) if t is not None and there else None for t, there in outs))
+
+
+def _qk_gradients_op(q, k, gq, gk, wq, wk, freqs, eps, need_wq, need_wk):
+    """(dq, dk, dwq, dwk) by the registered op, None where there is none."""
+    need_wq, need_wk = need_wq and wq is not None and gq is not None, need_wk and wk is not None and gk is not None
+    outs = torch.ops.dmad.qk_norm_rope_bwd(q, k, gq, gk, wq, wk, freqs, eps, need_wq, need_wk)
+    there = (gq is not None, gk is not None, need_wq, need_wk)
+    return tuple(t if y else None for t, y in zip(outs, there))
+
+
+def _qk_setup_context(ctx, inputs, output):
+    q, _, k, _, wq, wk, freqs, ctx.eps = inputs
+    ctx.save_for_backward(q, k, wq, wk, freqs)
+    ctx.set_materialize_grads(False)
+
+
+def _qk_op_backward(ctx, gq, _gtq, gk, _gtk):
+    q, k, wq, wk, freqs = ctx.saved_tensors
+    # the gradient of an absent operand's 0-element output is none
+    gq, gk, need = None if q is None else gq, None if k is None else gk, ctx.needs_input_grad
+    if gq is None and gk is None:
+        return (None,) * 8
+    dq, dk, dwq, dwk = _qk_gradients_op(q, k, gq, gk, wq, wk, freqs, ctx.eps, need[4], need[5])
+    return dq, None, dk, None, dwq, dwk, None, None
+
+
+qk_norm_rope_fwd.register_autograd(_qk_op_backward, setup_context=_qk_setup_context)
 
 
 def qk_norm_rope_with_tangent(q_withT, k_withT, q_weight, k_weight, eps, freqs):
@@ -344,28 +471,21 @@ def qk_norm_rope_with_tangent(q_withT, k_withT, q_weight, k_weight, eps, freqs):
     ``tq``/``tk``: tangents, given for both or for neither; their outputs are detached. ``k_withT``
     (or ``q_withT``) may be ``(None, None)``: the other alone. A weight of None skips that norm,
     ``freqs`` None the rotation; freqs are [S, D/2], or [B, S, D/2] for angles per sequence.
-    Weights have the operands' type or float32. Differentiable (once) in q, k and the weights.
+    Weights have the operands' type or float32. Differentiable (once) in q, k and the weights;
+    angles that require a gradient and torch's own forward-mode tangents are refused.
     """
-    op = "qk_norm_rope_with_tangent"
     (q, tq), (k, tk) = q_withT, k_withT
-    _check_same_device(op, q, tq, k, tk, q_weight, k_weight, freqs)
-    call = _QkCall()
-    x, call.B, call.S, call.Hq, call.Hk, call.D = _qk_shapes(op, q, k)
-    call.code, call.device = nat.dtype_code(x.dtype), x.device
-    call.eps = float(eps)
-    if not call.eps >= 0:
-        raise ValueError(f"{op}: eps must be non-negative, got {eps}")
-    if tq is not None or tk is not None:
-        for y, t in ((q, tq), (k, tk)):
-            if (y is None) != (t is None):
-                raise ValueError(f"{op}: tangents of both q and k, or of neither")
-            if t is not None and (t.shape != y.shape or t.dtype != y.dtype):
-                raise ValueError(f"{op}: a tangent has its operand's shape and type")
-    if (q is None and q_weight is not None) or (k is None and k_weight is not None):
-        raise ValueError(f"{op}: a weight without its operand")
-    # the weights' gradients are the operator's own
-    call.wq, call.wk, call.wcode = _norm_weights(op, x, call.D, q_weight, k_weight)
-    call.freqs, call.freqs_b = _angle_table(op, freqs, call.B, call.S, call.D)
+    eps = float(eps)
+    eager = _eager_call(q, tq, k, tk, q_weight, k_weight, freqs)
+    if not eager:
+        refuse_forward_mode(_QK, q, tq, k, tk, q_weight, k_weight, freqs)
+    sizes = _qk_check(q, tq, k, tk, q_weight, k_weight, freqs, eps)
+    if not eager:
+        tq, tk = (None if t is None else t.detach() for t in (tq, tk))
+        outs = torch.ops.dmad.qk_norm_rope_fwd(q, tq, k, tk, q_weight, k_weight, freqs, eps)
+        q, tq, k, tk = (None if t is None else y for t, y in zip((q, tq, k, tk), outs))
+        return (q, None if tq is None else tq.detach()), (k, None if tk is None else tk.detach())
+    call = _QkCall(sizes, q_weight, k_weight, freqs, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         q, tq, k, tk = _QkNormRope.apply(call, q, tq, k, tk, q_weight, k_weight)
     else:

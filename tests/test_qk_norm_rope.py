@@ -479,3 +479,207 @@ def test_c_backward_rejects_bad_arguments():
     assert call(gq=0) == 1 and b"gradient" in lib.dmad_last_error()
     assert call(ws=0) == 3 and call(size=16) == 3
     assert call(B=0) == 1
+
+
+# ---------------------------------------------------------------- what watches operators, and tensors that are not their memory
+
+
+def _mock_kernels(monkeypatch):
+    """Stand-ins in plain torch for the launches, which read the memory of their operands: dense CPU tensors with
+    data of their own only."""
+    from dmad_amd import prologue
+
+    def values(*ts):
+        for t in ts:
+            assert t is None or (t.data_ptr() and not t.is_neg()), "a tensor whose memory does not hold its values"
+
+    def forward(call, q, tq, k, tk):
+        values(q, tq, k, tk, call.wq, call.wk, call.freqs)
+        outs = []
+        for x, t, w in ((q, tq, call.wq), (k, tk, call.wk)):
+            outs.append(None if x is None else st.norm_rope(x, w, call.eps, call.freqs).to(x.dtype))
+            if t is not None and w is not None:  # without forward mode, which may be on around this
+                r = (x.double().pow(2).mean(-1, keepdim=True) + call.eps).rsqrt()
+                t = r * (t.double() - x * r * (x * r * t).mean(-1, keepdim=True)) * w
+            outs.append(None if t is None else st.rotate(t.double(), call.freqs).to(x.dtype))
+        return (*outs, q, k)
+
+    def gradients(call, q, k, gq, gk, wq, wk, need_wq, need_wk):
+        values(q, k, gq, gk, wq, wk, call.wq, call.wk, call.freqs)
+        dx, dw = [], []
+        for x, g, w, need in ((q, gq, wq, need_wq), (k, gk, wk, need_wk)):
+            if g is None:
+                dx.append(None), dw.append(None)
+                continue
+            a = st.rotate(g.double(), None if call.freqs is None else -call.freqs)
+            if w is not None:
+                r = (x.double().pow(2).mean(-1, keepdim=True) + call.eps).rsqrt()
+                n, u = x * r, a
+                a = u * w
+                a = r * (a - n * (a * n).mean(-1, keepdim=True))
+            dx.append(a.to(x.dtype))
+            dw.append((u * n).sum((0, 1, 2)).to(w.dtype) if need and w is not None else None)
+        return (*dx, *dw)
+
+    monkeypatch.setattr(prologue, "_check_same_device", lambda op, *ts: None)
+    monkeypatch.setattr(prologue, "_qk_forward", forward)
+    monkeypatch.setattr(prologue, "_qk_gradients", gradients)
+
+
+def _small(device="cpu", grad=False, dtype=torch.float32):
+    g = torch.Generator().manual_seed(3)
+    x = dict(q=torch.randn(2, 5, 4, 16, generator=g), k=torch.randn(2, 5, 2, 16, generator=g), tq=torch.randn(2, 5, 4, 16, generator=g),
+             tk=torch.randn(2, 5, 2, 16, generator=g), wq=torch.rand(16, generator=g) + 0.5, wk=torch.rand(16, generator=g) + 0.5)
+    x = {n: t.to(device, dtype) for n, t in x.items()}
+    x["freqs"] = (torch.rand(5, 8, generator=g) * 6).to(device)
+    for n in ("q", "k", "wq", "wk"):
+        x[n].requires_grad_(grad)
+    return x
+
+
+def _run(x):
+    from dmad_amd import qk_norm_rope_with_tangent
+
+    (q, tq), (k, tk) = qk_norm_rope_with_tangent((x["q"], x["tq"]), (x["k"], x["tk"]), x["wq"], x["wk"], 1e-6, x["freqs"])
+    return q, tq, k, tk
+
+
+OPERANDS = ("q", "tq", "k", "tk", "wq", "wk", "freqs")
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("gpu", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("name", OPERANDS)
+def test_forward_mode_is_refused(request, monkeypatch, device, name):
+    """torch's forward-mode tangents are not the operator's: they would be lost, so they are refused, whichever
+    operand carries them, by torch.autograd.forward_ad and by torch.func.jvp."""
+    if device == "cpu":
+        _mock_kernels(monkeypatch)
+    x = _small(request.getfixturevalue("gpu") if device == "gpu" else device)
+    with torch.no_grad(), torch.autograd.forward_ad.dual_level():
+        _run(x)  # none of them
+        dual = torch.autograd.forward_ad.make_dual(x[name], torch.ones_like(x[name]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            _run({**x, name: dual})
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: _run({**x, name: t})[0], (x[name],), (torch.ones_like(x[name]),))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("gpu", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("name", OPERANDS)
+def test_negated_views_have_their_sign(request, monkeypatch, device, name):
+    if device == "cpu":
+        _mock_kernels(monkeypatch)
+    x = _small(request.getfixturevalue("gpu") if device == "gpu" else device)
+    want = _run({**x, name: -x[name]})
+    odd = torch._neg_view(x[name])
+    assert odd.is_neg()
+    for a, b in zip(_run({**x, name: odd}), want):
+        assert torch.equal(a, b)
+    # and a cotangent
+    x = {**x, **{n: x[n].clone().requires_grad_(True) for n in ("q", "wk")}}
+    q, _, k, _ = _run(x)
+    g = torch.ones_like(q)
+    assert torch.equal(torch.autograd.grad(q, x["q"], torch._neg_view(g), retain_graph=True)[0], torch.autograd.grad(q, x["q"], -g)[0])
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("gpu", marks=pytest.mark.gpu)])
+def test_angles_that_want_a_gradient_are_refused(request, monkeypatch, device):
+    if device == "cpu":
+        _mock_kernels(monkeypatch)
+    x = _small(request.getfixturevalue("gpu") if device == "gpu" else device)
+    x["freqs"].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="gradient of the angles"):
+        _run(x)
+    with torch.no_grad():
+        _run(x)
+
+
+def test_meta_tensors_give_shapes():
+    x = _small("meta", grad=True)
+    outs = _run(x)
+    assert [tuple(o.shape) for o in outs] == [(2, 5, 4, 16)] * 2 + [(2, 5, 2, 16)] * 2 and all(o.is_meta for o in outs)
+    assert outs[0].requires_grad and not outs[1].requires_grad
+    leaves = [x[n] for n in ("q", "k", "wq", "wk")]
+    for t, g in zip(leaves, torch.autograd.grad(outs[0].sum() + outs[2].sum(), leaves)):
+        assert g.is_meta and g.shape == t.shape
+    with pytest.raises(ValueError, match="freqs"):
+        _run({**x, "freqs": x["freqs"][:4]})
+
+
+def test_batched_cotangents(monkeypatch):
+    _mock_kernels(monkeypatch)
+    x = _small(grad=True)
+    q, _, k, _ = _run(x)
+    leaves = [x[n] for n in ("q", "k", "wq", "wk")]
+    cts = [torch.randn(3, *o.shape) for o in (q, k)]
+    got = torch.autograd.grad((q, k), leaves, cts, is_grads_batched=True, retain_graph=True)
+    for i in range(3):
+        for a, b in zip(got, torch.autograd.grad((q, k), leaves, [c[i] for c in cts], retain_graph=True)):
+            torch.testing.assert_close(a[i], b)
+
+
+def test_fake_trace_has_one_node_per_pass():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def step(*ts):
+        x = dict(zip(OPERANDS, ts))
+        outs = _run(x)
+        return torch.autograd.grad(outs[0].square().sum() + outs[2].sum(), [x[n] for n in ("q", "k", "wq", "wk")])
+
+    x = _small("meta", grad=True)
+    gm = make_fx(step, tracing_mode="fake")(*(x[n] for n in OPERANDS))
+    ops = [n.target for n in gm.graph.nodes if n.op == "call_function" and "dmad" in str(n.target)]
+    assert ops == [torch.ops.dmad.qk_norm_rope_fwd.default, torch.ops.dmad.qk_norm_rope_bwd.default]
+
+
+def _watched(x, leaves, how):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Names(TorchDispatchMode):
+        names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    def step(*ls):
+        y = {**x, **dict(zip(leaves, ls))}
+        outs = _run(y)
+        loss = sum(o.float().square().sum() for o in (outs[0], outs[2]) if o is not None)
+        return [o for o in outs if o is not None] + list(torch.autograd.grad(loss, ls))
+
+    args = [x[n] for n in leaves]
+    if how == "direct":
+        return step(*args)
+    if how == "compiled":
+        def forward(*ls):
+            return [o for o in _run({**x, **dict(zip(leaves, ls))}) if o is not None]
+
+        outs = torch.compile(forward, fullgraph=True, backend="aot_eager")(*args)
+        primal = [o for o in outs if o.requires_grad]
+        return list(outs) + list(torch.autograd.grad(sum(o.float().square().sum() for o in primal), args))
+    if how == "profiled":
+        with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as p:
+            out = step(*args)
+        assert {"dmad::qk_norm_rope_fwd", "dmad::qk_norm_rope_bwd"} <= {e.key for e in p.key_averages()}
+        return out
+    with Names() as m:
+        out = step(*args)
+    assert [n for n in m.names if "dmad" in n] == ["dmad.qk_norm_rope_fwd.default", "dmad.qk_norm_rope_bwd.default"]
+    return out
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("gpu", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("how", ["dispatch mode", "profiled", "compiled"])
+@pytest.mark.parametrize("absent", [(), ("k", "tk", "wk"), ("wq",), ("tq", "tk", "freqs")])
+def test_op_and_direct_calls_agree_bitwise(request, monkeypatch, device, how, absent):
+    if device == "cpu":
+        _mock_kernels(monkeypatch)
+    x = _small(request.getfixturevalue("gpu") if device == "gpu" else device, grad=True)
+    x.update({n: None for n in absent})
+    leaves = [n for n in ("q", "k", "wq", "wk") if x[n] is not None]
+    want = _watched(x, leaves, "direct")
+    got = _watched(x, leaves, how)
+    assert len(got) == len(want)
+    for a, b in zip(got, want):
+        assert a.requires_grad == b.requires_grad and torch.equal(a, b)
