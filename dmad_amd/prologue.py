@@ -155,12 +155,13 @@ def _check_same_device(op, *ts):
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda and not t.is_meta:
-            raise RuntimeError(f"{op} runs on the GPU only (HIP kernel); got a tensor on {t.device}")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{op}: tensors on {dev} and on {t.device}")
+        d = t.device
+        if d != dev:
+            if d.type not in ("cuda", "meta"):
+                raise RuntimeError(f"{op} runs on the GPU only (HIP kernel); got a tensor on {d}")
+            if dev is not None:
+                raise ValueError(f"{op}: tensors on {dev} and on {d}")
+            dev = d
     return dev
 
 
@@ -307,7 +308,9 @@ def _qk_forward(call, q, tq, k, tk):
     tq, stq = _NOTHING if tq is None else readable_rows(tq)
     tk, stk = _NOTHING if tk is None else readable_rows(tk)
     dev = call.device
-    oq, otq, ok, otk = (None if t is None else torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, tq, k, tk))
+    # (half the host time of torch.empty with a device and a type)
+    oq, otq, ok, otk = (None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
+                        for t in (q, tq, k, tk))
     with nat.on_device(dev):
         nat.check(nat.lib().dmad_qk_norm_rope(
             call.code, call.wcode, call.B, call.S, call.Hq, call.Hk, call.D, nat.ptr(q), nat.ptr(tq), nat.ptr(k),
@@ -343,7 +346,7 @@ def _qk_backward(ctx, gq, gk):
     # an output whose gradient did not arrive adds nothing
     if gq is None and gk is None:
         return (None,) * 7
-    if _eager_call(q, k, gq, gk, wq, wk, freqs):
+    if _eager_call(gq, gk):  # what was saved was read by an eager forward
         dq, dk, dwq, dwk = _qk_gradients(call, q, k, gq, gk, wq, wk, need[5], need[6])
     else:
         dq, dk, dwq, dwk = _qk_gradients_op(q, k, gq, gk, wq, wk, freqs, call.eps, need[5], need[6])
@@ -361,7 +364,7 @@ def _qk_gradients(call, q, k, gq, gk, wq, wk, need_wq, need_wk):
     if gq is not None:
         q, sq = readable_rows(q)
         gq, sgq = readable_rows(gq)
-        dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        dq = torch.empty_like(q, memory_format=torch.contiguous_format)
         if cq is not None and need_wq:
             dwq = torch.empty_like(cq)
     else:
@@ -369,7 +372,7 @@ def _qk_gradients(call, q, k, gq, gk, wq, wk, need_wq, need_wk):
     if gk is not None:
         k, sk = readable_rows(k)
         gk, sgk = readable_rows(gk)
-        dk = torch.empty(k.shape, device=dev, dtype=k.dtype)
+        dk = torch.empty_like(k, memory_format=torch.contiguous_format)
         if ck is not None and need_wk:
             dwk = torch.empty_like(ck)
     else:
