@@ -9,7 +9,7 @@
     attention weight every slot receives;
   * ``evict_low_weight``: cuts long sequences to their heaviest slots.
 
-They run without gradients, put only kernel launches on the current stream and read lengths and
+They run without derivatives (operands that carry any are refused), put only kernel launches on the current stream and read lengths and
 page table on the device, so a captured step follows them. Nothing is copied to the host: what
 the device holds is checked by the kernels (see ``PagedKVCache``). Device work only: tensors off
 the GPU raise.
@@ -18,11 +18,16 @@ from __future__ import annotations
 
 import ctypes
 import math
+from typing import Optional, Tuple
 
 import torch
 
 from . import _native as nat
-from .prologue import HEAD_DIMS, _check_same_device, _norm_weights, readable_rows
+from .jvp_attention import _eager_call
+from .prologue import HEAD_DIMS, _check_same_device, _norm_weights, _weights_dtype, readable_rows, refuse_forward_mode
+
+
+CACHE_TENSORS = ("k_pages", "v_pages", "page_table", "lengths", "seen", "weight", "position")
 
 
 class PagedKVCache:
@@ -74,6 +79,10 @@ class PagedKVCache:
         for name, t, dtype in (("weight", weight, torch.float32), ("position", position, torch.int32)):
             if t is not None and (t.shape != (N, Hk, P) or t.dtype != dtype or not t.is_contiguous() or t.data_ptr() % 16):
                 raise ValueError(f"{op}: {name} must be [{N}, {Hk}, {P}] {dtype}, contiguous and 16-byte aligned")
+
+        for name, t in zip(CACHE_TENSORS, (k_pages, v_pages, page_table, lengths, seen, weight, position)):
+            if t is not None and (t.is_neg() or (t.numel() and not t.data_ptr())):
+                raise ValueError(f"{op}: {name} has no memory that holds its values")
 
         def strides(name, t):
             if t.stride(3) != 1 or t.data_ptr() % 16:
@@ -150,6 +159,59 @@ def _no_grad_only(op, *ts):
         raise RuntimeError(f"{op} has no backward: call it under torch.no_grad()")
 
 
+def _cache_tensors(cache):
+    return [getattr(cache, n) for n in CACHE_TENSORS]
+
+
+# Each call as a registered op, for whatever watches or replaces operators (compilers, dispatch modes, the profiler)
+# and for operands whose memory does not hold their values. An ordinary eager call does not go through them.
+@torch.library.custom_op("dmad::qk_norm_rope_append",
+                         mutates_args=("k_pages", "v_pages", "lengths", "seen", "weight", "position"))
+def _append_op(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, q_weight: Optional[torch.Tensor],
+               k_weight: Optional[torch.Tensor], eps: float, freqs: Optional[torch.Tensor], k_pages: torch.Tensor,
+               v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, seen: torch.Tensor,
+               weight: Optional[torch.Tensor], position: Optional[torch.Tensor]) -> torch.Tensor:
+    """q' of ``qk_norm_rope_append`` (0 elements without q)."""
+    cache = PagedKVCache(k_pages, v_pages, page_table, lengths, seen, weight, position)
+    out = _append(q, k, v, q_weight, k_weight, eps, freqs, cache)
+    return k.new_empty((0,)) if out is None else out
+
+
+@_append_op.register_fake
+def _(q, k, v, q_weight, k_weight, eps, freqs, *cache):
+    return k.new_empty((0,) if q is None else q.shape)
+
+
+@torch.library.custom_op("dmad::paged_attn", mutates_args=("weight",))
+def _attend_op(q: torch.Tensor, sm_scale: float, causal: bool, k_pages: torch.Tensor, v_pages: torch.Tensor,
+               page_table: torch.Tensor, lengths: torch.Tensor, seen: torch.Tensor, weight: Optional[torch.Tensor],
+               position: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(o, lse) of ``paged_attention``; adds to ``weight`` where it is given."""
+    cache = PagedKVCache(k_pages, v_pages, page_table, lengths, seen, weight, position)
+    return _attend(q, cache, sm_scale, causal, weight is not None)
+
+
+@_attend_op.register_fake
+def _(q, sm_scale, causal, *cache):
+    B, S, Hq, _ = q.shape
+    return q.new_empty(q.shape), q.new_empty((B, Hq, S), dtype=torch.float32)
+
+
+@torch.library.custom_op("dmad::kv_evict", mutates_args=("k_pages", "v_pages", "lengths", "weight", "position"))
+def _evict_op(keep: int, recent: int, sink: int, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+              lengths: torch.Tensor, seen: torch.Tensor, weight: torch.Tensor, position: torch.Tensor) -> None:
+    """``evict_low_weight``."""
+    _evict(PagedKVCache(k_pages, v_pages, page_table, lengths, seen, weight, position), keep, recent, sink)
+
+
+@_evict_op.register_fake
+def _(keep, recent, sink, *cache):
+    return None
+
+
+_APPEND = "qk_norm_rope_append"
+
+
 def qk_norm_rope_append(q, k, v, q_weight, k_weight, eps, freqs, cache):
     """Appends S new tokens to every sequence of the cache and returns their queries.
 
@@ -160,24 +222,35 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, eps, freqs, cache):
     that norm, freqs None the rotation. New slots start with weight 0. Tokens beyond the capacity
     are dropped (``lengths`` stays at it, ``seen`` advances), and those whose page holds nothing.
     """
-    op = "qk_norm_rope_append"
+    op = _APPEND
     if k is None or v is None:
         raise ValueError(f"{op}: k and v must be given")
     _check_new(op, cache, ("k", k), ("v", v), ("q", q))
     _check_same_device(op, k, q_weight, k_weight, freqs)
-    _no_grad_only(op, q, k, v, q_weight, k_weight)
+    _no_grad_only(op, q, k, v, q_weight, k_weight, freqs, cache.k_pages, cache.v_pages, cache.weight)
+    eps = float(eps)
     if not eps >= 0:
         raise ValueError(f"{op}: eps must be non-negative, got {eps}")
-    B, S, D = cache.batch, k.shape[1], cache.head_dim
+    D = cache.head_dim
     if q is None and q_weight is not None:
         raise ValueError(f"{op}: q_weight without q")
-    cq, ck, wcode = _norm_weights(op, k, D, q_weight, k_weight)
-    if freqs is not None:
-        if freqs.dim() != 2 or freqs.shape[1] != D // 2 or freqs.shape[0] < 1:
-            raise ValueError(f"{op}: freqs must be [positions, {D // 2}], got {tuple(freqs.shape)}")
+    if freqs is not None and (freqs.dim() != 2 or freqs.shape[1] != D // 2 or freqs.shape[0] < 1):
+        raise ValueError(f"{op}: freqs must be [positions, {D // 2}], got {tuple(freqs.shape)}")
+    if _eager_call(q, k, v, q_weight, k_weight, freqs):
+        return _append(q, k, v, q_weight, k_weight, eps, freqs, cache)
+    _weights_dtype(op, k, D, q_weight, k_weight)
+    refuse_forward_mode(op, q, k, v, q_weight, k_weight, freqs, *_cache_tensors(cache))
+    out = torch.ops.dmad.qk_norm_rope_append(q, k, v, q_weight, k_weight, eps, freqs, *_cache_tensors(cache))
+    return None if q is None else out
+
+
+def _append(q, k, v, q_weight, k_weight, eps, freqs, cache):
+    """The launch."""
+    S, Hq = k.shape[1], 0 if q is None else q.shape[2]
+    cq, ck, wcode = _norm_weights(_APPEND, k, cache.head_dim, q_weight, k_weight)
+    if freqs is not None and (freqs.dtype != torch.float32 or not freqs.is_contiguous()):
         freqs = freqs.to(torch.float32).contiguous()
-    Hq = 0 if q is None else q.shape[2]
-    out = None if q is None else torch.empty((B, S, Hq, D), device=q.device, dtype=q.dtype)
+    out = None if q is None else torch.empty_like(q, memory_format=torch.contiguous_format)
     if Hq == 0:
         q = None
     ops = [(None, None) if t is None else readable_rows(t) for t in (q, k, v)]
@@ -185,7 +258,7 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, eps, freqs, cache):
         nat.check(nat.lib().dmad_qk_norm_rope_append(
             nat.dtype_code(cache.dtype), wcode, S, Hq, *(nat.ptr(t) for t, _ in ops), *(s for _, s in ops),
             nat.ptr(cq if q is not None else None), nat.ptr(ck), nat.ptr(freqs), 0 if freqs is None else freqs.shape[0],
-            float(eps), nat.ptr(out), cache._ref, nat.stream_ptr(cache.device)))
+            eps, nat.ptr(out), cache._ref, nat.stream_ptr(cache.device)))
     return out
 
 
@@ -211,8 +284,8 @@ def paged_attention(q, cache, sm_scale=None, causal=False, accumulate=False, ret
     """
     op = "paged_attention"
     _check_new(op, cache, ("q", q))
-    _no_grad_only(op, q)
-    S, Hq = q.shape[1], q.shape[2]
+    _no_grad_only(op, q, cache.k_pages, cache.v_pages, cache.weight)
+    Hq = q.shape[2]
     if Hq < 1 or Hq % cache.kv_heads:
         raise ValueError(f"{op}: {Hq} query heads are not a multiple of the cache's {cache.kv_heads}")
     scale = cache.head_dim ** -0.5 if sm_scale is None else float(sm_scale)
@@ -220,17 +293,31 @@ def paged_attention(q, cache, sm_scale=None, causal=False, accumulate=False, ret
         raise NotImplementedError(f"{op}: sm_scale must be positive and finite, got {sm_scale}")
     if accumulate and cache.weight is None:
         raise ValueError(f"{op}: the cache keeps no weights to accumulate")
-    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    causal, accumulate = bool(causal), bool(accumulate)
+    if _eager_call(q):
+        o, lse = _attend(q, cache, scale, causal, accumulate)
+    else:
+        refuse_forward_mode(op, q, *_cache_tensors(cache))
+        tensors = _cache_tensors(cache)
+        if not accumulate:
+            tensors[-2:] = None, None
+        o, lse = torch.ops.dmad.paged_attn(q, scale, causal, *tensors)
+    return (o, lse) if return_lse else o
+
+
+def _attend(q, cache, scale, causal, accumulate):
+    """The launch: (o, lse)."""
+    S, Hq = q.shape[1], q.shape[2]
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((cache.batch, Hq, S), device=q.device, dtype=torch.float32)
     q, strides = readable_rows(q)
-    accumulate = bool(accumulate)
     ws_ptr, ws_size, ws = cache._workspace(
         (S, Hq, accumulate), lambda: nat.paged_attn_workspace_bytes(cache._c, S, Hq, accumulate))
     with nat.on_device(cache.device):
         nat.check(nat.lib().dmad_paged_attn(
-            nat.dtype_code(cache.dtype), cache._ref, S, Hq, nat.ptr(q), strides, int(bool(causal)), int(accumulate), scale,
+            nat.dtype_code(cache.dtype), cache._ref, S, Hq, nat.ptr(q), strides, int(causal), int(accumulate), scale,
             nat.ptr(o), nat.ptr(lse), ws_ptr, ws_size, nat.stream_ptr(cache.device)))
-    return (o, lse) if return_lse else o
+    return o, lse
 
 
 def evict_low_weight(cache, keep, recent=0, sink=0):
@@ -257,6 +344,16 @@ def evict_low_weight(cache, keep, recent=0, sink=0):
                          f"keep={keep}, recent={recent}, sink={sink}")
     if keep >= cache.capacity or cache.batch == 0:
         return  # no sequence can be longer
+    _no_grad_only(op, cache.k_pages, cache.v_pages, cache.weight)
+    if _eager_call():
+        _evict(cache, keep, recent, sink)
+    else:
+        refuse_forward_mode(op, *_cache_tensors(cache))
+        torch.ops.dmad.kv_evict(keep, recent, sink, *_cache_tensors(cache))
+
+
+def _evict(cache, keep, recent, sink):
+    """The launches."""
     ws_ptr, ws_size, ws = cache._workspace(("evict", keep), lambda: nat.kv_evict_workspace_bytes(cache._c, keep))
     with nat.on_device(cache.device):
         nat.check(nat.lib().dmad_kv_evict(nat.dtype_code(cache.dtype), cache._ref, keep, recent, sink, ws_ptr, ws_size,

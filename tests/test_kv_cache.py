@@ -984,3 +984,160 @@ def test_light_slots_keep_their_share(gpu, D, S, Hq, dtype, length, orders):
     print(f"  o: {worst:.2f} of its bound", flush=True)
     assert worst <= 1
     assert ((lse.cpu().double() - rlse).abs() <= es.amax(-1).transpose(1, 2)).all()
+
+
+# ---------------------------------------------------------------- what watches operators, and tensors that are not their memory
+
+
+def _mock_launches(monkeypatch):
+    """The oracle in place of the launches, on CPU tensors, which it takes as the kernels do: by their memory."""
+    from dmad_amd import kv_cache
+
+    def tensors(cache, *ts):
+        for t in (*ts, *(getattr(cache, n) for n in st.FIELDS)):
+            assert t is None or t.numel() == 0 or (t.data_ptr() and not t.is_neg()), "memory that does not hold the values"
+        return {n: getattr(cache, n) for n in st.FIELDS}
+
+    def append(q, k, v, wq, wk, eps, freqs, cache):
+        rq, _ = st.append(tensors(cache, q, k, v, wq, wk, freqs), q, k, v, wq, wk, eps, freqs)
+        return None if q is None else rq.to(q.dtype)
+
+    def attend(q, cache, scale, causal, accumulate):
+        c = tensors(cache, q)
+        o, lse, _ = st.attend(c, q, scale=scale, causal=causal, accumulate=accumulate)
+        if accumulate:
+            cache.weight.copy_(c["weight"])
+        return o.to(q.dtype), lse.float()
+
+    def evict(cache, keep, recent, sink):
+        st.evict(tensors(cache), keep, recent, sink)
+
+    monkeypatch.setattr(kv_cache, "_check_same_device", lambda op, *ts: ts[0].device)
+    for name, f in (("_append", append), ("_attend", attend), ("_evict", evict)):
+        monkeypatch.setattr(kv_cache, name, f)
+
+
+BOTH = pytest.mark.parametrize("device", ["cpu", pytest.param("gpu", marks=pytest.mark.gpu)])
+
+
+def _loop(request, monkeypatch, device, seed=70):
+    """A short serving loop's inputs: cache, q, k, v, weights, angles."""
+    if device == "cpu":
+        _mock_launches(monkeypatch)
+    dev = request.getfixturevalue("gpu") if device == "gpu" else torch.device("cpu")
+    cache = _make(dev, 2, 2, 16, torch.bfloat16, 16, [37, 20], room=6, seed=seed)
+    g = torch.Generator().manual_seed(seed)
+    x = dict(q=torch.randn(2, 2, 4, 16, generator=g).bfloat16(), k=torch.randn(2, 2, 2, 16, generator=g).bfloat16(),
+             v=torch.randn(2, 2, 2, 16, generator=g).bfloat16(), wq=torch.rand(16, generator=g) + 0.5, wk=torch.rand(16, generator=g) + 0.5,
+             freqs=torch.rand(60, 8, generator=g))
+    return cache, {n: t.to(dev) for n, t in x.items()}
+
+
+def _serve(cache, x):
+    from dmad_amd import append_kv, evict_low_weight, paged_attention, qk_norm_rope_append
+
+    q = qk_norm_rope_append(x["q"], x["k"], x["v"], x["wq"], x["wk"], 1e-6, x["freqs"], cache)
+    o, lse = paged_attention(q, cache, causal=True, accumulate=True, return_lse=True)
+    append_kv(x["k"], x["v"], cache)
+    evict_low_weight(cache, 24, recent=4, sink=1)
+    return [q, o, lse, paged_attention(q, cache)]
+
+
+@BOTH
+@pytest.mark.parametrize("how", ["dispatch mode", "profiled", "compiled", "inference"])
+def test_cache_ops_and_direct_calls_agree_bitwise(request, monkeypatch, device, how):
+    """The whole loop under what watches operators: the same outputs and the same cache as without."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    names = []
+
+    class Names(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    cache, x = _loop(request, monkeypatch, device)
+    want = _serve(cache, x)
+    other, x = _loop(request, monkeypatch, device)
+    ops = ["qk_norm_rope_append", "paged_attn", "qk_norm_rope_append", "kv_evict", "paged_attn"]
+    if how == "dispatch mode":
+        with Names():
+            got = _serve(other, x)
+        assert [n for n in names if "dmad" in n] == [f"dmad.{n}.default" for n in ops]
+    elif how == "profiled":
+        with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as p:
+            got = _serve(other, x)
+        assert {f"dmad::{n}" for n in ops} <= {e.key for e in p.key_averages()}
+    elif how == "compiled":
+        with torch.no_grad():
+            got = torch.compile(_serve, fullgraph=True, backend="aot_eager")(other, x)
+    else:
+        with torch.inference_mode():
+            got = _serve(other, x)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    for n in st.FIELDS:
+        _same(n, getattr(other, n), getattr(cache, n))
+
+
+@BOTH
+def test_cache_calls_refuse_derivatives(request, monkeypatch, device):
+    """Forward-mode tangents and tensors that require a gradient, of the operands and of the cache's own: their
+    derivatives would be lost in silence."""
+    from dmad_amd import evict_low_weight, paged_attention, qk_norm_rope_append
+
+    cache, x = _loop(request, monkeypatch, device)
+    before = st.cache_of(cache)
+
+    def calls(x, cache):
+        return [lambda: qk_norm_rope_append(x["q"], x["k"], x["v"], x["wq"], x["wk"], 1e-6, x["freqs"], cache),
+                lambda: paged_attention(x["q"], cache), lambda: evict_low_weight(cache, 24)]
+
+    fa = torch.autograd.forward_ad
+    with torch.no_grad(), fa.dual_level():
+        for name in x:
+            for call in calls({**x, name: fa.make_dual(x[name], torch.ones_like(x[name]))}, cache)[:2 if name == "q" else 1]:
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+        for name in ("k_pages", "v_pages", "weight"):
+            from dmad_amd import PagedKVCache
+
+            t = {n: getattr(cache, n) for n in st.FIELDS}
+            dual = PagedKVCache(**{**t, name: fa.make_dual(t[name], torch.ones_like(t[name]))})
+            for call in calls(x, dual):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: paged_attention(t, cache), (x["q"],), (x["q"],))
+    for name in ("k_pages", "v_pages", "weight"):
+        getattr(cache, name).requires_grad_(True)
+        for call in calls(x, cache):
+            with pytest.raises(RuntimeError, match="no backward"):
+                call()
+        getattr(cache, name).requires_grad_(False)
+    x["freqs"].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="no backward"):
+        calls(x, cache)[0]()
+    for n in st.FIELDS:
+        _same(n, getattr(cache, n), before[n])
+
+
+@BOTH
+def test_cache_calls_read_negated_views(request, monkeypatch, device):
+    from dmad_amd import PagedKVCache
+
+    for name in ("q", "k", "v", "wq", "wk", "freqs"):
+        cache, x = _loop(request, monkeypatch, device)
+        want = _serve(cache, {**x, name: -x[name]})
+        other, x = _loop(request, monkeypatch, device)
+        for a, b in zip(_serve(other, {**x, name: torch._neg_view(x[name])}), want):
+            assert torch.equal(a, b), name
+        for n in st.FIELDS:
+            _same(n, getattr(other, n), getattr(cache, n))
+    # the cache's own tensors are written in place and cannot be such views
+    t = {n: getattr(cache, n) for n in st.FIELDS}
+    for name in ("k_pages", "weight", "lengths"):
+        with pytest.raises(ValueError, match="memory"):
+            PagedKVCache(**{**t, name: torch._neg_view(t[name])})
+    with pytest.raises(ValueError, match="memory"):
+        PagedKVCache(**{**t, "k_pages": torch._efficientzerotensor(t["k_pages"].shape, dtype=torch.bfloat16, device=t["k_pages"].device)})
