@@ -50,7 +50,8 @@ class PagedKVCache:
     as it is only read; pages that are appended to, evicted from or whose weights are accumulated
     belong to one sequence. Calls that only read a cache may run on several streams at once; one
     that appends, accumulates or evicts is ordered by the caller against all others, as with any
-    tensor changed in place.
+    tensor changed in place. Such calls count as changes in place for autograd: a backward pass that
+    needs what they overwrote raises.
     """
 
     def __init__(self, k_pages, v_pages, page_table, lengths, seen, weight=None, position=None):
@@ -100,6 +101,10 @@ class PagedKVCache:
         self._c = nat.KvCache(N, Hk, P, D, B, M, nat.ptr(k_pages), nat.ptr(v_pages), strides("k_pages", k_pages),
                               strides("v_pages", v_pages), nat.ptr(page_table), page_table.stride(0) if B > 1 else M,
                               nat.ptr(lengths), nat.ptr(seen), nat.ptr(weight), nat.ptr(position))
+        # what each call changes, for autograd (which keeps no count of inference tensors)
+        self._written = {op: [t for t in ts if t is not None and not t.is_inference()] for op, ts in (
+            ("append", (k_pages, v_pages, lengths, seen, weight, position)), ("attend", (weight,)),
+            ("evict", (k_pages, v_pages, lengths, weight, position)))}
         self._ref = ctypes.byref(self._c)
 
     def __setattr__(self, name, value):
@@ -128,6 +133,11 @@ class PagedKVCache:
             torch.zeros(pages, device=device, dtype=torch.float32) if track_weights else None,
             torch.zeros(pages, device=device, dtype=torch.int32) if track_weights else None,
         )
+
+    def _changed(self, by):
+        """The launches of an ordinary eager call write through addresses: counted as changes in place here."""
+        if self._written[by]:
+            torch.autograd.graph.increment_version(self._written[by])
 
     def _workspace(self, key, query):
         """A fresh workspace whose size ``query`` gives, asked once per ``key``."""
@@ -237,7 +247,9 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, eps, freqs, cache):
     if freqs is not None and (freqs.dim() != 2 or freqs.shape[1] != D // 2 or freqs.shape[0] < 1):
         raise ValueError(f"{op}: freqs must be [positions, {D // 2}], got {tuple(freqs.shape)}")
     if _eager_call(q, k, v, q_weight, k_weight, freqs):
-        return _append(q, k, v, q_weight, k_weight, eps, freqs, cache)
+        out = _append(q, k, v, q_weight, k_weight, eps, freqs, cache)
+        cache._changed("append")
+        return out
     _weights_dtype(op, k, D, q_weight, k_weight)
     refuse_forward_mode(op, q, k, v, q_weight, k_weight, freqs, *_cache_tensors(cache))
     out = torch.ops.dmad.qk_norm_rope_append(q, k, v, q_weight, k_weight, eps, freqs, *_cache_tensors(cache))
@@ -296,6 +308,8 @@ def paged_attention(q, cache, sm_scale=None, causal=False, accumulate=False, ret
     causal, accumulate = bool(causal), bool(accumulate)
     if _eager_call(q):
         o, lse = _attend(q, cache, scale, causal, accumulate)
+        if accumulate:
+            cache._changed("attend")
     else:
         refuse_forward_mode(op, q, *_cache_tensors(cache))
         tensors = _cache_tensors(cache)
@@ -347,6 +361,7 @@ def evict_low_weight(cache, keep, recent=0, sink=0):
     _no_grad_only(op, cache.k_pages, cache.v_pages, cache.weight)
     if _eager_call():
         _evict(cache, keep, recent, sink)
+        cache._changed("evict")
     else:
         refuse_forward_mode(op, *_cache_tensors(cache))
         torch.ops.dmad.kv_evict(keep, recent, sink, *_cache_tensors(cache))

@@ -996,7 +996,8 @@ def _mock_launches(monkeypatch):
     def tensors(cache, *ts):
         for t in (*ts, *(getattr(cache, n) for n in st.FIELDS)):
             assert t is None or t.numel() == 0 or (t.data_ptr() and not t.is_neg()), "memory that does not hold the values"
-        return {n: getattr(cache, n) for n in st.FIELDS}
+        # .data: writes that autograd does not count, as the kernels'
+        return {n: None if getattr(cache, n) is None else getattr(cache, n).data for n in st.FIELDS}
 
     def append(q, k, v, wq, wk, eps, freqs, cache):
         rq, _ = st.append(tensors(cache, q, k, v, wq, wk, freqs), q, k, v, wq, wk, eps, freqs)
@@ -1006,7 +1007,7 @@ def _mock_launches(monkeypatch):
         c = tensors(cache, q)
         o, lse, _ = st.attend(c, q, scale=scale, causal=causal, accumulate=accumulate)
         if accumulate:
-            cache.weight.copy_(c["weight"])
+            cache.weight.data.copy_(c["weight"])
         return o.to(q.dtype), lse.float()
 
     def evict(cache, keep, recent, sink):
@@ -1141,3 +1142,46 @@ def test_cache_calls_read_negated_views(request, monkeypatch, device):
             PagedKVCache(**{**t, name: torch._neg_view(t[name])})
     with pytest.raises(ValueError, match="memory"):
         PagedKVCache(**{**t, "k_pages": torch._efficientzerotensor(t["k_pages"].shape, dtype=torch.bfloat16, device=t["k_pages"].device)})
+
+
+@BOTH
+def test_writes_count_as_changes_in_place(request, monkeypatch, device):
+    """A backward pass that saved a view of the pages, lengths or weights before a call that writes them raises; one
+    that saved them before a call that only reads them does not."""
+    from dmad_amd import append_kv, evict_low_weight, paged_attention
+
+    writes = {"append": {"k_pages", "v_pages", "lengths", "seen", "weight", "position"}, "accumulate": {"weight"},
+              "evict": {"k_pages", "v_pages", "lengths", "weight", "position"}, "read": set()}
+    for what, names in writes.items():
+        cache, x = _loop(request, monkeypatch, device)
+        versions = {n: getattr(cache, n)._version for n in st.FIELDS}
+        ones = torch.ones((), device=x["q"].device, requires_grad=True)
+        kept = {n: (getattr(cache, n)[:1] * ones.to(getattr(cache, n).dtype)).sum() for n in ("k_pages", "v_pages", "weight")}
+        if what == "append":
+            append_kv(x["k"], x["v"], cache)
+        elif what == "evict":
+            evict_low_weight(cache, 24)
+        else:
+            paged_attention(x["q"], cache, accumulate=what == "accumulate")
+        for n in st.FIELDS:
+            assert (getattr(cache, n)._version != versions[n]) == (n in names), (what, n)
+        for n, loss in kept.items():
+            if n in names:
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    loss.backward()
+            else:
+                loss.backward()
+
+
+@pytest.mark.gpu
+def test_caches_made_under_inference_mode(request, monkeypatch):
+    """Inference tensors have no count of changes: such a cache works inside and outside the mode."""
+    device = "gpu"
+    with torch.inference_mode():
+        cache, x = _loop(request, monkeypatch, device)
+        other, _ = _loop(request, monkeypatch, device)
+        assert cache.k_pages.is_inference()
+        want = _serve(cache, x)
+    with torch.no_grad():
+        got = _serve(other, x)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
