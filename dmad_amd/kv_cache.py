@@ -30,6 +30,10 @@ from .prologue import HEAD_DIMS, _check_same_device, _norm_weights, _weights_dty
 CACHE_TENSORS = ("k_pages", "v_pages", "page_table", "lengths", "seen", "weight", "position")
 
 
+def _cache_tensors(cache):
+    return [getattr(cache, n) for n in CACHE_TENSORS]
+
+
 class PagedKVCache:
     """Pages of keys and values, one page list per sequence.
 
@@ -46,7 +50,8 @@ class PagedKVCache:
                       its token's position; both or neither (None: no accumulation, no eviction)
 
     The tensors are used in place and stay the caller's: pages are handed out, shared or dropped
-    by writing to ``page_table`` and ``lengths``. A page may appear in several sequences as long
+    by writing to ``page_table`` and ``lengths``. Where a tensor's memory is replaced (``t.data = ...``)
+    the next call checks and uses the new one; a captured graph keeps the one it was captured with. A page may appear in several sequences as long
     as it is only read; pages that are appended to, evicted from or whose weights are accumulated
     belong to one sequence. Calls that only read a cache may run on several streams at once; one
     that appends, accumulates or evicts is ordered by the caller against all others, as with any
@@ -55,8 +60,15 @@ class PagedKVCache:
     """
 
     def __init__(self, k_pages, v_pages, page_table, lengths, seen, weight=None, position=None):
+        self.k_pages, self.v_pages, self.page_table = k_pages, v_pages, page_table
+        self.lengths, self.seen, self.weight, self.position = lengths, seen, weight, position
+        self._describe()
+
+    def _describe(self):
+        """Checks the tensors and fills the kernels' view of them."""
         op = "PagedKVCache"
-        self.device = _check_same_device(op, k_pages, v_pages, page_table, lengths, seen, weight, position)
+        k_pages, v_pages, page_table, lengths, seen, weight, position = _cache_tensors(self)
+        device = _check_same_device(op, k_pages, v_pages, page_table, lengths, seen, weight, position)
         if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
             raise ValueError(f"{op}: k_pages and v_pages must be [N, Hk, P, D], got {tuple(k_pages.shape)} and "
                              f"{tuple(v_pages.shape)}")
@@ -93,19 +105,27 @@ class PagedKVCache:
                 raise ValueError(f"{op}: strides of {name} must be multiples of 8 elements and at least {D}, got {t.stride()}")
             return (ctypes.c_int64 * 3)(*st)
 
-        self.k_pages, self.v_pages, self.page_table = k_pages, v_pages, page_table
-        self.lengths, self.seen, self.weight, self.position = lengths, seen, weight, position
-        self.dtype, self.batch, self.kv_heads, self.page_size, self.head_dim = k_pages.dtype, B, Hk, P, D
-        self.capacity = M * P
-        self._sizes = {}
-        self._c = nat.KvCache(N, Hk, P, D, B, M, nat.ptr(k_pages), nat.ptr(v_pages), strides("k_pages", k_pages),
-                              strides("v_pages", v_pages), nat.ptr(page_table), page_table.stride(0) if B > 1 else M,
-                              nat.ptr(lengths), nat.ptr(seen), nat.ptr(weight), nat.ptr(position))
-        # what each call changes, for autograd (which keeps no count of inference tensors)
-        self._written = {op: [t for t in ts if t is not None and not t.is_inference()] for op, ts in (
-            ("append", (k_pages, v_pages, lengths, seen, weight, position)), ("attend", (weight,)),
-            ("evict", (k_pages, v_pages, lengths, weight, position)))}
-        self._ref = ctypes.byref(self._c)
+        c = nat.KvCache(N, Hk, P, D, B, M, nat.ptr(k_pages), nat.ptr(v_pages), strides("k_pages", k_pages),
+                        strides("v_pages", v_pages), nat.ptr(page_table), page_table.stride(0) if B > 1 else M,
+                        nat.ptr(lengths), nat.ptr(seen), nat.ptr(weight), nat.ptr(position))
+        tensors = [t for t in _cache_tensors(self) if t is not None]
+        described = dict(
+            device=device, dtype=k_pages.dtype, batch=B, kv_heads=Hk, page_size=P, head_dim=D, capacity=M * P, _c=c,
+            _sizes={}, _addresses=[(t, t.data_ptr()) for t in tensors],
+            # what each call changes, for autograd (which keeps no count of inference tensors)
+            _written={by: [t for t in ts if t is not None and not t.is_inference()] for by, ts in (
+                ("append", (k_pages, v_pages, lengths, seen, weight, position)), ("attend", (weight,)),
+                ("evict", (k_pages, v_pages, lengths, weight, position)))},
+            _ref=ctypes.byref(c))
+        self.__dict__.update(described)
+
+    def _settle(self):
+        """Follows tensors whose memory was replaced since (``t.data = ...``, a storage that was resized)."""
+        if torch.compiler.is_compiling():
+            return  # the registered ops describe the tensors that they are given
+        for t, address in self._addresses:
+            if t.data_ptr() != address:
+                return self._describe()
 
     def __setattr__(self, name, value):
         if hasattr(self, "_ref"):
@@ -151,6 +171,7 @@ def _check_new(op, cache, *named):
     """Shapes of new tokens' q, k, v against the cache: (S, Hq)."""
     if not isinstance(cache, PagedKVCache):
         raise TypeError(f"{op}: cache must be a PagedKVCache, got {type(cache).__name__}")
+    cache._settle()
     given = [(n, t) for n, t in named if t is not None]
     dev = _check_same_device(op, *(t for _, t in given))
     if dev != cache.device:
@@ -167,10 +188,6 @@ def _check_new(op, cache, *named):
 def _no_grad_only(op, *ts):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
         raise RuntimeError(f"{op} has no backward: call it under torch.no_grad()")
-
-
-def _cache_tensors(cache):
-    return [getattr(cache, n) for n in CACHE_TENSORS]
 
 
 # Each call as a registered op, for whatever watches or replaces operators (compilers, dispatch modes, the profiler)
@@ -350,6 +367,7 @@ def evict_low_weight(cache, keep, recent=0, sink=0):
     op = "evict_low_weight"
     if not isinstance(cache, PagedKVCache):
         raise TypeError(f"{op}: cache must be a PagedKVCache, got {type(cache).__name__}")
+    cache._settle()
     if cache.weight is None:
         raise ValueError(f"{op}: the cache keeps no weights and positions")
     keep, recent, sink = int(keep), int(recent), int(sink)

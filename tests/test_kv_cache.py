@@ -1185,3 +1185,36 @@ def test_caches_made_under_inference_mode(request, monkeypatch):
     with torch.no_grad():
         got = _serve(other, x)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@BOTH
+def test_replaced_memory_is_followed(request, monkeypatch, device):
+    """A cache tensor whose memory is replaced (.data, as optimizers and offloading do it) is read and written where
+    it is now; one without memory, or of another shape or type, is refused by the next call."""
+    from dmad_amd import paged_attention
+
+    cache, x = _loop(request, monkeypatch, device)
+    other, _ = _loop(request, monkeypatch, device)
+    fields = ("k_pages", "v_pages", "page_table", "lengths", "seen", "weight", "position")
+    old = {n: getattr(cache, n).data for n in fields}  # kept alive: what a stale address would read and write
+    for n in fields:
+        getattr(cache, n).data = old[n].clone()
+    before = {n: t.clone() for n, t in old.items()}
+    for a, b in zip(_serve(cache, x), _serve(other, x)):
+        assert torch.equal(a, b)
+    for n in fields:
+        assert getattr(cache._c, n) == getattr(cache, n).data_ptr() != old[n].data_ptr()
+        _same(n, getattr(cache, n), getattr(other, n))
+        _same(f"the old {n}", old[n], before[n])
+    # a pool of more pages, then what is refused
+    for n in ("k_pages", "v_pages", "weight", "position"):
+        t = getattr(cache, n)
+        t.data = torch.cat((t.data, t.data))
+    assert torch.equal(paged_attention(x["q"], cache), paged_attention(x["q"], other)) and cache._c.num_pages == 2 * other._c.num_pages
+    good = cache.k_pages.data
+    for bad, error in ((good[:3].clone(), ValueError), (good[..., :8].clone(), ValueError), (torch.empty(0, dtype=good.dtype, device=good.device), ValueError)):
+        cache.k_pages.data = bad
+        with pytest.raises(error):
+            paged_attention(x["q"], cache)
+    cache.k_pages.data = good
+    assert torch.equal(paged_attention(x["q"], cache), paged_attention(x["q"], other))
