@@ -111,7 +111,10 @@ class PagedKVCache:
         tensors = [t for t in _cache_tensors(self) if t is not None]
         described = dict(
             device=device, dtype=k_pages.dtype, batch=B, kv_heads=Hk, page_size=P, head_dim=D, capacity=M * P, _c=c,
-            _sizes={}, _addresses=[(t, t.data_ptr()) for t in tensors],
+            _code=nat.dtype_code(k_pages.dtype), _sizes={}, _pointers=[t.data_ptr for t in tensors],
+            _addresses=[t.data_ptr() for t in tensors],
+            # their new_empty takes half the host time of torch.empty with a device and a type
+            _bytes=torch.empty(0, device=device, dtype=torch.uint8), _floats=torch.empty(0, device=device, dtype=torch.float32),
             # what each call changes, for autograd (which keeps no count of inference tensors)
             _written={by: [t for t in ts if t is not None and not t.is_inference()] for by, ts in (
                 ("append", (k_pages, v_pages, lengths, seen, weight, position)), ("attend", (weight,)),
@@ -123,9 +126,8 @@ class PagedKVCache:
         """Follows tensors whose memory was replaced since (``t.data = ...``, a storage that was resized)."""
         if torch.compiler.is_compiling():
             return  # the registered ops describe the tensors that they are given
-        for t, address in self._addresses:
-            if t.data_ptr() != address:
-                return self._describe()
+        if [pointer() for pointer in self._pointers] != self._addresses:
+            self._describe()
 
     def __setattr__(self, name, value):
         if hasattr(self, "_ref"):
@@ -159,35 +161,50 @@ class PagedKVCache:
         if self._written[by]:
             torch.autograd.graph.increment_version(self._written[by])
 
-    def _workspace(self, key, query):
-        """A fresh workspace whose size ``query`` gives, asked once per ``key``."""
-        size = self._sizes.get(key)
+    def _workspace(self, query, *args):
+        """(pointer, size, owner) of a fresh workspace whose size ``query`` gives, asked once per call's sizes."""
+        size = self._sizes.get(args)
         if size is None:
-            size = self._sizes[key] = query()
-        return nat.workspace(size, self.device)
+            size = self._sizes[args] = query(self._c, *args)
+        if size == 0:
+            return None, 0, None
+        ws = self._bytes.new_empty(size)
+        return ws.data_ptr(), size, ws
+
+
+def _on_cache(op, cache, t):
+    if t is not None and t.device != cache.device:
+        _check_same_device(op, t)
+        raise ValueError(f"{op}: tensors on {t.device}, the cache on {cache.device}")
 
 
 def _check_new(op, cache, *named):
-    """Shapes of new tokens' q, k, v against the cache: (S, Hq)."""
+    """Shapes of new tokens' q, k, v against the cache."""
     if not isinstance(cache, PagedKVCache):
         raise TypeError(f"{op}: cache must be a PagedKVCache, got {type(cache).__name__}")
     cache._settle()
-    given = [(n, t) for n, t in named if t is not None]
-    dev = _check_same_device(op, *(t for _, t in given))
-    if dev != cache.device:
-        raise ValueError(f"{op}: tensors on {dev}, the cache on {cache.device}")
-    for n, t in given:
-        if t.dim() != 4 or t.shape[0] != cache.batch or t.shape[3] != cache.head_dim or t.shape[1] != given[0][1].shape[1]:
-            raise ValueError(f"{op}: {n} must be [{cache.batch}, S, H, {cache.head_dim}], got {tuple(t.shape)}")
+    tokens = None
+    for n, t in named:
+        if t is None:
+            continue
+        _on_cache(op, cache, t)
+        shape = t.shape
+        if len(shape) == 4:
+            B, S, H, D = shape
+            tokens = S if tokens is None else tokens
+        if len(shape) != 4 or B != cache.batch or D != cache.head_dim or S != tokens:
+            raise ValueError(f"{op}: {n} must be [{cache.batch}, S, H, {cache.head_dim}], got {tuple(shape)}")
         if t.dtype != cache.dtype:
             raise ValueError(f"{op}: {n} is {t.dtype}, the cache {cache.dtype}")
-        if n != "q" and t.shape[2] != cache.kv_heads:
-            raise ValueError(f"{op}: {n} has {t.shape[2]} heads, the cache {cache.kv_heads}")
+        if n != "q" and H != cache.kv_heads:
+            raise ValueError(f"{op}: {n} has {H} heads, the cache {cache.kv_heads}")
 
 
-def _no_grad_only(op, *ts):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise RuntimeError(f"{op} has no backward: call it under torch.no_grad()")
+def _no_grad_only(op, cache, *ts):
+    if torch.is_grad_enabled():
+        for t in (cache.k_pages, cache.v_pages, cache.weight, *ts):
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{op} has no backward: call it under torch.no_grad()")
 
 
 # Each call as a registered op, for whatever watches or replaces operators (compilers, dispatch modes, the profiler)
@@ -253,8 +270,9 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, eps, freqs, cache):
     if k is None or v is None:
         raise ValueError(f"{op}: k and v must be given")
     _check_new(op, cache, ("k", k), ("v", v), ("q", q))
-    _check_same_device(op, k, q_weight, k_weight, freqs)
-    _no_grad_only(op, q, k, v, q_weight, k_weight, freqs, cache.k_pages, cache.v_pages, cache.weight)
+    for t in (q_weight, k_weight, freqs):
+        _on_cache(op, cache, t)
+    _no_grad_only(op, cache, q, k, v, q_weight, k_weight, freqs)
     eps = float(eps)
     if not eps >= 0:
         raise ValueError(f"{op}: eps must be non-negative, got {eps}")
@@ -285,7 +303,7 @@ def _append(q, k, v, q_weight, k_weight, eps, freqs, cache):
     ops = [(None, None) if t is None else readable_rows(t) for t in (q, k, v)]
     with nat.on_device(cache.device):
         nat.check(nat.lib().dmad_qk_norm_rope_append(
-            nat.dtype_code(cache.dtype), wcode, S, Hq, *(nat.ptr(t) for t, _ in ops), *(s for _, s in ops),
+            cache._code, wcode, S, Hq, *(nat.ptr(t) for t, _ in ops), *(s for _, s in ops),
             nat.ptr(cq if q is not None else None), nat.ptr(ck), nat.ptr(freqs), 0 if freqs is None else freqs.shape[0],
             eps, nat.ptr(out), cache._ref, nat.stream_ptr(cache.device)))
     return out
@@ -313,7 +331,7 @@ def paged_attention(q, cache, sm_scale=None, causal=False, accumulate=False, ret
     """
     op = "paged_attention"
     _check_new(op, cache, ("q", q))
-    _no_grad_only(op, q, cache.k_pages, cache.v_pages, cache.weight)
+    _no_grad_only(op, cache, q)
     Hq = q.shape[2]
     if Hq < 1 or Hq % cache.kv_heads:
         raise ValueError(f"{op}: {Hq} query heads are not a multiple of the cache's {cache.kv_heads}")
@@ -340,13 +358,12 @@ def _attend(q, cache, scale, causal, accumulate):
     """The launch: (o, lse)."""
     S, Hq = q.shape[1], q.shape[2]
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty((cache.batch, Hq, S), device=q.device, dtype=torch.float32)
+    lse = cache._floats.new_empty((cache.batch, Hq, S))
     q, strides = readable_rows(q)
-    ws_ptr, ws_size, ws = cache._workspace(
-        (S, Hq, accumulate), lambda: nat.paged_attn_workspace_bytes(cache._c, S, Hq, accumulate))
+    ws_ptr, ws_size, ws = cache._workspace(nat.paged_attn_workspace_bytes, S, Hq, accumulate)
     with nat.on_device(cache.device):
         nat.check(nat.lib().dmad_paged_attn(
-            nat.dtype_code(cache.dtype), cache._ref, S, Hq, nat.ptr(q), strides, int(causal), int(accumulate), scale,
+            cache._code, cache._ref, S, Hq, nat.ptr(q), strides, int(causal), int(accumulate), scale,
             nat.ptr(o), nat.ptr(lse), ws_ptr, ws_size, nat.stream_ptr(cache.device)))
     return o, lse
 
@@ -376,7 +393,7 @@ def evict_low_weight(cache, keep, recent=0, sink=0):
                          f"keep={keep}, recent={recent}, sink={sink}")
     if keep >= cache.capacity or cache.batch == 0:
         return  # no sequence can be longer
-    _no_grad_only(op, cache.k_pages, cache.v_pages, cache.weight)
+    _no_grad_only(op, cache)
     if _eager_call():
         _evict(cache, keep, recent, sink)
         cache._changed("evict")
@@ -387,7 +404,7 @@ def evict_low_weight(cache, keep, recent=0, sink=0):
 
 def _evict(cache, keep, recent, sink):
     """The launches."""
-    ws_ptr, ws_size, ws = cache._workspace(("evict", keep), lambda: nat.kv_evict_workspace_bytes(cache._c, keep))
+    ws_ptr, ws_size, ws = cache._workspace(nat.kv_evict_workspace_bytes, keep)
     with nat.on_device(cache.device):
-        nat.check(nat.lib().dmad_kv_evict(nat.dtype_code(cache.dtype), cache._ref, keep, recent, sink, ws_ptr, ws_size,
+        nat.check(nat.lib().dmad_kv_evict(cache._code, cache._ref, keep, recent, sink, ws_ptr, ws_size,
                                           nat.stream_ptr(cache.device)))
