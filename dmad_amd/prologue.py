@@ -377,19 +377,24 @@ def _qk_gradients(call, q, k, gq, gk, wq, wk, need_wq, need_wk):
             dwk = torch.empty_like(ck)
     else:
         k, ck, Hk = None, None, 0
-    if call.B * call.S == 0:
-        for dw in (dwq, dwk):
-            if dw is not None:
-                dw.zero_()
-    else:
-        if dwq is not None or dwk is not None:
+    tokens = call.B * call.S
+    # without rows a weight's gradient is zero, and the kernels are not asked for it
+    ask_q, ask_k = dwq, dwk
+    if dwq is not None and tokens * Hq == 0:
+        ask_q, cq = None, None
+        dwq.zero_()
+    if dwk is not None and tokens * Hk == 0:
+        ask_k, ck = None, None
+        dwk.zero_()
+    if tokens * (Hq + Hk):
+        if ask_q is not None or ask_k is not None:
             ws_ptr, ws_size, ws = nat.workspace(
                 nat.qk_norm_rope_bwd_workspace_bytes(call.B, call.S, Hq, Hk, call.D), dev)
         with nat.on_device(dev):
             nat.check(nat.lib().dmad_qk_norm_rope_bwd(
                 call.code, call.wcode, call.B, call.S, Hq, Hk, call.D, nat.ptr(q), nat.ptr(gq), nat.ptr(k), nat.ptr(gk),
                 sq, sgq, sk, sgk, nat.ptr(cq), nat.ptr(ck), nat.ptr(call.freqs), call.freqs_b, call.eps, nat.ptr(dq),
-                nat.ptr(dk), nat.ptr(dwq), nat.ptr(dwk), ws_ptr, ws_size, nat.stream_ptr(dev)))
+                nat.ptr(dk), nat.ptr(ask_q), nat.ptr(ask_k), ws_ptr, ws_size, nat.stream_ptr(dev)))
     if dwq is not None and dwq.dtype != wq.dtype:
         dwq = dwq.to(wq.dtype)
     if dwk is not None and dwk.dtype != wk.dtype:

@@ -683,3 +683,27 @@ def test_op_and_direct_calls_agree_bitwise(request, monkeypatch, device, how, ab
     assert len(got) == len(want)
     for a, b in zip(got, want):
         assert a.requires_grad == b.requires_grad and torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("empty", ["q", "k"])
+def test_an_operand_without_heads(gpu, empty):
+    """q or k of no heads beside the other: empty results and a zero gradient of its weight, the other as alone."""
+    from dmad_amd import qk_norm_rope_with_tangent
+
+    x = _small(gpu, dtype=torch.bfloat16)
+    other = "k" if empty == "q" else "q"
+    for n in ("q", "k", "wq", "wk"):
+        x[n] = (x[n][:, :, :0] if n == empty else x[n]).detach().requires_grad_(True)
+    (q, _), (k, _) = qk_norm_rope_with_tangent((x["q"], None), (x["k"], None), x["wq"], x["wk"], 1e-6, x["freqs"])
+    y, none = (k, q) if empty == "q" else (q, k)
+    assert none.shape == (2, 5, 0, 16)
+    gx, gw = torch.autograd.grad(y.float().square().sum(), (x[other], x["w" + other]), retain_graph=True)
+    both = torch.autograd.grad(y.float().square().sum() + none.float().sum(), (x[other], x["w" + other], x[empty], x["w" + empty]))
+    assert torch.equal(both[0], gx) and torch.equal(both[1], gw)
+    assert both[2].shape == (2, 5, 0, 16) and torch.equal(both[3], torch.zeros_like(both[3])) and both[3].shape == (16,)
+    # the empty one alone
+    (q, _), (k, _) = qk_norm_rope_with_tangent((x["q"], None), (x["k"], None), x["wq"], x["wk"], 1e-6, x["freqs"])
+    none = q if empty == "q" else k
+    ge, gw = torch.autograd.grad(none.float().sum(), (x[empty], x["w" + empty]))
+    assert ge.shape == (2, 5, 0, 16) and torch.equal(gw, torch.zeros_like(gw))
