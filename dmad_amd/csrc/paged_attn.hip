@@ -195,6 +195,9 @@ __device__ __forceinline__ void load_v(const char* base, uint32_t off, uint32_t 
 // CAUSAL: rows of different tokens see different slots.
 template <typename T, int D, int NT, bool ACC, bool CAUSAL>
 __global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged_attn_kernel(PagedAttnParams p) {
+  // no contraction but the written ones: a call that accumulates has the outputs
+  // of one that does not, bit for bit
+#pragma clang fp contract(off)
   using C = PagedCfg<D>;
   __shared__ float sm_o[kPagedWaves][16][C::OP];
   __shared__ float sm_m[kPagedWaves][NT * 16], sm_l[kPagedWaves][NT * 16];
@@ -500,6 +503,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged
 // Joins the pieces of one row: D/4 lanes per piece, the pieces over the rest.
 template <typename T, int D, bool ACC>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
+#pragma clang fp contract(off)  // as in paged_attn_kernel
   constexpr int LANES = D / 4, STRANDS = 256 / LANES;
   __shared__ float sm_o[STRANDS][D], sm_m[STRANDS], sm_l[STRANDS];
   const KvPages& kv = p.kv;

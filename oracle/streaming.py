@@ -120,6 +120,43 @@ def attend(c, q, scale=None, causal=False, accumulate=False):
     return o, lse, (pv, sv, size)
 
 
+def attend_long(c, q, scale=None, causal=False, accumulate=False):
+    """``attend`` a key head at a time, for long caches, on whichever device the cache lies."""
+    B, S, Hq, D = q.shape
+    N, Hk, P, _ = c["k_pages"].shape
+    G, dev = Hq // Hk, c["k_pages"].device
+    scale = D ** -0.5 if scale is None else scale
+    o = torch.zeros(B, S, Hq, D, dtype=torch.float64, device=dev)
+    lse = torch.full((B, Hq, S), -math.inf, dtype=torch.float64, device=dev)
+    pv, sv = torch.zeros_like(o), torch.zeros_like(o)
+    size = torch.zeros(B, S, Hq, 1, dtype=torch.float64, device=dev)
+    if accumulate:
+        c["weight"] = c["weight"].double()
+    for b in range(B):
+        n = length(c, b)
+        slot = torch.arange(n, device=dev)
+        page = c["page_table"][b].long()[slot // P]
+        there = (page >= 0) & (page < N)
+        slot, page = slot[there], page[there]
+        see = torch.arange(S, device=dev).repeat_interleave(G) + (n - S + 1) if causal else torch.full((S * G,), n, device=dev)
+        seen = slot[None] < see[:, None]
+        some = seen.any(1)
+        if not bool(some.any()):
+            continue
+        for h in range(Hk):
+            k, v = (c[x][page, h, slot % P].double() for x in ("k_pages", "v_pages"))
+            rows = q[b, :, h * G:(h + 1) * G].reshape(S * G, D).double()
+            s = (rows @ k.T.contiguous() * scale).masked_fill(~seen, -math.inf)
+            p = torch.where(some[:, None], torch.softmax(s, 1), torch.zeros((), dtype=torch.float64, device=dev))
+            at = (b, slice(None), slice(h * G, (h + 1) * G))
+            o[at], pv[at], sv[at] = (x.view(S, G, D) for x in (p @ v, p @ v.abs(), seen.double() @ v.abs()))
+            lse[b, h * G:(h + 1) * G] = torch.logsumexp(s, 1).view(S, G).T
+            size[at] = ((rows.abs() @ k.abs().T.contiguous() * scale) * seen).amax(1).view(S, G, 1)
+            if accumulate:
+                c["weight"].index_put_((page, torch.tensor(h, device=dev), slot % P), p.sum(0), accumulate=True)
+    return o, lse, (pv, sv, size)
+
+
 def evict(c, keep, recent=0, sink=0):
     """Cuts the cache in place. Only slots that a page holds count: the sequence then ends behind the
     keep-th of them."""

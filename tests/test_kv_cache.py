@@ -1218,3 +1218,118 @@ def test_replaced_memory_is_followed(request, monkeypatch, device):
             paged_attention(x["q"], cache)
     cache.k_pages.data = good
     assert torch.equal(paged_attention(x["q"], cache), paged_attention(x["q"], other))
+
+
+# ---------------------------------------------------------------- long pieces
+
+
+def test_oracle_attention_a_head_at_a_time():
+    """The oracle for long caches is the one of single tokens and heads."""
+    g = torch.Generator().manual_seed(80)
+    for causal in (False, True):
+        c = dict(k_pages=torch.randn(9, 2, 16, 16, generator=g), v_pages=torch.randn(9, 2, 16, 16, generator=g),
+                 page_table=torch.randperm(9, generator=g)[:8].view(2, 4).to(torch.int32), lengths=torch.tensor([2, 60]),
+                 seen=torch.tensor([2, 60]), weight=torch.rand(9, 2, 16, generator=g))
+        c["page_table"][1, 1] = -1
+        d = {n: t.clone() for n, t in c.items()}
+        q = torch.randn(2, 3, 4, 16, generator=g)
+        a, b = st.attend(c, q, causal=causal, accumulate=True), st.attend_long(d, q, causal=causal, accumulate=True)
+        for x, y in zip((*a[:2], *a[2]), (*b[:2], *b[2])):
+            assert torch.equal(torch.isinf(x), torch.isinf(y))
+            torch.testing.assert_close(x.nan_to_num(0, 0, 0), y.nan_to_num(0, 0, 0), rtol=1e-12, atol=1e-12)
+        torch.testing.assert_close(c["weight"], d["weight"], rtol=1e-12, atol=1e-12)
+
+
+LONG = [
+    # S, Hq, Hk, D, dtype, page, lengths, causal, accumulate; tiles of 128 slots per piece, at least
+    (1, 40, 40, 128, "bf16", 16, [3000, 1, 700, 5000, 129], False, True, 12),  # pieces over several sequences
+    (1, 64, 64, 128, "bf16", 64, [20001], False, False, 33),  # more steps per wave than page ids are looked up at once
+    (1, 128, 64, 16, "fp16", 16, [50000], False, True, 33),
+    (2, 64, 8, 64, "bf16", 32, [9001, 4000, 30, 12000, 11111, 9090], True, True, 4),
+    (4, 64, 8, 64, "fp16", 16, [9001, 4000, 4, 12000, 11111, 9090], True, False, 4),  # two row tiles
+    (16, 80, 40, 128, "bf16", 48, [4000, 2500], True, True, 8),  # two row tiles
+    (40, 16, 16, 128, "fp16", 16, [5000, 41], True, False, 3),  # two groups of rows
+    (3, 32, 32, 256, "bf16", 16, [3000, 2000], True, True, 5),
+    (20, 32, 32, 256, "fp16", 64, [2500], True, False, 2),
+    (1, 100, 100, 32, "bf16", 128, [9000, 0, 77, 6000], False, False, 20),
+    (1, 64, 64, 16, "bf16", 16, [(97 * i) % 900 for i in range(130)], False, True, 30),  # more than 64 sequences
+]
+
+
+def _tiles_per_piece(Hk, D, page, S, Hq, lengths, room):
+    """Tiles that a piece of the attention covers: the number of pieces from the scratch that it asks for."""
+    from dmad_amd import _native as nat
+
+    B, M = len(lengths), -(-(max(lengths) + room) // page)
+    c = _c_cache(nat, num_pages=B * M, kv_heads=Hk, page_size=page, head_dim=D, batch=B, pages_per_seq=M, table_stride=M,
+                 ks=(Hk * page * D, page * D, D), vs=(Hk * page * D, page * D, D))
+    row = Hk * (S * Hq // Hk) * (4 * D + 8)
+    pieces = (nat.paged_attn_workspace_bytes(c, S, Hq, False) - 512) // row - B  # the two parts are rounded up to 256
+    tiles = sum(max(1, -(-n // 128)) for n in lengths)
+    return -(-tiles // (pieces + 1)), pieces
+
+
+@pytest.mark.parametrize("S,Hq,Hk,D,dtype,page,lengths,causal,accumulate,least", LONG)
+def test_long_cases_have_long_pieces(S, Hq, Hk, D, dtype, page, lengths, causal, accumulate, least):
+    """A wave takes one step of 32 slots per tile: these cases run the attention's loop, not its last step alone."""
+    per_piece, pieces = _tiles_per_piece(Hk, D, page, S, Hq, lengths, 5)
+    assert per_piece >= least, (per_piece, pieces)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,Hq,Hk,D,dtype,page,lengths,causal,accumulate,least", LONG)
+def test_attention_of_long_pieces(gpu, S, Hq, Hk, D, dtype, page, lengths, causal, accumulate, least):
+    from dmad_amd import paged_attention
+
+    B, t = len(lengths), DTYPES[dtype]
+    print(f"case long B={B} S={S} Hq={Hq} Hk={Hk} D={D} {dtype} page={page} lengths={lengths[:4]} causal={causal}", flush=True)
+    cache = _make(gpu, B, Hk, D, t, page, lengths, room=5, seed=D + S)
+    # whole pages missing inside pieces, one of them in the last, and an id beyond the pool
+    longest = lengths.index(max(lengths))
+    cache.page_table[longest, [3, 17, (max(lengths) - 1) // page // 2]] = torch.tensor([-1, cache.k_pages.shape[0], -7], dtype=torch.int32, device=gpu)
+    q = (torch.randn(B, S, Hq, D, generator=torch.Generator().manual_seed(1)) * 1.5).to(t).to(gpu)
+    c = {n: getattr(cache, n) for n in st.FIELDS}
+    before = cache.weight.clone()
+    ref = st.attend_long(c, q, causal=causal, accumulate=accumulate)
+    got = paged_attention(q, cache, causal=causal, accumulate=accumulate, return_lse=True)
+    torch.cuda.synchronize()
+    ro, rlse, bound = ref[0].cpu(), ref[1].cpu(), tuple(x.cpu() for x in ref[2])
+    _check_attention(got, (ro, rlse, bound), t, D)
+    if accumulate:
+        w, r = cache.weight.cpu().double(), c["weight"].cpu()
+        _same("weights of unused slots", torch.isnan(w).float(), torch.isnan(r).float())
+        share = (r - before.cpu().double()).nan_to_num(0)
+        worst = float(bound[2].max()) * (D + 8) * F32 * 2 + 128 * F32 * (1 + float(rlse[~torch.isinf(rlse)].abs().max()))
+        assert ((w - r).abs().nan_to_num(0) <= worst * share + 2 * F32 * r.abs().nan_to_num(0) + 1e-30).all()
+    for _ in range(2):
+        assert torch.equal(paged_attention(q, cache, causal=causal), got[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,Hq,Hk,D,dtype,lengths", [(4, 64, 64, 128, "bf16", [3000, 2000]), (3, 128, 64, 64, "fp16", [4000]),
+                                                     (5, 40, 40, 256, "bf16", [2600]), (17, 80, 40, 32, "fp16", [70, 5000])])
+def test_hidden_tokens_after_long_pieces(gpu, S, Hq, Hk, D, dtype, lengths):
+    """Infinities and NaN in the new tokens' values, behind many steps that need no mask: they reach the tokens that
+    see them, of their key head and sequence, and no other."""
+    from dmad_amd import paged_attention
+
+    B, t, G = len(lengths), DTYPES[dtype], Hq // Hk
+    assert _tiles_per_piece(Hk, D, 16, S, Hq, lengths, 0)[0] >= 3
+    cache = _make(gpu, B, Hk, D, t, 16, lengths, seed=90 + D)
+    q = torch.randn(B, S, Hq, D, generator=torch.Generator().manual_seed(3)).to(t).to(gpu)
+    clean = paged_attention(q, cache, causal=True)
+    ref = st.attend_long({n: getattr(cache, n) for n in st.FIELDS}, q, causal=True)
+    _check_attention((clean, ref[1].float()), (ref[0].cpu(), ref[1].cpu(), tuple(x.cpu() for x in ref[2])), t, D)
+    head = Hk // 2
+    rows = slice(head * G, head * G + G)
+    for token in (0, 1, S - 1):
+        for name, value in (("v_pages", math.inf), ("v_pages", math.nan), ("k_pages", math.nan)):
+            page, slot = st.locate(st.cache_of(cache), B - 1, lengths[-1] - S + token)
+            pages = getattr(cache, name)
+            keep = pages[page, head, slot].clone()
+            pages[page, head, slot] = value
+            o = paged_attention(q, cache, causal=True)
+            assert not torch.isfinite(o[-1, token:, rows].float()).any(), (token, name)
+            o[-1, token:, rows] = clean[-1, token:, rows]
+            assert torch.equal(o, clean), (token, name)
+            pages[page, head, slot] = keep
