@@ -707,3 +707,64 @@ def test_an_operand_without_heads(gpu, empty):
     none = q if empty == "q" else k
     ge, gw = torch.autograd.grad(none.float().sum(), (x[empty], x["w" + empty]))
     assert ge.shape == (2, 5, 0, 16) and torch.equal(gw, torch.zeros_like(gw))
+
+
+# ---------------------------------------------------------------- sizes whose waves take several passes, past the caches
+
+
+LARGE = [
+    # S, Hq, Hk, D, dtype: odd numbers of wave passes per token, q's and k's within one wave's share
+    (12701, 20, 8, 128, "bf16"),
+    (17001, 33, 9, 64, "fp16"),
+    (8001, 20, 8, 128, "fp32"),
+    (15001, 9, 4, 256, "bf16"),
+    (8803, 5, 12, 256, "fp32"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,Hq,Hk,D,dtype", LARGE)
+def test_large_calls(gpu, S, Hq, Hk, D, dtype):
+    """What the large calls do and small ones do not: more than two passes per wave (from three rounds of 16384
+    waves on) and, with tangents and backwards, more bytes than the caches hold, which go past them."""
+    from dmad_amd import qk_norm_rope_with_tangent
+
+    t = DTYPES[dtype]
+    passes = -(-Hq * D // 512) + -(-Hk * D // 512)
+    assert S * passes >= 3 * 16384 and passes % 2 and 3 * S * (Hq + Hk) * D * t.itemsize > 256 << 20
+    print(f"case large norm S={S} Hq={Hq} Hk={Hk} D={D} {dtype}", flush=True)
+    g = torch.Generator(device=gpu).manual_seed(S)
+
+    def r(*shape, sd=1.0):
+        return (torch.randn(shape, generator=g, device=gpu) * sd).to(t)
+
+    x = dict(q=r(1, S, Hq, D), k=r(1, S, Hk, D), tq=r(1, S, Hq, D, sd=0.1), tk=r(1, S, Hk, D, sd=0.1), gq=r(1, S, Hq, D), gk=r(1, S, Hk, D),
+             wq=1 + 0.3 * r(D).float(), wk=1 + 0.3 * r(D).float())
+    f = torch.rand(S, D // 2, generator=g, device=gpu) * 200 - 100
+    leaves = [x[n].requires_grad_(True) for n in ("q", "k", "wq", "wk")]
+    (q, tq), (k, tk) = qk_norm_rope_with_tangent((x["q"], x["tq"]), (x["k"], x["tk"]), x["wq"], x["wk"], 1e-6, f)
+    grads = torch.autograd.grad((q, k), leaves, (x["gq"], x["gk"]))
+    torch.cuda.synchronize()
+    for n, y, ty, dx, dw in (("q", q, tq, grads[0], grads[2]), ("k", k, tk, grads[1], grads[3])):
+        z, w, d = x[n].detach().double(), x["w" + n].detach().double(), x["t" + n].double()
+        root = (z.pow(2).mean(-1, keepdim=True) + 1e-6).rsqrt()
+        m = z * root
+        _check_there(n, y, st.rotate(m * w, f), None)
+        mean = (m * d).mean(-1, keepdim=True)
+        size = _pair_size((d.abs() + m.abs() * (m * d).abs().mean(-1, keepdim=True)) * root * w.abs())
+        _check_there("t" + n, ty, st.rotate((d - m * mean) * root * w, f), size)
+        u = st.rotate(x["g" + n].double(), -f)
+        _check_there("dw" + n, dw, (u * m).sum((0, 1, 2)), (u * m).abs().sum((0, 1, 2)))
+        a = u * w
+        size = root * (_pair_size(a) + m.abs() * (a * m).abs().mean(-1, keepdim=True))
+        _check_there("d" + n, dx, root * (a - m * (a * m).mean(-1, keepdim=True)), size)
+
+
+def _check_there(name, got, ref, size):
+    """_check on the device, a part at a time."""
+    size = _pair_size(ref) if size is None else size
+    if got.dim() == 4:
+        for i in range(0, got.shape[1], 2000):
+            _check(name, *(t[:, i:i + 2000].cpu() for t in (got.detach(), ref, size)))
+    else:
+        _check(name, got.detach().cpu(), ref.cpu(), size.cpu())
