@@ -1333,3 +1333,23 @@ def test_hidden_tokens_after_long_pieces(gpu, S, Hq, Hk, D, dtype, lengths):
             o[-1, token:, rows] = clean[-1, token:, rows]
             assert torch.equal(o, clean), (token, name)
             pages[page, head, slot] = keep
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Hk,D,page,length,keep", [(4, 32, 256, 16, 900, 420), (130, 40, 128, 16, 44, 20), (1, 5, 64, 48, 7000, 33)])
+def test_evict_more_rows_than_workgroups(gpu, B, Hk, D, page, length, keep):
+    """Copies whose workgroups take several rows each, and a capacity of which nearly nothing moves."""
+    from dmad_amd import evict_low_weight
+
+    cache = _make(gpu, B, Hk, D, torch.bfloat16, page, [length - b % 7 for b in range(B)], seed=keep)
+    c = st.cache_of(cache)
+    st.evict(c, keep, 5, 1)
+    evict_low_weight(cache, keep, recent=5, sink=1)
+    torch.cuda.synchronize()
+    for n in st.FIELDS:
+        _same(n, getattr(cache, n), c[n])
+    cache.lengths.fill_(keep)  # nothing to cut
+    c = st.cache_of(cache)
+    evict_low_weight(cache, keep, recent=5)
+    for n in st.FIELDS:
+        _same(n, getattr(cache, n), c[n])
