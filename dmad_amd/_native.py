@@ -246,11 +246,13 @@ class _HereAlready:
 
 
 _here = _HereAlready()
+# (without torch.cuda.current_device's look at whether the GPU is in use yet: a tensor lies on it)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def on_device(device: torch.device):
     """A context in which ``device`` is the current one (launches need its streams' device current)."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == _current_device():
         return _here
     return torch.cuda.device(device)
 

@@ -27,6 +27,9 @@ from .jvp_attention import _eager_call
 from .prologue import HEAD_DIMS, _check_same_device, _norm_weights, _weights_dtype, readable_rows, refuse_forward_mode
 
 
+# torch.autograd.graph.increment_version of a list
+_increment_version = torch._C._increment_version
+
 CACHE_TENSORS = ("k_pages", "v_pages", "page_table", "lengths", "seen", "weight", "position")
 
 
@@ -158,8 +161,7 @@ class PagedKVCache:
 
     def _changed(self, by):
         """The launches of an ordinary eager call write through addresses: counted as changes in place here."""
-        if self._written[by]:
-            torch.autograd.graph.increment_version(self._written[by])
+        _increment_version(self._written[by])
 
     def _workspace(self, query, *args):
         """(pointer, size, owner) of a fresh workspace whose size ``query`` gives, asked once per call's sizes."""
