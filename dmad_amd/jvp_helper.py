@@ -132,8 +132,9 @@ class MinimalA2AAttnOpWithT(nn.Module):
     are already rotated, then the query, and the whole key otherwise; rotated
     tangents are detached. The remaining arguments go to ``local_attn_T``
     (``FlexOrSdpaLocalAttentionWithT`` takes ``attn_meta``). Context parallelism
-    (a process group of more than one rank) and the KV cache of streaming
-    inference are not part of this one-GPU build and raise.
+    (a process group of more than one rank) is not part of this one-GPU build,
+    and a KV cache with tangents is not either: both raise. Without tangents a
+    student streams through ``dmad_amd.PagedKVCache``.
     """
 
     def __init__(self, local_attn_T=torch_attention_op_withT):
@@ -153,7 +154,8 @@ class MinimalA2AAttnOpWithT(nn.Module):
         cache = getattr(attn_ctx, "kv_cache", None) if attn_ctx is not None else None
         mode = getattr(attn_ctx, "mode", None)
         if cache is not None and getattr(mode, "name", mode) != "DISABLED":
-            raise NotImplementedError("the KV cache of streaming inference is not part of this build")
+            raise NotImplementedError("a KV cache with tangents is not part of this build; streaming inference without "
+                                      "tangents runs on dmad_amd.PagedKVCache, append_kv and paged_attention")
         rope = attn_ctx.rope if attn_ctx is not None else None
         if rope is not None and rope.cached_k_rotated and rope.current_key_freqs is not None:
             key_withT = _rotate(key_withT, rope.current_key_freqs)

@@ -1353,3 +1353,46 @@ def test_evict_more_rows_than_workgroups(gpu, B, Hk, D, page, length, keep):
     evict_low_weight(cache, keep, recent=5)
     for n in st.FIELDS:
         _same(n, getattr(cache, n), c[n])
+
+
+# ---------------------------------------------------------------- a student of this package, block by block
+
+
+def test_the_tangent_module_names_the_cache():
+    from types import SimpleNamespace
+
+    from dmad_amd import MinimalA2AAttnOpWithT
+
+    with pytest.raises(NotImplementedError, match="PagedKVCache"):
+        MinimalA2AAttnOpWithT()(None, None, None, attn_ctx=SimpleNamespace(rope=None, kv_cache=object(), mode="APPEND"))
+
+
+@pytest.mark.gpu
+def test_a_student_that_norms_over_the_width(gpu):
+    """Queries and keys normalised over the model width and rotated by the prologue, block after block into the
+    cache: each block attends to itself and what came before, as the dense attention does over the same keys."""
+    from dmad_amd import PagedKVCache, append_kv, paged_attention, plain_attention, rmsnorm_rope_with_tangent
+
+    B, block, blocks, H, D = 2, 24, 4, 4, 64
+    g = torch.Generator().manual_seed(40)
+    qkv = torch.randn(B, block * blocks, 3, H * D, generator=g).bfloat16().to(gpu)
+    wq, wk = ((1 + 0.2 * torch.randn(H * D, generator=g)).bfloat16().to(gpu) for _ in range(2))
+    freqs = (torch.rand(block * blocks, D // 2, generator=g) * 50).to(gpu)
+    cache = PagedKVCache.allocate(B, block * blocks, H, D, device=gpu, page_size=16, track_weights=False)
+    keys, values = [], []
+    for i in range(blocks):
+        at = slice(i * block, (i + 1) * block)
+        y = qkv[:, at].contiguous()
+        with torch.no_grad():
+            q, _ = rmsnorm_rope_with_tangent((y[:, :, 0].contiguous(), None), wq, 1e-6, freqs[at], H)
+            k, _ = rmsnorm_rope_with_tangent((y[:, :, 1].contiguous(), None), wk, 1e-6, freqs[at], H)
+        v = y[:, :, 2].reshape(B, block, H, D)
+        append_kv(k, v, cache)
+        ref = st.attend(st.cache_of(cache), q.cpu())
+        got = paged_attention(q, cache, return_lse=True)
+        _check_attention(got, ref, torch.bfloat16, D)
+        keys.append(k), values.append(v)
+        dense = plain_attention(*(x.transpose(1, 2).contiguous() for x in (q, torch.cat(keys, 1), torch.cat(values, 1))))
+        dense = dense.transpose(1, 2).float()
+        assert float((got[0].float() - dense).norm() / dense.norm()) < 5e-3
+    assert cache.lengths.tolist() == cache.seen.tolist() == [block * blocks] * B
