@@ -56,7 +56,8 @@ class PagedKVCache:
     by writing to ``page_table`` and ``lengths``. Where a tensor's memory is replaced (``t.data = ...``)
     the next call checks and uses the new one; a captured graph keeps the one it was captured with. A page may appear in several sequences as long
     as it is only read; pages that are appended to, evicted from or whose weights are accumulated
-    belong to one sequence. Calls that only read a cache may run on several streams at once; one
+    belong to one sequence, whose row names them once. ``lengths`` and ``seen``, or ``k_pages`` and
+    ``v_pages``, may be one memory only where nothing is appended or evicted. Calls that only read a cache may run on several streams at once; one
     that appends, accumulates or evicts is ordered by the caller against all others, as with any
     tensor changed in place. Such calls count as changes in place for autograd: a backward pass that
     needs what they overwrote raises.
@@ -112,6 +113,12 @@ class PagedKVCache:
                         strides("v_pages", v_pages), nat.ptr(page_table), page_table.stride(0) if B > 1 else M,
                         nat.ptr(lengths), nat.ptr(seen), nat.ptr(weight), nat.ptr(position))
         tensors = [t for t in _cache_tensors(self) if t is not None]
+        # one memory for two of them serves a cache that is only read
+        shared = ""
+        if B and abs(lengths.data_ptr() - seen.data_ptr()) < 4 * B:
+            shared = "lengths and seen"
+        elif k_pages.data_ptr() == v_pages.data_ptr():
+            shared = "k_pages and v_pages"
         described = dict(
             device=device, dtype=k_pages.dtype, batch=B, kv_heads=Hk, page_size=P, head_dim=D, capacity=M * P, _c=c,
             _code=nat.dtype_code(k_pages.dtype), _sizes={}, _pointers=[t.data_ptr for t in tensors],
@@ -122,7 +129,7 @@ class PagedKVCache:
             _written={by: [t for t in ts if t is not None and not t.is_inference()] for by, ts in (
                 ("append", (k_pages, v_pages, lengths, seen, weight, position)), ("attend", (weight,)),
                 ("evict", (k_pages, v_pages, lengths, weight, position)))},
-            _ref=ctypes.byref(c))
+            _shared=shared, _ref=ctypes.byref(c))
         self.__dict__.update(described)
 
     def _settle(self):
@@ -158,6 +165,10 @@ class PagedKVCache:
             torch.zeros(pages, device=device, dtype=torch.float32) if track_weights else None,
             torch.zeros(pages, device=device, dtype=torch.int32) if track_weights else None,
         )
+
+    def _writable(self, op):
+        if self._shared:
+            raise ValueError(f"{op}: {self._shared} of the cache share memory, and each is written")
 
     def _changed(self, by):
         """The launches of an ordinary eager call write through addresses: counted as changes in place here."""
@@ -272,6 +283,7 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, eps, freqs, cache):
     if k is None or v is None:
         raise ValueError(f"{op}: k and v must be given")
     _check_new(op, cache, ("k", k), ("v", v), ("q", q))
+    cache._writable(op)
     for t in (q_weight, k_weight, freqs):
         _on_cache(op, cache, t)
     _no_grad_only(op, cache, q, k, v, q_weight, k_weight, freqs)
@@ -322,8 +334,8 @@ def paged_attention(q, cache, sm_scale=None, causal=False, accumulate=False, ret
     Made for few new tokens (S = 1, a draft of a few, a small block): the work is split over the
     cache's length. Hq is a multiple of the cache's heads; query head h reads key head
     h // (Hq // Hk). ``sm_scale`` defaults to D^-1/2. Every token sees all slots in use;
-    with ``causal`` the S tokens are the last S slots (just appended, nothing evicted since) and
-    each sees the slots up to its own. A token that sees no slot gets o = 0 and lse = -inf, and so
+    with ``causal`` the S tokens are the last S slots (just appended, none dropped for want of room,
+    nothing evicted since) and each sees the slots up to its own. A token that sees no slot gets o = 0 and lse = -inf, and so
     does one whose scores are all -inf. What a slot that a token does not see holds, infinities and
     NaN among it, does not reach the token.
 
@@ -395,6 +407,7 @@ def evict_low_weight(cache, keep, recent=0, sink=0):
                          f"keep={keep}, recent={recent}, sink={sink}")
     if keep >= cache.capacity or cache.batch == 0:
         return  # no sequence can be longer
+    cache._writable(op)
     _no_grad_only(op, cache)
     if _eager_call():
         _evict(cache, keep, recent, sink)

@@ -367,7 +367,8 @@ int dmad_qk_norm_rope_bwd(int dtype, int wdtype, int64_t B, int64_t S, int64_t H
  * outside [0, num_pages) marks a page that holds nothing: its slots are
  * neither read nor written, and no row attends to them. Lengths outside
  * [0, pages_per_seq * page_size] are clipped. Pages that are written belong to
- * one sequence.
+ * one sequence, whose row names them once; lengths and seen, and k_pages and
+ * v_pages, are memories of their own where they are written.
  *   k_strides, v_strides: elements between pages, heads and slots; the head
  *           dim's is 1
  *   weight, position: [num_pages][kv_heads][page_size], 16-byte aligned, or

@@ -1396,3 +1396,31 @@ def test_a_student_that_norms_over_the_width(gpu):
         dense = dense.transpose(1, 2).float()
         assert float((got[0].float() - dense).norm() / dense.norm()) < 5e-3
     assert cache.lengths.tolist() == cache.seen.tolist() == [block * blocks] * B
+
+
+@BOTH
+def test_one_memory_for_two_tensors_is_not_written(request, monkeypatch, device):
+    """lengths given as seen too ("equal until something is evicted") would advance twice per token, and keys and
+    values in one memory overwrite each other: refused by what writes, fine for what reads."""
+    from dmad_amd import PagedKVCache, append_kv, evict_low_weight, paged_attention
+
+    cache, x = _loop(request, monkeypatch, device)
+    t = {n: getattr(cache, n) for n in st.FIELDS}
+    both = torch.zeros(3, device=t["lengths"].device, dtype=torch.int32)
+    both[:2] = t["lengths"]
+    want = paged_attention(x["q"], cache)
+    for over, match in ((dict(seen=t["lengths"]), "lengths and seen"), (dict(lengths=both[:2], seen=both[1:]), "lengths and seen"),
+                        (dict(v_pages=t["k_pages"]), "k_pages and v_pages")):
+        same = PagedKVCache(**{**t, **over})
+        before = st.cache_of(same)
+        with pytest.raises(ValueError, match=match):
+            append_kv(x["k"], x["v"], same)
+        with pytest.raises(ValueError, match=match):
+            evict_low_weight(same, 24)
+        if "v_pages" not in over:
+            assert torch.equal(paged_attention(x["q"], same), want)
+        for n in st.FIELDS:
+            _same(n, getattr(same, n), before[n])
+    counts = torch.stack([t["lengths"], t["seen"]])  # beside each other in one tensor
+    append_kv(x["k"], x["v"], PagedKVCache(**{**t, "lengths": counts[0], "seen": counts[1]}))
+    assert counts[0].tolist() == [39, 22] and counts[1].tolist() == [39, 22]
