@@ -1424,3 +1424,49 @@ def test_one_memory_for_two_tensors_is_not_written(request, monkeypatch, device)
     counts = torch.stack([t["lengths"], t["seen"]])  # beside each other in one tensor
     append_kv(x["k"], x["v"], PagedKVCache(**{**t, "lengths": counts[0], "seen": counts[1]}))
     assert counts[0].tolist() == [39, 22] and counts[1].tolist() == [39, 22]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["qk_norm_rope_append", "append without q", "paged_attn", "paged_attn weights", "kv_evict"])
+def test_registered_ops_do_what_they_declare(gpu, op):
+    """torch's own checks: what is written is what the schema names, and the shapes are those of the fakes."""
+    from dmad_amd import PagedKVCache
+
+    cache = PagedKVCache.allocate(2, 64, 2, 16, device=gpu, page_size=16)
+    g = torch.Generator().manual_seed(95)
+    for n in ("k_pages", "v_pages"):
+        getattr(cache, n).copy_(torch.randn(cache.k_pages.shape, generator=g))
+    cache.weight.copy_(torch.rand(cache.weight.shape, generator=g))
+    cache.position.copy_(torch.arange(cache.position.numel()).view_as(cache.position) % 50)
+    cache.lengths.fill_(40), cache.seen.fill_(40)
+    c = [getattr(cache, n) for n in ("k_pages", "v_pages", "page_table", "lengths", "seen", "weight", "position")]
+    q, k = (torch.randn(2, 3, h, 16, generator=g).bfloat16().to(gpu) for h in (4, 2))
+    w, f = torch.ones(16, device=gpu), torch.rand(60, 8, generator=g).to(gpu)
+    args = {"qk_norm_rope_append": (q, k, k.clone(), w, None, 1e-6, f, *c), "append without q": (None, k, k.clone(), None, None, 0.0, None, *c),
+            "paged_attn": (q, 0.25, True, *c[:5], None, None), "paged_attn weights": (q, 0.25, False, *c), "kv_evict": (20, 3, 1, *c)}[op]
+    name = {"append without q": "qk_norm_rope_append", "paged_attn weights": "paged_attn"}.get(op, op)
+    torch.library.opcheck(getattr(torch.ops.dmad, name).default, args, test_utils=("test_schema", "test_faketensor", "test_aot_dispatch_dynamic"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_subnormal_keys_and_values(gpu, dtype):
+    """Keys and values below the type's smallest normal are not flushed."""
+    from dmad_amd import paged_attention
+
+    t = DTYPES[dtype]
+    for which in ("k_pages", "v_pages"):
+        cache = _make(gpu, 1, 1, 32, t, 16, [90], seed=96)
+        tiny = torch.finfo(t).smallest_normal
+        getattr(cache, which).copy_((torch.rand(cache.k_pages.shape, generator=torch.Generator().manual_seed(97)) * tiny).to(t))
+        q = torch.randn(1, 1, 2, 32, generator=torch.Generator().manual_seed(98)).to(t)
+        scale = 0.2 if which == "v_pages" else min(0.2 / tiny, 2.0 ** 126)
+        ref = st.attend(st.cache_of(cache), q, scale=scale)
+        o, lse = paged_attention(q.to(gpu), cache, sm_scale=scale, return_lse=True)
+        u, step = torch.finfo(t).eps / 2, tiny * torch.finfo(t).eps / 2
+        es = (32 + 8) * F32 * ref[2][2] + 64 * F32 * (1 + ref[1].transpose(1, 2)[..., None].abs())
+        tol = (u + 2 * es) * 1.001 * ref[2][0] + u * ref[0].abs() + step
+        if t == torch.float16:
+            tol = tol + 2.0 ** -40 * ref[2][1]
+        assert ((o.cpu().double() - ref[0]).abs() <= tol).all() and float(ref[0].abs().max()) > 0
+        assert ((lse.cpu().double() - ref[1]).abs() <= es.amax(-1).transpose(1, 2)).all()

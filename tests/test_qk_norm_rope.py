@@ -768,3 +768,12 @@ def _check_there(name, got, ref, size):
             _check(name, *(t[:, i:i + 2000].cpu() for t in (got.detach(), ref, size)))
     else:
         _check(name, got.detach().cpu(), ref.cpu(), size.cpu())
+
+
+@pytest.mark.gpu
+def test_registered_ops_do_what_they_declare(gpu):
+    x = _small(gpu, grad=True)
+    torch.library.opcheck(torch.ops.dmad.qk_norm_rope_fwd.default, (*(x[n] for n in OPERANDS), 1e-6))
+    torch.library.opcheck(torch.ops.dmad.qk_norm_rope_fwd.default, (x["q"], None, None, None, x["wq"], None, None, 1e-6))
+    y = {n: t.detach() for n, t in x.items()}
+    torch.library.opcheck(torch.ops.dmad.qk_norm_rope_bwd.default, (y["q"], y["k"], y["tq"], y["tk"], y["wq"], y["wk"], y["freqs"], 1e-6, True, False))
