@@ -23,12 +23,15 @@
 //     m D/16 + j of the row, so a lane's results are D/16 neighbours.
 // The next step's K is requested when this step's scores are done, and V when
 // its products are. The arithmetic hides behind the bytes: 16 rows per key head
-// take 82 us where 4 take 72 (352 MB).
+// take 76 us where 4 take 66 (355 MB). K and V are read once per 16 or 32 rows, by
+// workgroups that meet in one L2: up to 32 rows cost what one does (118-121 us for
+// 40 heads of 32760 slots), from about 64 on the arithmetic bounds (143 us for 64,
+// 243 for 128, 2.34 ms for 1560: 450 TFLOP/s).
 //
 // Split: the launch has `splits` pieces of equal work for all sequences
 // together; the device finds from the lengths which tiles are whose, so ragged
 // batches load the chip evenly and a captured graph follows the lengths (48
-// sequences of 1 to 16000 slots: 68 us against 74 with pieces that end where a
+// sequences of 1 to 16000 slots: 66 us against 74 with pieces that end where a
 // sequence does, 60 for equal lengths; the 16 sequences above 1.33 ms against
 // 1.59). A sequence that lies in several pieces leaves (maximum, sum, O) of each
 // in float32 and a second kernel joins them in order; one that lies in a single
@@ -586,16 +589,19 @@ __global__ __launch_bounds__(kPagedTile) void paged_weight_kernel(PagedAttnParam
 // Its workgroups: up to 32 per CU.
 constexpr int kPagedWeightGroups = 8192;
 
-// Two row tiles share one reading of K and V, where their registers allow (not
-// for 256-wide heads). Four were no faster up to 64 rows, whose two groups meet
-// in one L2: 67 us either way for 4 sequences of 8 tokens with 8 query heads
-// per key head.
+// Two row tiles share one reading of K and V where their registers allow, which
+// those of 256-wide heads do not: 119 us against 136 with one tile each for 32 rows
+// of 40 heads of 32760 slots, 140 against 233 for 64 rows; 50 against 55 us for 32
+// rows of 64-wide heads (8 sequences of 16000 slots). 256-wide heads pay: 158 us for
+// 40 rows where 16 take 103 (526 MB).
 static int paged_row_tiles(int D, int R) { return R <= 16 || D == 256 ? 1 : 2; }
 int paged_attn_rows(int D, int R) { return 16 * paged_row_tiles(D, R); }
 // Workgroups per CU that the cut aims at. Four waves with 16 KiB of K and V on
-// their way each (128-wide heads) keep a CU's share of the memory busy: two or
-// three workgroups were 0-17% slower, for their starts and ends, and one of
-// 64-wide heads 6% slower than two.
+// their way each (128-wide heads) keep a CU's share of the memory busy: one, two
+// and three took 115, 116, 119 us for 40 heads of 32760 slots, 634, 643, 642 for 8
+// sequences of 120000 and 80, 84, 81 for 48 ragged ones; 51, 52, 57 at 256-wide heads.
+// Narrower rows gain by two where they are many: 96, 89, 89 us for 32-wide heads, 96,
+// 98, 94 for 64-wide ones.
 int paged_attn_resident(int D) { return D >= 128 ? 1 : 2; }
 
 template <typename T, int D, bool ACC, bool CAUSAL>

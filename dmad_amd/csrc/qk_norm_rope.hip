@@ -16,7 +16,7 @@
 // one token (q's heads, then k's, then v's), and its lanes share the sines and
 // cosines (D <= 128: one each). HBM-bound: 2 D bytes in and out per row and
 // tensor for about 60 vector instructions per 8 elements. 14B with tangents,
-// 2.7 GB: 498 us, 5.4 TB/s; gradients of 1.3B, 604 MB: 103 us, 5.8 TB/s.
+// 2.7 GB: 500 us, 5.4 TB/s; gradients of 1.3B, 604 MB: 104 us, 5.8 TB/s.
 #include "kv_cache.h"
 #include "lanes.h"
 
@@ -340,8 +340,10 @@ __global__ __launch_bounds__(1024) void qk_weight_grad_kernel(const float* parti
 bool qk_past_caches(int64_t bytes) { return bytes > (int64_t)256 << 20; }
 
 // A workgroup per sequence saves the launch that advances the lengths and is
-// slower where a wave takes more than two passes (48 passes: 8.1 us against
-// 6.7 us; 12: 5.8 against 6.8 us for 32 sequences).
+// slower where a wave takes more than two passes. 32 sequences, one launch
+// against two, per replayed append: 4.0 against 5.2 us for 4 passes, 4.5 - 5.3 for
+// 12, 5.3 - 5.3 for 24, 5.6 to 5.9 - 5.5 for 32, 6.8 - 5.7 to 6.0 for 48. An eager call
+// also saves the second launch's host time.
 constexpr int kQkAppendPasses = 32;
 void qk_append_split(QkNormRopeParams& p) {
   const int64_t passes = (int64_t)p.S * p.passes;

@@ -332,7 +332,10 @@ def paged_attention(q, cache, sm_scale=None, causal=False, accumulate=False, ret
     """Attention of q [B, S, Hq, D] over each sequence's cache: o [B, S, Hq, D] (and lse [B, Hq, S]).
 
     Made for few new tokens (S = 1, a draft of a few, a small block): the work is split over the
-    cache's length. Hq is a multiple of the cache's heads; query head h reads key head
+    cache's length, and K and V are read once per 32 query rows (16 at 256-wide heads) of a key
+    head. Up to 32 rows that costs what one does; a block of 1560 tokens takes 20 times as long.
+    The softmax weights are rounded to the operands' type for their product with V (their sum, the
+    scores and lse are float32). Hq is a multiple of the cache's heads; query head h reads key head
     h // (Hq // Hk). ``sm_scale`` defaults to D^-1/2. Every token sees all slots in use;
     with ``causal`` the S tokens are the last S slots (just appended, none dropped for want of room,
     nothing evicted since) and each sees the slots up to its own. A token that sees no slot gets o = 0 and lse = -inf, and so
@@ -341,7 +344,8 @@ def paged_attention(q, cache, sm_scale=None, causal=False, accumulate=False, ret
 
     ``accumulate`` adds to ``cache.weight`` what each slot receives: its softmax weight summed over
     the S tokens and the query heads of its key head. It takes scratch of 4 bytes per query row and
-    slot of the cache's whole capacity.
+    slot of the cache's whole capacity, written and read back: made for few rows (1560 tokens of 40
+    heads over 32760 slots: 8.2 GB and 6.3 ms).
     """
     op = "paged_attention"
     _check_new(op, cache, ("q", q))

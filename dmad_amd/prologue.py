@@ -473,8 +473,9 @@ def qk_norm_rope_with_tangent(q_withT, k_withT, q_weight, k_weight, eps, freqs):
     and k [B, S, Hk, D] (any head counts; bf16, fp16 or fp32; D in 16, 32, 64, 128, 256; any strides
     with contiguous 16-byte-aligned rows are read in place). Each head's row x becomes
     R(x / sqrt(mean(x^2) + eps) * w), R turning the pairs (x[2i], x[2i+1]) by freqs[s, i] as
-    ``apply_rope_with_tangent`` does; float32 throughout, rounded once at the end. This is the
-    norm per head; ``rmsnorm_rope_with_tangent`` is the one over the whole model width.
+    ``apply_rope_with_tangent`` does; float32 throughout, rounded once at the end (rows whose squares
+    leave float32, elements above about 1e18 or, where eps is 0, below 1e-19, are not scaled first).
+    This is the norm per head; ``rmsnorm_rope_with_tangent`` is the one over the whole model width.
 
     ``tq``/``tk``: tangents, given for both or for neither; their outputs are detached. ``k_withT``
     (or ``q_withT``) may be ``(None, None)``: the other alone. A weight of None skips that norm,
