@@ -230,6 +230,7 @@ def _append_op(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, q_we
                weight: Optional[torch.Tensor], position: Optional[torch.Tensor]) -> torch.Tensor:
     """q' of ``qk_norm_rope_append`` (0 elements without q)."""
     cache = PagedKVCache(k_pages, v_pages, page_table, lengths, seen, weight, position)
+    _check_append(q, k, v, q_weight, k_weight, eps, freqs, cache)
     out = _append(q, k, v, q_weight, k_weight, eps, freqs, cache)
     return k.new_empty((0,)) if out is None else out
 
@@ -245,7 +246,7 @@ def _attend_op(q: torch.Tensor, sm_scale: float, causal: bool, k_pages: torch.Te
                position: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
     """(o, lse) of ``paged_attention``; adds to ``weight`` where it is given."""
     cache = PagedKVCache(k_pages, v_pages, page_table, lengths, seen, weight, position)
-    return _attend(q, cache, sm_scale, causal, weight is not None)
+    return _attend(q, cache, _check_attend(q, cache, sm_scale, weight is not None), causal, weight is not None)
 
 
 @_attend_op.register_fake
@@ -258,7 +259,9 @@ def _(q, sm_scale, causal, *cache):
 def _evict_op(keep: int, recent: int, sink: int, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
               lengths: torch.Tensor, seen: torch.Tensor, weight: torch.Tensor, position: torch.Tensor) -> None:
     """``evict_low_weight``."""
-    _evict(PagedKVCache(k_pages, v_pages, page_table, lengths, seen, weight, position), keep, recent, sink)
+    cache = PagedKVCache(k_pages, v_pages, page_table, lengths, seen, weight, position)
+    _check_evict(cache, keep, recent, sink)
+    _evict(cache, keep, recent, sink)
 
 
 @_evict_op.register_fake
@@ -267,6 +270,25 @@ def _(keep, recent, sink, *cache):
 
 
 _APPEND = "qk_norm_rope_append"
+
+
+def _check_append(q, k, v, q_weight, k_weight, eps, freqs, cache):
+    """Refuses what an append does not take (the weights' types apart, which the launch looks at)."""
+    op = _APPEND
+    if k is None or v is None:
+        raise ValueError(f"{op}: k and v must be given")
+    _check_new(op, cache, ("k", k), ("v", v), ("q", q))
+    cache._writable(op)
+    for t in (q_weight, k_weight, freqs):
+        _on_cache(op, cache, t)
+    _no_grad_only(op, cache, q, k, v, q_weight, k_weight, freqs)
+    if not eps >= 0:
+        raise ValueError(f"{op}: eps must be non-negative, got {eps}")
+    if q is None and q_weight is not None:
+        raise ValueError(f"{op}: q_weight without q")
+    D = cache.head_dim
+    if freqs is not None and (freqs.dim() != 2 or freqs.shape[1] != D // 2 or freqs.shape[0] < 1):
+        raise ValueError(f"{op}: freqs must be [positions, {D // 2}], got {tuple(freqs.shape)}")
 
 
 def qk_norm_rope_append(q, k, v, q_weight, k_weight, eps, freqs, cache):
@@ -279,28 +301,14 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, eps, freqs, cache):
     that norm, freqs None the rotation. New slots start with weight 0. Tokens beyond the capacity
     are dropped (``lengths`` stays at it, ``seen`` advances), and those whose page holds nothing.
     """
-    op = _APPEND
-    if k is None or v is None:
-        raise ValueError(f"{op}: k and v must be given")
-    _check_new(op, cache, ("k", k), ("v", v), ("q", q))
-    cache._writable(op)
-    for t in (q_weight, k_weight, freqs):
-        _on_cache(op, cache, t)
-    _no_grad_only(op, cache, q, k, v, q_weight, k_weight, freqs)
     eps = float(eps)
-    if not eps >= 0:
-        raise ValueError(f"{op}: eps must be non-negative, got {eps}")
-    D = cache.head_dim
-    if q is None and q_weight is not None:
-        raise ValueError(f"{op}: q_weight without q")
-    if freqs is not None and (freqs.dim() != 2 or freqs.shape[1] != D // 2 or freqs.shape[0] < 1):
-        raise ValueError(f"{op}: freqs must be [positions, {D // 2}], got {tuple(freqs.shape)}")
+    _check_append(q, k, v, q_weight, k_weight, eps, freqs, cache)
     if _eager_call(q, k, v, q_weight, k_weight, freqs):
         out = _append(q, k, v, q_weight, k_weight, eps, freqs, cache)
         cache._changed("append")
         return out
-    _weights_dtype(op, k, D, q_weight, k_weight)
-    refuse_forward_mode(op, q, k, v, q_weight, k_weight, freqs, *_cache_tensors(cache))
+    _weights_dtype(_APPEND, k, cache.head_dim, q_weight, k_weight)
+    refuse_forward_mode(_APPEND, q, k, v, q_weight, k_weight, freqs, *_cache_tensors(cache))
     out = torch.ops.dmad.qk_norm_rope_append(q, k, v, q_weight, k_weight, eps, freqs, *_cache_tensors(cache))
     return None if q is None else out
 
@@ -328,6 +336,22 @@ def append_kv(k, v, cache):
     qk_norm_rope_append(None, k, v, None, None, 0.0, None, cache)
 
 
+def _check_attend(q, cache, sm_scale, accumulate):
+    """Refuses what the attention does not take; the scale."""
+    op = "paged_attention"
+    _check_new(op, cache, ("q", q))
+    _no_grad_only(op, cache, q)
+    Hq = q.shape[2]
+    if Hq < 1 or Hq % cache.kv_heads:
+        raise ValueError(f"{op}: {Hq} query heads are not a multiple of the cache's {cache.kv_heads}")
+    scale = cache.head_dim ** -0.5 if sm_scale is None else float(sm_scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise NotImplementedError(f"{op}: sm_scale must be positive and finite, got {sm_scale}")
+    if accumulate and cache.weight is None:
+        raise ValueError(f"{op}: the cache keeps no weights to accumulate")
+    return scale
+
+
 def paged_attention(q, cache, sm_scale=None, causal=False, accumulate=False, return_lse=False):
     """Attention of q [B, S, Hq, D] over each sequence's cache: o [B, S, Hq, D] (and lse [B, Hq, S]).
 
@@ -347,24 +371,14 @@ def paged_attention(q, cache, sm_scale=None, causal=False, accumulate=False, ret
     slot of the cache's whole capacity, written and read back: made for few rows (1560 tokens of 40
     heads over 32760 slots: 8.2 GB and 6.3 ms).
     """
-    op = "paged_attention"
-    _check_new(op, cache, ("q", q))
-    _no_grad_only(op, cache, q)
-    Hq = q.shape[2]
-    if Hq < 1 or Hq % cache.kv_heads:
-        raise ValueError(f"{op}: {Hq} query heads are not a multiple of the cache's {cache.kv_heads}")
-    scale = cache.head_dim ** -0.5 if sm_scale is None else float(sm_scale)
-    if not (scale > 0 and math.isfinite(scale)):
-        raise NotImplementedError(f"{op}: sm_scale must be positive and finite, got {sm_scale}")
-    if accumulate and cache.weight is None:
-        raise ValueError(f"{op}: the cache keeps no weights to accumulate")
+    scale = _check_attend(q, cache, sm_scale, accumulate)
     causal, accumulate = bool(causal), bool(accumulate)
     if _eager_call(q):
         o, lse = _attend(q, cache, scale, causal, accumulate)
         if accumulate:
             cache._changed("attend")
     else:
-        refuse_forward_mode(op, q, *_cache_tensors(cache))
+        refuse_forward_mode("paged_attention", q, *_cache_tensors(cache))
         tensors = _cache_tensors(cache)
         if not accumulate:
             tensors[-2:] = None, None
@@ -386,6 +400,21 @@ def _attend(q, cache, scale, causal, accumulate):
     return o, lse
 
 
+def _check_evict(cache, keep, recent, sink):
+    """Refuses what the eviction does not take."""
+    op = "evict_low_weight"
+    if not isinstance(cache, PagedKVCache):
+        raise TypeError(f"{op}: cache must be a PagedKVCache, got {type(cache).__name__}")
+    cache._settle()
+    if cache.weight is None:
+        raise ValueError(f"{op}: the cache keeps no weights and positions")
+    if keep < 1 or recent < 0 or sink < 0 or recent + sink > keep:
+        raise ValueError(f"{op}: keep must be at least 1, recent and sink non-negative and together at most keep; got "
+                         f"keep={keep}, recent={recent}, sink={sink}")
+    cache._writable(op)
+    _no_grad_only(op, cache)
+
+
 def evict_low_weight(cache, keep, recent=0, sink=0):
     """Cuts every sequence of more than ``keep`` slots to ``keep``, in place, each key head by itself.
 
@@ -399,25 +428,15 @@ def evict_low_weight(cache, keep, recent=0, sink=0):
     pages were dropped keeps ``keep`` of the slots it still has (``cache.lengths`` is then larger
     than ``keep`` by the missing ones; without any it is ``keep``).
     """
-    op = "evict_low_weight"
-    if not isinstance(cache, PagedKVCache):
-        raise TypeError(f"{op}: cache must be a PagedKVCache, got {type(cache).__name__}")
-    cache._settle()
-    if cache.weight is None:
-        raise ValueError(f"{op}: the cache keeps no weights and positions")
     keep, recent, sink = int(keep), int(recent), int(sink)
-    if keep < 1 or recent < 0 or sink < 0 or recent + sink > keep:
-        raise ValueError(f"{op}: keep must be at least 1, recent and sink non-negative and together at most keep; got "
-                         f"keep={keep}, recent={recent}, sink={sink}")
+    _check_evict(cache, keep, recent, sink)
     if keep >= cache.capacity or cache.batch == 0:
         return  # no sequence can be longer
-    cache._writable(op)
-    _no_grad_only(op, cache)
     if _eager_call():
         _evict(cache, keep, recent, sink)
         cache._changed("evict")
     else:
-        refuse_forward_mode(op, *_cache_tensors(cache))
+        refuse_forward_mode("evict_low_weight", *_cache_tensors(cache))
         torch.ops.dmad.kv_evict(keep, recent, sink, *_cache_tensors(cache))
 
 

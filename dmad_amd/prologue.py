@@ -356,8 +356,19 @@ def _qk_backward(ctx, gq, gk):
 _qk_backward_once = torch.autograd.function.once_differentiable(_qk_backward)
 
 
+def _check_saved(x, g):
+    """The kernels read an operand as the forward did: one that came back from a saved-tensor hook in another
+    shape, type or place is refused."""
+    if g is not None and (x is None or x.shape != g.shape or x.dtype != g.dtype or x.device != g.device):
+        got = "nothing" if x is None else f"{tuple(x.shape)} {x.dtype} on {x.device}"
+        raise RuntimeError(f"{_QK}: the backward needs the operand of a gradient {tuple(g.shape)} {g.dtype} on "
+                           f"{g.device} as the forward read it, got {got}")
+
+
 def _qk_gradients(call, q, k, gq, gk, wq, wk, need_wq, need_wk):
     """The launch: (dq, dk, dwq, dwk), None where there is no gradient of that output or none is asked for."""
+    _check_saved(q, gq)
+    _check_saved(k, gk)
     cq, ck, Hq, Hk, dev = call.wq, call.wk, call.Hq, call.Hk, call.device
     sq = sgq = sk = sgk = dq = dk = dwq = dwk = ws = ws_ptr = None
     ws_size = 0

@@ -1470,3 +1470,28 @@ def test_subnormal_keys_and_values(gpu, dtype):
             tol = tol + 2.0 ** -40 * ref[2][1]
         assert ((o.cpu().double() - ref[0]).abs() <= tol).all() and float(ref[0].abs().max()) > 0
         assert ((lse.cpu().double() - ref[1]).abs() <= es.amax(-1).transpose(1, 2)).all()
+
+
+@BOTH
+def test_registered_ops_refuse_what_the_calls_refuse(request, monkeypatch, device):
+    """The registered ops check what they are given as the calls do, before a kernel reads it."""
+    cache, x = _loop(request, monkeypatch, device)
+    c = [getattr(cache, n) for n in ("k_pages", "v_pages", "page_table", "lengths", "seen", "weight", "position")]
+    before = st.cache_of(cache)
+    append, attend, evict = (getattr(torch.ops.dmad, n) for n in ("qk_norm_rope_append", "paged_attn", "kv_evict"))
+    q, k, v, wq, wk, f = (x[n] for n in ("q", "k", "v", "wq", "wk", "freqs"))
+    for call in [
+        lambda: append(q[:1], k, v, wq, wk, 1e-6, f, *c), lambda: append(q, k, v[:, :1], wq, wk, 1e-6, f, *c),
+        lambda: append(q, k[:, :, :1], v, wq, wk, 1e-6, f, *c), lambda: append(q, k.half(), v, wq, wk, 1e-6, f, *c),
+        lambda: append(q, k, v, wq, wk, 1e-6, f[:, :4], *c), lambda: append(q, k, v, wq, wk, -1.0, f, *c),
+        lambda: append(q, k, v, wq, wk, 1e-6, f, *c[:3], c[3][:1], *c[4:]),
+        lambda: attend(q[..., :8], 0.25, False, *c), lambda: attend(q[:, :, :3], 0.25, False, *c),
+        lambda: attend(q, 0.25, False, c[0][:2], *c[1:]), lambda: attend(q[:1], 0.25, True, *c[:5], None, None),
+        lambda: evict(0, 0, 0, *c), lambda: evict(8, 5, 4, *c), lambda: evict(8, 0, 0, *c[:5], c[5][:1], c[6]),
+    ]:
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(NotImplementedError):
+        attend(q, -0.25, False, *c)
+    for n in st.FIELDS:
+        _same(n, getattr(cache, n), before[n])

@@ -777,3 +777,69 @@ def test_registered_ops_do_what_they_declare(gpu):
     torch.library.opcheck(torch.ops.dmad.qk_norm_rope_fwd.default, (x["q"], None, None, None, x["wq"], None, None, 1e-6))
     y = {n: t.detach() for n, t in x.items()}
     torch.library.opcheck(torch.ops.dmad.qk_norm_rope_bwd.default, (y["q"], y["k"], y["tq"], y["tk"], y["wq"], y["wk"], y["freqs"], 1e-6, True, False))
+
+
+HOOKS = {"type": lambda t: t.to(torch.bfloat16), "shape": lambda t: t[:, :3], "place": lambda t: t.to("meta")}
+
+
+@pytest.mark.parametrize("kind", [*HOOKS, "a copy"])
+def test_saved_operands_are_checked(kind):
+    """What a saved-tensor hook brings back in another shape, type or place is refused before a kernel reads it as
+    what it was."""
+    from dmad_amd.prologue import _check_saved
+
+    x, g = torch.zeros(2, 5, 4, 16), torch.zeros(2, 5, 4, 16)
+    if kind == "a copy":
+        _check_saved(x.clone(), g)
+        _check_saved(None, None)
+        return
+    with pytest.raises(RuntimeError, match="as the forward read it"):
+        _check_saved(HOOKS[kind](x), g)
+    with pytest.raises(RuntimeError, match="nothing"):
+        _check_saved(None, g)
+
+
+@pytest.mark.gpu
+def test_saved_tensor_hooks(gpu):
+    """Through autograd: a hook that offloads and brings back works, one that changes what it brings back raises."""
+    x = _small(gpu, grad=True)
+    leaves = [x[n] for n in ("q", "k", "wq", "wk")]
+
+    def grads(pack, unpack):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            q, _, k, _ = _run(x)
+        return torch.autograd.grad(q.square().sum() + k.sum(), leaves)
+
+    same = lambda t: t  # noqa: E731
+    want = grads(same, same)
+    for a, b in zip(grads(lambda t: t.cpu(), lambda t: t.to(gpu)), want):
+        assert torch.equal(a, b)
+    for unpack in (lambda t: t.to(torch.bfloat16), lambda t: t[:1], lambda t: t.cpu()):
+        with pytest.raises(RuntimeError):
+            (_run_hooked(x, unpack)).backward()
+
+
+def _run_hooked(x, unpack):
+    def only_operands(t):
+        return unpack(t) if t.dim() == 4 else t
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, only_operands):
+        q, _, k, _ = _run(x)
+    return q.sum() + k.sum()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("gpu", marks=pytest.mark.gpu)])
+def test_registered_ops_refuse_what_the_calls_refuse(request, monkeypatch, device):
+    if device == "cpu":
+        _mock_kernels(monkeypatch)
+    x = _small(request.getfixturevalue("gpu") if device == "gpu" else device)
+    t = [x[n] for n in OPERANDS]
+    fwd, bwd = torch.ops.dmad.qk_norm_rope_fwd, torch.ops.dmad.qk_norm_rope_bwd
+    for i, bad in ((0, x["q"][:, :3]), (1, x["tq"][:1]), (2, x["k"].half()), (4, x["wq"][:8]), (6, x["freqs"][:4])):
+        with pytest.raises(ValueError):
+            fwd(*t[:i], bad, *t[i + 1:], 1e-6)
+    if device == "gpu":  # (the check is part of the launch)
+        with pytest.raises(RuntimeError, match="as the forward read it"):
+            bwd(x["q"], x["k"], x["q"][:1], x["k"], x["wq"], x["wk"], x["freqs"], 1e-6, True, True)
+        with pytest.raises(RuntimeError, match="nothing"):
+            bwd(x["q"], None, x["q"], x["k"], x["wq"], None, x["freqs"], 1e-6, True, True)
