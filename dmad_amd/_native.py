@@ -81,6 +81,14 @@ class KvCache(ctypes.Structure):
     ]
 
 
+class GatedNormSizes(ctypes.Structure):
+    """``dmad_gated_norm_sizes``: types, sizes and strides of a gated norm."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "wdtype", "norm")] + \
+        [(n, ctypes.c_int64) for n in ("B", "S", "C", "F")] + \
+        [(n, ctypes.c_int64 * 3) for n in ("x", "y", "tx", "ty", "gate", "scale", "shift", "tgate", "tscale", "tshift")]
+
+
 # Every function the header declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -91,6 +99,7 @@ _SZP = ctypes.POINTER(ctypes.c_size_t)
 _INT = ctypes.c_int
 _F = ctypes.c_float
 _KV = ctypes.POINTER(KvCache)
+_GN = ctypes.POINTER(GatedNormSizes)
 
 SIGNATURES = {
     "dmad_abi_version": (_INT, []),
@@ -127,8 +136,14 @@ SIGNATURES = {
                                         _P, _KV, _P]),
     "dmad_paged_attn_workspace_bytes": (_INT, [_KV, _I64, _I64, _INT, _SZP]),
     "dmad_paged_attn": (_INT, [_INT, _KV, _I64, _I64, _P, _I64P, _INT, _INT, _F, _P, _P, _P, _SZ, _P]),
+    "dmad_prefix_attn_workspace_bytes": (_INT, [_KV, _KV, _I64, _I64, _SZP]),
+    "dmad_prefix_attn": (_INT, [_INT, _KV, _KV, _I64, _I64, _P, _I64P, _INT, _F, _P, _P, _P, _SZ, _P]),
     "dmad_kv_evict_workspace_bytes": (_INT, [_KV, _I64, _SZP]),
     "dmad_kv_evict": (_INT, [_INT, _KV, _I64, _I64, _I64, _P, _SZ, _P]),
+    "dmad_gated_norm": (_INT, [_GN, *[_P] * 13, _F, _F, *[_P] * 5]),
+    "dmad_gated_norm_bwd_workspace_bytes": (_INT, [_GN, _SZP]),
+    "dmad_gated_norm_bwd": (_INT, [_GN, *[_P] * 9, _F, _F, *[_P] * 9, _SZ, _P]),
+    "dmad_qk_rotary": (_INT, [_INT, *[_I64] * 6, *[_P] * 4, *[_I64P] * 4, _P, _INT, _I64P, _P, _INT, _INT, _F, *[_P] * 5]),
     "dmad_attn_bwd_workspace_bytes": (_INT, [_INT, _I64, _I64, _I64, _I64, _I64, _SZP]),
     "dmad_attn_fwd_plan": (_INT, [_INT, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _I64, ctypes.POINTER(Plan)]),
     "dmad_attn_bwd_plan": (_INT, [_INT, _INT, _INT, _I64, _I64, _I64, _I64, _I64, ctypes.POINTER(Plan)]),
@@ -346,6 +361,12 @@ def qk_norm_rope_bwd_workspace_bytes(B: int, S: int, Hq: int, Hk: int, D: int) -
 def paged_attn_workspace_bytes(cache: KvCache, S: int, Hq: int, accumulate: bool) -> int:
     n = ctypes.c_size_t(0)
     check(lib().dmad_paged_attn_workspace_bytes(ctypes.byref(cache), S, Hq, int(accumulate), ctypes.byref(n)))
+    return int(n.value)
+
+
+def prefix_attn_workspace_bytes(cache: KvCache, prefix: KvCache, S: int, Hq: int) -> int:
+    n = ctypes.c_size_t(0)
+    check(lib().dmad_prefix_attn_workspace_bytes(ctypes.byref(prefix), ctypes.byref(cache), S, Hq, ctypes.byref(n)))
     return int(n.value)
 
 

@@ -3,11 +3,13 @@
 // allocation-free backward uses this file's static device array `scratch`.
 #include <cstdarg>
 #include <cstdio>
+#include <cstring>
 #include <limits>
 #include <mutex>
 #include <string>
 
 #include "dmad_attn.h"
+#include "block_ops.h"
 #include "kv_cache.h"
 #include "launch.h"
 
@@ -1385,6 +1387,143 @@ int paged_layout(const dmad_kv_cache* c, int64_t S, int64_t Hq, bool accumulate,
   return DMAD_OK;
 }
 
+// Attention behind shared prefixes: both caches' pieces side by side.
+struct PrefixLayout {
+  PagedLayout shared, own;
+  size_t shared_o, shared_ml, own_o, own_ml, total;
+};
+int prefix_layout(const dmad_kv_cache* prefix, const dmad_kv_cache* c, int64_t S, int64_t Hq, PrefixLayout& w) {
+  if (prefix->kv_heads != c->kv_heads || prefix->head_dim != c->head_dim)
+    return fail(DMAD_ERR_INVALID, "the prefixes' heads and head dim must be the cache's");
+  if (prefix->batch < 1 || c->batch % prefix->batch != 0)
+    return fail(DMAD_ERR_INVALID, "%lld sequences cannot share %lld prefixes evenly", (long long)c->batch,
+                (long long)prefix->batch);
+  const int64_t n = c->batch / prefix->batch;
+  if (n > 0 && S >= ((int64_t)1 << 31) / n) return fail(DMAD_ERR_UNSUPPORTED, "too many query rows");
+  int rc = paged_layout(prefix, n * S, Hq, false, w.shared);
+  if (rc != DMAD_OK || (rc = paged_layout(c, S, Hq, false, w.own)) != DMAD_OK) return rc;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  const size_t rows = (size_t)(w.shared.splits + prefix->batch) * c->kv_heads * w.shared.R;
+  const size_t own = (size_t)(w.own.splits + c->batch) * c->kv_heads * w.own.R;
+  w.shared_o = 0;
+  w.shared_ml = w.shared_o + up(rows * c->head_dim * 4);
+  w.own_o = w.shared_ml + up(rows * 8);
+  w.own_ml = w.own_o + up(own * c->head_dim * 4);
+  w.total = w.own_ml + up(own * 8);
+  return DMAD_OK;
+}
+
+// ---------------------------------------------------------------- gate, residual and norm; rotations by position
+
+// Infinite or not a number, by its bits (the build lets the compiler take NaN tests for false).
+bool not_finite(float x) {
+  uint32_t bits;
+  memcpy(&bits, &x, sizeof bits);
+  return (bits & 0x7f800000u) == 0x7f800000u;
+}
+
+// A row operand of the gated norm by strides {b, s, c}, or a vector per group by {b, f, c}.
+int norm_rows(const char* name, const void* ptr, const int64_t* st, int esz, int64_t& outer, int64_t& inner) {
+  if (st == nullptr) return fail(DMAD_ERR_INVALID, "%s: null strides", name);
+  if (st[2] != 1) return fail(DMAD_ERR_INVALID, "%s: stride of the channels must be 1, got %lld", name, (long long)st[2]);
+  const int align = 16 / esz;
+  for (int i = 0; i < 2; ++i)
+    if (st[i] < 0 || st[i] % align != 0)
+      return fail(DMAD_ERR_INVALID, "%s: strides must be non-negative multiples of %d elements, got %lld", name, align,
+                  (long long)st[i]);
+  if (((uintptr_t)ptr & 15) != 0) return fail(DMAD_ERR_INVALID, "%s: base pointer must be 16-byte aligned", name);
+  outer = st[0];
+  inner = st[1];
+  return DMAD_OK;
+}
+
+int norm_aligned(std::initializer_list<const void*> ptrs) {
+  for (const void* ptr : ptrs)
+    if (((uintptr_t)ptr & 15) != 0) return fail(DMAD_ERR_INVALID, "weights and outputs must be 16-byte aligned");
+  return DMAD_OK;
+}
+
+// Sizes and operands that forward and backward of the gated norm share.
+int norm_sizes(const dmad_gated_norm_sizes* z, float eps, float residual_scale, dmad::GatedNormParams& p) {
+  if (z == nullptr) return fail(DMAD_ERR_INVALID, "sizes: null pointer");
+  if (z->dtype != DMAD_BF16 && z->dtype != DMAD_F16 && z->dtype != DMAD_F32)
+    return fail(DMAD_ERR_UNSUPPORTED, "unsupported dtype code %d", z->dtype);
+  if (z->wdtype != z->dtype && z->wdtype != DMAD_F32)
+    return fail(DMAD_ERR_UNSUPPORTED, "small operands must have the operands' type or float32");
+  if (z->norm != DMAD_NORM_LAYER && z->norm != DMAD_NORM_RMS) return fail(DMAD_ERR_INVALID, "unknown norm %d", z->norm);
+  if (z->B < 0 || z->S < 0 || z->F < 1 || z->S % z->F != 0)
+    return fail(DMAD_ERR_INVALID, "bad sizes B=%lld S=%lld, %lld groups", (long long)z->B, (long long)z->S, (long long)z->F);
+  if (z->C < 8 || z->C % 8 != 0 || z->C > dmad::kNormMaxC)
+    return fail(DMAD_ERR_UNSUPPORTED, "channels must be a multiple of 8 up to %d, got %lld", dmad::kNormMaxC, (long long)z->C);
+  const int64_t lim = (int64_t)1 << 24;
+  if (z->B >= lim || z->S >= lim || (z->B > 0 && z->S >= lim / z->B))
+    return fail(DMAD_ERR_UNSUPPORTED, "too many tokens");
+  if (not_finite(eps) || eps < 0.f) return fail(DMAD_ERR_INVALID, "eps must be non-negative and finite");
+  if (not_finite(residual_scale)) return fail(DMAD_ERR_INVALID, "residual_scale must be finite");
+  p.B = (int)z->B;
+  p.S = (int)z->S;
+  p.F = (int)z->F;
+  p.T = (int)(z->S / z->F);
+  p.C = (int)z->C;
+  p.rows = z->B * z->S;
+  p.layer = z->norm == DMAD_NORM_LAYER;
+  p.eps = eps;
+  p.rs = residual_scale;
+  p.split = 1;
+  return DMAD_OK;
+}
+
+int norm_operand(const char* name, int dtype, const void* ptr, const int64_t* st, dmad::NormRows& o) {
+  if (ptr == nullptr) return DMAD_OK;
+  o.p = ptr;
+  return norm_rows(name, ptr, st, elem_size(dtype), o.b, o.s);
+}
+int norm_vector(const char* name, int dtype, const void* ptr, const int64_t* st, dmad::NormVec& o) {
+  if (ptr == nullptr) return DMAD_OK;
+  o.p = ptr;
+  return norm_rows(name, ptr, st, elem_size(dtype), o.b, o.f);
+}
+
+int norm_split(const dmad::GatedNormParams& p) { return dmad::gated_norm_split((int64_t)p.B * p.F, p.T, p.C); }
+size_t norm_workspace(const dmad::GatedNormParams& p) {
+  return (size_t)p.B * p.F * norm_split(p) * dmad::kNormSums * p.C * sizeof(float);
+}
+
+// Largest power of two up to 8 elements that divides n (a stride or an address in bytes over esz).
+int64_t low_bit(int64_t n) { return n == 0 ? 8 : (n & -n) < 8 ? (n & -n) : 8; }
+
+int rotary_operand(const char* name, int esz, int64_t H, const void* x, const void* t, const int64_t* xs, const int64_t* ts,
+                   void* out, void* tout, dmad::RotaryOperand& o, int64_t& align) {
+  o.H = (int)H;
+  if (H == 0) {
+    if (x != nullptr) return fail(DMAD_ERR_INVALID, "%s: given, but with no heads", name);
+    return DMAD_OK;
+  }
+  if (x == nullptr || xs == nullptr) return fail(DMAD_ERR_INVALID, "%s: null pointer", name);
+  if (out == nullptr || (t != nullptr && tout == nullptr)) return fail(DMAD_ERR_INVALID, "output: null pointer");
+  if (t != nullptr && ts == nullptr) return fail(DMAD_ERR_INVALID, "%s: null strides of its tangent", name);
+  for (const int64_t* st : {xs, t != nullptr ? ts : xs}) {
+    if (st[3] != 1) return fail(DMAD_ERR_INVALID, "%s: stride of the head dim must be 1, got %lld", name, (long long)st[3]);
+    for (int i = 0; i < 3; ++i) {
+      if (st[i] < 0) return fail(DMAD_ERR_INVALID, "%s: negative stride %lld", name, (long long)st[i]);
+      const int64_t bit = low_bit(st[i]);
+      if (bit < align) align = bit;
+    }
+  }
+  for (const void* ptr : {x, t, (const void*)out, (const void*)tout}) {
+    if (((uintptr_t)ptr & (esz - 1)) != 0) return fail(DMAD_ERR_INVALID, "%s: base pointer must be a multiple of its element", name);
+    const int64_t bit = low_bit((int64_t)((uintptr_t)ptr & 255) / esz);
+    if (bit < align) align = bit;
+  }
+  o.x = x;
+  o.t = t;
+  o.out = out;
+  o.tout = tout;
+  o.xb = xs[0]; o.xs = xs[1]; o.xh = xs[2];
+  if (t != nullptr) { o.tb = ts[0]; o.ts = ts[1]; o.th = ts[2]; }
+  return DMAD_OK;
+}
+
 int64_t evict_moves(const dmad_kv_cache* c, int64_t keep) {
   const int64_t cap = c->pages_per_seq * c->page_size, over = cap - keep;
   return over <= 0 ? 0 : over < keep ? over : keep;
@@ -1861,6 +2000,75 @@ int dmad_paged_attn(int dtype, const dmad_kv_cache* cache, int64_t S, int64_t Hq
   return ok();
 }
 
+int dmad_prefix_attn_workspace_bytes(const dmad_kv_cache* prefix, const dmad_kv_cache* cache, int64_t S, int64_t Hq,
+                                     size_t* bytes) {
+  if (bytes == nullptr) return fail(DMAD_ERR_INVALID, "bytes: null pointer");
+  dmad::KvPages kv;
+  int rc = check_cache(DMAD_BF16, prefix, kv);
+  if (rc != DMAD_OK || (rc = check_cache(DMAD_BF16, cache, kv)) != DMAD_OK) return rc;
+  PrefixLayout w;
+  if ((rc = prefix_layout(prefix, cache, S, Hq, w)) != DMAD_OK) return rc;
+  *bytes = w.total;
+  return ok();
+}
+
+int dmad_prefix_attn(int dtype, const dmad_kv_cache* prefix, const dmad_kv_cache* cache, int64_t S, int64_t Hq,
+                     const void* q, const int64_t q_strides[4], int causal, float sm_scale, void* o, float* lse,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  dmad::PagedAttnParams shared{}, p{};
+  int rc = check_cache(dtype, prefix, shared.kv);
+  if (rc != DMAD_OK || (rc = check_cache(dtype, cache, p.kv)) != DMAD_OK) return rc;
+  const float scale_log2 = sm_scale * 1.4426950408889634f;
+  if (!(sm_scale > 0.f && scale_log2 <= std::numeric_limits<float>::max()))
+    return fail(DMAD_ERR_UNSUPPORTED, "sm_scale must be positive, and finite times log2(e)");
+  PrefixLayout w;
+  if ((rc = prefix_layout(prefix, cache, S, Hq, w)) != DMAD_OK) return rc;
+  if (cache->batch == 0 || S == 0) return ok();
+  if ((rc = check_rows("q", q, q_strides, 2)) != DMAD_OK) return rc;
+  // the tokens of a prefix's sequences follow one another at one stride
+  const int64_t n = cache->batch / prefix->batch;
+  if (S > 1 && n > 1 && q_strides[0] != S * q_strides[1])
+    return fail(DMAD_ERR_INVALID, "q: sequences must follow one another as their tokens do (stride %lld, not %lld)",
+                (long long)(S * q_strides[1]), (long long)q_strides[0]);
+  if (o == nullptr || lse == nullptr) return fail(DMAD_ERR_INVALID, "output: null pointer");
+  if (((uintptr_t)o & 15) != 0) return fail(DMAD_ERR_INVALID, "o must be 16-byte aligned");
+  if (workspace == nullptr || workspace_bytes < w.total || ((uintptr_t)workspace & 255) != 0)
+    return fail(DMAD_ERR_WORKSPACE, "workspace: %zu bytes (256-byte aligned) needed, %zu given", w.total, workspace_bytes);
+  char* ws = (char*)workspace;
+  p.q = q;
+  p.qb = q_strides[0]; p.qs = q_strides[1]; p.qh = q_strides[2];
+  p.o = o;
+  p.lse = lse;
+  p.S = (int)S;
+  p.G = (int)(Hq / cache->kv_heads);
+  p.R = (int)w.own.R;
+  p.row_groups = (int)w.own.row_groups;
+  p.causal = causal != 0;
+  p.splits = (int)w.own.splits;
+  p.scale_log2 = scale_log2;
+  p.part_o = (float*)(ws + w.own_o);
+  p.part_ml = (float*)(ws + w.own_ml);
+  p.keep_parts = 1;
+  dmad::KvPages kv = shared.kv;
+  shared = p;
+  shared.kv = kv;
+  shared.qs = S > 1 ? q_strides[1] : q_strides[0];
+  shared.qb = n * q_strides[0];
+  shared.S = (int)(n * S);
+  shared.R = (int)w.shared.R;
+  shared.row_groups = (int)w.shared.row_groups;
+  shared.causal = 0;
+  shared.splits = (int)w.shared.splits;
+  shared.part_o = (float*)(ws + w.shared_o);
+  shared.part_ml = (float*)(ws + w.shared_ml);
+  hipStream_t s = (hipStream_t)stream;
+  mark(0, false, s);
+  const hipError_t e = dmad::launch_prefix_attn(shared, p, dtype, (int)cache->head_dim, s);
+  mark(0, true, s);
+  if (e != hipSuccess) return fail(DMAD_ERR_HIP, "prefix attention launch: %s", hipGetErrorString(e));
+  return ok();
+}
+
 int dmad_kv_evict_workspace_bytes(const dmad_kv_cache* cache, int64_t keep, size_t* bytes) {
   if (bytes == nullptr) return fail(DMAD_ERR_INVALID, "bytes: null pointer");
   dmad::KvPages kv;
@@ -1896,6 +2104,162 @@ int dmad_kv_evict(int dtype, const dmad_kv_cache* cache, int64_t keep, int64_t r
   const hipError_t e = dmad::launch_kv_evict(p, s);
   mark(0, true, s);
   if (e != hipSuccess) return fail(DMAD_ERR_HIP, "eviction launch: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int dmad_gated_norm(const dmad_gated_norm_sizes* sizes, const void* x, const void* tx, const void* y, const void* ty,
+                    const void* gate, const void* tgate, const void* scale, const void* tscale, const void* shift,
+                    const void* tshift, const void* weight, const void* bias, const void* post_weight, float eps,
+                    float residual_scale, void* xo, void* txo, void* no, void* tno, void* stream) {
+  dmad::GatedNormParams p{};
+  int rc = norm_sizes(sizes, eps, residual_scale, p);
+  if (rc != DMAD_OK || p.rows == 0) return rc != DMAD_OK ? rc : ok();
+  const int dt = sizes->dtype, wdt = sizes->wdtype;
+  if (x == nullptr || no == nullptr) return fail(DMAD_ERR_INVALID, "x and n: null pointer");
+  if ((rc = norm_operand("x", dt, x, sizes->x, p.x)) != DMAD_OK || (rc = norm_operand("tx", dt, tx, sizes->tx, p.tx)) != DMAD_OK ||
+      (rc = norm_operand("y", dt, y, sizes->y, p.y)) != DMAD_OK || (rc = norm_operand("ty", dt, ty, sizes->ty, p.ty)) != DMAD_OK ||
+      (rc = norm_vector("gate", wdt, gate, sizes->gate, p.gate)) != DMAD_OK ||
+      (rc = norm_vector("tgate", wdt, tgate, sizes->tgate, p.tgate)) != DMAD_OK ||
+      (rc = norm_vector("scale", wdt, scale, sizes->scale, p.scale)) != DMAD_OK ||
+      (rc = norm_vector("tscale", wdt, tscale, sizes->tscale, p.tscale)) != DMAD_OK ||
+      (rc = norm_vector("shift", wdt, shift, sizes->shift, p.shift)) != DMAD_OK ||
+      (rc = norm_vector("tshift", wdt, tshift, sizes->tshift, p.tshift)) != DMAD_OK ||
+      (rc = norm_aligned({weight, bias, post_weight, xo, txo, no, tno})) != DMAD_OK)
+    return rc;
+  if ((y != nullptr) != (xo != nullptr)) return fail(DMAD_ERR_INVALID, "y and x' must be both set or both null");
+  if (y == nullptr && (gate != nullptr || post_weight != nullptr || ty != nullptr))
+    return fail(DMAD_ERR_INVALID, "gate, post_weight or a tangent without y");
+  const bool jvp = tx != nullptr;
+  if (jvp != (tno != nullptr) || (jvp && y != nullptr) != (ty != nullptr) || (jvp && y != nullptr) != (txo != nullptr))
+    return fail(DMAD_ERR_INVALID, "tangents of x and y and their outputs together, or none");
+  if ((tgate != nullptr && (gate == nullptr || !jvp)) || (tscale != nullptr && (scale == nullptr || !jvp)) ||
+      (tshift != nullptr && (shift == nullptr || !jvp)))
+    return fail(DMAD_ERR_INVALID, "a tangent without its operand or without those of x and y");
+  p.weight = weight;
+  p.bias = bias;
+  p.post = post_weight;
+  p.xo = xo;
+  p.txo = txo;
+  p.no = no;
+  p.tno = tno;
+  hipStream_t s = (hipStream_t)stream;
+  mark(0, false, s);
+  const hipError_t e = dmad::launch_gated_norm(p, dt, wdt, s);
+  mark(0, true, s);
+  if (e != hipSuccess) return fail(DMAD_ERR_HIP, "gated norm launch: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int dmad_gated_norm_bwd_workspace_bytes(const dmad_gated_norm_sizes* sizes, size_t* bytes) {
+  if (bytes == nullptr) return fail(DMAD_ERR_INVALID, "bytes: null pointer");
+  dmad::GatedNormParams p{};
+  const int rc = norm_sizes(sizes, 0.f, 1.f, p);
+  if (rc != DMAD_OK) return rc;
+  *bytes = p.rows == 0 ? 0 : norm_workspace(p);
+  return ok();
+}
+
+int dmad_gated_norm_bwd(const dmad_gated_norm_sizes* sizes, const void* x, const void* y, const void* gx, const void* gn,
+                        const void* gate, const void* scale, const void* weight, const void* bias,
+                        const void* post_weight, float eps, float residual_scale, void* dx, void* dy, void* dgate,
+                        void* dscale, void* dshift, void* dweight, void* dbias, void* dpost, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  dmad::GatedNormParams p{};
+  int rc = norm_sizes(sizes, eps, residual_scale, p);
+  if (rc != DMAD_OK) return rc;
+  const bool groups = dgate != nullptr || dscale != nullptr || dshift != nullptr;
+  const bool weights = dweight != nullptr || dbias != nullptr || dpost != nullptr;
+  if (p.rows == 0) {
+    if (groups || weights) return fail(DMAD_ERR_INVALID, "no rows to sum the small operands' gradients over");
+    return ok();
+  }
+  const int dt = sizes->dtype, wdt = sizes->wdtype;
+  if (x == nullptr || dx == nullptr) return fail(DMAD_ERR_INVALID, "x and dx: null pointer");
+  if (gx == nullptr && gn == nullptr) return fail(DMAD_ERR_INVALID, "gradients: null pointers");
+  if ((rc = norm_operand("x", dt, x, sizes->x, p.x)) != DMAD_OK || (rc = norm_operand("y", dt, y, sizes->y, p.y)) != DMAD_OK ||
+      (rc = norm_operand("gx", dt, gx, sizes->tx, p.tx)) != DMAD_OK || (rc = norm_operand("gn", dt, gn, sizes->ty, p.ty)) != DMAD_OK ||
+      (rc = norm_vector("gate", wdt, gate, sizes->gate, p.gate)) != DMAD_OK ||
+      (rc = norm_vector("scale", wdt, scale, sizes->scale, p.scale)) != DMAD_OK ||
+      (rc = norm_aligned({weight, bias, post_weight, dx, dy, dgate, dscale, dshift, dweight, dbias, dpost})) != DMAD_OK)
+    return rc;
+  if (y == nullptr && (gate != nullptr || post_weight != nullptr || dy != nullptr))
+    return fail(DMAD_ERR_INVALID, "gate, post_weight or dy without y");
+  if ((dgate != nullptr && gate == nullptr) || (dscale != nullptr && scale == nullptr) || (dweight != nullptr && weight == nullptr) ||
+      (dbias != nullptr && bias == nullptr) || (dpost != nullptr && post_weight == nullptr))
+    return fail(DMAD_ERR_INVALID, "the gradient of an operand that is not there");
+  p.weight = weight;
+  p.bias = bias;
+  p.post = post_weight;
+  p.xo = dx;
+  p.txo = dy;
+  p.dgate = dgate;
+  p.dscale = dscale;
+  p.dshift = dshift;
+  p.dweight = dweight;
+  p.dbias = dbias;
+  p.dpost = dpost;
+  p.split = norm_split(p);
+  if (weights || (groups && p.split > 1)) {
+    const size_t need = norm_workspace(p);
+    if (workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)
+      return fail(DMAD_ERR_WORKSPACE, "workspace: %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
+    p.partial = (float*)workspace;
+  }
+  hipStream_t s = (hipStream_t)stream;
+  mark(0, false, s);
+  const hipError_t e = dmad::launch_gated_norm_bwd(p, dt, wdt, s);
+  mark(0, true, s);
+  if (e != hipSuccess) return fail(DMAD_ERR_HIP, "gated norm backward launch: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int dmad_qk_rotary(int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, int64_t R, const void* q,
+                   const void* tq, const void* k, const void* tk, const int64_t q_strides[4], const int64_t tq_strides[4],
+                   const int64_t k_strides[4], const int64_t tk_strides[4], const void* positions, int positions_64,
+                   const int64_t position_strides[2], const double* frequencies, int layout, int transposed, float factor,
+                   void* oq, void* otq, void* ok_, void* otk, void* stream) {
+  if (dtype != DMAD_BF16 && dtype != DMAD_F16 && dtype != DMAD_F32)
+    return fail(DMAD_ERR_UNSUPPORTED, "unsupported dtype code %d", dtype);
+  if (B < 0 || S < 0 || Hq < 0 || Hk < 0 || Hq + Hk == 0 || D < 1)
+    return fail(DMAD_ERR_INVALID, "bad sizes B=%lld S=%lld Hq=%lld Hk=%lld D=%lld", (long long)B, (long long)S, (long long)Hq,
+                (long long)Hk, (long long)D);
+  if (R < 2 || R % 2 != 0 || R > D) return fail(DMAD_ERR_INVALID, "the turned part must be even, from 2 to the head dim, got %lld", (long long)R);
+  if (layout != DMAD_ROTARY_INTERLEAVED && layout != DMAD_ROTARY_HALF) return fail(DMAD_ERR_INVALID, "unknown layout %d", layout);
+  if (not_finite(factor)) return fail(DMAD_ERR_INVALID, "factor must be finite");
+  const int64_t lim = (int64_t)1 << 31;
+  if (D > 8192 || Hq >= (1 << 20) || Hk >= (1 << 20) || B >= lim || S >= lim || (B > 0 && S > (lim - 1) / B))
+    return fail(DMAD_ERR_UNSUPPORTED, "too many heads or tokens");
+  if (B == 0 || S == 0) return ok();
+  const bool jvp = tq != nullptr || tk != nullptr;
+  if (jvp && ((Hq > 0 && tq == nullptr) || (Hk > 0 && tk == nullptr)))
+    return fail(DMAD_ERR_INVALID, "tangents must be given for q and k, or for neither");
+  dmad::RotaryParams p{};
+  const int esz = elem_size(dtype);
+  int64_t align = 8;
+  int rc = rotary_operand("q", esz, Hq, q, tq, q_strides, tq_strides, oq, otq, p.op[0], align);
+  if (rc != DMAD_OK || (rc = rotary_operand("k", esz, Hk, k, tk, k_strides, tk_strides, ok_, otk, p.op[1], align)) != DMAD_OK)
+    return rc;
+  if (positions == nullptr || position_strides == nullptr || frequencies == nullptr)
+    return fail(DMAD_ERR_INVALID, "positions and frequencies: null pointer");
+  p.positions = positions;
+  p.pos64 = positions_64 != 0;
+  p.pos_b = position_strides[0];
+  p.pos_s = position_strides[1];
+  p.frequencies = frequencies;
+  p.B = (int)B;
+  p.S = (int)S;
+  p.D = (int)D;
+  p.R = (int)R;
+  p.tokens = B * S;
+  p.interleaved = layout == DMAD_ROTARY_INTERLEAVED;
+  p.factor = factor;
+  p.sign = transposed ? -1 : 1;
+  if (!dmad::rotary_plan(p, esz, (int)align)) return fail(DMAD_ERR_UNSUPPORTED, "too many heads and tokens");
+  hipStream_t s = (hipStream_t)stream;
+  mark(0, false, s);
+  const hipError_t e = dmad::launch_rotary(p, dtype, s);
+  mark(0, true, s);
+  if (e != hipSuccess) return fail(DMAD_ERR_HIP, "rotation launch: %s", hipGetErrorString(e));
   return ok();
 }
 

@@ -62,12 +62,17 @@ struct PagedAttnParams {
   float* part_ml;          // [splits + B][heads][R][2]: maximum (log2 domain) and sum
   float* scores;           // [B][heads][R][M P], log2 domain; null: weights are not accumulated
   float* lse2;             // [B][heads][R], log2 domain (with scores)
+  int keep_parts;          // every segment stays in part_o and part_ml, for a join with another cache's
 };
 // Rows of a workgroup of paged attention at head dim D, of R rows per key head.
 int paged_attn_rows(int D, int R);
 // Its workgroups per CU that a launch aims at.
 int paged_attn_resident(int D);
 hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, int D, hipStream_t s);
+// Attention over prefixes and over each sequence's own slots behind its prefix:
+// sequence b of p follows prefix b / (p.kv.B / shared.kv.B), whose rows in
+// `shared` are those of its sequences one after the other. Both keep_parts.
+hipError_t launch_prefix_attn(const PagedAttnParams& shared, const PagedAttnParams& p, int dtype, int D, hipStream_t s);
 
 // ---------------------------------------------------------------- eviction
 // Up to this many slots per sequence the selection keeps its keys in LDS (128 KiB).

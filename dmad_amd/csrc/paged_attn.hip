@@ -36,109 +36,12 @@
 // 1.59). A sequence that lies in several pieces leaves (maximum, sum, O) of each
 // in float32 and a second kernel joins them in order; one that lies in a single
 // piece is finished by the first kernel.
-#include "kv_cache.h"
-#include "lanes.h"
+#include "paged_pieces.h"
 
 namespace dmad {
 
 constexpr int kPagedWaves = 4;
 constexpr int kStep = 32;  // slots per wave step
-
-// Running sum over the lanes, the lane's own included: within rows of 16
-// lanes, then the row before's last lane, then lane 31's.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int scan_step(int x) {
-  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int wave_scan(int x) {
-  x = scan_step<0x111, 0xf>(x);  // from 1, 2, 4 and 8 lanes below
-  x = scan_step<0x112, 0xf>(x);
-  x = scan_step<0x114, 0xf>(x);
-  x = scan_step<0x118, 0xf>(x);
-  x = scan_step<0x142, 0xa>(x);  // lane 15 to rows 1, 3
-  x = scan_step<0x143, 0xc>(x);  // lane 31 to rows 2, 3
-  return x;
-}
-__device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
-
-// How the work is cut. Each sequence is a run of 128-slot tiles (one at least),
-// the runs follow one another, and piece x takes tiles [x chunk, (x + 1) chunk)
-// of that line, whatever sequences they belong to: equal work for every
-// workgroup of a ragged batch. A piece's part of a sequence is a segment; with
-// the pieces and the sequences both in order, x + b numbers the segments
-// without a clash. Every read of a length may find another value where a caller
-// writes them meanwhile: pieces and sequences are kept in range whatever the
-// lengths were, so that such a call gives wrong results and nothing worse.
-__device__ __forceinline__ int paged_tiles(int n) { return max(1, (n + kPagedTile - 1) / kPagedTile); }
-
-// Lengths of all sequences, a lane each; the first 64 are read once.
-struct PagedLengths {
-  const KvPages& kv;
-  int lane, first;
-  __device__ __forceinline__ PagedLengths(const KvPages& k, int l) : kv(k), lane(l), first(l < k.B ? k.length(l) : 0) {}
-  // length of sequence b0 + lane (b0 a multiple of 64), and its tiles (0 beyond the last)
-  __device__ __forceinline__ int at(int b0) const { return b0 == 0 ? first : b0 + lane < kv.B ? kv.length(b0 + lane) : 0; }
-  __device__ __forceinline__ int tiles(int b0) const { return b0 + lane < kv.B ? paged_tiles(at(b0)) : 0; }
-  __device__ __forceinline__ int total() const {
-    int t = 0;
-    for (int b0 = 0; b0 < kv.B; b0 += 64) t += tiles(b0);
-    return wave_total(t);
-  }
-};
-
-// A sequence and where its run of tiles begins.
-struct PagedRun {
-  int b, n, base;
-};
-__device__ __forceinline__ PagedRun run_of_tile(const PagedLengths& len, int tile) {
-  int before = 0;
-  for (int b0 = 0; b0 < len.kv.B; b0 += 64) {
-    // one reading: a tile is never before its sequence's first
-    const int n = len.at(b0), end = before + wave_scan(b0 + len.lane < len.kv.B ? paged_tiles(n) : 0);
-    const uint64_t past = __ballot(end > tile);
-    if (past != 0) {
-      const int at = __builtin_ctzll(past);
-      const int m = __builtin_amdgcn_readlane(n, at);
-      return PagedRun{b0 + at, m, __builtin_amdgcn_readlane(end, at) - paged_tiles(m)};
-    }
-    before = __builtin_amdgcn_readlane(end, 63);
-  }
-  return PagedRun{len.kv.B, 0, before};  // beyond the last tile: not asked for
-}
-__device__ __forceinline__ PagedRun run_of_sequence(const PagedLengths& len, int b) {
-  int before = 0;
-  for (int b0 = 0; b0 < b; b0 += 64) before += b0 + len.lane < b ? len.tiles(b0) : 0;
-  return PagedRun{b, len.kv.length(b), wave_total(before)};
-}
-
-// Piece x, segment by segment.
-struct PagedPiece {
-  const KvPages& kv;
-  PagedRun run;
-  int tile, stop, end;  // this segment's first tile, the piece's end, the segment's end
-  __device__ __forceinline__ PagedPiece(const KvPages& k, int splits, int x, int lane) : kv(k), run{0, 0, 0}, tile(0), stop(0), end(0) {
-    const PagedLengths len(kv, lane);
-    const int total = len.total(), chunk = max(1, (total + splits - 1) / splits);
-    tile = x * chunk;
-    stop = min(total, tile + chunk);
-    if (tile < stop) run = run_of_tile(len, tile);
-    if (run.b >= kv.B) stop = tile;
-    end = min(stop, run.base + paged_tiles(run.n));
-  }
-  __device__ __forceinline__ bool done() const { return tile >= stop; }
-  __device__ __forceinline__ bool last() const { return end >= stop; }
-  __device__ __forceinline__ void next() {
-    tile = end;
-    if (run.b + 1 >= kv.B) stop = tile;
-    if (done()) return;
-    run = PagedRun{run.b + 1, kv.length(run.b + 1), run.base + paged_tiles(run.n)};
-    end = min(stop, run.base + paged_tiles(run.n));
-  }
-  // the segment's slots, and whether it is the whole sequence
-  __device__ __forceinline__ int first_slot() const { return (tile - run.base) * kPagedTile; }
-  __device__ __forceinline__ int end_slot() const { return min(run.n, (end - run.base) * kPagedTile); }
-  __device__ __forceinline__ bool whole() const { return tile == run.base && end == run.base + paged_tiles(run.n); }
-};
 
 // Elements of O, or of a partial: 4 floats to 4 elements.
 template <typename T>
@@ -480,7 +383,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, D * NT <= 128 ? 2 : 1) void paged
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = fmaf(f, y[k], o[k]);
       }
-      if (piece.whole()) {
+      if (piece.whole() && !p.keep_parts) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const int hq = hk * p.G + r % p.G, tok = r / p.G, Hq = kv.heads * p.G;
         store4<T>((T*)p.o + (((int64_t)b * p.S + tok) * Hq + hq) * D + d, o * inv);
@@ -556,6 +459,62 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
   }
 }
 
+// Joins a row's pieces over a prefix that sequences share with those over its own
+// slots: `shared` has a run of n = B / P sequences' rows per prefix, and row r of
+// sequence b is row (b % n) R + r of prefix b / n.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prefix_join_kernel(PagedAttnParams shared, PagedAttnParams p) {
+  constexpr int LANES = D / 4, STRANDS = 256 / LANES;
+  __shared__ float sm_o[STRANDS][D], sm_m[STRANDS], sm_l[STRANDS];
+  const int r = (int)blockIdx.x % p.R, hk = ((int)blockIdx.x / p.R) % p.kv.heads, b = (int)blockIdx.x / (p.R * p.kv.heads);
+  const int strand = threadIdx.x / LANES, d = (threadIdx.x % LANES) * 4;
+  const int n = p.kv.B / shared.kv.B;
+  float m = -__builtin_inff(), l = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  auto gather = [&](const PagedAttnParams& a, int seq, int row, int turn) {
+    const PagedLengths len(a.kv, lane_id());
+    const int chunk = max(1, (len.total() + a.splits - 1) / a.splits);
+    const PagedRun run = run_of_sequence(len, seq);
+    const int first = run.base / chunk, last = min((run.base + paged_tiles(run.n) - 1) / chunk, a.splits - 1);
+    for (int i = first + (strand + turn) % STRANDS; i <= last; i += STRANDS) {
+      const int64_t at = ((int64_t)(i + seq) * a.kv.heads + hk) * a.R + row;
+      const float mi = a.part_ml[2 * at], li = a.part_ml[2 * at + 1];
+      const f32x4_t oi = *(const f32x4_t*)(a.part_o + at * D + d);
+      const float up = fmaxf(m, mi), base = up == -__builtin_inff() ? 0.f : up;
+      const float f = fast_exp2(m - base), fi = fast_exp2(mi - base);
+      l = l * f + li * fi;
+      o = o * f + oi * fi;
+      m = up;
+    }
+  };
+  gather(shared, b / n, (b % n) * p.R + r, 0);
+  gather(p, b, r, STRANDS / 2);  // from the other end of the strands, which few pieces leave idle
+  *(f32x4_t*)&sm_o[strand][d] = o;
+  if (d == 0) {
+    sm_m[strand] = m;
+    sm_l[strand] = l;
+  }
+  __syncthreads();
+  if (strand != 0) return;
+  float top = -__builtin_inff();
+  for (int i = 0; i < STRANDS; ++i) top = fmaxf(top, sm_m[i]);
+  const float base = top == -__builtin_inff() ? 0.f : top;
+  float sum = 0.f;
+  o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < STRANDS; ++i) {
+    const float f = fast_exp2(sm_m[i] - base);
+    sum = fmaf(f, sm_l[i], sum);
+    o = o + *(const f32x4_t*)&sm_o[i][d] * f;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int hq = hk * p.G + r % p.G, tok = r / p.G, Hq = p.kv.heads * p.G;
+  store4<T>((T*)p.o + (((int64_t)b * p.S + tok) * Hq + hq) * D + d, o * inv);
+  if (d == 0) {
+    const float l2 = base + __builtin_amdgcn_logf(sum);
+    p.lse[((int64_t)b * Hq + hq) * p.S + tok] = sum == 0.f ? -__builtin_inff() : l2 * 0.6931471805599453f;
+  }
+}
+
 // weight_j += sum over the rows of exp2(score - lse2), a tile of slots at a time
 // and a slot per thread. The line of tiles is cut finer than for the attention:
 // short sequences follow one another through the same wait for every one (17
@@ -623,7 +582,7 @@ static hipError_t paged_launch(const PagedAttnParams& p, hipStream_t s) {
   else paged_launch_rows<T, D, ACC, false>(p, s);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if (p.part_o != nullptr) {
+  if (p.part_o != nullptr && !p.keep_parts) {
     hipLaunchKernelGGL((paged_join_kernel<T, D, ACC>), dim3((unsigned)(p.kv.B * p.kv.heads * p.R)), dim3(256), 0, s, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
@@ -650,6 +609,30 @@ static hipError_t paged_launch_t(const PagedAttnParams& p, int D, hipStream_t s)
     case 256: return paged_launch_d<T, 256>(p, s);
   }
   return hipErrorInvalidValue;
+}
+
+template <typename T, int D>
+static hipError_t prefix_launch_d(const PagedAttnParams& shared, const PagedAttnParams& p, hipStream_t s) {
+  hipError_t e = paged_launch<T, D, false>(shared, s);
+  if (e != hipSuccess || (e = paged_launch<T, D, false>(p, s)) != hipSuccess) return e;
+  hipLaunchKernelGGL((prefix_join_kernel<T, D>), dim3((unsigned)(p.kv.B * p.kv.heads * p.R)), dim3(256), 0, s, shared, p);
+  return hipGetLastError();
+}
+
+template <typename T>
+static hipError_t prefix_launch_t(const PagedAttnParams& shared, const PagedAttnParams& p, int D, hipStream_t s) {
+  switch (D) {
+    case 16: return prefix_launch_d<T, 16>(shared, p, s);
+    case 32: return prefix_launch_d<T, 32>(shared, p, s);
+    case 64: return prefix_launch_d<T, 64>(shared, p, s);
+    case 128: return prefix_launch_d<T, 128>(shared, p, s);
+    case 256: return prefix_launch_d<T, 256>(shared, p, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch_prefix_attn(const PagedAttnParams& shared, const PagedAttnParams& p, int dtype, int D, hipStream_t s) {
+  return dtype == 0 ? prefix_launch_t<__bf16>(shared, p, D, s) : prefix_launch_t<_Float16>(shared, p, D, s);
 }
 
 hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, int D, hipStream_t s) {

@@ -1,0 +1,206 @@
+// Rotations of queries and keys by their positions, and of their tangents or
+// gradients. With angle = position * frequency_i, c = m cos, s = m sin:
+//   (a, b) -> (a c - b s, b c + a s)
+// over pairs (a, b) of elements 2i, 2i + 1 (interleaved) or i, i + R/2 (halves) of
+// the first R of a head's D elements; the others are copied. m is one factor for
+// all (stretched frequencies come with one). Backwards the same by -angle.
+//
+// Far positions have angles of many turns: position times frequency is taken in
+// 64 bits, reduced to a part of a turn there, and only that part is rounded to
+// float32 (position 131072 in float32 would be off by 0.008 radians).
+//
+// Bound by its bytes: 4 D per row of 16 bits, in and out. A workgroup takes a tile of
+// tokens: its threads first compute the tile's sines and cosines into LDS, each
+// once for all heads and both operands, then walk over units of two 16-byte
+// accesses: both halves of 8 pairs, 8 pairs of neighbours, or 16 elements to
+// copy. Smaller accesses where sizes or strides ask for them.
+#include "block_ops.h"
+#include "lanes.h"
+
+namespace dmad {
+
+constexpr int kRotaryThreads = 256;
+constexpr int kRotaryLdsPairs = 4096;  // sines and cosines of a tile: 32 KiB
+constexpr int kRotaryMaxTile = 64;
+
+// V consecutive elements, in one access of up to 16 bytes.
+template <typename T, int V>
+struct Piece {
+  typedef T vec_t __attribute__((ext_vector_type(V)));
+  vec_t v;
+  __device__ __forceinline__ void load(const T* p) { v = *(const vec_t*)p; }
+  __device__ __forceinline__ void store(T* p) const { *(vec_t*)p = v; }
+  __device__ __forceinline__ float get(int i) const { return (float)v[i]; }
+  __device__ __forceinline__ void set(int i, float x) { v[i] = (T)x; }
+};
+template <typename T>
+struct Piece<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = v; }
+  __device__ __forceinline__ float get(int) const { return (float)v; }
+  __device__ __forceinline__ void set(int, float x) { v = (T)x; }
+};
+
+// x / d by d's multiplier, of which 1 has none.
+__device__ __forceinline__ int rotary_div(int x, uint32_t mul) { return mul == 0 ? x : (int)__umulhi((uint32_t)x, mul); }
+
+// One unit of a row: its two pieces turned.
+template <typename T, int V, bool INTERLEAVED>
+__device__ __forceinline__ void rotary_turn(Piece<T, V>& u, Piece<T, V>& w, const float* cs, const float* sn) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float c = cs[i], s = sn[i];
+    if constexpr (INTERLEAVED) {
+      // pairs 2i, 2i + 1 of the 2 V elements
+      auto at = [&](int k) -> float { return k < V ? u.get(k) : w.get(k - V); };
+      const float a = at(2 * i), b = at(2 * i + 1);
+      const float x = fmaf(a, c, -(b * s)), y = fmaf(b, c, a * s);
+      if constexpr (V == 1) {
+        u.set(0, x);
+        w.set(0, y);
+      } else {
+        if (2 * i < V) {
+          u.set(2 * i, x);
+          u.set(2 * i + 1, y);
+        } else {
+          w.set(2 * i - V, x);
+          w.set(2 * i + 1 - V, y);
+        }
+      }
+    } else {
+      const float a = u.get(i), b = w.get(i);
+      u.set(i, fmaf(a, c, -(b * s)));
+      w.set(i, fmaf(b, c, a * s));
+    }
+  }
+}
+
+template <typename T, int V, bool INTERLEAVED, bool JVP>
+__global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryParams p) {
+  __shared__ __attribute__((aligned(16))) float cs[kRotaryLdsPairs], sn[kRotaryLdsPairs];
+  __shared__ int tok_b[kRotaryMaxTile], tok_s[kRotaryMaxTile];
+  const int64_t token0 = (int64_t)blockIdx.x * p.tile;
+  const int tokens = (int)min((int64_t)p.tile, p.tokens - token0), pairs = p.R >> 1;
+  if ((int)threadIdx.x < tokens) {
+    const int64_t t = token0 + threadIdx.x;
+    tok_b[threadIdx.x] = (int)(t / p.S);
+    tok_s[threadIdx.x] = (int)(t % p.S);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < tokens * pairs; i += kRotaryThreads) {
+    const int k = i / pairs, f = i - k * pairs;
+    const int64_t at = tok_b[k] * p.pos_b + tok_s[k] * p.pos_s;
+    const int64_t pos = p.pos64 ? ((const int64_t*)p.positions)[at] : (int64_t)((const int32_t*)p.positions)[at];
+    double turns = (double)pos * p.frequencies[f] * 0.15915494309189535;  // 1 / (2 pi)
+    turns -= rint(turns);
+    float s, c;
+    sincospif((float)(2.0 * turns), &s, &c);
+    cs[i] = c * p.factor;
+    sn[i] = s * p.factor * (float)p.sign;
+  }
+  __syncthreads();
+  const int units = tokens * p.per_token, turned = pairs / V;
+  for (int i = threadIdx.x; i < units; i += kRotaryThreads) {
+    const int k = rotary_div(i, p.token_mul), in_token = i - k * p.per_token;
+    int h = rotary_div(in_token, p.head_mul);
+    const int unit = in_token - h * p.per_head;
+    const RotaryOperand& o = p.op[h >= p.op[0].H];
+    if (h >= p.op[0].H) h -= p.op[0].H;
+    const int b = tok_b[k], s = tok_s[k];
+    const int64_t in = b * o.xb + s * o.xs + h * o.xh;
+    const int64_t tin = b * o.tb + s * o.ts + h * o.th;
+    const int64_t out = (((int64_t)b * p.S + s) * o.H + h) * p.D;
+    const bool turns = unit < turned;
+    int first, second;  // elements of the two pieces
+    if (turns) {
+      first = INTERLEAVED ? 2 * V * unit : V * unit;
+      second = INTERLEAVED ? first + V : first + pairs;
+    } else {
+      first = p.R + 2 * V * (unit - turned);
+      second = first + V;
+    }
+    const bool two = second < p.D;
+    Piece<T, V> u, w, tu, tw;
+    u.load((const T*)o.x + in + first);
+    if (two) w.load((const T*)o.x + in + second);
+    if constexpr (JVP) {
+      tu.load((const T*)o.t + tin + first);
+      if (two) tw.load((const T*)o.t + tin + second);
+    }
+    if (turns) {
+      const float *c = cs + k * pairs + V * unit, *z = sn + k * pairs + V * unit;
+      rotary_turn<T, V, INTERLEAVED>(u, w, c, z);
+      if constexpr (JVP) rotary_turn<T, V, INTERLEAVED>(tu, tw, c, z);
+    }
+    u.store((T*)o.out + out + first);
+    if (two) w.store((T*)o.out + out + second);
+    if constexpr (JVP) {
+      tu.store((T*)o.tout + out + first);
+      if (two) tw.store((T*)o.tout + out + second);
+    }
+  }
+}
+
+// Units that a workgroup aims at, and workgroups that fill the chip.
+constexpr int kRotaryUnits = 1024, kRotaryFill = 1024;
+
+bool rotary_plan(RotaryParams& p, int elem_size, int align) {
+  const int heads = p.op[0].H + p.op[1].H, pairs = p.R / 2, rest = p.D - p.R;
+  int v = 16 / elem_size;
+  while (v > 1 && (pairs % v != 0 || rest % v != 0 || p.D % v != 0 || align % v != 0)) v >>= 1;
+  p.vec = v;
+  p.per_head = pairs / v + (rest + 2 * v - 1) / (2 * v);
+  const int64_t per_token = (int64_t)heads * p.per_head;
+  int64_t tile = (kRotaryUnits + per_token - 1) / per_token;
+  const int64_t fill = (p.tokens + kRotaryFill - 1) / kRotaryFill;
+  if (tile > fill) tile = fill;
+  if (tile > kRotaryMaxTile) tile = kRotaryMaxTile;
+  if (pairs > 0 && tile > kRotaryLdsPairs / pairs) tile = kRotaryLdsPairs / pairs;
+  if (tile < 1) tile = 1;
+  if (pairs > kRotaryLdsPairs || per_token >= (1 << 20)) return false;
+  p.per_token = (int)per_token;
+  p.tile = (int)tile;
+  // m = ceil(2^32 / d) is off by e = m d - 2^32 < d parts of d: x m >> 32 = x / d while x e < 2^32
+  auto mul = [&](int64_t d, uint32_t& m) {
+    const int64_t q = (((int64_t)1 << 32) + d - 1) / d, e = q * d - ((int64_t)1 << 32);
+    m = d == 1 ? 0u : (uint32_t)q;
+    return per_token * tile * e < ((int64_t)1 << 32);
+  };
+  if (!mul(p.per_head, p.head_mul) || !mul(per_token, p.token_mul)) return false;
+  return (p.tokens + tile - 1) / tile < ((int64_t)1 << 24);
+}
+
+template <typename T, int V>
+static hipError_t rotary_launch_v(const RotaryParams& p, hipStream_t s) {
+  const dim3 grid((unsigned)((p.tokens + p.tile - 1) / p.tile)), block(kRotaryThreads);
+  const bool jvp = p.op[0].t != nullptr || p.op[1].t != nullptr;
+  if (p.interleaved) {
+    if (jvp) hipLaunchKernelGGL((rotary_kernel<T, V, true, true>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((rotary_kernel<T, V, true, false>), grid, block, 0, s, p);
+  } else {
+    if (jvp) hipLaunchKernelGGL((rotary_kernel<T, V, false, true>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((rotary_kernel<T, V, false, false>), grid, block, 0, s, p);
+  }
+  return hipGetLastError();
+}
+
+template <typename T>
+static hipError_t rotary_launch_t(const RotaryParams& p, hipStream_t s) {
+  switch (p.vec) {
+    case 8:
+      if constexpr (sizeof(T) == 2) return rotary_launch_v<T, 8>(p, s);
+      return hipErrorInvalidValue;
+    case 4: return rotary_launch_v<T, 4>(p, s);
+    case 2: return rotary_launch_v<T, 2>(p, s);
+    default: return rotary_launch_v<T, 1>(p, s);
+  }
+}
+
+hipError_t launch_rotary(const RotaryParams& p, int dtype, hipStream_t s) {
+  if (dtype == 0) return rotary_launch_t<__bf16>(p, s);
+  if (dtype == 1) return rotary_launch_t<_Float16>(p, s);
+  return rotary_launch_t<float>(p, s);
+}
+
+}  // namespace dmad

@@ -1,12 +1,13 @@
 """A paged key-value cache for token-by-token and block-by-block inference on the gfx950 kernels.
 
-``PagedKVCache`` holds the pages and what its sequences hold. Three calls work on it:
+``PagedKVCache`` holds the pages and what its sequences hold. These calls work on it:
 
   * ``qk_norm_rope_append``: the new tokens' queries and keys are normalised per head and rotated
     (as ``qk_norm_rope_with_tangent`` does), keys and values go into the pages; ``append_kv`` is
     the same without queries, norm and rotation;
   * ``paged_attention``: attention of those queries over the cache, optionally adding up the
     attention weight every slot receives;
+  * ``shared_prefix_attention``: the same of sequences that share a prefix, a cache of its own;
   * ``evict_low_weight``: cuts long sequences to their heaviest slots.
 
 They run without derivatives (operands that carry any are refused), put only kernel launches on the current stream and read lengths and
@@ -255,6 +256,23 @@ def _(q, sm_scale, causal, *cache):
     return q.new_empty(q.shape), q.new_empty((B, Hq, S), dtype=torch.float32)
 
 
+@torch.library.custom_op("dmad::prefix_attn", mutates_args=())
+def _prefix_op(q: torch.Tensor, sm_scale: float, causal: bool, prefix_k_pages: torch.Tensor, prefix_v_pages: torch.Tensor,
+               prefix_table: torch.Tensor, prefix_lengths: torch.Tensor, prefix_seen: torch.Tensor, k_pages: torch.Tensor,
+               v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+               seen: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(o, lse) of ``shared_prefix_attention``."""
+    prefix = PagedKVCache(prefix_k_pages, prefix_v_pages, prefix_table, prefix_lengths, prefix_seen)
+    cache = PagedKVCache(k_pages, v_pages, page_table, lengths, seen)
+    return _prefix_attend(q, prefix, cache, _check_prefix(q, prefix, cache, sm_scale), causal)
+
+
+@_prefix_op.register_fake
+def _(q, sm_scale, causal, *caches):
+    B, S, Hq, _ = q.shape
+    return q.new_empty(q.shape), q.new_empty((B, Hq, S), dtype=torch.float32)
+
+
 @torch.library.custom_op("dmad::kv_evict", mutates_args=("k_pages", "v_pages", "lengths", "weight", "position"))
 def _evict_op(keep: int, recent: int, sink: int, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
               lengths: torch.Tensor, seen: torch.Tensor, weight: torch.Tensor, position: torch.Tensor) -> None:
@@ -398,6 +416,80 @@ def _attend(q, cache, scale, causal, accumulate):
             cache._code, cache._ref, S, Hq, nat.ptr(q), strides, int(causal), int(accumulate), scale,
             nat.ptr(o), nat.ptr(lse), ws_ptr, ws_size, nat.stream_ptr(cache.device)))
     return o, lse
+
+
+_PREFIX = "shared_prefix_attention"
+
+
+def _check_prefix(q, prefix, cache, sm_scale):
+    """Refuses what the attention behind prefixes does not take; the scale."""
+    op = _PREFIX
+    if not isinstance(prefix, PagedKVCache):
+        raise TypeError(f"{op}: prefix must be a PagedKVCache, got {type(prefix).__name__}")
+    _check_new(op, cache, ("q", q))
+    prefix._settle()
+    if prefix.device != cache.device:
+        raise ValueError(f"{op}: the prefix on {prefix.device}, the cache on {cache.device}")
+    if prefix.dtype != cache.dtype or prefix.kv_heads != cache.kv_heads or prefix.head_dim != cache.head_dim:
+        raise ValueError(f"{op}: the prefix holds {prefix.kv_heads} heads of {prefix.head_dim} {prefix.dtype}, the cache "
+                         f"{cache.kv_heads} of {cache.head_dim} {cache.dtype}")
+    if prefix.batch < 1 or cache.batch % prefix.batch:
+        raise ValueError(f"{op}: {cache.batch} sequences cannot share {prefix.batch} prefixes evenly")
+    _no_grad_only(op, cache, q, prefix.k_pages, prefix.v_pages)
+    Hq = q.shape[2]
+    if Hq < 1 or Hq % cache.kv_heads:
+        raise ValueError(f"{op}: {Hq} query heads are not a multiple of the cache's {cache.kv_heads}")
+    scale = cache.head_dim ** -0.5 if sm_scale is None else float(sm_scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise NotImplementedError(f"{op}: sm_scale must be positive and finite, got {sm_scale}")
+    return scale
+
+
+def shared_prefix_attention(q, prefix, cache, sm_scale=None, causal=False, return_lse=False):
+    """``paged_attention`` of sequences that share prefixes: o [B, S, Hq, D] (and lse [B, Hq, S]).
+
+    ``prefix`` is a PagedKVCache of P sequences, P a divisor of B: the B / P sequences from b B / P on share prefix b, as
+    the samples of one prompt or the continuations of one clip do. Every token sees all slots of its prefix, and of the
+    sequence's own ``cache`` what ``paged_attention`` shows it (``causal``: the S tokens are the last S of its own slots).
+    The result is that of caches whose page tables begin with the prefix's pages, but K and V of a prefix are read for all
+    rows of its sequences together rather than once per sequence. The two caches may share one pool of pages; a prefix or
+    a cache of no slots adds nothing, and a token that sees no slot of either gets o = 0 and lse = -inf. The caches are
+    only read; weights are not accumulated.
+    """
+    scale = _check_prefix(q, prefix, cache, sm_scale)
+    causal = bool(causal)
+    if _eager_call(q):
+        o, lse = _prefix_attend(q, prefix, cache, scale, causal)
+    else:
+        refuse_forward_mode(_PREFIX, q, *_cache_tensors(prefix), *_cache_tensors(cache))
+        o, lse = torch.ops.dmad.prefix_attn(q, scale, causal, *_cache_tensors(prefix)[:5], *_cache_tensors(cache)[:5])
+    return (o, lse) if return_lse else o
+
+
+def _prefix_attend(q, prefix, cache, scale, causal):
+    """The launches: (o, lse)."""
+    B, S, Hq, _ = q.shape
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = cache._floats.new_empty((B, Hq, S))
+    q, strides = readable_rows(q)
+    if S > 1 and B > 1 and q.stride(0) != S * q.stride(1):  # one stride for all tokens of a prefix
+        q, strides = readable_rows(q.clone(memory_format=torch.contiguous_format))
+    size = _prefix_workspace(prefix, cache, S, Hq)
+    ws = cache._bytes.new_empty(size)
+    with nat.on_device(cache.device):
+        nat.check(nat.lib().dmad_prefix_attn(
+            cache._code, prefix._ref, cache._ref, S, Hq, nat.ptr(q), strides, int(causal), scale, nat.ptr(o), nat.ptr(lse),
+            ws.data_ptr(), size, nat.stream_ptr(cache.device)))
+    return o, lse
+
+
+def _prefix_workspace(prefix, cache, S, Hq):
+    """Bytes of workspace, asked once per sizes of both caches."""
+    key = (S, Hq, prefix.batch, prefix.capacity)
+    size = cache._sizes.get(key)
+    if size is None:
+        size = cache._sizes[key] = nat.prefix_attn_workspace_bytes(cache._c, prefix._c, S, Hq)
+    return size
 
 
 def _check_evict(cache, keep, recent, sink):

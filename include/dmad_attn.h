@@ -362,6 +362,73 @@ int dmad_qk_norm_rope_bwd(int dtype, int wdtype, int64_t B, int64_t S, int64_t H
                           void* stream);
 
 /*
+ * Gate, residual and norm in one pass, between two parts of a block (no
+ * counterpart as one call in the reference, whose blocks write it out:
+ * train/wan/rcm/networks/wan2pt1_jvp.py:551-609):
+ *   y' = y, or y / sqrt(mean(y^2) + eps) * post_weight where that is given
+ *   x' = x + residual_scale * gate * y'
+ *   n  = (N(x') * weight + bias) * (1 + scale) + shift
+ * N(x') = (x' - mean(x')) / sqrt(var(x') + eps) (DMAD_NORM_LAYER) or
+ * x' / sqrt(mean(x'^2) + eps) (DMAD_NORM_RMS) over the C channels.
+ *   x, y   : [B, S, C] by element strides {b, s, c}, c = 1; y null: x' = x,
+ *            which is not written
+ *   gate, scale, shift: [B, F, C] by strides {b, f, c} in type wdtype (the
+ *            operands' or DMAD_F32); token s takes row s / (S / F); null: absent
+ *   weight, bias, post_weight: [C] in type wdtype, or null
+ *   t...   : tangents; tx and (with y) ty for a call with tangents, those of
+ *            gate, scale and shift where they are not zero
+ *   xo, txo, no, tno: contiguous [B, S, C]
+ * Rows start 16-byte aligned; C a multiple of 8 up to 8192; bf16, fp16 and
+ * fp32. Computed in float32 and rounded once (n from x' before its rounding).
+ */
+enum { DMAD_NORM_LAYER = 0, DMAD_NORM_RMS = 1 };
+typedef struct dmad_gated_norm_sizes {
+  int32_t dtype, wdtype, norm;
+  int64_t B, S, C, F;
+  /* strides; of operands that are null they are not looked at */
+  int64_t x[3], y[3], tx[3], ty[3];
+  int64_t gate[3], scale[3], shift[3], tgate[3], tscale[3], tshift[3];
+} dmad_gated_norm_sizes;
+int dmad_gated_norm(const dmad_gated_norm_sizes* sizes, const void* x, const void* tx, const void* y, const void* ty,
+                    const void* gate, const void* tgate, const void* scale, const void* tscale, const void* shift,
+                    const void* tshift, const void* weight, const void* bias, const void* post_weight, float eps,
+                    float residual_scale, void* xo, void* txo, void* no, void* tno, void* stream);
+
+/* Bytes of workspace of dmad_gated_norm_bwd (not looked at where no small operand's gradient is asked for). */
+int dmad_gated_norm_bwd_workspace_bytes(const dmad_gated_norm_sizes* sizes, size_t* bytes);
+
+/*
+ * Its backward: gx, gn the gradients of x' and n by the strides `tx` and `ty`
+ * of the sizes (one of them may be null), dx, dy contiguous [B, S, C] (dy may
+ * be null), dgate, dscale, dshift contiguous [B, F, C] and dweight, dbias,
+ * dpost [C] of type wdtype, each null where it is not wanted. Sums run in a
+ * fixed order.
+ */
+int dmad_gated_norm_bwd(const dmad_gated_norm_sizes* sizes, const void* x, const void* y, const void* gx, const void* gn,
+                        const void* gate, const void* scale, const void* weight, const void* bias,
+                        const void* post_weight, float eps, float residual_scale, void* dx, void* dy, void* dgate,
+                        void* dscale, void* dshift, void* dweight, void* dbias, void* dpost, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/*
+ * Queries and keys turned by their positions (the reference turns pairs of
+ * neighbours by a table of angles, train/wan/rcm/utils/rope.py:56-70). Pair i of
+ * the first R of a head's D elements, (2i, 2i+1) or (i, i + R/2), is turned by
+ * positions * frequencies[i] (taken in float64) and multiplied by factor; the
+ * other elements are copied. transposed: by the negative angle (the gradient).
+ *   q, k, tq, tk, oq, ok, otq, otk: as in dmad_qk_norm_rope, any alignment of
+ *           whole elements, D any from 1 to 8192
+ *   positions: [B, S] by strides {b, s}, int32, or int64 with positions_64
+ *   frequencies: [R/2] radians per position
+ */
+enum { DMAD_ROTARY_INTERLEAVED = 0, DMAD_ROTARY_HALF = 1 };
+int dmad_qk_rotary(int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, int64_t R, const void* q,
+                   const void* tq, const void* k, const void* tk, const int64_t q_strides[4], const int64_t tq_strides[4],
+                   const int64_t k_strides[4], const int64_t tk_strides[4], const void* positions, int positions_64,
+                   const int64_t position_strides[2], const double* frequencies, int layout, int transposed, float factor,
+                   void* oq, void* otq, void* ok, void* otk, void* stream);
+
+/*
  * A paged key-value cache in device memory. Sequence b's slot s is slot
  * s % page_size of page page_table[b * table_stride + s / page_size]; an id
  * outside [0, num_pages) marks a page that holds nothing: its slots are
@@ -415,6 +482,22 @@ int dmad_paged_attn_workspace_bytes(const dmad_kv_cache* cache, int64_t S, int64
 int dmad_paged_attn(int dtype, const dmad_kv_cache* cache, int64_t S, int64_t Hq, const void* q,
                     const int64_t q_strides[4], int causal, int accumulate, float sm_scale, void* o, float* lse,
                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of dmad_prefix_attn. */
+int dmad_prefix_attn_workspace_bytes(const dmad_kv_cache* prefix, const dmad_kv_cache* cache, int64_t S, int64_t Hq,
+                                     size_t* bytes);
+
+/*
+ * The same where consecutive sequences share a prefix: sequence b sees all slots
+ * of sequence b / (batch / prefix batch) of `prefix` and then its own as in
+ * dmad_paged_attn (causal: the S tokens are the last S of its own slots). K and V of a prefix are
+ * read for all its sequences together. Both caches have the same heads, head
+ * dim and type; the prefix batch divides the cache's. q's sequences follow one
+ * another as their tokens do (stride b = S times stride s where S > 1).
+ */
+int dmad_prefix_attn(int dtype, const dmad_kv_cache* prefix, const dmad_kv_cache* cache, int64_t S, int64_t Hq,
+                     const void* q, const int64_t q_strides[4], int causal, float sm_scale, void* o, float* lse,
+                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* Bytes of workspace of dmad_kv_evict. */
 int dmad_kv_evict_workspace_bytes(const dmad_kv_cache* cache, int64_t keep, size_t* bytes);
