@@ -60,6 +60,7 @@ def units():
     # the per-head norm and the paged cache test for NaN (weights, positions without angles)
     out += [("qk_norm_rope.hip", "qk_norm_rope", ["-fhonor-nans"]), ("kv_evict.hip", "kv_evict", ["-fhonor-nans"]),
             ("paged_attn.hip", "paged_attn", ["-fhonor-nans", "-mllvm", "-amdgpu-mfma-vgpr-form"])]
+    out.append(("prefix_rows.hip", "prefix_rows", ["-mllvm", "-amdgpu-mfma-vgpr-form"]))
     # gate, residual and norm: operands of one type, small ones of the same or fp32
     for t, w, name in ((0, 0, "bf16"), (0, 1, "bf16_wide"), (1, 0, "f16"), (1, 1, "f16_wide"), (2, 0, "f32")):
         out.append(("gated_norm.hip", f"gated_norm_{name}", [f"-DDMAD_T={t}", f"-DDMAD_W={w}", "-fhonor-nans"]))

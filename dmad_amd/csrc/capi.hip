@@ -1353,19 +1353,20 @@ struct PagedLayout {
   int64_t R, row_groups, splits;
   size_t part_o, part_ml, scores, lse2, total;  // offsets; equal to the next where a part is absent
 };
-int paged_layout(const dmad_kv_cache* c, int64_t S, int64_t Hq, bool accumulate, PagedLayout& w) {
+int paged_layout(const dmad_kv_cache* c, int64_t S, int64_t Hq, bool accumulate, PagedLayout& w, bool prefix = false) {
   if (S < 0 || Hq < 1 || Hq % c->kv_heads != 0)
     return fail(DMAD_ERR_INVALID, "query heads (%lld) must be a multiple of the cache's key heads (%lld)", (long long)Hq,
                 (long long)c->kv_heads);
   const int64_t lim = (int64_t)1 << 31;
   if (S >= lim / Hq) return fail(DMAD_ERR_UNSUPPORTED, "too many query rows");
   w.R = S * (Hq / c->kv_heads);
-  const int64_t rows = dmad::paged_attn_rows((int)c->head_dim, (int)w.R);
+  const bool many = prefix && dmad::prefix_rows_takes((int)c->head_dim, (int)w.R);
+  const int64_t rows = many ? dmad::kPrefixRows : dmad::paged_attn_rows((int)c->head_dim, (int)w.R);
   w.row_groups = (w.R + rows - 1) / rows;
   const int64_t cap = c->pages_per_seq * c->page_size;
   const int64_t tiles = cap > 0 ? (cap + dmad::kPagedTile - 1) / dmad::kPagedTile : 1;
   const int64_t per = c->kv_heads * (w.row_groups > 0 ? w.row_groups : 1);
-  w.splits = paged_splits(per, dmad::paged_attn_resident((int)c->head_dim));
+  w.splits = paged_splits(per, many ? dmad::prefix_rows_resident((int)c->head_dim) : dmad::paged_attn_resident((int)c->head_dim));
   if (w.splits > c->batch * tiles) w.splits = c->batch * tiles;
   const bool join = tiles > 1;
   const size_t BR = (size_t)c->batch * c->kv_heads * w.R;
@@ -1400,7 +1401,7 @@ int prefix_layout(const dmad_kv_cache* prefix, const dmad_kv_cache* c, int64_t S
                 (long long)prefix->batch);
   const int64_t n = c->batch / prefix->batch;
   if (n > 0 && S >= ((int64_t)1 << 31) / n) return fail(DMAD_ERR_UNSUPPORTED, "too many query rows");
-  int rc = paged_layout(prefix, n * S, Hq, false, w.shared);
+  int rc = paged_layout(prefix, n * S, Hq, false, w.shared, true);
   if (rc != DMAD_OK || (rc = paged_layout(c, S, Hq, false, w.own)) != DMAD_OK) return rc;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   const size_t rows = (size_t)(w.shared.splits + prefix->batch) * c->kv_heads * w.shared.R;

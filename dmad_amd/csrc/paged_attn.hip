@@ -613,7 +613,8 @@ static hipError_t paged_launch_t(const PagedAttnParams& p, int D, hipStream_t s)
 
 template <typename T, int D>
 static hipError_t prefix_launch_d(const PagedAttnParams& shared, const PagedAttnParams& p, hipStream_t s) {
-  hipError_t e = paged_launch<T, D, false>(shared, s);
+  hipError_t e = prefix_rows_takes(D, shared.R) ? launch_prefix_rows(shared, __is_same(T, _Float16) ? 1 : 0, D, s)
+                                                : paged_launch<T, D, false>(shared, s);
   if (e != hipSuccess || (e = paged_launch<T, D, false>(p, s)) != hipSuccess) return e;
   hipLaunchKernelGGL((prefix_join_kernel<T, D>), dim3((unsigned)(p.kv.B * p.kv.heads * p.R)), dim3(256), 0, s, shared, p);
   return hipGetLastError();
