@@ -72,17 +72,30 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void prefix_ro
     roff_k[j] = (uint32_t)((row & 15) * (int64_t)kv.k_sl * 2) + logical * 16;
     roff_v[j] = (uint32_t)((row & 15) * (int64_t)kv.v_sl * 2) + logical * 16;
   }
-  int kx0, tx0[2];
+  // (256-wide heads keep the first ones: slice s lies at kx ^ 32 s, block db at tx ^ 64 db)
+  constexpr int NKX = D == 256 ? 1 : KS, NTX = D == 256 ? 1 : DB;
+  int kx[NKX], tx[NTX][2];
   {
-    const int r = perm32(col);
-    kx0 = r * ROWB + ((half ^ trswz<CR>(r & 15)) << 4);  // slice s at kx0 ^ 32 s
-    const int g = lane >> 4, rr = (lane & 15) >> 2, c = lane & 3;
+    const int r = perm32(col), g = lane >> 4, rr = (lane & 15) >> 2, c = lane & 3;
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const int row = 8 * (g >> 1) + 4 * hh + rr, chunk = 2 * (g & 1) + (c >> 1);
-      tx0[hh] = row * ROWB + ((chunk ^ trswz<CR>(row & 15)) << 4) + 8 * (c & 1);  // block db at tx0 ^ 64 db
-    }
+    for (int s = 0; s < NKX; ++s) kx[s] = r * ROWB + (((2 * s + half) ^ trswz<CR>(r & 15)) << 4);
+#pragma unroll
+    for (int db = 0; db < NTX; ++db)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int row = 8 * (g >> 1) + 4 * hh + rr, chunk = 4 * db + 2 * (g & 1) + (c >> 1);
+        tx[db][hh] = row * ROWB + ((chunk ^ trswz<CR>(row & 15)) << 4) + 8 * (c & 1);
+      }
   }
+  auto k_off = [&](int s) { return NKX == 1 ? kx[0] ^ (32 * s) : kx[s % NKX]; };
+  auto v_off = [&](int db, int hh) { return NTX == 1 ? tx[0][hh] ^ (64 * db) : tx[db % NTX][hh]; };
+  // re-defined at each step: stage and offset fold into the LDS instructions
+  auto pin = [&]() {
+#pragma unroll
+    for (int s = 0; s < NKX; ++s) asm volatile("" : "+v"(kx[s]));
+#pragma unroll
+    for (int db = 0; db < NTX; ++db) asm volatile("" : "+v"(tx[db][0]), "+v"(tx[db][1]));
+  };
   auto stage = [&](auto kk) -> lds_char_t* {
     constexpr int k = decltype(kk)::value % 4;
     if constexpr (k == 0) return (lds_char_t*)stg0;
@@ -106,38 +119,36 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void prefix_ro
         if (r < p.R) qreg[s] = *(const i32x4_t*)(q + s * 16);
       }
     }
-    // Pages of 32 steps' halves, one per lane: step lane/2, half lane%2; whether
-    // all 16 slots of each are there, of these steps and of the 32 before.
-    int pages = 0, slots = 0;
+    // Where 32 steps' halves begin and what of them is there, one half per lane (step
+    // lane/2, half lane%2): addresses of K's and V's 16 rows, bytes up to the last row
+    // in use (none for a missing page). And whether all 16 slots of each are there, of
+    // these steps and of the 32 before.
+    uint64_t k_at = 0, v_at = 0;
+    uint32_t k_bytes = 0, v_bytes = 0;
     uint64_t whole = 0, whole_before = 0;
     int window = -1;
     auto look_up = [&](int j0) {
       const int j = j0 + (lane >> 1), key = first + j * C::BN + (lane & 1) * 16;
-      pages = -1;
-      slots = 0;
-      if (j < ntiles && key < last) {
-        const KvSlot at = kv.locate(b, key);
-        pages = at.page;
-        slots = at.slot;
-      }
+      KvSlot at{-1, 0};
+      if (j < ntiles && key < last) at = kv.locate(b, key);
+      const int there = at.page < 0 ? 0 : min(last - key, 16);
+      const KvSlot from{max(at.page, 0), at.slot};
+      k_at = (uint64_t)kv.k + 2 * kv.k_offset(from, hk);
+      v_at = (uint64_t)kv.v + 2 * kv.v_offset(from, hk);
+      k_bytes = there ? (uint32_t)(((there - 1) * kv.k_sl + D) * 2) : 0;
+      v_bytes = there ? (uint32_t)(((there - 1) * kv.v_sl + D) * 2) : 0;
       whole_before = whole;
-      whole = __ballot(pages >= 0 && key + 16 <= last);
+      whole = __ballot(there == 16);
       window = j0 >> 5;
     };
-    // slots of half hh of step j that are there, and where they begin
+    auto lane_of = [](uint32_t v, int at) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
+    // request li of step j
     auto request = [&](lds_char_t* st, int j, int li) {
-      const int jj = li >> 1, i = wave + jj * C::NW, hh = __builtin_amdgcn_readfirstlane(i * C::RPR / 16);
-      const int at = 2 * (j & 31) + hh;
-      const int page = __builtin_amdgcn_readlane(pages, at), slot = __builtin_amdgcn_readlane(slots, at);
-      const int there = page < 0 ? 0 : min(max(last - (first + j * C::BN + hh * 16), 0), 16);
-      const KvSlot from{max(page, 0), slot};
-      if (li & 1) {
-        const uint32_t bytes = there ? (uint32_t)(((there - 1) * kv.v_sl + D) * 2) : 0;
-        buf_load16_lds(make_rsrc((const char*)kv.v + 2 * kv.v_offset(from, hk), bytes), st + C::TILE + i * 1024, roff_v[jj], 0);
-      } else {
-        const uint32_t bytes = there ? (uint32_t)(((there - 1) * kv.k_sl + D) * 2) : 0;
-        buf_load16_lds(make_rsrc((const char*)kv.k + 2 * kv.k_offset(from, hk), bytes), st + i * 1024, roff_k[jj], 0);
-      }
+      const int jj = li >> 1, i = wave + jj * C::NW, at = 2 * (j & 31) + i * C::RPR / 16;
+      const uint64_t from = li & 1 ? v_at : k_at;
+      const uint64_t base = (uint64_t)lane_of((uint32_t)(from >> 32), at) << 32 | lane_of((uint32_t)from, at);
+      const __amdgpu_buffer_rsrc_t rows = make_rsrc((const void*)base, lane_of(li & 1 ? v_bytes : k_bytes, at));
+      buf_load16_lds(rows, st + (li & 1 ? C::TILE : 0) + i * 1024, li & 1 ? roff_v[jj] : roff_k[jj], 0);
     };
 
     f32x16_t oacc[DB];
@@ -189,10 +200,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void prefix_ro
     auto all_there = [&](int i) { return (((i >> 5) == window ? whole : whole_before) >> (2 * (i & 31)) & 3) == 3; };
 
     auto load_op = [&](const lds_char_t* s_next, const lds_char_t* s_cur, int o) -> i32x4_t {
-      if (o < KS) return *(lds_i32x4_t*)(s_next + (kx0 ^ (32 * o)));
+      if (o < KS) return *(lds_i32x4_t*)(s_next + k_off(o));
       const int t = (o - KS) / DB, db = (o - KS) % DB;
       const lds_char_t* base = s_cur + C::TILE + t * 16 * ROWB;
-      const u32x2_t lo = lds_read_tr16(base + (tx0[0] ^ (64 * db))), hi = lds_read_tr16(base + (tx0[1] ^ (64 * db)));
+      const u32x2_t lo = lds_read_tr16(base + v_off(db, 0)), hi = lds_read_tr16(base + v_off(db, 1));
       return i32x4_t{(int)lo[0], (int)lo[1], (int)hi[0], (int)hi[1]};
     };
     auto mfma_op = [&](int o, i32x4_t a, f32x16_t& sn, const i32x4_t (&pk)[2]) {
@@ -201,9 +212,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void prefix_ro
     };
     auto rescale = [&](float alpha) {
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+      for (int d = 0; d < DB; ++d) {
+        asm volatile("" : "+v"(oacc[d]));  // not to be computed ahead of the branch around it
 #pragma unroll
         for (int v = 0; v < 16; ++v) oacc[d][v] *= alpha;
+      }
     };
     // step i: scores of step i + 1 with the softmax of step i between them, then its
     // products with V, the requests of step i + 3 between those
@@ -211,7 +224,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void prefix_ro
       constexpr int k = decltype(kk)::value;
       if (((i + 3) & 31) == 0) look_up(i + 3);
       ring_sync<C::LOADS>();  // step i + 1 has landed, step i + 2 may be in flight
-      asm volatile("" : "+v"(kx0), "+v"(tx0[0]), "+v"(tx0[1]));
+      pin();
       const lds_char_t *s_next = stage(IC<k + 1>{}), *s_cur = stage(IC<k>{});
       lds_char_t* s_req = stage(IC<k + 3>{});
       if (!all_there(i)) mask(sc, i);
