@@ -30,10 +30,10 @@ struct GatedNormParams {
   int layer;                 // the norm subtracts the mean
   float eps, rs;             // rs: scale of the branch
   int past_caches;           // more than the caches hold
-  // backward: `split` workgroups per group of tokens. Either each leaves its sums
-  // in partial [B F split][kNormSums][C], or (partial null, split 1) writes the
-  // groups' gradients itself.
-  int split;
+  int split;                 // workgroups per group of tokens
+  // backward: either each leaves its sums in partial
+  // [B F split][kNormSums][C], or (partial null, split 1) writes the group's
+  // gradients itself
   float* partial;
   void *dgate, *dscale, *dshift;     // contiguous [B, F, C], or null
   void *dweight, *dbias, *dpost;     // [C], or null
@@ -41,12 +41,14 @@ struct GatedNormParams {
 
 // Widest rows.
 constexpr int kNormMaxC = 8192;
-// Channels from which a row takes a workgroup, not a wave.
-constexpr int kNormWaveC = 2048;
+// Waves of a workgroup for rows of C channels, and waves that a forward and a
+// backward pass aim at.
+int norm_waves(int C);
+constexpr int kNormFwdWaves = 16384, kNormBwdWaves = 4096;
 
 hipError_t launch_gated_norm(const GatedNormParams& p, int dtype, int wdtype, hipStream_t s);
-// Workgroups per group of tokens in the backward pass.
-int gated_norm_split(int64_t groups, int T, int C);
+// Workgroups per group of tokens.
+int gated_norm_split(int64_t groups, int T, int C, bool backward);
 hipError_t launch_gated_norm_bwd(const GatedNormParams& p, int dtype, int wdtype, hipStream_t s);
 
 // ---------------------------------------------------------------- rotations by position

@@ -1485,9 +1485,15 @@ int norm_vector(const char* name, int dtype, const void* ptr, const int64_t* st,
   return norm_rows(name, ptr, st, elem_size(dtype), o.b, o.f);
 }
 
-int norm_split(const dmad::GatedNormParams& p) { return dmad::gated_norm_split((int64_t)p.B * p.F, p.T, p.C); }
+// Cuts the tokens; a launch takes fewer than 2^32 threads.
+int norm_cut(dmad::GatedNormParams& p, bool backward) {
+  p.split = dmad::gated_norm_split((int64_t)p.B * p.F, p.T, p.C, backward);
+  if ((int64_t)p.B * p.F * p.split * 64 * dmad::norm_waves(p.C) >= ((int64_t)1 << 32))
+    return fail(DMAD_ERR_UNSUPPORTED, "too many groups of tokens");
+  return DMAD_OK;
+}
 size_t norm_workspace(const dmad::GatedNormParams& p) {
-  return (size_t)p.B * p.F * norm_split(p) * dmad::kNormSums * p.C * sizeof(float);
+  return (size_t)p.B * p.F * p.split * dmad::kNormSums * p.C * sizeof(float);
 }
 
 // Largest power of two up to 8 elements that divides n (a stride or an address in bytes over esz).
@@ -2143,6 +2149,8 @@ int dmad_gated_norm(const dmad_gated_norm_sizes* sizes, const void* x, const voi
   p.txo = txo;
   p.no = no;
   p.tno = tno;
+  if ((rc = norm_cut(p, false)) != DMAD_OK) return rc;
+  p.past_caches = dmad::qk_past_caches((y != nullptr ? 8 : 4) * p.rows * p.C * elem_size(dt));
   hipStream_t s = (hipStream_t)stream;
   mark(0, false, s);
   const hipError_t e = dmad::launch_gated_norm(p, dt, wdt, s);
@@ -2154,8 +2162,8 @@ int dmad_gated_norm(const dmad_gated_norm_sizes* sizes, const void* x, const voi
 int dmad_gated_norm_bwd_workspace_bytes(const dmad_gated_norm_sizes* sizes, size_t* bytes) {
   if (bytes == nullptr) return fail(DMAD_ERR_INVALID, "bytes: null pointer");
   dmad::GatedNormParams p{};
-  const int rc = norm_sizes(sizes, 0.f, 1.f, p);
-  if (rc != DMAD_OK) return rc;
+  int rc = norm_sizes(sizes, 0.f, 1.f, p);
+  if (rc != DMAD_OK || (rc = norm_cut(p, true)) != DMAD_OK) return rc;
   *bytes = p.rows == 0 ? 0 : norm_workspace(p);
   return ok();
 }
@@ -2199,13 +2207,14 @@ int dmad_gated_norm_bwd(const dmad_gated_norm_sizes* sizes, const void* x, const
   p.dweight = dweight;
   p.dbias = dbias;
   p.dpost = dpost;
-  p.split = norm_split(p);
+  if ((rc = norm_cut(p, true)) != DMAD_OK) return rc;
   if (weights || (groups && p.split > 1)) {
     const size_t need = norm_workspace(p);
     if (workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)
       return fail(DMAD_ERR_WORKSPACE, "workspace: %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
     p.partial = (float*)workspace;
   }
+  p.past_caches = dmad::qk_past_caches((y != nullptr ? 6 : 3) * p.rows * p.C * elem_size(dt));
   hipStream_t s = (hipStream_t)stream;
   mark(0, false, s);
   const hipError_t e = dmad::launch_gated_norm_bwd(p, dt, wdt, s);

@@ -15,68 +15,39 @@
 // x' is normed as computed, not as rounded for its store; everything is in
 // float32 and rounded once. The backward pass computes x' again from x and y.
 //
-// A row of up to 2048 channels is one wave's, a wider one a workgroup's; a
-// thread holds 8 neighbouring channels of every 8 TPR, so that the whole row is
-// in registers and each operand is read once with 16-byte loads.
+// Bound by its bytes. A lane holds 8 neighbouring channels (one 16-byte access per
+// operand), so a row is ceil(C / 512) waves, which make one workgroup and exchange
+// their sums through LDS, two barriers per row; a row of one wave needs none, and
+// four of them share a workgroup. A workgroup takes a run of a group's tokens: gate,
+// scale, shift and the weights stay in its registers, and the next token's rows are
+// requested before this one's are worked on.
 #include "block_ops.h"
 #include "lanes.h"
 
 namespace dmad {
 
-constexpr int kNormThreads = 256;
+constexpr int kNormRowsPerGroup = 4;  // waves of a workgroup whose rows are one wave's
 
-// Sums over the threads of a row. W waves: each leaves its part in LDS. `slot`
-// numbers the reductions between two uses of the same memory, of which there
-// is a barrier in between as long as a row makes two.
-template <int W, int N>
-__device__ __forceinline__ void row_sums(float (&x)[N], float* slot) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = group_sum<64>(x[i]);
-  if constexpr (W > 1) {
-    const int wave = threadIdx.x >> 6;
-    if (lane_id() == 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) slot[wave * N + i] = x[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float s = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) s += slot[w * N + i];
-      x[i] = s;
-    }
-  }
-}
-
-// What a thread holds of a row: 8 channels at col0 + j STEP.
-template <int TPR_, int NCH_>
-struct NormShape {
-  static constexpr int TPR = TPR_, NCH = NCH_, W = TPR / 64, STEP = 8 * TPR, RPB = kNormThreads / TPR;
-};
-
-template <typename T, typename S>
-struct NormRow {
-  Row8<T> v[S::NCH];
+// One token's operands as loaded: up to four rows, 8 channels each.
+template <typename T, int N>
+struct NormToken {
+  Row8<T> v[N];
   template <bool NT>
-  __device__ __forceinline__ void load(const NormRows& o, int b, int s, int col0, int C, bool there) {
-    const T* p = (const T*)o.p + b * o.b + s * o.s;
+  __device__ __forceinline__ void load(const NormRows* const (&o)[N], int b, int s, int col, bool there) {
 #pragma unroll
-    for (int j = 0; j < S::NCH; ++j) {
-      v[j].zero();
-      if (there && col0 + j * S::STEP < C) v[j].template load<NT>(p + col0 + j * S::STEP);
+    for (int k = 0; k < N; ++k) {
+      v[k].zero();
+      if (there && o[k]->p != nullptr) v[k].template load<NT>((const T*)o[k]->p + b * o[k]->b + s * o[k]->s + col);
     }
   }
 };
 
 // 8 channels of a vector, widened; `none` where it is absent.
 template <typename W>
-__device__ __forceinline__ void vec8(const W* p, int col, float none, float (&x)[8]) {
-  if (p == nullptr) {
+__device__ __forceinline__ void vec8(const W* p, int col, bool there, float none, float (&x)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = none;
-    return;
-  }
+  for (int e = 0; e < 8; ++e) x[e] = none;
+  if (p == nullptr || !there) return;
   Row8<W> r;
   r.load(p + col);
 #pragma unroll
@@ -89,374 +60,359 @@ __device__ __forceinline__ const W* vec_row(const NormVec& v, int b, int f) {
 
 enum class Branch { kNone, kPlain, kNormed };
 
-// Mean and sum of squares about it of a row in one exchange: each wave's about
-// its own mean, put together by the parallel form. With a tangent t also
-// sum t and sum (x - mean) t.
-template <typename S, bool JVP>
-__device__ __forceinline__ void row_moments(const float (&x)[S::NCH][8], const float (&t)[S::NCH][8], bool layer, int col0, int C,
-                                            float* slot, float& mean, float& m2, float& st, float& xt) {
-  float own = 0.f;
-  if (layer) {
-    float sum = 0.f;
+constexpr int kNormMaxWaves = kNormMaxC / 512;
+typedef float NormSlot[kNormMaxWaves][4];  // what the waves of a row exchange at once
+
+// Sums over a row. Each wave leaves its own in `slot`, then a lane takes a wave's
+// and 16 lanes add them up. The same slot may be used again behind another barrier.
+template <bool ONE, int N>
+__device__ __forceinline__ void row_sums(float (&x)[N], NormSlot& slot, int waves) {
+  static_assert(N <= 4);
 #pragma unroll
-    for (int j = 0; j < S::NCH; ++j)
+  for (int i = 0; i < N; ++i) x[i] = group_sum<64>(x[i]);
+  if constexpr (!ONE) {
+    const int lane = lane_id(), w = lane & 15;
+    if (lane == 0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += x[j][e];  // zero beyond the row
-    sum = group_sum<64>(sum);
-    // channels of this wave
-    int n = 0;
-    const int first = col0 - 8 * lane_id();
-#pragma unroll
-    for (int j = 0; j < S::NCH; ++j) n += min(max(C - first - j * S::STEP, 0), 512);
-    own = n > 0 ? sum / (float)n : 0.f;
-    mean = own;
-    if constexpr (S::W > 1) {
-      // (sum, count are exact enough to be exchanged as they are)
-      if (lane_id() == 0) {
-        slot[16 + 2 * (threadIdx.x >> 6)] = sum;
-        slot[17 + 2 * (threadIdx.x >> 6)] = (float)n;
-      }
-    }
-  } else {
-    mean = 0.f;
-  }
-  float sums[JVP ? 3 : 1] = {};
-#pragma unroll
-  for (int j = 0; j < S::NCH; ++j) {
-    const bool in = col0 + j * S::STEP < C;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float d = in ? x[j][e] - own : 0.f;
-      sums[0] = fmaf(d, d, sums[0]);
-      if constexpr (JVP) {
-        sums[1] += t[j][e];
-        sums[2] = fmaf(d, t[j][e], sums[2]);
-      }
-    }
-  }
-  constexpr int N = JVP ? 3 : 1;
-  if constexpr (S::W == 1) {
-    row_sums<1, N>(sums, slot);
-    m2 = sums[0];
-    if constexpr (JVP) {
-      st = sums[1];
-      xt = sums[2];
-    }
-  } else {
-    const int wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int i = 0; i < N; ++i) sums[i] = group_sum<64>(sums[i]);
-    if (lane_id() == 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) slot[wave * N + i] = sums[i];
+      for (int i = 0; i < N; ++i) slot[threadIdx.x >> 6][i] = x[i];
     }
     __syncthreads();
-    if (layer) {
-      float total = 0.f;
 #pragma unroll
-      for (int w = 0; w < S::W; ++w) total += slot[16 + 2 * w];
-      mean = total / (float)C;
+    for (int i = 0; i < N; ++i) x[i] = group_sum<16>(w < waves ? slot[w < waves ? w : 0][i] : 0.f);
+  }
+}
+
+// Mean (layer) and sum of squares about it of a row in one exchange: each wave's
+// about its own mean, put together by the parallel form. With a tangent t also
+// sum t and sum (x - mean) t.
+template <bool ONE, bool JVP>
+__device__ __forceinline__ void row_moments(const float (&x)[8], const float (&t)[8], bool layer, bool there, int C, int waves,
+                                            NormSlot& slot, float& mean, float& m2, float& st, float& xt) {
+  const int lane = lane_id();
+  float sum = 0.f, own = 0.f;
+  if (layer) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += x[e];  // zero beyond the row
+    sum = group_sum<64>(sum);
+    const int n = min(C - (int)(ONE ? 0 : threadIdx.x >> 6) * 512, 512);
+    own = sum / (float)n;
+  }
+  constexpr int N = JVP ? 3 : 1;
+  float s[N] = {};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float d = there ? x[e] - own : 0.f;
+    s[0] = fmaf(d, d, s[0]);
+    if constexpr (JVP) {
+      s[1] += t[e];
+      s[2] = fmaf(d, t[e], s[2]);
     }
-    m2 = st = xt = 0.f;
+  }
 #pragma unroll
-    for (int w = 0; w < S::W; ++w) {
-      const float n = layer ? slot[17 + 2 * w] : 0.f, off = n > 0.f ? slot[16 + 2 * w] / n - mean : 0.f;
-      m2 += fmaf(n * off, off, slot[w * N]);
-      if constexpr (JVP) {
-        st += slot[w * N + 1];
-        xt += fmaf(off, slot[w * N + 1], slot[w * N + 2]);
-      }
+  for (int i = 0; i < N; ++i) s[i] = group_sum<64>(s[i]);
+  mean = own;
+  m2 = s[0];
+  if constexpr (JVP) {
+    st = s[1];
+    xt = s[2];
+  }
+  if constexpr (!ONE) {
+    const int w = lane & 15;
+    if (lane == 0) {
+      slot[threadIdx.x >> 6][0] = sum;
+#pragma unroll
+      for (int i = 0; i < N; ++i) slot[threadIdx.x >> 6][1 + i] = s[i];
+    }
+    __syncthreads();
+    const bool in = w < waves;
+    const NormSlot& r = slot;
+    const int at = in ? w : 0;
+    const float n = in ? (float)min(C - 512 * w, 512) : 0.f, ws = in ? r[at][0] : 0.f;
+    float off = 0.f;
+    if (layer) {
+      mean = group_sum<16>(ws) / (float)C;
+      off = in ? ws / n - mean : 0.f;
+    }
+    m2 = group_sum<16>(in ? fmaf(n * off, off, r[at][1]) : 0.f);
+    if constexpr (JVP) {
+      st = group_sum<16>(in ? r[at][2] : 0.f);
+      xt = group_sum<16>(in ? fmaf(off, r[at][2], r[at][3]) : 0.f);
     }
   }
 }
-constexpr int kMomentSlot = 24;  // floats of LDS that row_moments takes
 
-template <typename T, typename W, typename S, bool JVP, Branch BR, bool NT>
-__global__ __launch_bounds__(kNormThreads) void gated_norm_kernel(GatedNormParams p) {
-  __shared__ float slots[2][kMomentSlot];
-  const int64_t row = (int64_t)blockIdx.x * S::RPB + threadIdx.x / S::TPR;
-  const bool there = row < p.rows;
-  if (S::W == 1 && !there) return;  // a whole wave, and no barriers
-  const int b = (int)(row / p.S), s = (int)(row % p.S), f = s / p.T;
-  const int col0 = (threadIdx.x % S::TPR) * 8;
+// The tokens of a workgroup (ONE: of a wave in turn): [first, last) of group
+// blockIdx.x / split, every `step`-th from `i` on.
+struct NormRun {
+  int group, b, f, i, last, step;
+};
+template <bool ONE>
+__device__ __forceinline__ NormRun norm_run(const GatedNormParams& p) {
+  NormRun r;
+  const int piece = (int)blockIdx.x % p.split;
+  r.group = (int)blockIdx.x / p.split;
+  r.b = r.group / p.F;
+  r.f = r.group % p.F;
+  r.i = (int)((int64_t)p.T * piece / p.split) + (ONE ? (int)(threadIdx.x >> 6) : 0);
+  r.last = (int)((int64_t)p.T * (piece + 1) / p.split);
+  r.step = ONE ? kNormRowsPerGroup : 1;
+  return r;
+}
+
+template <typename T, typename W, bool ONE, bool JVP, Branch BR, bool NT>
+__global__ __launch_bounds__(ONE ? 64 * kNormRowsPerGroup : 64 * kNormMaxWaves) void gated_norm_kernel(GatedNormParams p) {
+  __shared__ NormSlot slots[2][2];
+  const NormRun run = norm_run<ONE>(p);
+  const int col = (ONE ? lane_id() : (int)threadIdx.x) * 8, waves = (int)blockDim.x >> 6;
+  const bool there = col < p.C;
   const float inv_c = 1.f / (float)p.C;
+  constexpr bool BRANCH = BR != Branch::kNone;
+  constexpr int N = (BRANCH ? 2 : 1) * (JVP ? 2 : 1), TX = BRANCH ? 2 : 1;
+  const NormRows* ops[N];
+  ops[0] = &p.x;
+  if constexpr (BRANCH) ops[1] = &p.y;
+  if constexpr (JVP) ops[TX] = &p.tx;
+  if constexpr (JVP && BRANCH) ops[3] = &p.ty;
 
-  float x[S::NCH][8], t[S::NCH][8];
-  NormRow<T, S> rx, ry, rtx, rty;
-  rx.template load<NT>(p.x, b, s, col0, p.C, there);
-  if constexpr (BR != Branch::kNone) ry.template load<NT>(p.y, b, s, col0, p.C, there);
-  if constexpr (JVP) rtx.template load<NT>(p.tx, b, s, col0, p.C, there);
-  if constexpr (JVP && BR != Branch::kNone) rty.template load<NT>(p.ty, b, s, col0, p.C, there);
-
-  const W* gate = vec_row<W>(p.gate, b, f);
-  const W* tgate = vec_row<W>(p.tgate, b, f);
-  float yr = 1.f, ym = 0.f;
-  if constexpr (BR == Branch::kNormed) {
-    float sums[JVP ? 2 : 1] = {};
-#pragma unroll
-    for (int j = 0; j < S::NCH; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = ry.v[j].get(e);
-        sums[0] = fmaf(y, y, sums[0]);
-        if constexpr (JVP) sums[1] = fmaf(y, rty.v[j].get(e), sums[1]);
-      }
-    row_sums<S::W>(sums, slots[0]);
-    yr = rsqrtf(sums[0] * inv_c + p.eps);
-    if constexpr (JVP) ym = sums[1] * inv_c * yr;
-  }
-#pragma unroll
-  for (int j = 0; j < S::NCH; ++j) {
-    const int col = col0 + j * S::STEP;
+  // n = u A + O and its tangent u. A + u B + Q
+  float g[8], tg[8], wp[8], A[8], O[8], tB[8], tQ[8];
+  {
+    float w[8], o[8], sc[8];
+    vec8((const W*)p.weight, col, there, 1.f, w);
+    vec8((const W*)p.bias, col, there, 0.f, o);
+    vec8(vec_row<W>(p.scale, run.b, run.f), col, there, 0.f, sc);
+    vec8(vec_row<W>(p.shift, run.b, run.f), col, there, 0.f, O);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      x[j][e] = rx.v[j].get(e);
-      t[j][e] = JVP ? rtx.v[j].get(e) : 0.f;
+      A[e] = fmaf(w[e], sc[e], w[e]);
+      O[e] += fmaf(o[e], sc[e], o[e]);
     }
-    if (col >= p.C) continue;
-    if constexpr (BR != Branch::kNone) {
-      float g[8], tg[8], wp[8];
-      vec8(gate, col, 1.f, g);
-      if constexpr (JVP) vec8(tgate, col, 0.f, tg);
-      if constexpr (BR == Branch::kNormed) vec8((const W*)p.post, col, 1.f, wp);
+    if constexpr (JVP) {
+      vec8(vec_row<W>(p.tscale, run.b, run.f), col, there, 0.f, sc);
+      vec8(vec_row<W>(p.tshift, run.b, run.f), col, there, 0.f, tQ);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float y = ry.v[j].get(e), ty = JVP ? rty.v[j].get(e) : 0.f;
+        tB[e] = w[e] * sc[e];
+        tQ[e] = fmaf(o[e], sc[e], tQ[e]);
+      }
+    }
+    if constexpr (BRANCH) {
+      vec8(vec_row<W>(p.gate, run.b, run.f), col, there, 1.f, g);
+      if constexpr (JVP) vec8(vec_row<W>(p.tgate, run.b, run.f), col, there, 0.f, tg);
+      if constexpr (BR == Branch::kNormed) vec8((const W*)p.post, col, there, 1.f, wp);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        g[e] *= p.rs;
+        if constexpr (JVP) tg[e] *= p.rs;
+      }
+    }
+  }
+
+  NormToken<T, N> next;
+  next.template load<NT>(ops, run.b, run.f * p.T + run.i, col, there && run.i < run.last);
+  int odd = 0;
+  for (int i = run.i; i < run.last; i += run.step, odd ^= 1) {
+    const NormToken<T, N> now = next;
+    next.template load<NT>(ops, run.b, run.f * p.T + i + run.step, col, there && i + run.step < run.last);
+    const int64_t at = ((int64_t)run.b * p.S + run.f * p.T + i) * p.C + col;
+    float x[8], t[8];
+    float yr = 1.f, ym = 0.f;
+    if constexpr (BR == Branch::kNormed) {
+      float sums[JVP ? 2 : 1] = {};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = now.v[1].get(e);
+        sums[0] = fmaf(y, y, sums[0]);
+        if constexpr (JVP) sums[1] = fmaf(y, now.v[3].get(e), sums[1]);
+      }
+      row_sums<ONE>(sums, slots[odd][0], waves);
+      yr = rsqrtf(sums[0] * inv_c + p.eps);
+      if constexpr (JVP) ym = sums[1] * inv_c * yr;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = now.v[0].get(e);
+      t[e] = JVP ? now.v[JVP ? TX : 0].get(e) : 0.f;
+      if constexpr (BRANCH) {
+        float y = now.v[1].get(e), ty = JVP ? now.v[JVP ? 3 : 0].get(e) : 0.f;
         if constexpr (BR == Branch::kNormed) {
           y *= yr;
           if constexpr (JVP) ty = fmaf(-y, ym, ty) * yr * wp[e];
           y *= wp[e];
         }
-        x[j][e] = fmaf(p.rs * g[e], y, x[j][e]);
-        if constexpr (JVP) t[j][e] += p.rs * fmaf(tg[e], y, g[e] * ty);
-      }
-      if (there) {
-        const int64_t at = row * p.C + col;
-        Row8<T>::template store<NT>((T*)p.xo + at, x[j]);
-        if constexpr (JVP) Row8<T>::template store<NT>((T*)p.txo + at, t[j]);
+        x[e] = fmaf(g[e], y, x[e]);
+        if constexpr (JVP) t[e] += fmaf(tg[e], y, g[e] * ty);
       }
     }
-  }
-
-  float mean, m2, st, xt;
-  row_moments<S, JVP>(x, t, p.layer, col0, p.C, slots[1], mean, m2, st, xt);
-  const float r = rsqrtf(m2 * inv_c + p.eps);
-  const float tm = p.layer ? st * inv_c : 0.f, nt = xt * inv_c * r;
-
-  const W* scale = vec_row<W>(p.scale, b, f);
-  const W* shift = vec_row<W>(p.shift, b, f);
-  const W* tscale = vec_row<W>(p.tscale, b, f);
-  const W* tshift = vec_row<W>(p.tshift, b, f);
-#pragma unroll
-  for (int j = 0; j < S::NCH; ++j) {
-    const int col = col0 + j * S::STEP;
-    if (col >= p.C || !there) continue;
-    float w[8], o[8], sc[8], sh[8], tsc[8], tsh[8], n[8], tn[8];
-    vec8((const W*)p.weight, col, 1.f, w);
-    vec8((const W*)p.bias, col, 0.f, o);
-    vec8(scale, col, 0.f, sc);
-    vec8(shift, col, 0.f, sh);
-    if constexpr (JVP) {
-      vec8(tscale, col, 0.f, tsc);
-      vec8(tshift, col, 0.f, tsh);
+    if (BRANCH && there) {
+      Row8<T>::template store<NT>((T*)p.xo + at, x);
+      if constexpr (JVP) Row8<T>::template store<NT>((T*)p.txo + at, t);
     }
+    float mean, m2, st, xt;
+    row_moments<ONE, JVP>(x, t, p.layer, there, p.C, waves, slots[odd][1], mean, m2, st, xt);
+    if (!there) continue;
+    const float r = rsqrtf(m2 * inv_c + p.eps);
+    float n[8], tn[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float u = (x[j][e] - mean) * r, v = fmaf(u, w[e], o[e]);  // normed, and with weight and bias
-      n[e] = fmaf(v, sc[e], v) + sh[e];
+      const float u = (x[e] - mean) * r;
+      n[e] = fmaf(u, A[e], O[e]);
       if constexpr (JVP) {
-        const float tv = (t[j][e] - tm - u * nt) * r * w[e];
-        tn[e] = fmaf(tv, sc[e], tv) + fmaf(v, tsc[e], tsh[e]);
+        const float tm = p.layer ? st * inv_c : 0.f, nt = xt * inv_c * r;
+        tn[e] = fmaf((t[e] - tm - u * nt) * r, A[e], fmaf(u, tB[e], tQ[e]));
       }
     }
-    const int64_t at = row * p.C + col;
     Row8<T>::template store<NT>((T*)p.no + at, n);
     if constexpr (JVP) Row8<T>::template store<NT>((T*)p.tno + at, tn);
   }
 }
 
-// Backward: a workgroup takes a run of a group's tokens, one after the other
-// (a token per wave, or all four waves on one), and keeps the group's sums P, Q,
-// R in registers.
-template <typename T, typename W, typename S, Branch BR, bool NT>
-__global__ __launch_bounds__(kNormThreads) void gated_norm_bwd_kernel(GatedNormParams p) {
-  __shared__ float slots[3][kMomentSlot];
-  __shared__ float strip[S::W == 1 ? S::RPB : 1][S::W == 1 ? 512 : 1];
-  const int group = (int)blockIdx.x / p.split, piece = (int)blockIdx.x % p.split;
-  const int b = group / p.F, f = group % p.F;
-  const int first = (int)((int64_t)p.T * piece / p.split), last = (int)((int64_t)p.T * (piece + 1) / p.split);
-  const int col0 = (threadIdx.x % S::TPR) * 8;
+// Backward: the run's sums P, Q, R stay in registers.
+template <typename T, typename W, bool ONE, Branch BR, bool NT>
+__global__ __launch_bounds__(ONE ? 64 * kNormRowsPerGroup : 64 * kNormMaxWaves) void gated_norm_bwd_kernel(GatedNormParams p) {
+  __shared__ NormSlot slots[4];
+  __shared__ float strip[ONE ? kNormRowsPerGroup : 1][ONE ? 512 : 1];
+  const NormRun run = norm_run<ONE>(p);
+  const int col = (ONE ? lane_id() : (int)threadIdx.x) * 8, waves = (int)blockDim.x >> 6;
+  const bool there = col < p.C;
   const float inv_c = 1.f / (float)p.C;
-  const W* gate = vec_row<W>(p.gate, b, f);
-  const W* scale = vec_row<W>(p.scale, b, f);
-  float P[S::NCH][8] = {}, Q[S::NCH][8] = {}, R[S::NCH][8] = {};
+  constexpr bool BRANCH = BR != Branch::kNone;
+  constexpr int N = BRANCH ? 4 : 3;
+  const NormRows* ops[N];
+  ops[0] = &p.x;
+  ops[1] = &p.tx;  // the gradient of x'
+  ops[2] = &p.ty;  // and of n
+  if constexpr (BRANCH) ops[3] = &p.y;
 
-  for (int i = first + (int)threadIdx.x / S::TPR; i < last; i += S::RPB) {
-    const int s = f * p.T + i;
-    const int64_t row = (int64_t)b * p.S + s;
-    NormRow<T, S> rx, ry, rgx, rgn;
-    rx.template load<NT>(p.x, b, s, col0, p.C, true);
-    if constexpr (BR != Branch::kNone) ry.template load<NT>(p.y, b, s, col0, p.C, true);
-    rgx.template load<NT>(p.tx, b, s, col0, p.C, p.tx.p != nullptr);
-    rgn.template load<NT>(p.ty, b, s, col0, p.C, p.ty.p != nullptr);
+  float g[8], wp[8], A[8];
+  {
+    float sc[8];
+    vec8((const W*)p.weight, col, there, 1.f, A);
+    vec8(vec_row<W>(p.scale, run.b, run.f), col, there, 0.f, sc);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) A[e] = fmaf(A[e], sc[e], A[e]);
+    if constexpr (BRANCH) {
+      vec8(vec_row<W>(p.gate, run.b, run.f), col, there, 1.f, g);
+      if constexpr (BR == Branch::kNormed) vec8((const W*)p.post, col, there, 1.f, wp);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[e] *= p.rs;
+    }
+  }
+  float P[8] = {}, Q[8] = {}, R[8] = {};
 
+  NormToken<T, N> next;
+  next.template load<NT>(ops, run.b, run.f * p.T + run.i, col, there && run.i < run.last);
+  for (int i = run.i; i < run.last; i += run.step) {
+    const NormToken<T, N> now = next;
+    next.template load<NT>(ops, run.b, run.f * p.T + i + run.step, col, there && i + run.step < run.last);
+    const int64_t at = ((int64_t)run.b * p.S + run.f * p.T + i) * p.C + col;
     float yr = 1.f;
     if constexpr (BR == Branch::kNormed) {
       float sums[1] = {0.f};
 #pragma unroll
-      for (int j = 0; j < S::NCH; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sums[0] = fmaf(ry.v[j].get(e), ry.v[j].get(e), sums[0]);
-      row_sums<S::W>(sums, slots[2]);
+      for (int e = 0; e < 8; ++e) sums[0] = fmaf(now.v[3].get(e), now.v[3].get(e), sums[0]);
+      row_sums<ONE>(sums, slots[2], waves);
       yr = rsqrtf(sums[0] * inv_c + p.eps);
     }
-    float x[S::NCH][8];
+    float x[8];
 #pragma unroll
-    for (int j = 0; j < S::NCH; ++j) {
-      const int col = col0 + j * S::STEP;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[j][e] = rx.v[j].get(e);
-      if (col >= p.C) continue;
-      if constexpr (BR != Branch::kNone) {
-        float g[8], wp[8];
-        vec8(gate, col, 1.f, g);
-        if constexpr (BR == Branch::kNormed) vec8((const W*)p.post, col, 1.f, wp);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float y = ry.v[j].get(e);
-          if constexpr (BR == Branch::kNormed) y = y * yr * wp[e];
-          x[j][e] = fmaf(p.rs * g[e], y, x[j][e]);
-        }
+    for (int e = 0; e < 8; ++e) {
+      x[e] = now.v[0].get(e);
+      if constexpr (BRANCH) {
+        float y = now.v[3].get(e);
+        if constexpr (BR == Branch::kNormed) y = y * yr * wp[e];
+        x[e] = fmaf(g[e], y, x[e]);
       }
     }
     float mean, m2, st, xt;
-    row_moments<S, false>(x, x, p.layer, col0, p.C, slots[0], mean, m2, st, xt);
+    row_moments<ONE, false>(x, x, p.layer, there, p.C, waves, slots[0], mean, m2, st, xt);
     const float r = rsqrtf(m2 * inv_c + p.eps);
-
     // a = gn A, its mean and its mean with N
-    float sums[2] = {0.f, 0.f};
-    float a[S::NCH][8];
+    float sums[2] = {0.f, 0.f}, a[8];
 #pragma unroll
-    for (int j = 0; j < S::NCH; ++j) {
-      const int col = col0 + j * S::STEP;
-      if (col >= p.C) continue;
-      float w[8], sc[8];
-      vec8((const W*)p.weight, col, 1.f, w);
-      vec8(scale, col, 0.f, sc);
+    for (int e = 0; e < 8; ++e) {
+      const float gn = now.v[2].get(e), n = there ? (x[e] - mean) * r : 0.f;
+      x[e] = n;
+      P[e] = fmaf(gn, n, P[e]);
+      Q[e] += gn;
+      a[e] = gn * A[e];
+      sums[0] += a[e];
+      sums[1] = fmaf(a[e], n, sums[1]);
+    }
+    row_sums<ONE>(sums, slots[1], waves);
+    const float am = p.layer ? sums[0] * inv_c : 0.f, an = sums[1] * inv_c;
+    float d[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d[e] = fmaf(r, a[e] - am - x[e] * an, now.v[1].get(e));
+    if (there) Row8<T>::template store<NT>((T*)p.xo + at, d);
+    if constexpr (BR == Branch::kPlain) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float g = rgn.v[j].get(e), n = (x[j][e] - mean) * r, gw = g * w[e];
-        x[j][e] = n;
-        P[j][e] = fmaf(g, n, P[j][e]);
-        Q[j][e] += g;
-        a[j][e] = fmaf(gw, sc[e], gw);
-        sums[0] += a[j][e];
-        sums[1] = fmaf(a[j][e], n, sums[1]);
+        R[e] = fmaf(d[e], now.v[3].get(e), R[e]);
+        d[e] *= g[e];
       }
-    }
-    row_sums<S::W>(sums, slots[1]);
-    const float am = p.layer ? sums[0] * inv_c : 0.f, an = sums[1] * inv_c;
-    float yu[1] = {0.f};
-#pragma unroll
-    for (int j = 0; j < S::NCH; ++j) {
-      const int col = col0 + j * S::STEP;
-      if (col >= p.C) continue;
-      const int64_t at = row * p.C + col;
-      float d[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) d[e] = fmaf(r, a[j][e] - am - x[j][e] * an, rgx.v[j].get(e));
-      Row8<T>::template store<NT>((T*)p.xo + at, d);
-      if constexpr (BR != Branch::kNone) {
-        float g[8];
-        vec8(gate, col, 1.f, g);
-        if constexpr (BR == Branch::kPlain) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            R[j][e] = fmaf(d[e], ry.v[j].get(e), R[j][e]);
-            d[e] *= p.rs * g[e];
-          }
-          if (p.txo != nullptr) Row8<T>::template store<NT>((T*)p.txo + at, d);
-        } else {
-          float wp[8];
-          vec8((const W*)p.post, col, 1.f, wp);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float y = ry.v[j].get(e) * yr;
-            R[j][e] = fmaf(d[e], y, R[j][e]);
-            a[j][e] = d[e] * p.rs * g[e] * wp[e];
-            yu[0] = fmaf(a[j][e], y, yu[0]);
-          }
-        }
-      }
+      if (there && p.txo != nullptr) Row8<T>::template store<NT>((T*)p.txo + at, d);
     }
     if constexpr (BR == Branch::kNormed) {
-      row_sums<S::W>(yu, slots[2] + 8);
+      float yu[1] = {0.f};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = now.v[3].get(e) * yr;
+        // (beyond the row y is zero, and d is not: it may not be a number there)
+        if (there) R[e] = fmaf(d[e], y, R[e]);
+        d[e] = there ? d[e] * g[e] * wp[e] : 0.f;
+        yu[0] = fmaf(d[e], y, yu[0]);
+      }
+      row_sums<ONE>(yu, slots[3], waves);
       const float m = yu[0] * inv_c;
 #pragma unroll
-      for (int j = 0; j < S::NCH; ++j) {
-        const int col = col0 + j * S::STEP;
-        if (col >= p.C || p.txo == nullptr) continue;
-        float d[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = yr * fmaf(-(ry.v[j].get(e) * yr), m, a[j][e]);
-        Row8<T>::template store<NT>((T*)p.txo + row * p.C + col, d);
-      }
+      for (int e = 0; e < 8; ++e) d[e] = yr * fmaf(-(now.v[3].get(e) * yr), m, d[e]);
+      if (there && p.txo != nullptr) Row8<T>::template store<NT>((T*)p.txo + at, d);
     }
   }
 
-  // the tokens of the waves put together, 512 channels at a time
-  if constexpr (S::W == 1) {
-    const int wave = threadIdx.x >> 6, lane = lane_id();
+  // the tokens of the waves put together
+  if constexpr (ONE) {
+    const int wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int j = 0; j < S::NCH; ++j)
+    for (int q = 0; q < (BRANCH ? 3 : 2); ++q) {
+      float(&acc)[8] = q == 0 ? P : q == 1 ? Q : R;
+      if (q > 0) __syncthreads();
 #pragma unroll
-      for (int q = 0; q < kNormSums; ++q) {
-        if (q == 2 && BR == Branch::kNone) continue;
-        float(&acc)[8] = q == 0 ? P[j] : q == 1 ? Q[j] : R[j];
-        __syncthreads();
+      for (int e = 0; e < 8; ++e) strip[wave][col + e] = acc[e];
+      __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) strip[wave][lane * 8 + e] = acc[e];
-        __syncthreads();
-        if (wave == 0) {
+      for (int e = 0; e < 8; ++e) {
+        acc[e] = strip[0][col + e];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float sum = strip[0][lane * 8 + e];
-#pragma unroll
-            for (int w = 1; w < S::RPB; ++w) sum += strip[w][lane * 8 + e];
-            acc[e] = sum;
-          }
-        }
+        for (int w = 1; w < kNormRowsPerGroup; ++w) acc[e] += strip[ONE ? w : 0][col + e];
       }
+    }
     if (wave != 0) return;
   }
+  if (!there) return;
+  if (p.partial != nullptr) {
+    float* out = p.partial + (int64_t)blockIdx.x * kNormSums * p.C + col;
+    Row8<float>::store(out, P);
+    Row8<float>::store(out + p.C, Q);
+    if constexpr (BRANCH) Row8<float>::store(out + 2 * p.C, R);
+    return;
+  }
+  const int64_t at = (int64_t)run.group * p.C + col;
+  if (p.dscale != nullptr) {
+    float w[8], o[8], d[8];
+    vec8((const W*)p.weight, col, true, 1.f, w);
+    vec8((const W*)p.bias, col, true, 0.f, o);
 #pragma unroll
-  for (int j = 0; j < S::NCH; ++j) {
-    const int col = col0 + j * S::STEP;
-    if (col >= p.C) continue;
-    if (p.partial != nullptr) {
-      float* out = p.partial + (int64_t)blockIdx.x * kNormSums * p.C + col;
-      Row8<float>::store(out, P[j]);
-      Row8<float>::store(out + p.C, Q[j]);
-      if constexpr (BR != Branch::kNone) Row8<float>::store(out + 2 * p.C, R[j]);
-      continue;
-    }
-    const int64_t at = (int64_t)group * p.C + col;
-    if (p.dscale != nullptr) {
-      float w[8], o[8], d[8];
-      vec8((const W*)p.weight, col, 1.f, w);
-      vec8((const W*)p.bias, col, 0.f, o);
+    for (int e = 0; e < 8; ++e) d[e] = fmaf(w[e], P[e], o[e] * Q[e]);
+    Row8<W>::store((W*)p.dscale + at, d);
+  }
+  if (p.dshift != nullptr) Row8<W>::store((W*)p.dshift + at, Q);
+  if (BRANCH && p.dgate != nullptr) {
+    float d[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d[e] = fmaf(w[e], P[j][e], o[e] * Q[j][e]);
-      Row8<W>::store((W*)p.dscale + at, d);
-    }
-    if (p.dshift != nullptr) Row8<W>::store((W*)p.dshift + at, Q[j]);
-    if (BR != Branch::kNone && p.dgate != nullptr) {
-      float wp[8], d[8];
-      vec8((const W*)p.post, col, 1.f, wp);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) d[e] = p.rs * wp[e] * R[j][e];
-      Row8<W>::store((W*)p.dgate + at, d);
-    }
+    for (int e = 0; e < 8; ++e) d[e] = p.rs * (BR == Branch::kNormed ? wp[e] : 1.f) * R[e];
+    Row8<W>::store((W*)p.dgate + at, d);
   }
 }
 
@@ -517,47 +473,43 @@ __global__ __launch_bounds__(1024) void gated_norm_grad_kernel(GatedNormParams p
 }
 
 #if DMAD_T == 0 && DMAD_W == 0
-// Workgroups that a backward pass aims at, and the fewest tokens that one takes.
-constexpr int kNormBwdBlocks = 768;
-int gated_norm_split(int64_t groups, int T, int C) {
-  const int least = C <= kNormWaveC ? 4 : 1;
-  int64_t split = (kNormBwdBlocks + groups - 1) / groups;
-  const int64_t most = (T + least - 1) / least;
+int norm_waves(int C) { return C <= 512 ? kNormRowsPerGroup : (C + 511) / 512; }
+// Workgroups that a pass aims at: as many as the chip holds at once for a backward
+// pass, which leaves sums behind for each; four times that for a forward pass.
+int gated_norm_split(int64_t groups, int T, int C, bool backward) {
+  const int64_t aim = backward ? kNormBwdWaves / norm_waves(C) : kNormFwdWaves / norm_waves(C);
+  int64_t split = (aim + groups - 1) / groups;
+  const int64_t least = C <= 512 ? kNormRowsPerGroup : 1, most = (T + least - 1) / least;
   if (split > most) split = most;
   return split < 1 ? 1 : (int)split;
 }
 #endif
 
-template <typename T, typename W, typename S>
+template <typename T, typename W, bool ONE, bool NT>
 static hipError_t norm_launch_s(const GatedNormParams& p, bool backward, hipStream_t s) {
   const bool branch = p.y.p != nullptr, normed = p.post != nullptr;
-  const dim3 block(kNormThreads);
+  const dim3 grid((unsigned)(p.B * p.F * p.split)), block(64 * norm_waves(p.C));
   if (backward) {
-    const dim3 grid((unsigned)(p.B * p.F * p.split));
-    if (normed) hipLaunchKernelGGL((gated_norm_bwd_kernel<T, W, S, Branch::kNormed, false>), grid, block, 0, s, p);
-    else if (branch) hipLaunchKernelGGL((gated_norm_bwd_kernel<T, W, S, Branch::kPlain, false>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((gated_norm_bwd_kernel<T, W, S, Branch::kNone, false>), grid, block, 0, s, p);
+    if (normed) hipLaunchKernelGGL((gated_norm_bwd_kernel<T, W, ONE, Branch::kNormed, NT>), grid, block, 0, s, p);
+    else if (branch) hipLaunchKernelGGL((gated_norm_bwd_kernel<T, W, ONE, Branch::kPlain, NT>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((gated_norm_bwd_kernel<T, W, ONE, Branch::kNone, NT>), grid, block, 0, s, p);
     return hipGetLastError();
   }
-  const dim3 grid((unsigned)((p.rows + S::RPB - 1) / S::RPB));
-  auto go = [&](auto jvp) {
-    constexpr bool JVP = decltype(jvp)::value != 0;
-    if (normed) hipLaunchKernelGGL((gated_norm_kernel<T, W, S, JVP, Branch::kNormed, false>), grid, block, 0, s, p);
-    else if (branch) hipLaunchKernelGGL((gated_norm_kernel<T, W, S, JVP, Branch::kPlain, false>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((gated_norm_kernel<T, W, S, JVP, Branch::kNone, false>), grid, block, 0, s, p);
+  auto go = [&](auto jvp, auto nt) {
+    constexpr bool JVP = decltype(jvp)::value != 0, PAST = decltype(nt)::value != 0;
+    if (normed) hipLaunchKernelGGL((gated_norm_kernel<T, W, ONE, JVP, Branch::kNormed, PAST>), grid, block, 0, s, p);
+    else if (branch) hipLaunchKernelGGL((gated_norm_kernel<T, W, ONE, JVP, Branch::kPlain, PAST>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((gated_norm_kernel<T, W, ONE, JVP, Branch::kNone, PAST>), grid, block, 0, s, p);
   };
-  if (p.tx.p != nullptr) go(IC<1>{});
-  else go(IC<0>{});
+  if (p.tx.p != nullptr) go(IC<1>{}, IC<NT>{});
+  else go(IC<0>{}, IC<0>{});
   return hipGetLastError();
 }
 
 template <typename T, typename W>
 static hipError_t norm_launch_t(const GatedNormParams& p, bool backward, hipStream_t s) {
-  if (p.C <= 512) return norm_launch_s<T, W, NormShape<64, 1>>(p, backward, s);
-  if (p.C <= 1536) return norm_launch_s<T, W, NormShape<64, 3>>(p, backward, s);
-  if (p.C <= kNormWaveC) return norm_launch_s<T, W, NormShape<64, 4>>(p, backward, s);
-  if (p.C <= 6144) return norm_launch_s<T, W, NormShape<256, 3>>(p, backward, s);
-  return norm_launch_s<T, W, NormShape<256, 4>>(p, backward, s);
+  if (p.past_caches) return p.C <= 512 ? norm_launch_s<T, W, true, true>(p, backward, s) : norm_launch_s<T, W, false, true>(p, backward, s);
+  return p.C <= 512 ? norm_launch_s<T, W, true, false>(p, backward, s) : norm_launch_s<T, W, false, false>(p, backward, s);
 }
 
 // One unit per operand type and type of the small operands (DMAD_T, DMAD_W).
