@@ -41,14 +41,14 @@ struct GatedNormParams {
 
 // Widest rows.
 constexpr int kNormMaxC = 8192;
-// Waves of a workgroup for rows of C channels, and waves that a forward and a
-// backward pass aim at.
+// Waves of a workgroup for rows of C channels, and waves that a pass aims at.
 int norm_waves(int C);
-constexpr int kNormFwdWaves = 16384, kNormBwdWaves = 4096;
+enum class NormPass { kForward, kTangent, kBackward };
+constexpr int kNormFwdWaves = 16384, kNormTangentWaves = 65536, kNormBwdWaves = 4096;
 
 hipError_t launch_gated_norm(const GatedNormParams& p, int dtype, int wdtype, hipStream_t s);
 // Workgroups per group of tokens.
-int gated_norm_split(int64_t groups, int T, int C, bool backward);
+int gated_norm_split(int64_t groups, int T, int C, NormPass pass);
 hipError_t launch_gated_norm_bwd(const GatedNormParams& p, int dtype, int wdtype, hipStream_t s);
 
 // ---------------------------------------------------------------- rotations by position

@@ -1486,8 +1486,8 @@ int norm_vector(const char* name, int dtype, const void* ptr, const int64_t* st,
 }
 
 // Cuts the tokens; a launch takes fewer than 2^32 threads.
-int norm_cut(dmad::GatedNormParams& p, bool backward) {
-  p.split = dmad::gated_norm_split((int64_t)p.B * p.F, p.T, p.C, backward);
+int norm_cut(dmad::GatedNormParams& p, dmad::NormPass pass) {
+  p.split = dmad::gated_norm_split((int64_t)p.B * p.F, p.T, p.C, pass);
   if ((int64_t)p.B * p.F * p.split * 64 * dmad::norm_waves(p.C) >= ((int64_t)1 << 32))
     return fail(DMAD_ERR_UNSUPPORTED, "too many groups of tokens");
   return DMAD_OK;
@@ -2149,7 +2149,7 @@ int dmad_gated_norm(const dmad_gated_norm_sizes* sizes, const void* x, const voi
   p.txo = txo;
   p.no = no;
   p.tno = tno;
-  if ((rc = norm_cut(p, false)) != DMAD_OK) return rc;
+  if ((rc = norm_cut(p, jvp ? dmad::NormPass::kTangent : dmad::NormPass::kForward)) != DMAD_OK) return rc;
   p.past_caches = dmad::qk_past_caches((y != nullptr ? 8 : 4) * p.rows * p.C * elem_size(dt));
   hipStream_t s = (hipStream_t)stream;
   mark(0, false, s);
@@ -2163,7 +2163,7 @@ int dmad_gated_norm_bwd_workspace_bytes(const dmad_gated_norm_sizes* sizes, size
   if (bytes == nullptr) return fail(DMAD_ERR_INVALID, "bytes: null pointer");
   dmad::GatedNormParams p{};
   int rc = norm_sizes(sizes, 0.f, 1.f, p);
-  if (rc != DMAD_OK || (rc = norm_cut(p, true)) != DMAD_OK) return rc;
+  if (rc != DMAD_OK || (rc = norm_cut(p, dmad::NormPass::kBackward)) != DMAD_OK) return rc;
   *bytes = p.rows == 0 ? 0 : norm_workspace(p);
   return ok();
 }
@@ -2207,7 +2207,7 @@ int dmad_gated_norm_bwd(const dmad_gated_norm_sizes* sizes, const void* x, const
   p.dweight = dweight;
   p.dbias = dbias;
   p.dpost = dpost;
-  if ((rc = norm_cut(p, true)) != DMAD_OK) return rc;
+  if ((rc = norm_cut(p, dmad::NormPass::kBackward)) != DMAD_OK) return rc;
   if (weights || (groups && p.split > 1)) {
     const size_t need = norm_workspace(p);
     if (workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)

@@ -208,12 +208,19 @@ __global__ __launch_bounds__(ONE ? 64 * kNormRowsPerGroup : 64 * kNormMaxWaves) 
     }
   }
 
-  NormToken<T, N> next;
-  next.template load<NT>(ops, run.b, run.f * p.T + run.i, col, there && run.i < run.last);
+  // (with tangents the registers for a second token cost a workgroup per CU: 541 us
+  // against 510 for 14B)
+  constexpr bool AHEAD = !JVP;
+  NormToken<T, N> now, next;
+  if constexpr (AHEAD) next.template load<NT>(ops, run.b, run.f * p.T + run.i, col, there && run.i < run.last);
   int odd = 0;
   for (int i = run.i; i < run.last; i += run.step, odd ^= 1) {
-    const NormToken<T, N> now = next;
-    next.template load<NT>(ops, run.b, run.f * p.T + i + run.step, col, there && i + run.step < run.last);
+    if constexpr (AHEAD) {
+      now = next;
+      next.template load<NT>(ops, run.b, run.f * p.T + i + run.step, col, there && i + run.step < run.last);
+    } else {
+      now.template load<NT>(ops, run.b, run.f * p.T + i, col, there);
+    }
     const int64_t at = ((int64_t)run.b * p.S + run.f * p.T + i) * p.C + col;
     float x[8], t[8];
     float yr = 1.f, ym = 0.f;
@@ -476,8 +483,9 @@ __global__ __launch_bounds__(1024) void gated_norm_grad_kernel(GatedNormParams p
 int norm_waves(int C) { return C <= 512 ? kNormRowsPerGroup : (C + 511) / 512; }
 // Workgroups that a pass aims at: as many as the chip holds at once for a backward
 // pass, which leaves sums behind for each; four times that for a forward pass.
-int gated_norm_split(int64_t groups, int T, int C, bool backward) {
-  const int64_t aim = backward ? kNormBwdWaves / norm_waves(C) : kNormFwdWaves / norm_waves(C);
+int gated_norm_split(int64_t groups, int T, int C, NormPass pass) {
+  const int64_t aim = (pass == NormPass::kBackward ? kNormBwdWaves : pass == NormPass::kTangent ? kNormTangentWaves : kNormFwdWaves) /
+                      norm_waves(C);
   int64_t split = (aim + groups - 1) / groups;
   const int64_t least = C <= 512 ? kNormRowsPerGroup : 1, most = (T + least - 1) / least;
   if (split > most) split = most;
