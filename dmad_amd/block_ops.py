@@ -18,33 +18,33 @@ import torch
 
 from . import _native as nat
 from .jvp_attention import _eager_call
-from .prologue import _check_same_device, _or_empty, readable_rows, refuse_forward_mode
+from .prologue import _check_same_device, _or_empty, refuse_forward_mode
 
 _GN = "gated_residual_norm_with_tangent"
 _NORMS = {"layer": 0, "rms": 1}
 MAX_CHANNELS = 8192
 
 
-def _stride3(t):
-    """Strides of a [B, S, C] operand whose rows are contiguous and 16-byte aligned, as ints (an axis of one element is
-    never stepped along); None where the kernels cannot read it in place."""
+def _strides3(t):
+    """Strides of a [B, S, C] operand as the kernels take them (an axis of one element is never stepped along), None where
+    its rows are not contiguous or not a multiple of 16 bytes apart."""
     (b, s, _), (sb, ss, sc) = t.shape, t.stride()
     sb, ss, step = 0 if b == 1 else sb, 0 if s == 1 else ss, 16 // t.element_size()
-    return None if sc != 1 or sb % step or ss % step or t.data_ptr() % 16 else (sb, ss, 1)
+    return None if sc != 1 or sb % step or ss % step else (sb, ss, 1)
 
 
 def _readable3(t):
     """(tensor, strides): ``t`` itself where the kernels read it in place, else a contiguous copy."""
-    st = _stride3(t)
-    if st is None:
+    st = _strides3(t)
+    if st is None or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-        st = _stride3(t)
+        st = _strides3(t)
     return t, st
 
 
 def _small_as_read(t, dtype):
     """A vector as the kernels take it: in the one type of all of them, rows readable in place."""
-    if t is None or (t.dtype == dtype and t.stride(-1) == 1 and (not t.data_ptr() % 16) and (t.dim() == 1 or _stride3(t))):
+    if t is None or (t.dtype == dtype and t.stride(-1) == 1 and not t.data_ptr() % 16 and (t.dim() == 1 or _strides3(t))):
         return t
     return torch.empty(t.shape, device=t.device, dtype=dtype).copy_(t.detach())
 
@@ -53,36 +53,57 @@ _SMALL = ("gate", "scale", "shift")
 _PER_CHANNEL = ("weight", "bias", "post_weight")
 
 
-class _NormCall:
-    """What forward and backward of one call share: sizes, and the small operands as the kernels take them."""
+class _NormPlan:
+    """What the sizes, types and strides of a call's operands settle, made once for them."""
 
-    __slots__ = ("device", "B", "S", "C", "F", "code", "wcode", "norm", "eps", "residual_scale", *_SMALL, *_PER_CHANNEL)
+    __slots__ = ("device", "B", "S", "C", "F", "code", "wcode", "dtype", "norm", "in_place", "forward_sizes", "backward_sizes",
+                 "workspace")
 
-    def __init__(self, checked, gate, scale, shift, weight, bias, post_weight, eps, norm, residual_scale):
-        x, self.F, wdtype = checked
+    def __init__(self, checked, norm, operands):
+        x, self.F, self.dtype = checked
         self.B, self.S, self.C = x.shape
-        self.device, self.code, self.wcode = x.device, nat.dtype_code(x.dtype), nat.dtype_code(wdtype)
-        self.norm, self.eps, self.residual_scale = _NORMS[norm], eps, residual_scale
-        self.gate, self.scale, self.shift = (_small_as_read(t, wdtype) for t in (gate, scale, shift))
-        self.weight, self.bias, self.post_weight = (_small_as_read(t, wdtype) for t in (weight, bias, post_weight))
-
-    def dtype(self):
-        return (torch.bfloat16, torch.float16, torch.float32)[self.wcode]
+        self.device, self.code, self.wcode = x.device, nat.dtype_code(x.dtype), nat.dtype_code(self.dtype)
+        self.norm, self.backward_sizes, self.workspace = _NORMS[norm], {}, None
+        # whether the kernels read every operand where it lies, if it starts aligned
+        strides = [None if t is None else _strides3(t) for t in operands[:10]]
+        self.in_place = all(t is None or st is not None for t, st in zip(operands, strides)) and all(
+            t is None or t.dtype == self.dtype and (i < 10 or t.stride(0) == 1) for i, t in enumerate(operands) if i >= 4)
+        self.forward_sizes = None
+        if self.in_place:
+            x, tx, y, ty, gate, tgate, scale, tscale, shift, tshift = strides
+            self.forward_sizes = self.sizes(x, y, tx, ty, gate, scale, shift, tgate, tscale, tshift)
 
     def sizes(self, *strides):
-        """``dmad_gated_norm_sizes`` of this call, made once per sizes and strides."""
-        key = (self.code, self.wcode, self.norm, self.B, self.S, self.C, self.F, *strides)
-        found = _norm_sizes.get(key)
+        """``dmad_gated_norm_sizes`` of these strides, for ctypes."""
+        none = (0, 0, 1)
+        return ctypes.byref(nat.GatedNormSizes(self.code, self.wcode, self.norm, self.B, self.S, self.C, self.F,
+                                               *((ctypes.c_int64 * 3)(*(none if s is None else s)) for s in strides)))
+
+    def sizes_back(self, *strides):
+        found = self.backward_sizes.get(strides)
         if found is None:
-            if len(_norm_sizes) > 4096:
-                _norm_sizes.clear()
-            none = (0, 0, 1)
-            found = nat.GatedNormSizes(*key[:7], *((ctypes.c_int64 * 3)(*(none if s is None else s)) for s in strides))
-            found = _norm_sizes[key] = ctypes.byref(found), found
-        return found[0]
+            if len(self.backward_sizes) > 64:
+                self.backward_sizes.clear()
+            found = self.backward_sizes[strides] = self.sizes(*strides, None, None, None)
+        return found
 
 
-_norm_sizes: dict = {}
+class _NormCall:
+    """What forward and backward of one call share: the plan, and the small operands as the kernels take them."""
+
+    __slots__ = ("plan", "in_place", "eps", "residual_scale", *_SMALL, *_PER_CHANNEL)
+
+    def __init__(self, plan, in_place, gate, scale, shift, weight, bias, post_weight, eps, residual_scale):
+        self.plan, self.in_place, self.eps, self.residual_scale = plan, in_place, eps, residual_scale
+        if not in_place:
+            gate, scale, shift, weight, bias, post_weight = (_small_as_read(t, plan.dtype) for t in
+                                                             (gate, scale, shift, weight, bias, post_weight))
+        self.gate, self.scale, self.shift = gate, scale, shift
+        self.weight, self.bias, self.post_weight = weight, bias, post_weight
+
+
+# plans by what they are made from
+_norm_plans: dict = {}
 
 
 def _norm_check(x, tx, y, ty, gate, tgate, scale, tscale, shift, tshift, weight, bias, post_weight, eps, norm, residual_scale):
@@ -140,27 +161,39 @@ def _small_type(op, name, t, dtype):
     return dtype if t.dtype == dtype else torch.float32
 
 
+def _norm_plan(tensors, eps, norm, residual_scale):
+    """The plan of an ordinary call's operands; what the operator does not take is refused."""
+    key = (norm, *(None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors))
+    plan = _norm_plans.get(key)
+    # (the two numbers are not part of the key)
+    if plan is None or not (0 <= eps < math.inf) or not math.isfinite(residual_scale):
+        checked = _norm_check(*tensors, eps, norm, residual_scale)
+        if len(_norm_plans) > 1024:
+            _norm_plans.clear()
+        plan = _norm_plans[key] = _NormPlan(checked, norm, tensors)
+    return plan
+
+
 def _norm_forward(call, x, tx, y, ty, tgate, tscale, tshift):
     """The launch: (x', tx', n, tn) and x and y as they were read."""
-    dev, none = call.device, (None, None)
-    x, sx = _readable3(x)
-    tx, stx = none if tx is None else _readable3(tx)
-    y, sy = none if y is None else _readable3(y)
-    ty, sty = none if ty is None else _readable3(ty)
-    small = []
-    for t in (tgate, tscale, tshift):
-        small.append(None if t is None else _small_as_read(t, call.dtype()))
+    plan, ptr = call.plan, nat.ptr
+    if call.in_place:
+        sizes = plan.forward_sizes
+    else:
+        none = (None, None)
+        (x, sx), (tx, stx), (y, sy), (ty, sty) = (none if t is None else _readable3(t) for t in (x, tx, y, ty))
+        tgate, tscale, tshift = (None if t is None else _small_as_read(t, plan.dtype) for t in (tgate, tscale, tshift))
+        sizes = plan.sizes(sx, sy, stx, sty, *(None if t is None else _strides3(t) for t in
+                                               (call.gate, call.scale, call.shift, tgate, tscale, tshift)))
     n = torch.empty_like(x, memory_format=torch.contiguous_format)
     tn = None if tx is None else torch.empty_like(n)
     xo = None if y is None else torch.empty_like(n)
     txo = None if ty is None else torch.empty_like(n)
-    sizes = call.sizes(sx, sy, stx, sty, *(None if t is None else _stride3(t) for t in (call.gate, call.scale, call.shift, *small)))
-    ptr = nat.ptr
-    with nat.on_device(dev):
+    with nat.on_device(plan.device):
         nat.check(nat.lib().dmad_gated_norm(
-            sizes, ptr(x), ptr(tx), ptr(y), ptr(ty), ptr(call.gate), ptr(small[0]), ptr(call.scale), ptr(small[1]),
-            ptr(call.shift), ptr(small[2]), ptr(call.weight), ptr(call.bias), ptr(call.post_weight), call.eps,
-            call.residual_scale, ptr(xo), ptr(txo), ptr(n), ptr(tn), nat.stream_ptr(dev)))
+            sizes, ptr(x), ptr(tx), ptr(y), ptr(ty), ptr(call.gate), ptr(tgate), ptr(call.scale), ptr(tscale),
+            ptr(call.shift), ptr(tshift), ptr(call.weight), ptr(call.bias), ptr(call.post_weight), call.eps,
+            call.residual_scale, ptr(xo), ptr(txo), ptr(n), ptr(tn), nat.stream_ptr(plan.device)))
     return xo, txo, n, tn, x, y
 
 
@@ -178,40 +211,37 @@ def _norm_gradients(call, x, y, gx, gn, originals, need):
     ``originals``: the small operands as the caller has them; ``need``: which of the eight are wanted."""
     g = gn if gx is None else gx
     _check_norm_saved(x, g)
-    if call.gate is not None or call.post_weight is not None or y is not None:
+    if y is not None or call.gate is not None or call.post_weight is not None:
         _check_norm_saved(y, g)
-    dev = call.device
+    plan, ptr = call.plan, nat.ptr
     x, sx = _readable3(x)
     y, sy = (None, None) if y is None else _readable3(y)
     gx, sgx = (None, None) if gx is None else _readable3(gx)
     gn, sgn = (None, None) if gn is None else _readable3(gn)
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dy = torch.empty_like(dx) if need[1] and y is not None else None
-    shape, dtype = (call.B, call.F, call.C), call.dtype()
-    small = []
-    for i, name in enumerate((*_SMALL, *_PER_CHANNEL)):
-        if getattr(call, name) is None or not need[2 + i]:
-            small.append(None)
-        else:
-            small.append(dx.new_empty(shape if i < 3 else shape[2:], dtype=dtype))
+    shape, dtype = (plan.B, plan.F, plan.C), plan.dtype
+    as_read = (call.gate, call.scale, call.shift, call.weight, call.bias, call.post_weight)
+    small = [None if t is None or not n else dx.new_empty(shape if i < 3 else shape[2:], dtype=dtype)
+             for i, (t, n) in enumerate(zip(as_read, need[2:]))]
     if x.numel() == 0:
         for t in small:
             if t is not None:
                 t.zero_()
     else:
-        sizes = call.sizes(sx, sy, sgx, sgn, *(None if t is None else _stride3(t) for t in (call.gate, call.scale)),
-                           None, None, None, None)
+        sizes = plan.sizes_back(sx, sy, sgx, sgn, *(None if t is None else _strides3(t) for t in as_read[:3]))
         ws_ptr, ws_size, ws = None, 0, None
         if any(t is not None for t in small):
-            n = ctypes.c_size_t(0)
-            nat.check(nat.lib().dmad_gated_norm_bwd_workspace_bytes(sizes, ctypes.byref(n)))
-            ws_ptr, ws_size, ws = nat.workspace(n.value, dev)
-        ptr = nat.ptr
-        with nat.on_device(dev):
+            if plan.workspace is None:
+                n = ctypes.c_size_t(0)
+                nat.check(nat.lib().dmad_gated_norm_bwd_workspace_bytes(sizes, ctypes.byref(n)))
+                plan.workspace = n.value
+            ws_ptr, ws_size, ws = nat.workspace(plan.workspace, plan.device)
+        with nat.on_device(plan.device):
             nat.check(nat.lib().dmad_gated_norm_bwd(
                 sizes, ptr(x), ptr(y), ptr(gx), ptr(gn), ptr(call.gate), ptr(call.scale), ptr(call.weight), ptr(call.bias),
                 ptr(call.post_weight), call.eps, call.residual_scale, ptr(dx), ptr(dy), *map(ptr, small), ws_ptr, ws_size,
-                nat.stream_ptr(dev)))
+                nat.stream_ptr(plan.device)))
     small = [t if t is None or t.dtype == o.dtype else t.to(o.dtype) for t, o in zip(small, originals)]
     return (dx, dy, *small)
 
@@ -259,7 +289,7 @@ def _norm_backward(ctx, gx, gn):
     if _eager_call(gx, gn):  # what was saved was read by an eager forward
         grads = _norm_gradients(call, x, y, gx, gn, small, need)
     else:
-        grads = _norm_gradients_op(x, y, gx, gn, *small, call.eps, call.norm == 1, call.residual_scale, need)
+        grads = _norm_gradients_op(x, y, gx, gn, *small, call.eps, call.plan.norm == 1, call.residual_scale, need)
     return (None, *_spread(grads))
 
 
@@ -277,9 +307,9 @@ def gated_norm_fwd(x: torch.Tensor, tx: Optional[torch.Tensor], y: Optional[torc
                    residual_scale: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(x', tx', n, tn) of ``gated_residual_norm_with_tangent``."""
     norm = "rms" if rms else "layer"
-    checked = _norm_check(x, tx, y, ty, gate, tgate, scale, tscale, shift, tshift, weight, bias, post_weight, eps, norm,
-                          residual_scale)
-    call = _NormCall(checked, gate, scale, shift, weight, bias, post_weight, eps, norm, residual_scale)
+    tensors = (x, tx, y, ty, gate, tgate, scale, tscale, shift, tshift, weight, bias, post_weight)
+    plan = _NormPlan(_norm_check(*tensors, eps, norm, residual_scale), norm, tensors)
+    call = _NormCall(plan, False, gate, scale, shift, weight, bias, post_weight, eps, residual_scale)
     return _or_empty(x, _norm_forward(call, x, tx, y, ty, tgate, tscale, tshift)[:4])
 
 
@@ -298,14 +328,14 @@ def gated_norm_bwd(x: torch.Tensor, y: Optional[torch.Tensor], gx: Optional[torc
     """Gradients of (x, y, gate, scale, shift, weight, bias, post_weight) over those of the primal outputs, of which one
     may be absent."""
     norm = "rms" if rms else "layer"
-    checked = _norm_check(x, None, y, None, gate, None, scale, None, shift, None, weight, bias, post_weight, eps, norm,
-                          residual_scale)
+    tensors = (x, None, y, None, gate, None, scale, None, shift, None, weight, bias, post_weight)
+    plan = _NormPlan(_norm_check(*tensors, eps, norm, residual_scale), norm, tensors)
     if gx is None and gn is None:
         raise ValueError(f"{_GN}: the gradient of neither output")
     for g in (gx, gn):
         if g is not None:
             _check_norm_saved(x, g)
-    call = _NormCall(checked, gate, scale, shift, weight, bias, post_weight, eps, norm, residual_scale)
+    call = _NormCall(plan, False, gate, scale, shift, weight, bias, post_weight, eps, residual_scale)
     return _or_empty(x, _norm_gradients(call, x, y, gx, gn, (gate, scale, shift, weight, bias, post_weight), need))
 
 
@@ -364,21 +394,21 @@ def gated_residual_norm_with_tangent(x_withT, y_withT=(None, None), gate_withT=(
     (x, tx), (y, ty), (gate, tgate), (scale, tscale), (shift, tshift) = x_withT, y_withT, gate_withT, scale_withT, shift_withT
     eps, residual_scale = float(eps), float(residual_scale)
     tensors = (x, tx, y, ty, gate, tgate, scale, tscale, shift, tshift, weight, bias, post_weight)
-    eager = _eager_call(*tensors)
-    if not eager:
+    if not _eager_call(*tensors):
         refuse_forward_mode(_GN, *tensors)
-    checked = _norm_check(*tensors, eps, norm, residual_scale)
-    if not eager:
+        _norm_check(*tensors, eps, norm, residual_scale)
         detached = [t if t is None or i % 2 == 0 or i > 9 else t.detach() for i, t in enumerate(tensors)]
         xo, txo, n, tn = torch.ops.dmad.gated_norm_fwd(*detached, eps, norm == "rms", residual_scale)
         txo, tn = (None if t is None else o.detach() for t, o in ((ty, txo), (tx, tn)))
     else:
-        call = _NormCall(checked, gate, scale, shift, weight, bias, post_weight, eps, norm, residual_scale)
+        plan = _norm_plan(tensors, eps, norm, residual_scale)
+        in_place = plan.in_place and not any(t is not None and t.data_ptr() & 15 for t in tensors)
+        call = _NormCall(plan, in_place, gate, scale, shift, weight, bias, post_weight, eps, residual_scale)
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in
                                            (x, y, gate, scale, shift, weight, bias, post_weight)):
             xo, txo, n, tn = _GatedNorm.apply(call, *tensors)
         else:
-            xo, txo, n, tn = _norm_forward(call, x, tx, y, ty, tgate, tscale, tshift)[:4]
+            xo, txo, n, tn, _, _ = _norm_forward(call, x, tx, y, ty, tgate, tscale, tshift)
     return ((x, tx) if y is None else (xo, txo)), (n, tn)
 
 
@@ -423,22 +453,39 @@ def rotary_frequencies(dim, theta=10000.0, scaling=None, factor=1.0, trained_len
 
 
 class _RotaryCall:
-    """What forward and backward of one call share: the positions and frequencies as the kernels take them."""
+    """What forward and backward of one call share: sizes, and the positions and frequencies as the kernels take them."""
 
-    __slots__ = ("device", "code", "B", "S", "Hq", "Hk", "D", "R", "positions", "pos64", "pos_strides", "frequencies", "layout",
-                 "factor")
+    __slots__ = ("device", "code", "B", "S", "D", "R", "positions", "pos64", "pos_strides", "frequencies", "layout", "factor")
 
     def __init__(self, sizes, positions, frequencies, layout, factor):
-        x, self.B, self.S, self.Hq, self.Hk, self.D, self.R = sizes
-        self.code, self.device, self.layout, self.factor = nat.dtype_code(x.dtype), x.device, _LAYOUTS[layout], factor
-        st = positions.stride()
-        self.positions, self.pos64 = positions, int(positions.dtype == torch.int64)
-        self.pos_strides = nat.int64_array((st[0] if len(st) == 2 and positions.shape[0] > 1 else 0, st[-1]))
+        self.device, self.code, self.B, self.S, self.D, self.R, self.pos64, self.pos_strides = sizes
+        self.positions, self.layout, self.factor = positions, _LAYOUTS[layout], factor
         self.frequencies = frequencies if frequencies.is_contiguous() else frequencies.contiguous()
 
 
+# the sizes of a _RotaryCall by shapes, types and strides of its operands
+_rotary_sizes: dict = {}
+
+
+def _rotary_plan(q, tq, k, tk, positions, frequencies, layout, factor):
+    """The sizes of an ordinary call's operands; what the operator does not take is refused."""
+    tensors = (q, tq, k, tk, positions, frequencies)
+    key = (layout, *(None if t is None else (t.shape, t.dtype, t.device) for t in tensors),
+           None if positions is None else positions.stride())
+    sizes = _rotary_sizes.get(key)
+    # (the factor and whether a gradient is wanted are not part of the key)
+    if sizes is None or not math.isfinite(factor) or frequencies.requires_grad:
+        x, B, S, D, R = _rotary_check(*tensors, layout, factor)
+        if len(_rotary_sizes) > 1024:
+            _rotary_sizes.clear()
+        st = positions.stride()
+        pos_strides = nat.int64_array((st[0] if len(st) == 2 and positions.shape[0] > 1 else 0, st[-1]))
+        sizes = _rotary_sizes[key] = (x.device, nat.dtype_code(x.dtype), B, S, D, R, int(positions.dtype == torch.int64), pos_strides)
+    return sizes
+
+
 def _rotary_check(q, tq, k, tk, positions, frequencies, layout, factor):
-    """Refuses what the operator does not take; (an operand, B, S, Hq, Hk, D, R)."""
+    """Refuses what the operator does not take; (an operand, B, S, D, R)."""
     op = _QR
     _check_same_device(op, q, tq, k, tk, positions, frequencies)
     x = q if q is not None else k
@@ -474,7 +521,7 @@ def _rotary_check(q, tq, k, tk, positions, frequencies, layout, factor):
         raise ValueError(f"{op}: layout must be one of {tuple(_LAYOUTS)}, got {layout!r}")
     if not math.isfinite(factor):
         raise ValueError(f"{op}: factor must be finite, got {factor}")
-    return x, B, S, 0 if q is None else q.shape[2], 0 if k is None else k.shape[2], D, 2 * frequencies.shape[0]
+    return x, B, S, D, 2 * frequencies.shape[0]
 
 
 _head_strides: dict = {}
@@ -557,7 +604,7 @@ def qk_rotary_fwd(q: Optional[torch.Tensor], tq: Optional[torch.Tensor], k: Opti
                   factor: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(q', tq', k', tk') of ``qk_rotary_with_tangent``."""
     layout = "half" if half else "interleaved"
-    call = _RotaryCall(_rotary_check(q, tq, k, tk, positions, frequencies, layout, factor), positions, frequencies, layout, factor)
+    call = _RotaryCall(_rotary_plan(q, tq, k, tk, positions, frequencies, layout, factor), positions, frequencies, layout, factor)
     return _or_empty(k if q is None else q, _rotary_launch(call, q, tq, k, tk, 0))
 
 
@@ -571,7 +618,7 @@ def qk_rotary_bwd(gq: Optional[torch.Tensor], gk: Optional[torch.Tensor], positi
                   half: bool, factor: float) -> Tuple[torch.Tensor, torch.Tensor]:
     """(dq, dk): the outputs' gradients, of which one may be absent, turned back."""
     layout = "half" if half else "interleaved"
-    call = _RotaryCall(_rotary_check(gq, None, gk, None, positions, frequencies, layout, factor), positions, frequencies, layout,
+    call = _RotaryCall(_rotary_plan(gq, None, gk, None, positions, frequencies, layout, factor), positions, frequencies, layout,
                        factor)
     dq, _, dk, _ = _rotary_launch(call, gq, None, gk, None, 1)
     return _or_empty(gk if gq is None else gq, (dq, dk))
@@ -624,16 +671,14 @@ def qk_rotary_with_tangent(q_withT, k_withT, positions, frequencies, layout="int
     (q, tq), (k, tk) = q_withT, k_withT
     factor = float(factor)
     tensors = (q, tq, k, tk, positions, frequencies)
-    eager = _eager_call(*tensors)
-    if not eager:
+    if not _eager_call(*tensors):
         refuse_forward_mode(_QR, *tensors)
-    sizes = _rotary_check(*tensors, layout, factor)
-    if not eager:
+        _rotary_check(*tensors, layout, factor)
         tq, tk = (None if t is None else t.detach() for t in (tq, tk))
         outs = torch.ops.dmad.qk_rotary_fwd(q, tq, k, tk, positions, frequencies, layout == "half", factor)
         q, tq, k, tk = (None if t is None else y for t, y in zip((q, tq, k, tk), outs))
         return (q, None if tq is None else tq.detach()), (k, None if tk is None else tk.detach())
-    call = _RotaryCall(sizes, positions, frequencies, layout, factor)
+    call = _RotaryCall(_rotary_plan(*tensors, layout, factor), positions, frequencies, layout, factor)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
         q, tq, k, tk = _Rotary.apply(call, q, tq, k, tk, positions, frequencies)
     else:

@@ -597,11 +597,11 @@ def _mock_kernels(monkeypatch):
         small = [getattr(call, n) for n in (*SMALL, *PER_CHANNEL)]
         values(x, tx, y, ty, tgate, tscale, tshift, *small)
         d = lambda t: None if t is None else t.detach().double()  # noqa: E731
-        kind = ("layer", "rms")[call.norm]
+        kind = ("layer", "rms")[call.plan.norm]
         xo, n = ob.gated_norm(d(x), d(y), *map(d, small), call.eps, kind, call.residual_scale)
         txo = tn = None
         if tx is not None:  # by hand: forward mode may be on around this
-            S, z = call.S, torch.zeros((), dtype=torch.float64)
+            S, z = call.plan.S, torch.zeros((), dtype=torch.float64)
             g, s, h = (z if t is None else ob.rows_of(d(t), S) for t in (tgate, tscale, tshift))
             gate = 1.0 if call.gate is None else ob.rows_of(d(call.gate), S)
             txo = d(tx)
@@ -628,7 +628,7 @@ def _mock_kernels(monkeypatch):
     def gradients(call, x, y, gx, gn, originals, need):
         """By hand: a registered op runs below autograd."""
         values(x, y, gx, gn, *originals)
-        kind, S, rs = ("layer", "rms")[call.norm], call.S, call.residual_scale
+        kind, S, rs = ("layer", "rms")[call.plan.norm], call.plan.S, call.residual_scale
         d = lambda t: None if t is None else t.detach().double()  # noqa: E731
         mean = lambda t: t.mean(-1, keepdim=True)  # noqa: E731
         one, zero = torch.ones(()).double(), torch.zeros(()).double()
@@ -642,7 +642,7 @@ def _mock_kernels(monkeypatch):
         a = gn * w * by
         a = a - N * mean(a * N)
         dx = r * (a - mean(a) if kind == "layer" else a) + (zero if gx is None else d(gx))
-        per = lambda t: t.view(call.B, call.F, -1, call.C).sum(2)  # noqa: E731
+        per = lambda t: t.view(call.plan.B, call.plan.F, -1, call.plan.C).sum(2)  # noqa: E731
         out = [dx, None, None, per(gn * (N * w + b)), per(gn), (gn * by * N).sum((0, 1)), (gn * by * one).sum((0, 1)), None]
         if y is not None:
             g, yy, ry = one if gate is None else ob.rows_of(gate, S), d(y), one
