@@ -2264,6 +2264,7 @@ int dmad_qk_rotary(int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int6
   p.interleaved = layout == DMAD_ROTARY_INTERLEAVED;
   p.factor = factor;
   p.sign = transposed ? -1 : 1;
+  p.past_caches = dmad::qk_past_caches((jvp ? 4 : 2) * p.tokens * (Hq + Hk) * D * esz);
   if (!dmad::rotary_plan(p, esz, (int)align)) return fail(DMAD_ERR_UNSUPPORTED, "too many heads and tokens");
   hipStream_t s = (hipStream_t)stream;
   mark(0, false, s);

@@ -428,8 +428,14 @@ int main() {
               const int h = quot(in, p.head_mul), unit = in - h * p.per_head, turned = pairs / V;
               if (k != i / p.per_token || h != in / p.per_head || k >= tokens || h >= heads) { printf("bad quotient\n"); return 1; }
               const bool turns = unit < turned;
-              const int first = turns ? (inter ? 2 * V * unit : V * unit) : p.R + 2 * V * (unit - turned);
-              const int second = turns ? (inter ? first + V : first + pairs) : first + V;
+              const bool pair = inter && V == 1;
+              const int first = turns ? (pair ? 2 * unit : V * unit) : p.R + 2 * V * (unit - turned);
+              const int second = turns ? (pair ? first + 1 : first + pairs) : first + V;
+              const int angle = (inter && V > 1 ? V / 2 : V) * unit;
+              if (turns && inter && V > 1 && (pairs % 2 || angle != first / 2 || angle + pairs / 2 != second / 2 || angle + pairs / 2 + V / 2 > pairs)) {
+                printf("angles of neighbours\n");
+                return 1;
+              }
               if (turns && V * unit + V > pairs) { printf("angles beyond the row\n"); return 1; }
               for (int f : {first, second}) {
                 if (f == second && second >= p.D) continue;
