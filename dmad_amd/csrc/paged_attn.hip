@@ -461,13 +461,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnParams p) {
 
 // Joins a row's pieces over a prefix that sequences share with those over its own
 // slots: `shared` has a run of n = B / P sequences' rows per prefix, and row r of
-// sequence b is row (b % n) R + r of prefix b / n.
-template <typename T, int D>
+// sequence b is row (b % n) R + r of prefix b / n. D/4 lanes hold a row, WAYS such
+// strands share its pieces, and a workgroup has 256 / (D/4 WAYS) rows of one
+// sequence; each strand requests four pieces at a time.
+template <typename T, int D, int WAYS>
 __global__ __launch_bounds__(256) void prefix_join_kernel(PagedAttnParams shared, PagedAttnParams p) {
-  constexpr int LANES = D / 4, STRANDS = 256 / LANES;
-  __shared__ float sm_o[STRANDS][D], sm_m[STRANDS], sm_l[STRANDS];
-  const int r = (int)blockIdx.x % p.R, hk = ((int)blockIdx.x / p.R) % p.kv.heads, b = (int)blockIdx.x / (p.R * p.kv.heads);
-  const int strand = threadIdx.x / LANES, d = (threadIdx.x % LANES) * 4;
+  constexpr int LANES = D / 4, ROWS = 256 / (LANES * WAYS), AHEAD = 4;
+  __shared__ float sm_o[WAYS > 1 ? WAYS : 1][ROWS][D], sm_m[WAYS][ROWS], sm_l[WAYS][ROWS];
+  const int rows = p.kv.heads * p.R, groups = (rows + ROWS - 1) / ROWS;  // of a sequence
+  const int b = (int)blockIdx.x / groups;
+  const int strand = threadIdx.x / LANES, way = strand / ROWS, slot = strand % ROWS, d = (threadIdx.x % LANES) * 4;
+  const int at_row = ((int)blockIdx.x % groups) * ROWS + slot;
+  const bool there = at_row < rows;
+  const int hk = min(at_row, rows - 1) / p.R, r = min(at_row, rows - 1) % p.R;
   const int n = p.kv.B / shared.kv.B;
   float m = -__builtin_inff(), l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
@@ -476,42 +482,61 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PagedAttnParams shared
     const int chunk = max(1, (len.total() + a.splits - 1) / a.splits);
     const PagedRun run = run_of_sequence(len, seq);
     const int first = run.base / chunk, last = min((run.base + paged_tiles(run.n) - 1) / chunk, a.splits - 1);
-    for (int i = first + (strand + turn) % STRANDS; i <= last; i += STRANDS) {
-      const int64_t at = ((int64_t)(i + seq) * a.kv.heads + hk) * a.R + row;
-      const float mi = a.part_ml[2 * at], li = a.part_ml[2 * at + 1];
-      const f32x4_t oi = *(const f32x4_t*)(a.part_o + at * D + d);
-      const float up = fmaxf(m, mi), base = up == -__builtin_inff() ? 0.f : up;
-      const float f = fast_exp2(m - base), fi = fast_exp2(mi - base);
-      l = l * f + li * fi;
-      o = o * f + oi * fi;
+    for (int i = first + (way + turn) % WAYS; i <= last; i += AHEAD * WAYS) {
+      float mi[AHEAD], li[AHEAD];
+      f32x4_t oi[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int64_t at = ((int64_t)(min(i + j * WAYS, last) + seq) * a.kv.heads + hk) * a.R + row;
+        mi[j] = a.part_ml[2 * at];
+        li[j] = a.part_ml[2 * at + 1];
+        oi[j] = *(const f32x4_t*)(a.part_o + at * D + d);
+      }
+      float up = m;
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (i + j * WAYS > last) mi[j] = -__builtin_inff(), li[j] = 0.f, oi[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        up = fmaxf(up, mi[j]);
+      }
+      const float base = up == -__builtin_inff() ? 0.f : up, f = fast_exp2(m - base);
+      l *= f;
+      o *= f;
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const float fi = fast_exp2(mi[j] - base);
+        l = l + li[j] * fi;
+        o = o + oi[j] * fi;
+      }
       m = up;
     }
   };
   gather(shared, b / n, (b % n) * p.R + r, 0);
-  gather(p, b, r, STRANDS / 2);  // from the other end of the strands, which few pieces leave idle
-  *(f32x4_t*)&sm_o[strand][d] = o;
-  if (d == 0) {
-    sm_m[strand] = m;
-    sm_l[strand] = l;
+  gather(p, b, r, WAYS / 2);  // from the other end of the strands, which few pieces leave idle
+  if constexpr (WAYS > 1) {
+    *(f32x4_t*)&sm_o[way][slot][d] = o;
+    if (d == 0) {
+      sm_m[way][slot] = m;
+      sm_l[way][slot] = l;
+    }
+    __syncthreads();
+    if (way != 0) return;
+    for (int i = 0; i < WAYS; ++i) m = fmaxf(m, sm_m[i][slot]);
+    const float base = m == -__builtin_inff() ? 0.f : m;
+    l = 0.f;
+    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < WAYS; ++i) {
+      const float f = fast_exp2(sm_m[i][slot] - base);
+      l = fmaf(f, sm_l[i][slot], l);
+      o = o + *(const f32x4_t*)&sm_o[i][slot][d] * f;
+    }
   }
-  __syncthreads();
-  if (strand != 0) return;
-  float top = -__builtin_inff();
-  for (int i = 0; i < STRANDS; ++i) top = fmaxf(top, sm_m[i]);
-  const float base = top == -__builtin_inff() ? 0.f : top;
-  float sum = 0.f;
-  o = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < STRANDS; ++i) {
-    const float f = fast_exp2(sm_m[i] - base);
-    sum = fmaf(f, sm_l[i], sum);
-    o = o + *(const f32x4_t*)&sm_o[i][d] * f;
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (!there) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   const int hq = hk * p.G + r % p.G, tok = r / p.G, Hq = p.kv.heads * p.G;
   store4<T>((T*)p.o + (((int64_t)b * p.S + tok) * Hq + hq) * D + d, o * inv);
   if (d == 0) {
-    const float l2 = base + __builtin_amdgcn_logf(sum);
-    p.lse[((int64_t)b * Hq + hq) * p.S + tok] = sum == 0.f ? -__builtin_inff() : l2 * 0.6931471805599453f;
+    const float l2 = (m == -__builtin_inff() ? 0.f : m) + __builtin_amdgcn_logf(l);
+    p.lse[((int64_t)b * Hq + hq) * p.S + tok] = l == 0.f ? -__builtin_inff() : l2 * 0.6931471805599453f;
   }
 }
 
@@ -611,12 +636,21 @@ static hipError_t paged_launch_t(const PagedAttnParams& p, int D, hipStream_t s)
   return hipErrorInvalidValue;
 }
 
+constexpr int kJoinRowsFrom = 2048, kJoinWays = 1;
+
 template <typename T, int D>
 static hipError_t prefix_launch_d(const PagedAttnParams& shared, const PagedAttnParams& p, hipStream_t s) {
   hipError_t e = prefix_rows_takes(D, shared.R) ? launch_prefix_rows(shared, __is_same(T, _Float16) ? 1 : 0, D, s)
                                                 : paged_launch<T, D, false>(shared, s);
   if (e != hipSuccess || (e = paged_launch<T, D, false>(p, s)) != hipSuccess) return e;
-  hipLaunchKernelGGL((prefix_join_kernel<T, D>), dim3((unsigned)(p.kv.B * p.kv.heads * p.R)), dim3(256), 0, s, shared, p);
+  constexpr int LANES = D / 4, ALL = 256 / LANES;
+  const int rows = p.kv.heads * p.R;
+  if (rows * p.kv.B >= kJoinRowsFrom) {
+    constexpr int WAYS = kJoinWays;
+    hipLaunchKernelGGL((prefix_join_kernel<T, D, WAYS>), dim3((unsigned)(p.kv.B * ((rows * WAYS + ALL - 1) / ALL))), dim3(256), 0, s, shared, p);
+  } else {
+    hipLaunchKernelGGL((prefix_join_kernel<T, D, ALL>), dim3((unsigned)(p.kv.B * rows)), dim3(256), 0, s, shared, p);
+  }
   return hipGetLastError();
 }
 
