@@ -1353,20 +1353,19 @@ struct PagedLayout {
   int64_t R, row_groups, splits;
   size_t part_o, part_ml, scores, lse2, total;  // offsets; equal to the next where a part is absent
 };
-int paged_layout(const dmad_kv_cache* c, int64_t S, int64_t Hq, bool accumulate, PagedLayout& w, bool prefix = false) {
+int paged_layout(const dmad_kv_cache* c, int64_t S, int64_t Hq, bool accumulate, PagedLayout& w, int64_t block_rows = 0, int64_t resident = 0) {
   if (S < 0 || Hq < 1 || Hq % c->kv_heads != 0)
     return fail(DMAD_ERR_INVALID, "query heads (%lld) must be a multiple of the cache's key heads (%lld)", (long long)Hq,
                 (long long)c->kv_heads);
   const int64_t lim = (int64_t)1 << 31;
   if (S >= lim / Hq) return fail(DMAD_ERR_UNSUPPORTED, "too many query rows");
   w.R = S * (Hq / c->kv_heads);
-  const bool many = prefix && dmad::prefix_rows_takes((int)c->head_dim, (int)w.R);
-  const int64_t rows = many ? dmad::kPrefixRows : dmad::paged_attn_rows((int)c->head_dim, (int)w.R);
+  const int64_t rows = block_rows > 0 ? block_rows : dmad::paged_attn_rows((int)c->head_dim, (int)w.R);
   w.row_groups = (w.R + rows - 1) / rows;
   const int64_t cap = c->pages_per_seq * c->page_size;
   const int64_t tiles = cap > 0 ? (cap + dmad::kPagedTile - 1) / dmad::kPagedTile : 1;
   const int64_t per = c->kv_heads * (w.row_groups > 0 ? w.row_groups : 1);
-  w.splits = paged_splits(per, many ? dmad::prefix_rows_resident((int)c->head_dim) : dmad::paged_attn_resident((int)c->head_dim));
+  w.splits = paged_splits(per, resident > 0 ? resident : dmad::paged_attn_resident((int)c->head_dim));
   if (w.splits > c->batch * tiles) w.splits = c->batch * tiles;
   const bool join = tiles > 1;
   const size_t BR = (size_t)c->batch * c->kv_heads * w.R;
@@ -1401,8 +1400,13 @@ int prefix_layout(const dmad_kv_cache* prefix, const dmad_kv_cache* c, int64_t S
                 (long long)prefix->batch);
   const int64_t n = c->batch / prefix->batch;
   if (n > 0 && S >= ((int64_t)1 << 31) / n) return fail(DMAD_ERR_UNSUPPORTED, "too many query rows");
-  int rc = paged_layout(prefix, n * S, Hq, false, w.shared, true);
-  if (rc != DMAD_OK || (rc = paged_layout(c, S, Hq, false, w.own)) != DMAD_OK) return rc;
+  const int D = (int)c->head_dim;
+  // many rows: one launch for both, in which the own slots take 16 rows per workgroup
+  const bool many = S >= 0 && Hq > 0 && dmad::prefix_rows_takes(D, n * S * (Hq / c->kv_heads));
+  int rc = paged_layout(prefix, n * S, Hq, false, w.shared, many ? dmad::kPrefixRows : 0, many ? dmad::prefix_rows_resident(D) : 0);
+  if (rc != DMAD_OK || (rc = paged_layout(c, S, Hq, false, w.own, many ? 16 : 0)) != DMAD_OK) return rc;
+  if ((w.shared.splits * w.shared.row_groups + w.own.splits * w.own.row_groups) * c->kv_heads >= (int64_t)1 << 23)
+    return fail(DMAD_ERR_UNSUPPORTED, "too many pieces for one launch");
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   const size_t rows = (size_t)(w.shared.splits + prefix->batch) * c->kv_heads * w.shared.R;
   const size_t own = (size_t)(w.own.splits + c->batch) * c->kv_heads * w.own.R;

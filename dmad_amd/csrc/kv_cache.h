@@ -73,9 +73,9 @@ hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, int D, hipStre
 // workgroup, whether a call is one of these, and its workgroups per CU.
 constexpr int kPrefixRows = 128;
 constexpr int kPrefixRowsFrom = 32;
-bool prefix_rows_takes(int D, int R);
+bool prefix_rows_takes(int D, int64_t R);
 int prefix_rows_resident(int D);
-hipError_t launch_prefix_rows(const PagedAttnParams& p, int dtype, int D, hipStream_t s);
+hipError_t launch_prefix_rows(const PagedAttnParams& shared, const PagedAttnParams& p, int dtype, int D, hipStream_t s);
 // Attention over prefixes and over each sequence's own slots behind its prefix:
 // sequence b of p follows prefix b / (p.kv.B / shared.kv.B), whose rows in
 // `shared` are those of its sequences one after the other. Both keep_parts.

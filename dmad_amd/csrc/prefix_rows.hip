@@ -22,7 +22,7 @@
 // The line of slots is cut into `splits` pieces (paged_pieces.h); each leaves
 // (maximum, sum, O) per row in float32 for prefix_join_kernel.
 #include "attn_fwd.h"
-#include "paged_pieces.h"
+#include "paged_body.h"
 
 namespace dmad {
 
@@ -47,20 +47,21 @@ struct PrefixP {
   static constexpr float DOWN = HALF ? 1.f / 32768.f : 1.f;
 };
 
+// The ring's stages.
+struct PrefixRing {
+  lds_char_t *s0, *s1, *s2, *s3;
+};
+
 template <typename T, int D>
-__global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void prefix_rows_kernel(PagedAttnParams p) {
+__device__ __forceinline__ void prefix_rows_body(const PagedAttnParams& p, int block, const PrefixRing& ring) {
   using C = PrefixCfg<D>;
   using PP = PrefixP<T>;
   constexpr int KS = C::KS, DB = C::DB, CR = C::CR, ROWB = C::ROWB, NOP = C::NOP, PF = 4;
-  __shared__ __attribute__((aligned(1024))) char stg0[C::STAGE];
-  __shared__ __attribute__((aligned(1024))) char stg1[C::STAGE];
-  __shared__ __attribute__((aligned(1024))) char stg2[C::STAGE];
-  __shared__ __attribute__((aligned(1024))) char stg3[C::STAGE];
   const KvPages& kv = p.kv;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   // the row groups of one piece and head on one XCD, as in paged_attn_kernel
-  const int work = (int)blockIdx.x / (8 * p.row_groups) * 8 + ((int)blockIdx.x & 7), rg = (int)blockIdx.x / 8 % p.row_groups;
+  const int work = block / (8 * p.row_groups) * 8 + (block & 7), rg = block / 8 % p.row_groups;
   const int hk = work % kv.heads, x = work / kv.heads;
   if (x >= p.splits) return;
 
@@ -98,10 +99,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void prefix_ro
   };
   auto stage = [&](auto kk) -> lds_char_t* {
     constexpr int k = decltype(kk)::value % 4;
-    if constexpr (k == 0) return (lds_char_t*)stg0;
-    else if constexpr (k == 1) return (lds_char_t*)stg1;
-    else if constexpr (k == 2) return (lds_char_t*)stg2;
-    else return (lds_char_t*)stg3;
+    if constexpr (k == 0) return ring.s0;
+    else if constexpr (k == 1) return ring.s1;
+    else if constexpr (k == 2) return ring.s2;
+    else return ring.s3;
   };
 
   PagedPiece piece(kv, p.splits, x, lane);
@@ -327,24 +328,57 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void prefix_ro
   }
 }
 
-template <typename T>
-static hipError_t prefix_rows_t(const PagedAttnParams& p, int D, hipStream_t s) {
-  const int work = (p.splits * p.kv.heads + 7) / 8 * 8;
-  const dim3 grid((unsigned)(work * p.row_groups)), block(256);
-  switch (D) {
-    case 64: hipLaunchKernelGGL((prefix_rows_kernel<T, 64>), grid, block, 0, s, p); break;
-    case 128: hipLaunchKernelGGL((prefix_rows_kernel<T, 128>), grid, block, 0, s, p); break;
-    case 256: hipLaunchKernelGGL((prefix_rows_kernel<T, 256>), grid, block, 0, s, p); break;
-    default: return hipErrorInvalidValue;
+// The prefix's pass and, with the launch's last blocks, that over the sequences' own
+// slots, which starts wherever the first one's workgroups end.
+template <typename T, int D, bool CAUSAL>
+__global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void prefix_rows_kernel(PagedAttnParams shared, PagedAttnParams p,
+                                                                                         int rows_blocks) {
+  using C = PrefixCfg<D>;
+  __shared__ __attribute__((aligned(1024))) char stg0[C::STAGE];
+  __shared__ __attribute__((aligned(1024))) char stg1[C::STAGE];
+  __shared__ __attribute__((aligned(1024))) char stg2[C::STAGE];
+  __shared__ __attribute__((aligned(1024))) char stg3[C::STAGE];
+  constexpr int O = 16 * PagedCfg<D>::OP;
+  static_assert((O + 32) * 4 <= C::STAGE);
+  struct Lds {  // a wave's part is one stage
+    __device__ __forceinline__ float* o(int w) const { return (float*)(w == 0 ? stg0 : w == 1 ? stg1 : w == 2 ? stg2 : stg3); }
+    __device__ __forceinline__ float* m(int w) const { return o(w) + O; }
+    __device__ __forceinline__ float* l(int w) const { return o(w) + O + 16; }
+  };
+  const int own = (int)blockIdx.x - rows_blocks;
+  if (own >= 0) {
+    paged_attn_body<T, D, 1, false, CAUSAL>(p, own, Lds{});
+  } else {
+    prefix_rows_body<T, D>(shared, (int)blockIdx.x,
+                           PrefixRing{(lds_char_t*)stg0, (lds_char_t*)stg1, (lds_char_t*)stg2, (lds_char_t*)stg3});
   }
+}
+
+template <typename T, int D>
+static hipError_t prefix_rows_d(const PagedAttnParams& shared, const PagedAttnParams& p, hipStream_t s) {
+  auto blocks = [](const PagedAttnParams& a) { return (a.splits * a.kv.heads + 7) / 8 * 8 * a.row_groups; };
+  const int rows = blocks(shared);
+  const dim3 grid((unsigned)(rows + blocks(p))), block(256);
+  if (p.causal && p.S > 1) hipLaunchKernelGGL((prefix_rows_kernel<T, D, true>), grid, block, 0, s, shared, p, rows);
+  else hipLaunchKernelGGL((prefix_rows_kernel<T, D, false>), grid, block, 0, s, shared, p, rows);
   return hipGetLastError();
 }
 
-hipError_t launch_prefix_rows(const PagedAttnParams& p, int dtype, int D, hipStream_t s) {
-  return dtype == 0 ? prefix_rows_t<__bf16>(p, D, s) : prefix_rows_t<_Float16>(p, D, s);
+template <typename T>
+static hipError_t prefix_rows_t(const PagedAttnParams& shared, const PagedAttnParams& p, int D, hipStream_t s) {
+  switch (D) {
+    case 64: return prefix_rows_d<T, 64>(shared, p, s);
+    case 128: return prefix_rows_d<T, 128>(shared, p, s);
+    case 256: return prefix_rows_d<T, 256>(shared, p, s);
+  }
+  return hipErrorInvalidValue;
 }
 
-bool prefix_rows_takes(int D, int R) { return (D == 64 || D == 128 || D == 256) && R > kPrefixRowsFrom; }
+hipError_t launch_prefix_rows(const PagedAttnParams& shared, const PagedAttnParams& p, int dtype, int D, hipStream_t s) {
+  return dtype == 0 ? prefix_rows_t<__bf16>(shared, p, D, s) : prefix_rows_t<_Float16>(shared, p, D, s);
+}
+
+bool prefix_rows_takes(int D, int64_t R) { return (D == 64 || D == 128 || D == 256) && R > kPrefixRowsFrom; }
 int prefix_rows_resident(int D) { return D == 64 ? 3 : D == 128 ? 2 : 1; }
 
 }  // namespace dmad
