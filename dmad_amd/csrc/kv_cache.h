@@ -72,7 +72,7 @@ hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, int D, hipStre
 // The same for many rows per key head (prefix_rows.hip), partials only: rows per
 // workgroup, whether a call is one of these, and its workgroups per CU.
 constexpr int kPrefixRows = 128;
-constexpr int kPrefixRowsFrom = 32;
+constexpr int kPrefixRowsFrom = 16;
 bool prefix_rows_takes(int D, int64_t R);
 int prefix_rows_resident(int D);
 hipError_t launch_prefix_rows(const PagedAttnParams& shared, const PagedAttnParams& p, int dtype, int D, hipStream_t s);

@@ -378,7 +378,16 @@ hipError_t launch_prefix_rows(const PagedAttnParams& shared, const PagedAttnPara
   return dtype == 0 ? prefix_rows_t<__bf16>(shared, p, D, s) : prefix_rows_t<_Float16>(shared, p, D, s);
 }
 
+// More than 16 rows per key head (one row tile of paged_attn_kernel) go here, whose
+// K and V pass through LDS once for 128 rows. 40 heads of 128 over 32760 slots: 135
+// against 136 us for 24 rows, 136 - 144 for 32, 140 - 167 for 48, 159 - 304 for 128; 64-wide
+// heads 80 - 81 us for 32 rows, 105 - 169 for 128; 16 heads of 256 113 - 121 for 17, 150 - 389
+// for 128. Up to 16 rows 124 to 134 there against 130 to 135 here.
 bool prefix_rows_takes(int D, int64_t R) { return (D == 64 || D == 128 || D == 256) && R > kPrefixRowsFrom; }
-int prefix_rows_resident(int D) { return D == 64 ? 3 : D == 128 ? 2 : 1; }
+// Workgroups per CU that the cut aims at; a CU holds 3, 2, 1. Fewer are fewer pieces to
+// leave and join, and leave room for the own slots: 128-wide heads 159 us with one
+// against 205 with two for 128 rows as above (88 - 98 for 96 samples behind two
+// prefixes); 64-wide ones 111, 105 and 107 us with one, two and three.
+int prefix_rows_resident(int D) { return D == 64 ? 2 : 1; }
 
 }  // namespace dmad
