@@ -250,6 +250,60 @@ def test_forward_tangent_backward(gpu, B, S, C, F, dtype, wdtype, kind, there, l
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C", [512, 5120])
+def test_calls_past_the_caches(gpu, C):
+    """Calls of more than the caches hold (256 MB): bit for bit what their chunks of tokens give, and the gradient of a
+    chunk's shift, a sum of 1500 terms in float32 in some order: n eps / 2 times the sum of their sizes, and its rounding."""
+    parts, n = 4, 1500 * (5120 // C)
+    S = parts * n
+    assert 6 * S * C * 2 > 256e6 > 8 * n * C * 2
+    g = torch.Generator(device=gpu).manual_seed(3)
+    d = {k: torch.randn(1, S, C, generator=g, device=gpu).to(torch.bfloat16) for k in ("x", "tx", "y", "ty", "gx", "gn")}
+    d.update({k: torch.randn(1, parts, C, generator=g, device=gpu) for k in ("gate", "scale", "shift")})
+
+    def run(rows, group):
+        x, y = (d[k][:, rows].detach().requires_grad_() for k in "xy")
+        small = {k: d[k][:, group].detach().requires_grad_() for k in ("gate", "scale", "shift")}
+        print(f"case past caches C={C} rows={x.shape[1]}", flush=True)
+        (xo, txo), (o, to) = _call({"x": x, "tx": d["tx"][:, rows], "y": y, "ty": d["ty"][:, rows], **small})
+        torch.autograd.backward((xo, o), (d["gx"][:, rows], d["gn"][:, rows]))
+        return (xo.detach(), txo, o.detach(), to, x.grad, y.grad), small["shift"].grad
+
+    every = slice(None)
+    whole, dshift = run(every, every)
+    assert all(torch.isfinite(t).all() for t in whole)
+    for i in range(parts):
+        rows = slice(i * n, (i + 1) * n)
+        some, part = run(rows, slice(i, i + 1))
+        for a, b in zip(whole, some):
+            assert torch.equal(a[:, rows], b)
+        ref, size = d["gn"][0, rows].double().sum(0), d["gn"][0, rows].double().abs().sum(0)
+        for got in (dshift[0, i], part[0, 0]):
+            assert ((got.double() - ref).abs() <= (n + 1) * 2.0 ** -24 * size).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [64, 1536])
+def test_one_shape_at_many_places(gpu, C):
+    """Calls of one shape, some of whose operands start off 16 bytes: what is planned for the shape holds for none else."""
+    d = {k: torch.randn(2, 6, C, device=gpu).to(torch.bfloat16) for k in ("x", "y")}
+    d["gate"] = torch.randn(2, 1, C, device=gpu)
+
+    def off(t):
+        at = torch.empty(t.numel() + 1, device=gpu, dtype=t.dtype)[1:].view(t.shape)
+        return at.copy_(t)
+
+    (want, _), (wn, _) = _call(d)
+    for moved in ((), ("x",), ("gate",), ("y", "x"), ()):
+        (xo, _), (n, _) = _call({k: off(t) if k in moved else t for k, t in d.items()})
+        assert torch.equal(xo, want) and torch.equal(n, wn)
+    with pytest.raises(ValueError, match="eps"):
+        _call(d, eps=-1.0)
+    with pytest.raises(ValueError, match="residual_scale"):
+        _call(d, rs=math.inf)
+
+
+@pytest.mark.gpu
 def test_gradient_is_the_difference_quotient(gpu):
     """fp32 gradients against central differences of the kernel's own outputs. With step h = 2^-6 the quotient of
     sum(x' gx + n gn) is off by h^2 / 6 times a third derivative of order 10 and by the outputs' float32 errors, 64 half

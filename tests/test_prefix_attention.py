@@ -94,6 +94,20 @@ CASES = [
     (1, 64, 4, 8, 2, 128, "bf16", (64, 16), [2000], [4 + 3 * i for i in range(64)], True),
     (4, 64, 1, 32, 4, 128, "fp16", (48, 16), [129, 128, 127, 1000], [(11 * i) % 90 for i in range(64)], False),
     (1, 300, 1, 2, 2, 128, "bf16", (16, 16), [97], [1] * 300, False),
+    # 16 and 17 rows per key head, behind each head dim
+    (1, 16, 1, 3, 3, 128, "fp16", (16, 16), [400], [11 * i for i in range(16)], False),
+    (1, 17, 1, 3, 3, 128, "bf16", (16, 16), [400], [11 * i for i in range(17)], False),
+    (1, 17, 1, 3, 3, 64, "fp16", (32, 16), [190], [140 - i for i in range(17)], False),
+    (1, 17, 1, 2, 2, 256, "fp16", (16, 64), [410], [1] * 17, False),
+    (1, 16, 1, 2, 2, 256, "bf16", (16, 64), [410], [150] * 16, False),
+    (1, 17, 1, 2, 2, 16, "bf16", (16, 16), [300], [3] * 17, False),
+    # own slots of more than 16 rows, in several pieces, behind a prefix of one step
+    (1, 3, 20, 4, 2, 128, "bf16", (16, 16), [400], [20, 300, 77], True),
+    (1, 2, 1, 40, 2, 64, "fp16", (16, 16), [5], [3000, 2500], False),
+    (2, 4, 3, 12, 2, 256, "bf16", (16, 16), [31, 0], [3, 500, 0, 129], False),
+    # pieces of more than 32 steps
+    (1, 17, 1, 64, 64, 128, "bf16", (64, 16), [5003], [1 + i for i in range(17)], False),
+    (1, 20, 1, 64, 64, 64, "fp16", (16, 16), [9000], [2 * i for i in range(20)], False),
 ]
 
 
@@ -220,6 +234,30 @@ def test_low_and_heavy_scores(gpu, dtype, B, Hq):
     prefix.k_pages[at][..., 0] = 24.0
     prefix.v_pages[at] = 2.0 ** -14
     _check(shared_prefix_attention(q, prefix, cache, return_lse=True), ob.prefix_attend(_fields(prefix), _fields(cache), q), t, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [4, 40])
+def test_pages_beyond_32_bits(gpu, B):
+    """Pages at the far end of pools of more than 2^31 elements: bit for bit what small pools give."""
+    from dmad_amd import PagedKVCache, shared_prefix_attention
+
+    t, Hk, D, page = torch.bfloat16, 8, 128, 16
+    prefix, cache = _caches(gpu, 1, B, Hk, D, t, (page, page), [700], [3 + 5 * i for i in range(B)], seed=2, one_pool=True)
+    q = _queries(gpu, B, 1, 16, D, t)
+    want = shared_prefix_attention(q, prefix, cache, return_lse=True)
+    n, far = prefix.k_pages.shape[0], 132000
+    assert far * Hk * page * D > 2 ** 31
+    pools = []
+    for small in (prefix.k_pages, prefix.v_pages):
+        pool = torch.empty(far + n, Hk, page, D, device=gpu, dtype=t)
+        pool[:n] = math.nan
+        pool[far:] = small
+        pools.append(pool)
+    moved = [PagedKVCache(*pools, c.page_table + far, c.lengths, c.seen) for c in (prefix, cache)]
+    got = shared_prefix_attention(q, *moved, return_lse=True)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
 
 
 @pytest.mark.gpu

@@ -174,6 +174,37 @@ def test_forward_tangent_backward(gpu, B, S, Hq, Hk, D, R, dtype, half, layout, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("half,R", [(False, 128), (True, 128), (False, 64)])
+def test_calls_past_the_caches(gpu, half, R):
+    """Calls of more than the caches hold (256 MB): bit for bit what their chunks of tokens give, forwards and backwards."""
+    n, parts, H, D = 1500, 4, 40, 128
+    S = parts * n
+    assert 4 * S * 2 * H * D * 2 > 256e6 > 4 * n * 2 * H * D * 2 and 2 * 2 * S * 2 * H * D * 2 > 256e6
+    g = torch.Generator(device=gpu).manual_seed(4)
+    x = {k: torch.randn(1, S, H, D, generator=g, device=gpu).to(torch.bfloat16) for k in ("q", "tq", "k", "tk")}
+    x["positions"] = torch.arange(S, device=gpu, dtype=torch.int32) + 7
+    x["frequencies"] = 10000.0 ** (torch.arange(R // 2, device=gpu, dtype=torch.float64) * (-2.0 / R))
+    whole = _call(x, half)
+    q = x["q"].expand(2, S, H, D).detach().requires_grad_()  # two sequences: past the caches without tangents too
+    k = x["k"].expand(2, S, H, D).detach().requires_grad_()
+    (qo, _), (ko, _) = _call(x, half, tangents=False, q=q, k=k)
+    torch.autograd.backward((qo, ko), (x["tq"].expand(2, S, H, D), x["tk"].expand(2, S, H, D)))
+    for i in range(parts):
+        rows = slice(i * n, (i + 1) * n)
+        part = {m: t[:, rows] for m, t in x.items() if t.dim() == 4}
+        part["positions"], part["frequencies"] = x["positions"][rows], x["frequencies"]
+        some = _call(part, half)
+        for a, b in zip((*whole[0], *whole[1]), (*some[0], *some[1])):
+            assert torch.equal(a[:, rows], b)
+        sq, sk = (part[m].detach().requires_grad_() for m in "qk")
+        (oq, _), (ok, _) = _call(part, half, tangents=False, q=sq, k=sk)
+        torch.autograd.backward((oq, ok), (part["tq"], part["tk"]))
+        for b in range(2):
+            for a, c in ((qo, oq), (ko, ok), (q.grad, sq.grad), (k.grad, sk.grad)):
+                assert torch.equal(a[b:b + 1, rows], c)
+
+
+@pytest.mark.gpu
 def test_far_and_negative_positions(gpu):
     """Angles of many turns are as exact as near ones; positions are any whole numbers."""
     x = _inputs(1, 6, 2, 1, 64, 64, torch.float32, 3)
