@@ -439,18 +439,36 @@ __global__ __launch_bounds__(1024) void gated_norm_grad_kernel(GatedNormParams p
   const bool branch = p.y.p != nullptr;
   float s[kNormSums] = {};
   if (col < p.C) {
-#pragma unroll 4
-    for (int64_t i = first + strand; i < last; i += kNormGradStrands) {
-      const float* x = p.partial + i * kNormSums * p.C + col;
-      float by = 1.f, g = 1.f;
-      if (all) {
+    if (all && (p.scale.p != nullptr || p.gate.p != nullptr)) {
+#pragma unroll 2
+      for (int64_t i = first + strand; i < last; i += kNormGradStrands) {
+        const float* x = p.partial + i * kNormSums * p.C + col;
         const int gr = (int)(i / p.split), b = gr / p.F, f = gr % p.F;
-        if (p.scale.p != nullptr) by += (float)vec_row<W>(p.scale, b, f)[col];
-        if (p.gate.p != nullptr) g = (float)vec_row<W>(p.gate, b, f)[col];
+        const float by = p.scale.p != nullptr ? 1.f + (float)vec_row<W>(p.scale, b, f)[col] : 1.f;
+        const float g = p.gate.p != nullptr ? (float)vec_row<W>(p.gate, b, f)[col] : 1.f;
+        s[0] = fmaf(by, x[0], s[0]);
+        s[1] = fmaf(by, x[p.C], s[1]);
+        if (branch) s[2] = fmaf(g, x[2 * (int64_t)p.C], s[2]);
       }
-      s[0] = fmaf(by, x[0], s[0]);
-      s[1] = fmaf(by, x[p.C], s[1]);
-      if (branch) s[2] = fmaf(g, x[2 * (int64_t)p.C], s[2]);
+    } else if (all) {
+      // many workgroups, few gradients: 27 us in the loop below for two weights' over 2997
+      // tokens of 1536, 9 with only their sums read and eight loads in flight
+      const bool take[kNormSums] = {p.dweight != nullptr, p.dbias != nullptr, p.dpost != nullptr};
+#pragma unroll
+      for (int q = 0; q < kNormSums; ++q) {
+        if (!take[q]) continue;
+        const float* x = p.partial + q * (int64_t)p.C + col;
+#pragma unroll 8
+        for (int64_t i = first + strand; i < last; i += kNormGradStrands) s[q] += x[i * kNormSums * p.C];
+      }
+    } else {
+#pragma unroll 4
+      for (int64_t i = first + strand; i < last; i += kNormGradStrands) {
+        const float* x = p.partial + i * kNormSums * p.C + col;
+        s[0] += x[0];
+        s[1] += x[p.C];
+        if (branch) s[2] += x[2 * (int64_t)p.C];
+      }
     }
   }
 #pragma unroll
