@@ -15,7 +15,9 @@
 // x' is normed as computed, not as rounded for its store; everything is in
 // float32 and rounded once. The backward pass computes x' again from x and y.
 //
-// Bound by its bytes. A lane holds 8 neighbouring channels (one 16-byte access per
+// Bound by its bytes: 32760 tokens of 1536 channels in bf16 take 83 us forward (403 MB, 4.9
+// TB/s) and 118 + 8 us backward (604 MB and 19 MB of sums, 5.3 TB/s), of 5120 with tangents
+// 512 us (2.7 GB, 5.2 TB/s); a 4 GiB copy reaches 4.7. A lane holds 8 neighbouring channels (one 16-byte access per
 // operand), so a row is ceil(C / 512) waves, which make one workgroup and exchange
 // their sums through LDS, two barriers per row; a row of one wave needs none, and
 // four of them share a workgroup. A workgroup takes a run of a group's tokens: gate,
@@ -499,8 +501,10 @@ __global__ __launch_bounds__(1024) void gated_norm_grad_kernel(GatedNormParams p
 
 #if DMAD_T == 0 && DMAD_W == 0
 int norm_waves(int C) { return C <= 512 ? kNormRowsPerGroup : (C + 511) / 512; }
-// Workgroups that a pass aims at: as many as the chip holds at once for a backward
-// pass, which leaves sums behind for each; four times that for a forward pass.
+// Workgroups that a pass aims at: about as many as the chip holds at once for a backward
+// pass, which leaves sums behind for each (1024, 2048, 3072, 4096 waves with the joining
+// of their sums: 174, 122, 127, 132 us for 32760 tokens of 1536 in 21 groups, 40, 34, 30,
+// 36 for 2997 tokens of weights); four to twenty times that for the others.
 int gated_norm_split(int64_t groups, int T, int C, NormPass pass) {
   const int64_t aim = (pass == NormPass::kBackward ? kNormBwdWaves : pass == NormPass::kTangent ? kNormTangentWaves : kNormFwdWaves) /
                       norm_waves(C);

@@ -19,6 +19,11 @@
 // once in fp16, where P enters as 2^15 P so that light slots keep their precision).
 // Scores of slots that are not there are -inf.
 //
+// 48 sequences of 4 tokens, 64 query heads over 8 key heads, behind 131072 slots: 0.82
+// ms for 8.3e11 flops, 1.0 PFLOP/s (a large matrix product reaches 1.23, plain attention
+// of this package 1.04 on the same heads): what is left lies between the MFMAs, the
+// softmax's VALU work (about 3 instructions per score and row) foremost.
+//
 // The line of slots is cut into `splits` pieces (paged_pieces.h); each leaves
 // (maximum, sum, O) per row in float32 for prefix_join_kernel.
 #include "attn_fwd.h"

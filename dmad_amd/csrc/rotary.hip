@@ -9,7 +9,8 @@
 // 64 bits, reduced to a part of a turn there, and only that part is rounded to
 // float32 (position 131072 in float32 would be off by 0.008 radians).
 //
-// Bound by its bytes: 4 D per row of 16 bits, in and out. A workgroup takes a tile of
+// Bound by its bytes: 4 D per row of 16 bits, in and out; 40 + 40 heads of 128 over 32760
+// tokens with tangents take 455 us (2.7 GB, 5.9 TB/s). A workgroup takes a tile of
 // tokens: its threads first compute the tile's sines and cosines into LDS, each
 // once for all heads and both operands, then walk over units of two 16-byte
 // accesses: both halves of 8 pairs, 8 pairs of neighbours, or 16 elements to
