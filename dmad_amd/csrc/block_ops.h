@@ -41,10 +41,11 @@ struct GatedNormParams {
 
 // Widest rows.
 constexpr int kNormMaxC = 8192;
-// Waves of a workgroup for rows of C channels, and waves that a pass aims at.
+// Waves of a workgroup for rows of C channels, waves that a pass aims at, and waves of a
+// CU in the backward pass.
 int norm_waves(int C);
 enum class NormPass { kForward, kTangent, kBackward };
-constexpr int kNormFwdWaves = 16384, kNormTangentWaves = 65536, kNormBwdWaves = 3072;
+constexpr int kNormFwdWaves = 16384, kNormTangentWaves = 65536, kNormBwdWaves = 16;
 
 hipError_t launch_gated_norm(const GatedNormParams& p, int dtype, int wdtype, hipStream_t s);
 // Workgroups per group of tokens.

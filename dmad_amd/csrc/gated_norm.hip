@@ -309,11 +309,18 @@ __global__ __launch_bounds__(ONE ? 64 * kNormRowsPerGroup : 64 * kNormMaxWaves) 
   }
   float P[8] = {}, Q[8] = {}, R[8] = {};
 
+  // (in float32 a second token's registers spill: 469 us against 454 for 12480 tokens of 5120)
+  constexpr bool AHEAD = sizeof(T) == 2;
   NormToken<T, N> next;
-  next.template load<NT>(ops, run.b, run.f * p.T + run.i, col, there && run.i < run.last);
+  if constexpr (AHEAD) next.template load<NT>(ops, run.b, run.f * p.T + run.i, col, there && run.i < run.last);
   for (int i = run.i; i < run.last; i += run.step) {
-    const NormToken<T, N> now = next;
-    next.template load<NT>(ops, run.b, run.f * p.T + i + run.step, col, there && i + run.step < run.last);
+    NormToken<T, N> now;
+    if constexpr (AHEAD) {
+      now = next;
+      next.template load<NT>(ops, run.b, run.f * p.T + i + run.step, col, there && i + run.step < run.last);
+    } else {
+      now.template load<NT>(ops, run.b, run.f * p.T + i, col, there);
+    }
     const int64_t at = ((int64_t)run.b * p.S + run.f * p.T + i) * p.C + col;
     float yr = 1.f;
     if constexpr (BR == Branch::kNormed) {
@@ -501,14 +508,28 @@ __global__ __launch_bounds__(1024) void gated_norm_grad_kernel(GatedNormParams p
 
 #if DMAD_T == 0 && DMAD_W == 0
 int norm_waves(int C) { return C <= 512 ? kNormRowsPerGroup : (C + 511) / 512; }
-// Workgroups that a pass aims at: about as many as the chip holds at once for a backward
-// pass, which leaves sums behind for each (1024, 2048, 3072, 4096 waves with the joining
-// of their sums: 174, 122, 127, 132 us for 32760 tokens of 1536 in 21 groups, 40, 34, 30,
-// 36 for 2997 tokens of weights); four to twenty times that for the others.
+// Workgroups per group of tokens. A forward pass has four to twenty times as many as the
+// chip holds. A backward pass leaves sums behind for each, and of rows of ten waves a CU
+// holds one (16 waves of 128 registers): it has as few as fill a round of those, or a few
+// rounds, best. 32760 tokens of 5120 with 410 workgroups 553 us, with 256 371; of 1536 in 21
+// groups 116 us with 1029, 110 with 1260.
 int gated_norm_split(int64_t groups, int T, int C, NormPass pass) {
-  const int64_t aim = (pass == NormPass::kBackward ? kNormBwdWaves : pass == NormPass::kTangent ? kNormTangentWaves : kNormFwdWaves) /
-                      norm_waves(C);
-  int64_t split = (aim + groups - 1) / groups;
+  const int waves = norm_waves(C);
+  int64_t split;
+  if (pass != NormPass::kBackward) {
+    split = ((pass == NormPass::kTangent ? kNormTangentWaves : kNormFwdWaves) / waves + groups - 1) / groups;
+  } else {
+    const int64_t slots = 256 * (waves < kNormBwdWaves ? kNormBwdWaves / waves : 1);
+    split = slots / groups;
+    if (groups > slots / 16) {
+      double fullest = 0;
+      for (int64_t n = 1; n <= 16 && fullest < 0.95; ++n) {
+        const int64_t rounds = (n * groups + slots - 1) / slots;
+        const double full = (double)(n * groups) / (double)(rounds * slots);
+        if (full > fullest) fullest = full, split = n;
+      }
+    }
+  }
   const int64_t least = C <= 512 ? kNormRowsPerGroup : 1, most = (T + least - 1) / least;
   if (split > most) split = most;
   return split < 1 ? 1 : (int)split;
