@@ -41,11 +41,11 @@ struct GatedNormParams {
 
 // Widest rows.
 constexpr int kNormMaxC = 8192;
-// Waves of a workgroup for rows of C channels, waves that a pass aims at, and waves of a
-// CU in the backward pass.
+// Waves of a workgroup for rows of C channels, waves that a pass aims at, and waves that a
+// CU holds in the forward and the backward pass.
 int norm_waves(int C);
 enum class NormPass { kForward, kTangent, kBackward };
-constexpr int kNormFwdWaves = 16384, kNormTangentWaves = 65536, kNormBwdWaves = 16;
+constexpr int kNormFwdWaves = 40960, kNormTangentWaves = 65536, kNormFwdHeld = 20, kNormBwdHeld = 16;
 
 hipError_t launch_gated_norm(const GatedNormParams& p, int dtype, int wdtype, hipStream_t s);
 // Workgroups per group of tokens.

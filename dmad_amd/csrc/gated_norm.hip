@@ -15,9 +15,10 @@
 // x' is normed as computed, not as rounded for its store; everything is in
 // float32 and rounded once. The backward pass computes x' again from x and y.
 //
-// Bound by its bytes: 32760 tokens of 1536 channels in bf16 take 83 us forward (403 MB, 4.9
-// TB/s) and 118 + 8 us backward (604 MB and 19 MB of sums, 5.3 TB/s), of 5120 with tangents
-// 512 us (2.7 GB, 5.2 TB/s); a 4 GiB copy reaches 4.7. A lane holds 8 neighbouring channels (one 16-byte access per
+// Bound by its bytes: 32760 tokens of 1536 channels in bf16 take 77 us forward (403 MB, 5.2
+// TB/s) and 108 + 8 us backward (604 MB and 23 MB of sums, 5.8 TB/s), of 5120 264, 428 + 18
+// and, forward with tangents, 508 us (5.1, 4.7 and 5.3 TB/s); a 4 GiB copy reaches 4.7. A
+// lane holds 8 neighbouring channels (one 16-byte access per
 // operand), so a row is ceil(C / 512) waves, which make one workgroup and exchange
 // their sums through LDS, two barriers per row; a row of one wave needs none, and
 // four of them share a workgroup. A workgroup takes a run of a group's tokens: gate,
@@ -508,18 +509,24 @@ __global__ __launch_bounds__(1024) void gated_norm_grad_kernel(GatedNormParams p
 
 #if DMAD_T == 0 && DMAD_W == 0
 int norm_waves(int C) { return C <= 512 ? kNormRowsPerGroup : (C + 511) / 512; }
-// Workgroups per group of tokens. A forward pass has four to twenty times as many as the
-// chip holds. A backward pass leaves sums behind for each, and of rows of ten waves a CU
+// Workgroups per group of tokens. A forward pass takes short runs, eight times what the
+// chip holds, and a call too small for runs of two tokens one round of it: 32760 tokens of
+// 5120 264 us with 4096 workgroups, 293 with 1638, 288 with 512; 6000 tokens 55, 50 and 42. A
+// backward pass leaves sums behind for each, and of rows of ten waves a CU
 // holds one (16 waves of 128 registers): it has as few as fill a round of those, or a few
 // rounds, best. 32760 tokens of 5120 with 410 workgroups 553 us, with 256 371; of 1536 in 21
 // groups 116 us with 1029, 110 with 1260.
 int gated_norm_split(int64_t groups, int T, int C, NormPass pass) {
   const int waves = norm_waves(C);
   int64_t split;
-  if (pass != NormPass::kBackward) {
-    split = ((pass == NormPass::kTangent ? kNormTangentWaves : kNormFwdWaves) / waves + groups - 1) / groups;
+  if (pass == NormPass::kTangent) {
+    split = (kNormTangentWaves / waves + groups - 1) / groups;
+  } else if (pass == NormPass::kForward) {
+    int64_t aim = kNormFwdWaves / waves;
+    if (groups * T < 2 * aim * (C <= 512 ? kNormRowsPerGroup : 1)) aim = 256 * (waves < kNormFwdHeld ? kNormFwdHeld / waves : 1);
+    split = aim / groups;
   } else {
-    const int64_t slots = 256 * (waves < kNormBwdWaves ? kNormBwdWaves / waves : 1);
+    const int64_t slots = 256 * (waves < kNormBwdHeld ? kNormBwdHeld / waves : 1);
     split = slots / groups;
     if (groups > slots / 16) {
       double fullest = 0;
