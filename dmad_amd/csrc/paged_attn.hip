@@ -299,7 +299,7 @@ static hipError_t paged_launch_t(const PagedAttnParams& p, int D, hipStream_t s)
 }
 
 // Rows of all sequences from which one strand joins a row's pieces: enough to fill the
-// chip. 14 us against 31 for 12288 rows of six pieces, 8 against 13 for 3072 of seventeen;
+// chip. 14 us against 31 for 12288 rows of six pieces, 8 against 13 for 96 sequences of 32 with seventeen each;
 // fewer rows need the strands where their pieces are many.
 constexpr int kJoinRowsFrom = 2048;
 
