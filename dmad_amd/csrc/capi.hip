@@ -1392,7 +1392,7 @@ struct PrefixLayout {
   PagedLayout shared, own;
   size_t shared_o, shared_ml, own_o, own_ml, total;
 };
-int prefix_layout(const dmad_kv_cache* prefix, const dmad_kv_cache* c, int64_t S, int64_t Hq, PrefixLayout& w) {
+int prefix_layout(const dmad_kv_cache* prefix, const dmad_kv_cache* c, int64_t S, int64_t Hq, bool causal, PrefixLayout& w) {
   if (prefix->kv_heads != c->kv_heads || prefix->head_dim != c->head_dim)
     return fail(DMAD_ERR_INVALID, "the prefixes' heads and head dim must be the cache's");
   if (prefix->batch < 1 || c->batch % prefix->batch != 0)
@@ -1401,10 +1401,13 @@ int prefix_layout(const dmad_kv_cache* prefix, const dmad_kv_cache* c, int64_t S
   const int64_t n = c->batch / prefix->batch;
   if (n > 0 && S >= ((int64_t)1 << 31) / n) return fail(DMAD_ERR_UNSUPPORTED, "too many query rows");
   const int D = (int)c->head_dim;
-  // many rows: one launch for both, in which the own slots take 16 rows per workgroup
+  // many rows: one launch for both, in which the own slots take 16 rows per workgroup, or as many
   const bool many = S >= 0 && Hq > 0 && dmad::prefix_rows_takes(D, n * S * (Hq / c->kv_heads));
   int rc = paged_layout(prefix, n * S, Hq, false, w.shared, many ? dmad::kPrefixRows : 0, many ? dmad::prefix_rows_resident(D) : 0);
-  if (rc != DMAD_OK || (rc = paged_layout(c, S, Hq, false, w.own, many ? 16 : 0)) != DMAD_OK) return rc;
+  const bool own_rows = many && dmad::prefix_own_rows(S * (Hq / c->kv_heads), causal, S);
+  if (rc != DMAD_OK || (rc = paged_layout(c, S, Hq, false, w.own, own_rows ? dmad::kPrefixRows : many ? 16 : 0,
+                                          own_rows ? dmad::prefix_rows_resident(D) : 0)) != DMAD_OK)
+    return rc;
   if ((w.shared.splits * w.shared.row_groups + w.own.splits * w.own.row_groups) * c->kv_heads >= (int64_t)1 << 23)
     return fail(DMAD_ERR_UNSUPPORTED, "too many pieces for one launch");
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
@@ -2017,9 +2020,11 @@ int dmad_prefix_attn_workspace_bytes(const dmad_kv_cache* prefix, const dmad_kv_
   dmad::KvPages kv;
   int rc = check_cache(DMAD_BF16, prefix, kv);
   if (rc != DMAD_OK || (rc = check_cache(DMAD_BF16, cache, kv)) != DMAD_OK) return rc;
-  PrefixLayout w;
-  if ((rc = prefix_layout(prefix, cache, S, Hq, w)) != DMAD_OK) return rc;
-  *bytes = w.total;
+  PrefixLayout w, causal;  // for either
+  if ((rc = prefix_layout(prefix, cache, S, Hq, false, w)) != DMAD_OK ||
+      (rc = prefix_layout(prefix, cache, S, Hq, true, causal)) != DMAD_OK)
+    return rc;
+  *bytes = std::max(w.total, causal.total);
   return ok();
 }
 
@@ -2033,7 +2038,7 @@ int dmad_prefix_attn(int dtype, const dmad_kv_cache* prefix, const dmad_kv_cache
   if (!(sm_scale > 0.f && scale_log2 <= std::numeric_limits<float>::max()))
     return fail(DMAD_ERR_UNSUPPORTED, "sm_scale must be positive, and finite times log2(e)");
   PrefixLayout w;
-  if ((rc = prefix_layout(prefix, cache, S, Hq, w)) != DMAD_OK) return rc;
+  if ((rc = prefix_layout(prefix, cache, S, Hq, causal != 0, w)) != DMAD_OK) return rc;
   if (cache->batch == 0 || S == 0) return ok();
   if ((rc = check_rows("q", q, q_strides, 2)) != DMAD_OK) return rc;
   // the tokens of a prefix's sequences follow one another at one stride

@@ -74,6 +74,9 @@ hipError_t launch_paged_attn(const PagedAttnParams& p, int dtype, int D, hipStre
 constexpr int kPrefixRows = 128;
 constexpr int kPrefixRowsFrom = 16;
 bool prefix_rows_takes(int D, int64_t R);
+// Whether such a call's own slots, of R rows per key head, are one too.
+constexpr int kPrefixOwnRowsFrom = 32;
+bool prefix_own_rows(int64_t R, bool causal, int64_t S);
 int prefix_rows_resident(int D);
 hipError_t launch_prefix_rows(const PagedAttnParams& shared, const PagedAttnParams& p, int dtype, int D, hipStream_t s);
 // Attention over prefixes and over each sequence's own slots behind its prefix:

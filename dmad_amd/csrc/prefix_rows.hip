@@ -334,8 +334,11 @@ __device__ __forceinline__ void prefix_rows_body(const PagedAttnParams& p, int b
 }
 
 // The prefix's pass and, with the launch's last blocks, that over the sequences' own
-// slots, which starts wherever the first one's workgroups end.
-template <typename T, int D, bool CAUSAL>
+// slots, which starts wherever the first one's workgroups end: 16 rows at a time, or many
+// rows like the prefix's where every row sees every slot.
+enum class OwnPass { kAll, kCausal, kRows };
+
+template <typename T, int D, OwnPass OWN>
 __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void prefix_rows_kernel(PagedAttnParams shared, PagedAttnParams p,
                                                                                          int rows_blocks) {
   using C = PrefixCfg<D>;
@@ -350,12 +353,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void prefix_ro
     __device__ __forceinline__ float* m(int w) const { return o(w) + O; }
     __device__ __forceinline__ float* l(int w) const { return o(w) + O + 16; }
   };
+  const PrefixRing ring{(lds_char_t*)stg0, (lds_char_t*)stg1, (lds_char_t*)stg2, (lds_char_t*)stg3};
   const int own = (int)blockIdx.x - rows_blocks;
   if (own >= 0) {
-    paged_attn_body<T, D, 1, false, CAUSAL>(p, own, Lds{});
+    if constexpr (OWN != OwnPass::kRows) paged_attn_body<T, D, 1, false, OWN == OwnPass::kCausal>(p, own, Lds{});
+    else prefix_rows_body<T, D>(p, own, ring);
   } else {
-    prefix_rows_body<T, D>(shared, (int)blockIdx.x,
-                           PrefixRing{(lds_char_t*)stg0, (lds_char_t*)stg1, (lds_char_t*)stg2, (lds_char_t*)stg3});
+    prefix_rows_body<T, D>(shared, (int)blockIdx.x, ring);
   }
 }
 
@@ -364,8 +368,9 @@ static hipError_t prefix_rows_d(const PagedAttnParams& shared, const PagedAttnPa
   auto blocks = [](const PagedAttnParams& a) { return (a.splits * a.kv.heads + 7) / 8 * 8 * a.row_groups; };
   const int rows = blocks(shared);
   const dim3 grid((unsigned)(rows + blocks(p))), block(256);
-  if (p.causal && p.S > 1) hipLaunchKernelGGL((prefix_rows_kernel<T, D, true>), grid, block, 0, s, shared, p, rows);
-  else hipLaunchKernelGGL((prefix_rows_kernel<T, D, false>), grid, block, 0, s, shared, p, rows);
+  if (prefix_own_rows(p.R, p.causal, p.S)) hipLaunchKernelGGL((prefix_rows_kernel<T, D, OwnPass::kRows>), grid, block, 0, s, shared, p, rows);
+  else if (p.causal && p.S > 1) hipLaunchKernelGGL((prefix_rows_kernel<T, D, OwnPass::kCausal>), grid, block, 0, s, shared, p, rows);
+  else hipLaunchKernelGGL((prefix_rows_kernel<T, D, OwnPass::kAll>), grid, block, 0, s, shared, p, rows);
   return hipGetLastError();
 }
 
@@ -389,6 +394,11 @@ hipError_t launch_prefix_rows(const PagedAttnParams& shared, const PagedAttnPara
 // heads 80 - 81 us for 32 rows, 105 - 169 for 128; 16 heads of 256 113 - 121 for 17, 150 - 389
 // for 128. Up to 16 rows 124 to 134 there against 130 to 135 here.
 bool prefix_rows_takes(int D, int64_t R) { return (D == 64 || D == 128 || D == 256) && R > kPrefixRowsFrom; }
+// Own slots of more than 32 rows whose tokens all see the same: 4 continuations by a frame
+// of 1560 tokens (12 heads, 1560 to 3120 own slots, behind 4000) 322 us against 737 with 16
+// rows per workgroup, 40 rows of 8 x 40 heads (1000 to 2000) 95 - 117, 48 of 4 x 16 64-wide
+// ones 32 - 29. Causal blocks stay with 16.
+bool prefix_own_rows(int64_t R, bool causal, int64_t S) { return !(causal && S > 1) && R > kPrefixOwnRowsFrom; }
 // Workgroups per CU that the cut aims at; a CU holds 3, 2, 1. Fewer are fewer pieces to
 // leave and join, and leave room for the own slots: 128-wide heads 159 us with one
 // against 205 with two for 128 rows as above (88 - 98 for 96 samples behind two

@@ -105,6 +105,12 @@ CASES = [
     (1, 3, 20, 4, 2, 128, "bf16", (16, 16), [400], [20, 300, 77], True),
     (1, 2, 1, 40, 2, 64, "fp16", (16, 16), [5], [3000, 2500], False),
     (2, 4, 3, 12, 2, 256, "bf16", (16, 16), [31, 0], [3, 500, 0, 129], False),
+    # own slots of more than 32 rows, seen by all of them and causal
+    (1, 2, 40, 4, 2, 128, "bf16", (16, 16), [400], [700, 40], False),
+    (1, 2, 40, 4, 2, 128, "bf16", (16, 16), [400], [700, 40], True),
+    (2, 4, 33, 1, 1, 64, "fp16", (32, 16), [100, 17], [33, 150, 64, 1000], False),
+    (1, 3, 1, 136, 2, 256, "bf16", (16, 64), [90], [0, 1, 200], False),
+    (1, 5, 150, 2, 2, 128, "fp16", (64, 16), [0], [150, 151, 1200, 160, 300], False),
     # pieces of more than 32 steps
     (1, 17, 1, 64, 64, 128, "bf16", (64, 16), [5003], [1 + i for i in range(17)], False),
     (1, 20, 1, 64, 64, 64, "fp16", (16, 16), [9000], [2 * i for i in range(20)], False),
