@@ -1,6 +1,7 @@
 // C ABI entry points (include/dmad_attn.h): argument validation, workspace
 // carving and kernel dispatch. Nothing here allocates device memory; the
 // allocation-free backward uses this file's static device array `scratch`.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
