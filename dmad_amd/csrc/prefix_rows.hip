@@ -15,7 +15,7 @@
 //     in use, and everything beyond (a missing page: everything) reads as zeros.
 //   * V^T is read from the row-major tile by transposing LDS reads.
 //   * The softmax of one step runs between the MFMAs of the next one's scores.
-// The maximum follows lazily (it moves once a score exceeds it by 2^8 in bf16; at
+// A row's maximum follows lazily (it moves once a score exceeds it by 2^8 in bf16; at
 // once in fp16, where P enters as 2^15 P so that light slots keep their precision).
 // Scores of slots that are not there are -inf.
 //
@@ -179,8 +179,10 @@ __device__ __forceinline__ void prefix_rows_body(const PagedAttnParams& p, int b
         sm.ls = 0.f;
       } else if (u == 1) {
         sm.mx = fmaxf(sm.mx, other_half(sm.mx)) * p.scale_log2;
-        sm.moved = __builtin_amdgcn_ballot_w64(sm.mx > m_i + PP::SLACK) != 0;
-        const float m_new = sm.moved ? fmaxf(m_i, sm.mx) : m_i;
+        // row by row: whether its neighbours in the wave move changes nothing for one that stays
+        const bool move = sm.mx > m_i + PP::SLACK;
+        sm.moved = __builtin_amdgcn_ballot_w64(move) != 0;
+        const float m_new = move ? sm.mx : m_i;
         sm.alpha = fast_exp2(m_i - m_new);
         m_i = m_new;
         sm.neg_m = PP::UP - m_new;

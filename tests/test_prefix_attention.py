@@ -219,6 +219,32 @@ def test_what_is_not_seen_does_not_reach(gpu, B, S, Hq):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_sequence_does_not_depend_on_its_neighbours(gpu, dtype, D):
+    """Scores that grow along the prefix, so that every row's running maximum moves many times, each row's at slots of its
+    own: with other queries beside it a sequence's output stays bit for bit what it is."""
+    from dmad_amd import shared_prefix_attention
+
+    t, B, n = DTYPES[dtype], 40, 2000
+    prefix, cache = _caches(gpu, 1, B, 2, D, t, (16, 16), [n], [1 + i % 5 for i in range(B)], seed=17)
+    slots = torch.arange(prefix.capacity, device=gpu).view(-1, 1, 16).expand(-1, 2, -1)
+    prefix.k_pages[prefix.page_table[0].long(), ..., 0] = (slots * (320.0 / n)).to(t)
+    q = _queries(gpu, B, 1, 4, D, t)
+    # scores that grow by up to 200 over the prefix, by 0.3 to 13 over a tile of 128 slots; a maximum may lag by 5.5
+    q[..., 0] = torch.arange(1, B + 1, device=gpu).view(B, 1, 1).to(t) * 0.25
+    want = shared_prefix_attention(q, prefix, cache, sm_scale=1 / 16, return_lse=True)
+    _check(want, ob.prefix_attend(_fields(prefix), _fields(cache), q, scale=1 / 16), t, D)
+    other = q.clone()
+    other[1::2, ..., 0] *= 1.7
+    other[3::4, ..., 1:] = 0.0
+    got = shared_prefix_attention(other, prefix, cache, sm_scale=1 / 16, return_lse=True)
+    for a, b in zip(got, want):
+        assert torch.equal(a[::2], b[::2])
+        assert not torch.equal(a[1::2], b[1::2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("B,Hq", [(2, 2), (64, 8)])
 def test_low_and_heavy_scores(gpu, dtype, B, Hq):
     """All scores very low; and one slot far above all others, which are many: the light ones keep their share."""
