@@ -142,6 +142,7 @@ SIGNATURES = {
     "dmad_kv_evict": (_INT, [_INT, _KV, _I64, _I64, _I64, _P, _SZ, _P]),
     "dmad_gated_norm": (_INT, [_GN, *[_P] * 13, _F, _F, *[_P] * 5]),
     "dmad_gated_norm_bwd_workspace_bytes": (_INT, [_GN, _SZP]),
+    "dmad_gated_norm_bwd_workspace_bytes_for": (_INT, [_GN, _INT, _SZP]),
     "dmad_gated_norm_bwd": (_INT, [_GN, *[_P] * 9, _F, _F, *[_P] * 9, _SZ, _P]),
     "dmad_qk_rotary": (_INT, [_INT, *[_I64] * 6, *[_P] * 4, *[_I64P] * 4, _P, _INT, _I64P, _P, _INT, _INT, _F, *[_P] * 5]),
     "dmad_attn_bwd_workspace_bytes": (_INT, [_INT, _I64, _I64, _I64, _I64, _I64, _SZP]),

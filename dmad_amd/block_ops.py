@@ -63,7 +63,7 @@ class _NormPlan:
         x, self.F, self.dtype = checked
         self.B, self.S, self.C = x.shape
         self.device, self.code, self.wcode = x.device, nat.dtype_code(x.dtype), nat.dtype_code(self.dtype)
-        self.norm, self.backward_sizes, self.workspace = _NORMS[norm], {}, None
+        self.norm, self.backward_sizes, self.workspace = _NORMS[norm], {}, {}
         # whether the kernels read every operand where it lies, if it starts aligned
         strides = [None if t is None else _strides3(t) for t in operands[:10]]
         self.in_place = all(t is None or st is not None for t, st in zip(operands, strides)) and all(
@@ -232,11 +232,13 @@ def _norm_gradients(call, x, y, gx, gn, originals, need):
         sizes = plan.sizes_back(sx, sy, sgx, sgn, *(None if t is None else _strides3(t) for t in as_read[:3]))
         ws_ptr, ws_size, ws = None, 0, None
         if any(t is not None for t in small):
-            if plan.workspace is None:
+            per_channel = any(t is not None for t in small[3:])
+            size = plan.workspace.get(per_channel)
+            if size is None:
                 n = ctypes.c_size_t(0)
-                nat.check(nat.lib().dmad_gated_norm_bwd_workspace_bytes(sizes, ctypes.byref(n)))
-                plan.workspace = n.value
-            ws_ptr, ws_size, ws = nat.workspace(plan.workspace, plan.device)
+                nat.check(nat.lib().dmad_gated_norm_bwd_workspace_bytes_for(sizes, per_channel, ctypes.byref(n)))
+                size = plan.workspace[per_channel] = n.value
+            ws_ptr, ws_size, ws = nat.workspace(size, plan.device)
         with nat.on_device(plan.device):
             nat.check(nat.lib().dmad_gated_norm_bwd(
                 sizes, ptr(x), ptr(y), ptr(gx), ptr(gn), ptr(call.gate), ptr(call.scale), ptr(call.weight), ptr(call.bias),
@@ -389,7 +391,9 @@ def gated_residual_norm_with_tangent(x_withT, y_withT=(None, None), gate_withT=(
 
     Tangents: of x and y both or of neither, then also of gate, scale and shift where they are not zero; tangent outputs
     are detached. Differentiable (once) in x, y and the small operands, whose gradients are summed in a fixed order;
-    torch's own forward-mode tangents are refused.
+    torch's own forward-mode tangents are refused. The backward's scratch is 12 C bytes per workgroup, of which a
+    group of tokens has one or more; none where it has one, as with a row per token, and no gradient of weight, bias or
+    post_weight is wanted.
     """
     (x, tx), (y, ty), (gate, tgate), (scale, tscale), (shift, tshift) = x_withT, y_withT, gate_withT, scale_withT, shift_withT
     eps, residual_scale = float(eps), float(residual_scale)

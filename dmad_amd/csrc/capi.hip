@@ -1500,7 +1500,9 @@ int norm_cut(dmad::GatedNormParams& p, dmad::NormPass pass) {
     return fail(DMAD_ERR_UNSUPPORTED, "too many groups of tokens");
   return DMAD_OK;
 }
-size_t norm_workspace(const dmad::GatedNormParams& p) {
+// Workgroups leave their sums behind where several share a group, or a gradient runs over all groups.
+size_t norm_workspace(const dmad::GatedNormParams& p, bool per_channel) {
+  if (p.rows == 0 || (!per_channel && p.split == 1)) return 0;
   return (size_t)p.B * p.F * p.split * dmad::kNormSums * p.C * sizeof(float);
 }
 
@@ -2170,11 +2172,15 @@ int dmad_gated_norm(const dmad_gated_norm_sizes* sizes, const void* x, const voi
 }
 
 int dmad_gated_norm_bwd_workspace_bytes(const dmad_gated_norm_sizes* sizes, size_t* bytes) {
+  return dmad_gated_norm_bwd_workspace_bytes_for(sizes, 1, bytes);
+}
+
+int dmad_gated_norm_bwd_workspace_bytes_for(const dmad_gated_norm_sizes* sizes, int per_channel, size_t* bytes) {
   if (bytes == nullptr) return fail(DMAD_ERR_INVALID, "bytes: null pointer");
   dmad::GatedNormParams p{};
   int rc = norm_sizes(sizes, 0.f, 1.f, p);
   if (rc != DMAD_OK || (rc = norm_cut(p, dmad::NormPass::kBackward)) != DMAD_OK) return rc;
-  *bytes = p.rows == 0 ? 0 : norm_workspace(p);
+  *bytes = norm_workspace(p, per_channel != 0);
   return ok();
 }
 
@@ -2218,8 +2224,8 @@ int dmad_gated_norm_bwd(const dmad_gated_norm_sizes* sizes, const void* x, const
   p.dbias = dbias;
   p.dpost = dpost;
   if ((rc = norm_cut(p, dmad::NormPass::kBackward)) != DMAD_OK) return rc;
-  if (weights || (groups && p.split > 1)) {
-    const size_t need = norm_workspace(p);
+  const size_t need = groups || weights ? norm_workspace(p, weights) : 0;
+  if (need > 0) {
     if (workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)
       return fail(DMAD_ERR_WORKSPACE, "workspace: %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
     p.partial = (float*)workspace;

@@ -394,8 +394,14 @@ int dmad_gated_norm(const dmad_gated_norm_sizes* sizes, const void* x, const voi
                     const void* tshift, const void* weight, const void* bias, const void* post_weight, float eps,
                     float residual_scale, void* xo, void* txo, void* no, void* tno, void* stream);
 
-/* Bytes of workspace of dmad_gated_norm_bwd (not looked at where no small operand's gradient is asked for). */
+/* Bytes of workspace of dmad_gated_norm_bwd (not looked at where no small operand's gradient is asked for), enough for any
+ * gradients. */
 int dmad_gated_norm_bwd_workspace_bytes(const dmad_gated_norm_sizes* sizes, size_t* bytes);
+
+/* The same of a call whose dweight, dbias and dpost are all null (per_channel 0): none where every group of tokens is
+ * worked on by one workgroup, which then writes the group's gradients itself, as with a row of gate, scale and shift per
+ * token. per_channel 1: as above. */
+int dmad_gated_norm_bwd_workspace_bytes_for(const dmad_gated_norm_sizes* sizes, int per_channel, size_t* bytes);
 
 /*
  * Its backward: gx, gn the gradients of x' and n by the strides `tx` and `ty`

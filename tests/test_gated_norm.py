@@ -367,6 +367,27 @@ def test_partial_gradients(gpu, C):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C", [256, 1536])
+def test_a_row_per_token_takes_no_workspace(gpu, C):
+    """Gate, scale and shift per token, whose gradients the workgroups write themselves: the backward allocates them and
+    those of x and y, and nothing beside them."""
+    S = 2048
+    x = _inputs(1, S, C, S, torch.bfloat16, torch.bfloat16, WAN, 23)
+    d = {n: t.to(gpu).contiguous() for n, t in x.items()}
+    leaves = [d[n].requires_grad_(True) for n in WAN]
+    (xo, _), (n, _) = _call(d, tangents=False)
+    print(f"case a row per token C={C}", flush=True)
+    before = torch.cuda.memory_stats()["requested_bytes.all.current"]
+    torch.cuda.reset_peak_memory_stats()
+    grads = torch.autograd.grad((xo, n), leaves, (d["gx"], d["gn"]))
+    took = torch.cuda.memory_stats()["requested_bytes.all.peak"] - before
+    assert took == sum(t.numel() * t.element_size() for t in grads)
+    ref, size = _reference(x, WAN, "layer", 1e-6, 1.0, True)
+    for name, got in zip(WAN, grads):
+        _check("d" + name, got, ref["d" + name], size["d" + name])
+
+
+@pytest.mark.gpu
 def test_no_second_derivative(gpu):
     x = _inputs(1, 4, 32, 1, torch.float32, torch.float32, WAN, 6)
     d = {n: t.to(gpu) for n, t in x.items()}
@@ -633,6 +654,28 @@ def test_c_backward_rejects_bad_arguments():
     assert call(y=0, gate=0, dgate=0) == 1 and b"without y" in lib.dmad_last_error()
     assert call(ws=0) == 3 and call(size=16) == 3 and call(ws=264) == 3
     assert call(z=_sizes(B=0)) == 1 and b"no rows" in lib.dmad_last_error()
+
+
+def test_workspace_goes_by_the_gradients_that_are_wanted():
+    """3 rows of sums per workgroup where gradients run over all groups or several workgroups share one; else none."""
+    from dmad_amd import _native as nat
+
+    def size(per_channel, **over):
+        z, n = _sizes(**over), ctypes.c_size_t(99)
+        assert nat.lib().dmad_gated_norm_bwd_workspace_bytes_for(ctypes.byref(z), per_channel, ctypes.byref(n)) == 0
+        most = ctypes.c_size_t(99)
+        assert nat.lib().dmad_gated_norm_bwd_workspace_bytes(ctypes.byref(z), ctypes.byref(most)) == 0
+        assert n.value <= most.value and (not per_channel or n.value == most.value)
+        return n.value
+
+    for C in (256, 5120):
+        assert size(0, S=32760, F=32760, C=C) == 0
+        assert size(1, S=32760, F=32760, C=C) == 32760 * 3 * C * 4
+        assert size(0, S=32760, F=1, C=C) == size(1, S=32760, F=1, C=C) > 0
+        assert size(0, S=0, F=1, C=C) == size(1, S=0, F=1, C=C) == 0
+    z, n = _sizes(), ctypes.c_size_t(0)
+    assert nat.lib().dmad_gated_norm_bwd_workspace_bytes_for(None, 0, ctypes.byref(n)) == 1
+    assert nat.lib().dmad_gated_norm_bwd_workspace_bytes_for(ctypes.byref(z), 0, None) == 1
 
 
 # ---------------------------------------------------------------- what watches operators, and tensors that are not their memory
