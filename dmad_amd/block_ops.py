@@ -56,22 +56,33 @@ _PER_CHANNEL = ("weight", "bias", "post_weight")
 class _NormPlan:
     """What the sizes, types and strides of a call's operands settle, made once for them."""
 
-    __slots__ = ("device", "B", "S", "C", "F", "code", "wcode", "dtype", "norm", "in_place", "forward_sizes", "backward_sizes",
-                 "workspace")
+    __slots__ = ("device", "B", "S", "C", "F", "code", "wcode", "dtype", "norm", "small", "in_place", "group_strides",
+                 "dense", "forward_sizes", "backward_sizes", "workspace")
 
     def __init__(self, checked, norm, operands):
         x, self.F, self.dtype = checked
         self.B, self.S, self.C = x.shape
         self.device, self.code, self.wcode = x.device, nat.dtype_code(x.dtype), nat.dtype_code(self.dtype)
         self.norm, self.backward_sizes, self.workspace = _NORMS[norm], {}, {}
+        # strides of a contiguous operand
+        self.dense = (0 if self.B == 1 else self.S * self.C, 0 if self.S == 1 else self.C, 1)
+        # gate, scale, shift, weight, bias and post_weight
+        self.small = [None if t is None else (t.shape, t.dtype, t.stride()) for t in (*operands[4:10:2], *operands[10:])]
         # whether the kernels read every operand where it lies, if it starts aligned
         strides = [None if t is None else _strides3(t) for t in operands[:10]]
         self.in_place = all(t is None or st is not None for t, st in zip(operands, strides)) and all(
             t is None or t.dtype == self.dtype and (i < 10 or t.stride(0) == 1) for i, t in enumerate(operands) if i >= 4)
-        self.forward_sizes = None
+        self.forward_sizes = self.group_strides = None
         if self.in_place:
             x, tx, y, ty, gate, tgate, scale, tscale, shift, tshift = strides
+            self.group_strides = gate, scale, shift
             self.forward_sizes = self.sizes(x, y, tx, ty, gate, scale, shift, tgate, tscale, tshift)
+
+    def readable(self, t):
+        """``_readable3`` of an operand [B, S, C] or None."""
+        if t is None:
+            return None, None
+        return (t, self.dense) if t.is_contiguous() and not t.data_ptr() & 15 else _readable3(t)
 
     def sizes(self, *strides):
         """``dmad_gated_norm_sizes`` of these strides, for ctypes."""
@@ -89,7 +100,7 @@ class _NormPlan:
 
 
 class _NormCall:
-    """What forward and backward of one call share: the plan, and the small operands as the kernels take them."""
+    """What a forward or a backward launch goes by: the plan, and the small operands as the kernels take them."""
 
     __slots__ = ("plan", "in_place", "eps", "residual_scale", *_SMALL, *_PER_CHANNEL)
 
@@ -180,8 +191,7 @@ def _norm_forward(call, x, tx, y, ty, tgate, tscale, tshift):
     if call.in_place:
         sizes = plan.forward_sizes
     else:
-        none = (None, None)
-        (x, sx), (tx, stx), (y, sy), (ty, sty) = (none if t is None else _readable3(t) for t in (x, tx, y, ty))
+        (x, sx), (tx, stx), (y, sy), (ty, sty) = map(plan.readable, (x, tx, y, ty))
         tgate, tscale, tshift = (None if t is None else _small_as_read(t, plan.dtype) for t in (tgate, tscale, tshift))
         sizes = plan.sizes(sx, sy, stx, sty, *(None if t is None else _strides3(t) for t in
                                                (call.gate, call.scale, call.shift, tgate, tscale, tshift)))
@@ -206,6 +216,20 @@ def _check_norm_saved(t, g):
                            f"{g.device} as the forward read it, got {got}")
 
 
+def _saved_call(plan, small, eps, residual_scale):
+    """The call of a backward, from the saved small operands, which are those that the plan was made from: one that came
+    back in another shape, type or place is refused, and one that lies otherwise is copied (what was absent stays so)."""
+    in_place = plan.in_place
+    for t, want in zip(small, plan.small):
+        if want is None:
+            continue
+        if t is None or t.dtype != want[1] or t.shape != want[0] or t.device != plan.device:
+            got = "nothing" if t is None else f"{tuple(t.shape)} {t.dtype} on {t.device}"
+            raise RuntimeError(f"{_GN}: the backward needs a small operand as the forward read it, got {got}")
+        in_place = in_place and t.stride() == want[2] and not t.data_ptr() & 15
+    return _NormCall(plan, in_place, *small, eps, residual_scale)
+
+
 def _norm_gradients(call, x, y, gx, gn, originals, need):
     """The launch: gradients of (x, y, gate, scale, shift, weight, bias, post_weight), None where none is asked for.
     ``originals``: the small operands as the caller has them; ``need``: which of the eight are wanted."""
@@ -214,10 +238,7 @@ def _norm_gradients(call, x, y, gx, gn, originals, need):
     if y is not None or call.gate is not None or call.post_weight is not None:
         _check_norm_saved(y, g)
     plan, ptr = call.plan, nat.ptr
-    x, sx = _readable3(x)
-    y, sy = (None, None) if y is None else _readable3(y)
-    gx, sgx = (None, None) if gx is None else _readable3(gx)
-    gn, sgn = (None, None) if gn is None else _readable3(gn)
+    (x, sx), (y, sy), (gx, sgx), (gn, sgn) = map(plan.readable, (x, y, gx, gn))
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dy = torch.empty_like(dx) if need[1] and y is not None else None
     shape, dtype = (plan.B, plan.F, plan.C), plan.dtype
@@ -229,10 +250,11 @@ def _norm_gradients(call, x, y, gx, gn, originals, need):
             if t is not None:
                 t.zero_()
     else:
-        sizes = plan.sizes_back(sx, sy, sgx, sgn, *(None if t is None else _strides3(t) for t in as_read[:3]))
+        groups = plan.group_strides if call.in_place else (None if t is None else _strides3(t) for t in as_read[:3])
+        sizes = plan.sizes_back(sx, sy, sgx, sgn, *groups)
         ws_ptr, ws_size, ws = None, 0, None
-        if any(t is not None for t in small):
-            per_channel = any(t is not None for t in small[3:])
+        per_channel = not (small[3] is None and small[4] is None and small[5] is None)
+        if per_channel or not (small[0] is None and small[1] is None and small[2] is None):
             size = plan.workspace.get(per_channel)
             if size is None:
                 n = ctypes.c_size_t(0)
@@ -255,8 +277,9 @@ class _GatedNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, call, x, tx, y, ty, gate, tgate, scale, tscale, shift, tshift, weight, bias, post_weight):
         xo, txo, n, tn, x, y = _norm_forward(call, x, tx, y, ty, tgate, tscale, tshift)
+        # no operand is kept but by its saved tensor, which hooks may move and the backward frees
         ctx.save_for_backward(x, y, gate, scale, shift, weight, bias, post_weight)
-        ctx.call = call
+        ctx.plan, ctx.eps, ctx.residual_scale = call.plan, call.eps, call.residual_scale
         ctx.set_materialize_grads(False)
         tangents = [t for t in (txo, tn) if t is not None]
         if tangents:
@@ -284,14 +307,15 @@ def _needed(ctx, first):
 
 
 def _norm_backward(ctx, gx, gn):
-    x, y, gate, scale, shift, weight, bias, post_weight = ctx.saved_tensors  # unpacked, so that a change in place is noticed
+    x, y, *small = ctx.saved_tensors
     if gx is None and gn is None:
         return (None,) * 14
-    call, small, need = ctx.call, (gate, scale, shift, weight, bias, post_weight), _needed(ctx, 1)
-    if _eager_call(gx, gn):  # what was saved was read by an eager forward
+    plan, eps, residual_scale, need = ctx.plan, ctx.eps, ctx.residual_scale, _needed(ctx, 1)
+    if _eager_call(gx, gn, x, y, *small):
+        call = _saved_call(plan, small, eps, residual_scale)
         grads = _norm_gradients(call, x, y, gx, gn, small, need)
     else:
-        grads = _norm_gradients_op(x, y, gx, gn, *small, call.eps, call.plan.norm == 1, call.residual_scale, need)
+        grads = _norm_gradients_op(x, y, gx, gn, *small, eps, plan.norm == 1, residual_scale, need)
     return (None, *_spread(grads))
 
 

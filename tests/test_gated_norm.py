@@ -10,8 +10,10 @@ reciprocal root around it, every result is off by less than STEPS = 128 half ste
 adds up for it. Sums over tokens (gradients of small operands) are at most 43 additions in a wave, 4 waves and 32 more
 of each of 32 strands in these tests: the same bound.
 """
+import contextlib
 import ctypes
 import math
+import weakref
 
 import pytest
 import torch
@@ -930,6 +932,66 @@ def test_saved_tensor_hooks(gpu):
     for unpack in (lambda t: t.to(torch.bfloat16), lambda t: t[:1], lambda t: t.cpu()):
         with pytest.raises(RuntimeError):
             grads(lambda t: t, lambda t: unpack(t) if t.dim() == 3 and t.shape[1] == 6 else t)
+
+
+@BOTH
+@pytest.mark.parametrize("when", ["packed", "after the backward"])
+def test_operands_are_kept_by_their_saved_tensors_alone(request, monkeypatch, device, when):
+    """Hooks that move what is saved move all of it, and a graph that lives on after its backward holds no operand."""
+    leaves = _set_up(request, monkeypatch, device, grad=True)
+    x = {n: t if n.startswith("g") and n != "gate" else t * 1 for n, t in leaves.items()}
+    there = {n: weakref.ref(t) for n, t in x.items() if n in ALL}
+    clone = (lambda t: t.clone(), lambda t: t)
+    with torch.autograd.graph.saved_tensors_hooks(*clone) if when == "packed" else contextlib.nullcontext():
+        outs = _run(x)
+    if when != "packed":
+        torch.autograd.grad(outs[2].sum(), [leaves[n] for n in ALL], allow_unused=True)
+    del x
+    assert [n for n, r in there.items() if r() is not None] == []
+    assert outs[2].requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wdtype", ["bf16", "fp32", "mixed"])
+def test_hooks_that_offload_leave_nothing_on_the_device(gpu, wdtype):
+    """Nor do copies of small operands of several types stay, and what comes back may lie otherwise than it did."""
+    x = _inputs(2, 6, 1536, 2, torch.bfloat16, torch.float32 if wdtype != "bf16" else torch.bfloat16, ALL, 31)
+    if wdtype == "mixed":
+        x["gate"], x["weight"] = x["gate"].to(torch.bfloat16), x["weight"].to(torch.bfloat16)
+    d = {n: t.to(gpu).requires_grad_(n in ALL) for n, t in x.items()}
+    into = (d["gx"], d["gn"])
+
+    def current():
+        torch.cuda.synchronize()
+        return torch.cuda.memory_stats()["requested_bytes.all.current"]
+
+    def run(*hooks):
+        before = current()
+        with torch.autograd.graph.saved_tensors_hooks(*hooks):
+            (xo, _), (n, _) = _call({m: d[m] * 1 for m in ALL}, tangents=False)
+        kept = current() - before - 2 * n.numel() * n.element_size()
+        return kept, torch.autograd.grad((xo, n), [d[m] for m in ALL], into)
+
+    kept, want = run(lambda t: t, lambda t: t)
+    assert kept >= sum(d[m].numel() * d[m].element_size() for m in ALL)
+    wide = lambda t: torch.stack((t, t), -2)[..., 0, :]  # noqa: E731
+    for back in (lambda t: t.to(gpu), lambda t: wide(t.to(gpu)), lambda t: torch.cat((t.new_zeros(1), t.flatten())).to(gpu)[1:].view(t.shape)):
+        kept, got = run(lambda t: t.cpu(), back)
+        assert kept == 0
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_small_operands_from_hooks_are_checked(gpu):
+    x = _small(gpu, grad=True)
+    for name in (*SMALL, *PER_CHANNEL):
+        for change in (lambda t: t.to(torch.float16), lambda t: t[..., :-8], lambda t: t.cpu(), lambda t: t[:1] if t.dim() == 3 else t[None]):
+            at = x[name].data_ptr()
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: (t, t.data_ptr() == at), lambda p: change(p[0]) if p[1] else p[0]):
+                xo, _, n, _ = _run(x)
+            with pytest.raises(RuntimeError, match="as the forward read it"):
+                torch.autograd.grad(xo.square().sum() + n.sum(), [x[m] for m in ALL])
 
 
 @BOTH
