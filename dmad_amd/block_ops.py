@@ -481,17 +481,17 @@ def rotary_frequencies(dim, theta=10000.0, scaling=None, factor=1.0, trained_len
 
 
 class _RotaryCall:
-    """What forward and backward of one call share: sizes, and the positions and frequencies as the kernels take them."""
+    """What a forward or a backward launch goes by: sizes, and the positions and frequencies as the kernels take them."""
 
-    __slots__ = ("device", "code", "B", "S", "D", "R", "positions", "pos64", "pos_strides", "frequencies", "layout", "factor")
+    __slots__ = ("sizes", "positions", "pos_strides", "frequencies", "layout", "factor")
 
-    def __init__(self, sizes, positions, frequencies, layout, factor):
-        self.device, self.code, self.B, self.S, self.D, self.R, self.pos64, self.pos_strides = sizes
-        self.positions, self.layout, self.factor = positions, _LAYOUTS[layout], factor
+    def __init__(self, sizes, positions, pos_strides, frequencies, layout, factor):
+        self.sizes, self.positions, self.pos_strides, self.layout, self.factor = sizes, positions, pos_strides, layout, factor
         self.frequencies = frequencies if frequencies.is_contiguous() else frequencies.contiguous()
 
 
-# the sizes of a _RotaryCall by shapes, types and strides of its operands
+# the sizes of a _RotaryCall by shapes, types and strides of its operands: (device, type code, B, S, D, R, whether positions have
+# 64 bits, their strides for ctypes, (shape, type and strides of positions, shape of frequencies))
 _rotary_sizes: dict = {}
 
 
@@ -506,10 +506,15 @@ def _rotary_plan(q, tq, k, tk, positions, frequencies, layout, factor):
         x, B, S, D, R = _rotary_check(*tensors, layout, factor)
         if len(_rotary_sizes) > 1024:
             _rotary_sizes.clear()
-        st = positions.stride()
-        pos_strides = nat.int64_array((st[0] if len(st) == 2 and positions.shape[0] > 1 else 0, st[-1]))
-        sizes = _rotary_sizes[key] = (x.device, nat.dtype_code(x.dtype), B, S, D, R, int(positions.dtype == torch.int64), pos_strides)
+        sizes = _rotary_sizes[key] = (x.device, nat.dtype_code(x.dtype), B, S, D, R, int(positions.dtype == torch.int64),
+                                      _position_strides(positions),
+                                      (positions.shape, positions.dtype, positions.stride(), frequencies.shape))
     return sizes
+
+
+def _position_strides(positions):
+    st = positions.stride()
+    return nat.int64_array((st[0] if len(st) == 2 and positions.shape[0] > 1 else 0, st[-1]))
 
 
 def _rotary_check(q, tq, k, tk, positions, frequencies, layout, factor):
@@ -553,11 +558,14 @@ def _rotary_check(q, tq, k, tk, positions, frequencies, layout, factor):
 
 
 _head_strides: dict = {}
+_ABSENT = (None, None)
 
 
 def _heads4(t):
     """(tensor, ctypes strides) of a [B, S, H, D] operand, copied only where its rows are not contiguous: the kernel takes
     any alignment of whole elements. An axis of one element is never stepped along."""
+    if t is None:
+        return _ABSENT
     key = (t.shape, t.stride())
     arr = _head_strides.get(key, 0)
     if arr == 0:
@@ -572,22 +580,24 @@ def _heads4(t):
 
 def _rotary_launch(call, q, tq, k, tk, transposed):
     """The launch: (q', tq', k', tk')."""
-    none, dev, ptr = (None, None), call.device, nat.ptr
-    outs = [None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, tq, k, tk)]
+    dev, code, B, S, D, R, pos64, _, _ = call.sizes
+    ptr, dense = nat.ptr, torch.contiguous_format
+    oq = None if q is None else torch.empty_like(q, memory_format=dense)
+    ok = None if k is None else torch.empty_like(k, memory_format=dense)
+    otq = None if tq is None else torch.empty_like(tq, memory_format=dense)
+    otk = None if tk is None else torch.empty_like(tk, memory_format=dense)
     # an operand without heads has nothing to turn
     Hq, Hk = 0 if q is None else q.shape[2], 0 if k is None else k.shape[2]
-    q, tq = (q, tq) if Hq else none
-    k, tk = (k, tk) if Hk else none
-    if call.B * call.S * (Hq + Hk) == 0:
-        return outs
-    (q, sq), (tq, stq), (k, sk), (tk, stk) = (none if t is None else _heads4(t) for t in (q, tq, k, tk))
-    oq, otq, ok, otk = outs
+    if B * S * (Hq + Hk) == 0:
+        return [oq, otq, ok, otk]
+    (q, sq), (tq, stq) = (_heads4(q), _heads4(tq)) if Hq else (_ABSENT, _ABSENT)
+    (k, sk), (tk, stk) = (_heads4(k), _heads4(tk)) if Hk else (_ABSENT, _ABSENT)
     with nat.on_device(dev):
         nat.check(nat.lib().dmad_qk_rotary(
-            call.code, call.B, call.S, Hq, Hk, call.D, call.R, ptr(q), ptr(tq), ptr(k), ptr(tk), sq, stq, sk, stk,
-            ptr(call.positions), call.pos64, call.pos_strides, ptr(call.frequencies), call.layout, transposed, call.factor,
+            code, B, S, Hq, Hk, D, R, ptr(q), ptr(tq), ptr(k), ptr(tk), sq, stq, sk, stk, ptr(call.positions), pos64,
+            call.pos_strides, ptr(call.frequencies), call.layout, transposed, call.factor,
             ptr(oq), ptr(otq), ptr(ok), ptr(otk), nat.stream_ptr(dev)))
-    return outs
+    return [oq, otq, ok, otk]
 
 
 class _Rotary(torch.autograd.Function):
@@ -596,8 +606,9 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, call, q, tq, k, tk, positions, frequencies):
         outs = _rotary_launch(call, q, tq, k, tk, 0)
+        # positions and frequencies are kept by their saved tensors alone, which hooks may move and the backward frees
         ctx.save_for_backward(positions, frequencies)
-        ctx.call = call
+        ctx.plan = call.sizes, call.layout, call.factor
         ctx.set_materialize_grads(False)
         tangents = [t for t in (outs[1], outs[3]) if t is not None]
         if tangents:
@@ -612,14 +623,22 @@ class _Rotary(torch.autograd.Function):
 
 
 def _rotary_backward(ctx, gq, gk):
-    positions, frequencies = ctx.saved_tensors  # unpacked, so that a change in place is noticed
+    positions, frequencies = ctx.saved_tensors
     if gq is None and gk is None:
         return (None,) * 7
-    call = ctx.call
-    if _eager_call(gq, gk):
+    sizes, layout, factor = ctx.plan
+    dev, pos_strides, (shape, dtype, strides, table) = sizes[0], *sizes[-2:]
+    if positions is None or frequencies is None or positions.shape != shape or positions.dtype != dtype or \
+            frequencies.shape != table or frequencies.dtype != torch.float64 or positions.device != dev or frequencies.device != dev:
+        got = ", ".join("nothing" if t is None else f"{tuple(t.shape)} {t.dtype} on {t.device}" for t in (positions, frequencies))
+        raise RuntimeError(f"{_QR}: the backward needs positions and frequencies as the forward read them, got {got}")
+    if _eager_call(gq, gk, positions, frequencies):
+        if positions.stride() != strides:
+            pos_strides = _position_strides(positions)
+        call = _RotaryCall(sizes, positions, pos_strides, frequencies, layout, factor)
         dq, _, dk, _ = _rotary_launch(call, gq, None, gk, None, 1)
     else:
-        dq, dk = _rotary_gradients_op(gq, gk, positions, frequencies, call.layout == 1, call.factor)
+        dq, dk = _rotary_gradients_op(gq, gk, positions, frequencies, layout == 1, factor)
     return None, dq, None, dk, None, None, None
 
 
@@ -632,7 +651,8 @@ def qk_rotary_fwd(q: Optional[torch.Tensor], tq: Optional[torch.Tensor], k: Opti
                   factor: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(q', tq', k', tk') of ``qk_rotary_with_tangent``."""
     layout = "half" if half else "interleaved"
-    call = _RotaryCall(_rotary_plan(q, tq, k, tk, positions, frequencies, layout, factor), positions, frequencies, layout, factor)
+    sizes = _rotary_plan(q, tq, k, tk, positions, frequencies, layout, factor)
+    call = _RotaryCall(sizes, positions, sizes[7], frequencies, int(half), factor)
     return _or_empty(k if q is None else q, _rotary_launch(call, q, tq, k, tk, 0))
 
 
@@ -646,8 +666,8 @@ def qk_rotary_bwd(gq: Optional[torch.Tensor], gk: Optional[torch.Tensor], positi
                   half: bool, factor: float) -> Tuple[torch.Tensor, torch.Tensor]:
     """(dq, dk): the outputs' gradients, of which one may be absent, turned back."""
     layout = "half" if half else "interleaved"
-    call = _RotaryCall(_rotary_plan(gq, None, gk, None, positions, frequencies, layout, factor), positions, frequencies, layout,
-                       factor)
+    sizes = _rotary_plan(gq, None, gk, None, positions, frequencies, layout, factor)
+    call = _RotaryCall(sizes, positions, sizes[7], frequencies, int(half), factor)
     dq, _, dk, _ = _rotary_launch(call, gq, None, gk, None, 1)
     return _or_empty(gk if gq is None else gq, (dq, dk))
 
@@ -706,7 +726,8 @@ def qk_rotary_with_tangent(q_withT, k_withT, positions, frequencies, layout="int
         outs = torch.ops.dmad.qk_rotary_fwd(q, tq, k, tk, positions, frequencies, layout == "half", factor)
         q, tq, k, tk = (None if t is None else y for t, y in zip((q, tq, k, tk), outs))
         return (q, None if tq is None else tq.detach()), (k, None if tk is None else tk.detach())
-    call = _RotaryCall(_rotary_plan(*tensors, layout, factor), positions, frequencies, layout, factor)
+    sizes = _rotary_plan(*tensors, layout, factor)
+    call = _RotaryCall(sizes, positions, sizes[7], frequencies, _LAYOUTS[layout], factor)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
         q, tq, k, tk = _Rotary.apply(call, q, tq, k, tk, positions, frequencies)
     else:

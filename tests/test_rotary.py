@@ -8,8 +8,10 @@ and cosine come within 2 units in the last place, the factor and the two product
 element is off by half a step of its type plus less than STEPS = 16 half steps of float32 of |factor| times the larger
 element of its pair. Elements behind the turned part are copied.
 """
+import contextlib
 import ctypes
 import math
+import weakref
 
 import pytest
 import torch
@@ -625,6 +627,46 @@ def test_registered_ops_do_what_they_declare(gpu):
     torch.library.opcheck(torch.ops.dmad.qk_rotary_fwd.default, (*(x[n] for n in OPERANDS), True, 1.5))
     torch.library.opcheck(torch.ops.dmad.qk_rotary_fwd.default, (None, None, x["k"], None, x["positions"], x["frequencies"], False, 1.0))
     torch.library.opcheck(torch.ops.dmad.qk_rotary_bwd.default, (x["gq"], None, x["positions"], x["frequencies"], True, 1.5))
+
+
+@BOTH
+@pytest.mark.parametrize("when", ["packed", "after the backward"])
+def test_angles_are_kept_by_their_saved_tensors_alone(request, monkeypatch, device, when):
+    """Hooks that move what is saved move all of it, and a graph that lives on after its backward holds nothing."""
+    leaves = _set_up(request, monkeypatch, device, grad=True)
+    x = {n: t * 1 for n, t in leaves.items()}
+    there = {n: weakref.ref(t) for n, t in x.items()}
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t) if when == "packed" else contextlib.nullcontext():
+        q, _, k, _ = _run(x)
+    if when != "packed":
+        torch.autograd.grad(q.sum() + k.sum(), (leaves["q"], leaves["k"]))
+    del x
+    assert [n for n, r in there.items() if r() is not None] == []
+    assert q.requires_grad
+
+
+@BOTH
+@pytest.mark.parametrize("shared", [False, True])
+def test_angles_from_hooks(request, monkeypatch, device, shared):
+    """What comes back from hooks may lie otherwise than it did; in another shape, type or place it is refused."""
+    x = _set_up(request, monkeypatch, device, grad=True)
+    if shared:
+        x["positions"], x["frequencies"] = x["positions"][:1].expand(2, -1), torch.stack((x["frequencies"],) * 2, -1)[:, 0]
+
+    def grads(pack, unpack):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            q, _, k, _ = _run(x)
+        return torch.autograd.grad(q.square().sum() + k.sum(), (x["q"], x["k"]))
+
+    want = grads(lambda t: t, lambda t: t)
+    for unpack in (lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: torch.stack((t, t), -1)[..., 0]):
+        for a, b in zip(grads(lambda t: t, unpack), want):
+            assert torch.equal(a, b)
+    wrong = [lambda t: t[..., :-1], lambda t: t.to(torch.int16), lambda t: t[None, None]]
+    for change in wrong + ([lambda t: t.cpu()] if device == "gpu" else []):
+        for dtype in (x["positions"].dtype, torch.float64):
+            with pytest.raises((RuntimeError, ValueError), match="as the forward read them"):
+                grads(lambda t: t, lambda t: change(t) if t.dtype == dtype else t)
 
 
 @BOTH
