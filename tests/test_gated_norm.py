@@ -284,6 +284,70 @@ def test_calls_past_the_caches(gpu, C):
             assert ((got.double() - ref).abs() <= (n + 1) * 2.0 ** -24 * size).all()
 
 
+def _check_within(name, got, ref, size, steps):
+    u, tiny = torch.finfo(got.dtype).eps / 2, torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
+    tol = u * ref.abs() * (1 + 1e-3) + steps * F32 * size + tiny
+    assert torch.isfinite(got).all(), name
+    worst = float(((got.double() - ref).abs() / tol).max())
+    print(f"  {name}: worst error {worst:.2f} of its bound", flush=True)
+    assert worst <= 1.0, name
+
+
+def _on_device(gpu, B, S, C, F, dtype, wdtype, there, seed):
+    """As _inputs(), made on the device, for large calls."""
+    g = torch.Generator(device=gpu).manual_seed(seed)
+    r = lambda *shape, sd=1.0, mean=0.0: torch.randn(shape, generator=g, device=gpu) * sd + mean  # noqa: E731
+    x = {n: r(B, S, C).to(dtype) for n in ("x", "y", "tx", "ty", "gx", "gn")}
+    x.update({n: r(B, F, C, sd=0.3).to(wdtype) for n in ("gate", "scale", "shift")})
+    x.update({n: r(C, sd=0.2, mean=m).to(wdtype) for n, m in (("weight", 1.0), ("bias", 0.0), ("post_weight", 1.0))})
+    return {n: t for n, t in x.items() if n in there or n in ("tx", "gx", "gn") or (n == "ty" and "y" in there)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,C,F,dtype,wdtype,kind,there,rs", [
+    (60000, 512, 4, "bf16", "fp32", "layer", ALL, 1.0),
+    (6000, 5120, 3, "fp16", "fp16", "rms", ALL, 0.5),
+    (12000, 1544, 1, "fp32", "fp32", "layer", ("x", "y", "weight", "post_weight"), -1.0),
+    (30000, 1536, 4, "bf16", "bf16", "layer", ("x", "scale", "weight", "bias"), 1.0),
+    (90000, 504, 1, "bf16", "fp32", "rms", ("x", "weight"), 1.0),
+    (31000, 1536, 2, "fp16", "fp32", "layer", WAN, 1.0),
+])
+def test_gradients_of_calls_past_the_caches(gpu, S, C, F, dtype, wdtype, kind, there, rs):
+    """Every gradient of calls of more than the caches hold, with and without a branch and a norm after it, against
+    float64. Sums over tokens are up to 30 additions in a wave, 4 waves, and 40 of each of 32 strands, together fewer than
+    the module's bound counts."""
+    d = _on_device(gpu, 1, S, C, F, DTYPES[dtype], DTYPES[wdtype], there, C)
+    assert (6 if "y" in there else 3) * S * C * d["x"].element_size() > 2 ** 28
+    branch = "y" in there
+    print(f"case past caches S={S} C={C} F={F} {dtype} {wdtype} {kind} {there}", flush=True)
+    leaves = [d[n].requires_grad_(True) for n in ALL if n in there]
+    (xo, _), (n, _) = _call(d, kind, 1e-6, rs, tangents=False)
+    outs, into = ((xo, n), (d["gx"], d["gn"])) if branch else ((n,), (d["gn"],))
+    grads = torch.autograd.grad(outs, leaves, into)
+    torch.cuda.synchronize()
+    ref, size = _reference({k: t.detach() for k, t in d.items()}, there, kind, 1e-6, rs, branch)
+    for name, leaf, got in zip([n for n in ALL if n in there], leaves, grads):
+        assert got.dtype == leaf.dtype and got.shape == leaf.shape
+        _check_within("d" + name, got, ref["d" + name], size["d" + name], STEPS)
+
+
+@pytest.mark.gpu
+def test_more_groups_than_rows_of_a_grid(gpu):
+    """34000 groups of two tokens, whose gradients take two launches; those of the weights are sums over 34000 workgroups,
+    of which a strand adds 1063 after one another: as many half steps more."""
+    B, F, C = 2, 17000, 64
+    d = _on_device(gpu, B, 2 * F, C, F, torch.bfloat16, torch.float32, ALL, 8)
+    assert B * F > 32768
+    leaves = [d[n].requires_grad_(True) for n in ALL]
+    print(f"case groups {B * F}", flush=True)
+    (xo, _), (n, _) = _call(d, tangents=False)
+    grads = torch.autograd.grad((xo, n), leaves, (d["gx"], d["gn"]))
+    torch.cuda.synchronize()
+    ref, size = _reference({k: t.detach() for k, t in d.items()}, ALL, "layer", 1e-6, 1.0, True)
+    for name, got in zip(ALL, grads):
+        _check_within("d" + name, got, ref["d" + name], size["d" + name], STEPS + (1063 if name in PER_CHANNEL else 0))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("C", [64, 1536])
 def test_one_shape_at_many_places(gpu, C):
