@@ -24,6 +24,16 @@ constexpr int kRotaryThreads = 256;
 constexpr int kRotaryLdsPairs = 4096;  // sines and cosines of a tile: 32 KiB
 constexpr int kRotaryMaxTile = 64;
 
+// A float32 result to its element. The compiler makes one instruction with one rounding of
+// some of the products and conversions to fp16 and two of others, which ones by the kernel's
+// form: about one element in 4000 then depended on whether there are tangents and on the
+// alignment. The empty asm keeps the two apart: float32, then fp16, for every element.
+template <typename T>
+__device__ __forceinline__ T rotary_round(float x) {
+  if constexpr (__is_same(T, _Float16)) asm("" : "+v"(x));
+  return (T)x;
+}
+
 // V consecutive elements, in one access of up to 16 bytes.
 template <typename T, int V>
 struct Piece {
@@ -40,7 +50,7 @@ struct Piece {
     else *(vec_t*)p = v;
   }
   __device__ __forceinline__ float get(int i) const { return (float)v[i]; }
-  __device__ __forceinline__ void set(int i, float x) { v[i] = (T)x; }
+  __device__ __forceinline__ void set(int i, float x) { v[i] = rotary_round<T>(x); }
 };
 template <typename T>
 struct Piece<T, 1> {
@@ -50,7 +60,7 @@ struct Piece<T, 1> {
   template <bool>
   __device__ __forceinline__ void store(T* p) const { *p = v; }
   __device__ __forceinline__ float get(int) const { return (float)v; }
-  __device__ __forceinline__ void set(int, float x) { v = (T)x; }
+  __device__ __forceinline__ void set(int, float x) { v = rotary_round<T>(x); }
 };
 
 // x / d by d's multiplier, of which 1 has none.

@@ -207,6 +207,28 @@ def test_calls_past_the_caches(gpu, half, R):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("D,R", [(16, 16), (128, 128), (80, 40)])
+def test_bits_do_not_depend_on_tangents_or_alignment(gpu, dtype, half, D, R):
+    """Over a million elements: with tangents, without, and from rows that start anywhere, where the accesses are single."""
+    S, H = 2 ** 20 // (5 * D), 3
+    print(f"case bits {dtype} half={half} D={D} R={R}", flush=True)
+    x = {n: _to(t, gpu) for n, t in _inputs(1, S, H, 2, D, R, DTYPES[dtype], 41).items()}
+
+    def off(t):
+        return torch.empty(t.numel() + 1, device=gpu, dtype=t.dtype)[1:].view(t.shape).copy_(t)
+
+    with torch.no_grad():
+        (q, tq), (k, tk) = _call(x, half, 1.25)
+        for y in ({**x, "tq": None, "tk": None}, {n: off(t) if n in ("q", "k", "tq", "tk") else t for n, t in x.items()}):
+            (q2, tq2), (k2, tk2) = _call(y, half, 1.25)
+            assert torch.equal(q2, q) and torch.equal(k2, k)
+            if tq2 is not None:
+                assert torch.equal(tq2, tq) and torch.equal(tk2, tk)
+
+
+@pytest.mark.gpu
 def test_far_and_negative_positions(gpu):
     """Angles of many turns are as exact as near ones; positions are any whole numbers."""
     x = _inputs(1, 6, 2, 1, 64, 64, torch.float32, 3)
