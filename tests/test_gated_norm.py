@@ -349,6 +349,31 @@ def test_more_groups_than_rows_of_a_grid(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("wdtype", ["same", "fp32"])
+@pytest.mark.parametrize("C", [512, 1536])
+@pytest.mark.parametrize("there", [("x", "scale", "shift", "weight", "bias"), WAN, ALL])
+def test_bits_do_not_depend_on_tangents_or_gradients(gpu, dtype, wdtype, C, there):
+    """Over a million elements: outputs with tangents and without, gradients with those of the weights and without."""
+    d = _on_device(gpu, 1, 2 ** 21 // C // 8 * 8, C, 8, DTYPES[dtype], DTYPES[dtype if wdtype == "same" else wdtype], there, 3)
+    print(f"case bits {dtype} {wdtype} C={C} {there}", flush=True)
+
+    def run(tangents, leaves):
+        ops = {n: t.detach().requires_grad_(n in leaves) for n, t in d.items()}
+        (xo, txo), (n, tn) = _call(ops, tangents=tangents)
+        outs, into = ((xo, n), (d["gx"], d["gn"])) if "y" in there else ((n,), (d["gn"],))
+        return [xo.detach(), n.detach()], dict(zip(leaves, torch.autograd.grad(outs, [ops[m] for m in leaves], into)))
+
+    every = [n for n in ALL if n in there]
+    outs, grads = run(True, every)
+    for tangents, leaves in ((False, every), (False, [n for n in every if n not in PER_CHANNEL]), (False, ["x"])):
+        o, g = run(tangents, leaves)
+        assert all(torch.equal(a, b) for a, b in zip(o, outs))
+        for n in leaves:
+            assert torch.equal(g[n], grads[n]), n
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("C", [64, 1536])
 def test_one_shape_at_many_places(gpu, C):
     """Calls of one shape, some of whose operands start off 16 bytes: what is planned for the shape holds for none else."""
