@@ -349,6 +349,31 @@ def test_more_groups_than_rows_of_a_grid(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("S,C", [(270000, 8192), (4400000, 504)])
+def test_more_elements_than_32_bits_count(gpu, S, C):
+    """The last tokens of calls of more than 2^31 elements: bit for bit what a call of them alone gives."""
+    F, n = S // 1000, 2000
+    assert S * C > 2 ** 31
+    print(f"case beyond 32 bits S={S} C={C}", flush=True)
+    d = {k: torch.empty(1, S, C, device=gpu, dtype=torch.bfloat16) for k in ("x", "tx", "y", "ty", "gx", "gn")}
+    for t in d.values():
+        t.view(-1, 1000 * C)[:] = torch.randn(1000 * C, device=gpu).to(torch.bfloat16)
+        t[:, -n:] = torch.randn(n, C, device=gpu).to(torch.bfloat16)
+    d.update({k: torch.randn(1, F, C, device=gpu) for k in ("gate", "scale", "shift")})
+
+    def run(rows, groups):
+        y = {k: t[:, groups if k in SMALL else rows] for k, t in d.items()}
+        leaves = [y[k].detach().requires_grad_() for k in WAN]
+        y.update(zip(WAN, leaves))
+        (xo, txo), (o, to) = _call(y)
+        grads = torch.autograd.grad((xo, o), leaves[:2], (y["gx"], y["gn"]))
+        return [t.detach()[:, -n:].clone() for t in (xo, txo, o, to, *grads)]
+
+    for a, b in zip(run(slice(None), slice(None)), run(slice(S - n, S), slice(F - n // 1000, F))):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("wdtype", ["same", "fp32"])
 @pytest.mark.parametrize("C", [512, 1536])

@@ -229,6 +229,24 @@ def test_bits_do_not_depend_on_tangents_or_alignment(gpu, dtype, half, D, R):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("half", [False, True])
+def test_more_elements_than_32_bits_count(gpu, half):
+    """The last tokens of a call of more than 2^31 elements: bit for bit what a call of them alone gives."""
+    S, H, D, n = 420000, 40, 128, 500
+    assert S * H * D > 2 ** 31
+    print(f"case beyond 32 bits half={half}", flush=True)
+    x = {k: torch.empty(1, S, H, D, device=gpu, dtype=torch.bfloat16) for k in ("q", "tq")}
+    for t in x.values():
+        t.view(-1, 1000 * H * D)[:] = torch.randn(1000 * H * D, device=gpu).to(torch.bfloat16)
+    x["positions"], x["frequencies"] = torch.arange(S, device=gpu), 10000.0 ** (-torch.arange(64, dtype=torch.float64, device=gpu) / 64)
+    x["k"] = x["tk"] = None
+    outs = _call(x, half)[0]
+    last = {k: t if k in ("k", "tk", "frequencies") else t[-n:] if k == "positions" else t[:, -n:] for k, t in x.items()}
+    for a, b in zip(outs, _call(last, half)[0]):
+        assert torch.equal(a[:, -n:], b)
+
+
+@pytest.mark.gpu
 def test_far_and_negative_positions(gpu):
     """Angles of many turns are as exact as near ones; positions are any whole numbers."""
     x = _inputs(1, 6, 2, 1, 64, 64, torch.float32, 3)
