@@ -455,7 +455,8 @@ def rotary_frequencies(dim, theta=10000.0, scaling=None, factor=1.0, trained_len
         the highest as it is;
       * "yarn": frequencies that make at least ``fast`` turns over ``trained_length`` positions stay, those that make at
         most ``slow`` are divided by ``factor``, those between are blended linearly in their turns; sines and cosines are
-        multiplied by 0.1 ln(factor) + 1.
+        multiplied by 0.1 ln(factor) + 1. (Some programs blend linearly in i between the two instead: weights trained so
+        need that table, which ``qk_rotary_with_tangent`` takes like any other.)
     """
     op = "rotary_frequencies"
     if dim < 2 or dim % 2:

@@ -41,8 +41,9 @@ struct GatedNormParams {
 
 // Widest rows.
 constexpr int kNormMaxC = 8192;
-// Waves of a workgroup for rows of C channels, waves that a pass aims at, and waves that a
-// CU holds in the forward and the backward pass.
+// Waves of a workgroup for rows of C channels, waves that a pass aims at, and waves per CU in
+// a round of the forward and of the backward pass. The backward's are what a CU holds; of the
+// forward's it would hold 32 (28 with a norm after the branch; with tangents 20 and 16).
 int norm_waves(int C);
 enum class NormPass { kForward, kTangent, kBackward };
 constexpr int kNormFwdWaves = 40960, kNormTangentWaves = 65536, kNormFwdHeld = 20, kNormBwdHeld = 16;

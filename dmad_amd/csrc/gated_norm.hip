@@ -20,7 +20,8 @@
 // and, forward with tangents, 508 us (5.1, 4.7 and 5.3 TB/s); a 4 GiB copy reaches 4.7. A
 // lane holds 8 neighbouring channels (one 16-byte access per
 // operand), so a row is ceil(C / 512) waves, which make one workgroup and exchange
-// their sums through LDS, two barriers per row; a row of one wave needs none, and
+// their sums through LDS: behind one barrier per row forwards, two backwards, and with
+// a norm after the branch two and four; a row of one wave needs none, and
 // four of them share a workgroup. A workgroup takes a run of a group's tokens: gate,
 // scale, shift and the weights stay in its registers, and the next token's rows are
 // requested before this one's are worked on.
@@ -509,13 +510,15 @@ __global__ __launch_bounds__(1024) void gated_norm_grad_kernel(GatedNormParams p
 
 #if DMAD_T == 0 && DMAD_W == 0
 int norm_waves(int C) { return C <= 512 ? kNormRowsPerGroup : (C + 511) / 512; }
-// Workgroups per group of tokens. A forward pass takes short runs, eight times what the
-// chip holds, and a call too small for runs of two tokens one round of it: 32760 tokens of
+// Workgroups per group of tokens. A forward pass takes short runs, eight rounds of 20 waves
+// per CU, and a call too small for runs of two tokens one such round: 32760 tokens of
 // 5120 264 us with 4096 workgroups, 293 with 1638, 288 with 512; 6000 tokens 55, 50 and 42. A
 // backward pass leaves sums behind for each, and of rows of ten waves a CU
 // holds one (16 waves of 128 registers): it has as few as fill a round of those, or a few
-// rounds, best. 32760 tokens of 5120 with 410 workgroups 553 us, with 256 371; of 1536 in 21
-// groups 116 us with 1029, 110 with 1260.
+// rounds, best. 32760 tokens of 5120 with the weights' gradients alone take 553 us with 410
+// workgroups, 371 with 256; of 1536 in 21 modulated groups 116 us with 1029, 110 with 1260. The rule
+// does not weigh the sums' bytes, which count where groups are many: 32256 tokens of 1536 in 672
+// groups get 7392 workgroups, whose 272 MB of sums take 123 + 118 us with the data's 595 MB.
 int gated_norm_split(int64_t groups, int T, int C, NormPass pass) {
   const int waves = norm_waves(C);
   int64_t split;

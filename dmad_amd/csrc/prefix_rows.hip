@@ -17,7 +17,9 @@
 //   * The softmax of one step runs between the MFMAs of the next one's scores.
 // A row's maximum follows lazily (it moves once a score exceeds it by 2^8 in bf16; at
 // once in fp16, where P enters as 2^15 P so that light slots keep their precision).
-// Scores of slots that are not there are -inf.
+// Scores of slots that are not there are -inf. P is rounded to the operand type for its
+// product with V alone (off by at most 2^-8 of each in bf16, 2^-11 in fp16, as in
+// paged_attn_kernel); maxima, sums of P and O are float32.
 //
 // 48 sequences of 4 tokens, 64 query heads over 8 key heads, behind 131072 slots: 0.82
 // ms for 8.3e11 flops, 1.0 PFLOP/s (a large matrix product reaches 1.23, plain attention
@@ -399,7 +401,8 @@ bool prefix_rows_takes(int D, int64_t R) { return (D == 64 || D == 128 || D == 2
 // Own slots of more than 32 rows whose tokens all see the same: 4 continuations by a frame
 // of 1560 tokens (12 heads, 1560 to 3120 own slots, behind 4000) 322 us against 737 with 16
 // rows per workgroup, 40 rows of 8 x 40 heads (1000 to 2000) 95 - 117, 48 of 4 x 16 64-wide
-// ones 32 - 29. Causal blocks stay with 16.
+// ones 32 - 29. Causal blocks go 16 at a time: the LDS kernel masks slots for all rows
+// alike, not row by row. The same frame, causal, takes 897 us.
 bool prefix_own_rows(int64_t R, bool causal, int64_t S) { return !(causal && S > 1) && R > kPrefixOwnRowsFrom; }
 // Workgroups per CU that the cut aims at; a CU holds 3, 2, 1. Fewer are fewer pieces to
 // leave and join, and leave room for the own slots: 128-wide heads 159 us with one
