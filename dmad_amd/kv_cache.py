@@ -454,9 +454,9 @@ def shared_prefix_attention(q, prefix, cache, sm_scale=None, causal=False, retur
     The result is that of caches whose page tables begin with the prefix's pages, but K and V of a prefix are read for all
     rows of its sequences together rather than once per sequence. The softmax weights are rounded to the operands' type for
     their product with V, as in ``paged_attention`` (off by at most half a step of each: 2^-8 in bf16, 2^-11 in fp16); their
-    sum, the scores and lse are float32. A sequence's result does not depend on the other sequences' queries. The two caches may share one pool of pages; a prefix or
-    a cache of no slots adds nothing, and a token that sees no slot of either gets o = 0 and lse = -inf. The caches are
-    only read; weights are not accumulated.
+    sum, the scores and lse are float32. A sequence's result does not depend on the other sequences' queries. The two caches
+    may share one pool of pages; a prefix or a cache of no slots adds nothing, and a token that sees no slot of either gets
+    o = 0 and lse = -inf. The caches are only read; weights are not accumulated.
     """
     scale = _check_prefix(q, prefix, cache, sm_scale)
     causal = bool(causal)
